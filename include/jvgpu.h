@@ -279,6 +279,64 @@ int jv_merge_topk_device(int32_t device, const int32_t* d_docs, const float* d_s
                          int32_t lists, int32_t k, int32_t* d_out_docs, float* d_out_scores,
                          void* hip_stream);
 
+/* ---- training and 8-bit scoring of vectors ----
+ * Operators on rows of vectors in HBM that belong to no index handle (though an index created with JV_DESC_BORROW may share the
+ * rows).  Every pointer but the structs is a DEVICE pointer on `device`; the calls allocate nothing, keep nothing between calls and
+ * make no host round trip, so they can be captured into a graph; the caller's current device is left as it was.
+ * `hip_stream`: NULL = the legacy default stream, and the call returns when its work is done; any other handle (hipStreamLegacy, (void*)1,
+ * names the default stream too) = the call returns after enqueueing.  Outputs must not overlap inputs.  Calls may run at the same time from
+ * any number of threads as long as they do not share outputs or a workspace. */
+typedef enum jv_dtype { JV_DTYPE_F32 = 0, JV_DTYPE_BF16 = 1 } jv_dtype;
+#define JV_OPS_MAX_D 65536 /* components of a row; JV_EUNSUPPORTED beyond, and beyond 2^31 - 65 537 rows */
+
+/* Rows of 8-bit floats: codes [n][B][128] e4m3 bytes (16-byte aligned, zeros behind component d), scales [n][B] bytes, B = ceil(d / 128).
+ * A block stands for  code * 2^(scale byte - 127)  with the least power of two that brings its largest finite magnitude to 448 or below;
+ * components are rounded to the nearest code, ties to the even one.  NaN and infinities become NaN codes (scores against them are NaN), a
+ * block of zeros has scale byte 127, magnitudes below 2^-136 become zero.  Any run of rows of such a matrix is one itself. */
+int jv_encode_blocks_device(int32_t device, const void* d_vectors, int32_t dtype, int64_t row_stride, int32_t n, int32_t d,
+                            uint8_t* d_out_codes, uint8_t* d_out_scales, void* hip_stream);
+/* The values that the codes stand for: 4 significant bits, exact in both types but where they pass the type's range (a component next to
+ * float32's largest may be held as 2^128: infinity). */
+int jv_decode_blocks_device(int32_t device, const uint8_t* d_codes, const uint8_t* d_scales, int32_t n, int32_t d, int32_t dtype,
+                            void* d_out_vectors, int64_t row_stride, void* hip_stream);
+/* out[i][j] = the dot product of query i and row j, both as such codes.  JV_DTYPE_F32: exact products, float32 sums (components below 2^-126 may count as
+ * zero).  JV_DTYPE_BF16: the 8-bit matrix unit's own sums (each group of 64 products is off by up to 2^-11 of its largest), rounded to bf16.
+ * row_stride: components from one query's scores to the next one's (>= n). */
+int jv_score_blocks_device(int32_t device, const uint8_t* d_query_codes, const uint8_t* d_query_scales, int32_t nq,
+                           const uint8_t* d_codes, const uint8_t* d_scales, int32_t n, int32_t d, int32_t dtype, void* d_out_scores,
+                           int64_t row_stride, void* hip_stream);
+
+/* Softmax cross entropy of queries over ALL rows of a matrix, as an embedding model or a query adapter is trained against a corpus:
+ *   lse_i = log sum_j exp(scale q_i . v_j),   loss_i = lse_i - scale q_i . v_t(i)
+ * in pieces of the rows: the nq x n logits are never held.  A target outside [0, n) is none: its loss is 0 and it adds to no gradient. */
+#define JV_SOFTMAX_MAX_QUERIES (1 << 22)
+typedef struct jv_softmax_params {
+    uint32_t struct_size;   /* sizeof(jv_softmax_params) */
+    int32_t device;
+    int32_t dtype;          /* jv_dtype of the queries, the vectors and their gradients */
+    int32_t nq, n, d;       /* queries, rows, components */
+    float scale;            /* 1 / temperature; finite */
+    int32_t reserved;
+    const void* queries;    /* [nq] rows, query_stride components apart */
+    int64_t query_stride;
+    const void* vectors;    /* [n] rows, vector_stride components apart */
+    int64_t vector_stride;
+    const int32_t* targets; /* [nq] or NULL = none has one (lse alone) */
+    void* workspace;        /* 256-byte aligned; in use until the call's work is done (graphs that may run at the same time need one each) */
+    int64_t workspace_bytes;
+} jv_softmax_params;
+#define JV_SOFTMAX_LOSS 0x1u
+#define JV_SOFTMAX_QUERY_GRAD 0x2u
+#define JV_SOFTMAX_VECTOR_GRAD 0x4u
+/* Bytes of workspace that the calls named by `what` (JV_SOFTMAX_*) need for this dtype, nq, n and d. */
+int jv_softmax_workspace(const jv_softmax_params* params, uint32_t what, int64_t* out_bytes);
+/* out_loss [nq], out_lse [nq] (natural logarithm; -inf if n == 0). */
+int jv_softmax_loss_device(const jv_softmax_params* params, float* d_out_loss, float* d_out_lse, void* hip_stream);
+/* Gradients of sum_i loss_grad_i loss_i (loss_grad NULL = 1 each) for the lse that jv_softmax_loss_device returned, each row rounded once
+ * to `dtype` and overwritten; a gradient whose pointer is NULL is not computed.  Sums are taken in a fixed order: two calls agree bit for bit. */
+int jv_softmax_grad_device(const jv_softmax_params* params, const float* d_lse, const float* d_loss_grad, void* d_out_query_grad,
+                           int64_t query_grad_stride, void* d_out_vector_grad, int64_t vector_grad_stride, void* hip_stream);
+
 /* Introspection used by the benchmark's roofline accounting. */
 typedef struct jv_index_info {
     int32_t n, d, R, similarity, pq_M, pq_K, num_upper_layers, device;

@@ -27,7 +27,12 @@ ABI_SYMBOLS = [
     "jv_abi_version", "jv_search_ex", "jv_search_batch_ex", "jv_index_set_option", "jv_index_get_counter", "jv_shard_group_create",
     "jv_shard_group_destroy", "jv_search_sharded_batch", "jv_search_sharded_batch_ex", "jv_shard_group_set_option",
     "jv_score_ordinals_batch", "jv_score_ordinals_batch_device", "jv_exact_search",
+    "jv_encode_blocks_device", "jv_decode_blocks_device", "jv_score_blocks_device", "jv_softmax_workspace", "jv_softmax_loss_device",
+    "jv_softmax_grad_device",
 ]
+DTYPE_F32, DTYPE_BF16 = 0, 1
+OPS_MAX_D, SOFTMAX_MAX_QUERIES = 65536, 1 << 22
+SOFTMAX_LOSS, SOFTMAX_QUERY_GRAD, SOFTMAX_VECTOR_GRAD = 0x1, 0x2, 0x4
 XB_NO_PREFILTER, XB_FORCE_PREFILTER, XB_TOPK_MAX, XB_INFO_WORDS = 0x1, 0x2, 1024, 4
 QFLAG_RETRIED_BIG, QFLAG_EARLY_TERMINATED = 0x1, 0x2
 
@@ -69,6 +74,14 @@ class JvIndexInfo(C.Structure):
         ("pq_K", C.c_int32), ("num_upper_layers", C.c_int32), ("device", C.c_int32), ("hbm_bytes", C.c_int64),
         ("row_stride_floats", C.c_int32), ("fused_adc", C.c_int32), ("scratch_bytes", C.c_int64),
         ("filter_cache_hits", C.c_int64), ("filter_cache_misses", C.c_int64),
+    ]
+
+
+class JvSoftmaxParams(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("device", C.c_int32), ("dtype", C.c_int32), ("nq", C.c_int32), ("n", C.c_int32), ("d", C.c_int32),
+        ("scale", C.c_float), ("reserved", C.c_int32), ("queries", C.c_void_p), ("query_stride", C.c_int64), ("vectors", C.c_void_p),
+        ("vector_stride", C.c_int64), ("targets", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
     ]
 
 
@@ -248,6 +261,18 @@ def load_library(path: str = LIB_PATH) -> C.CDLL:
     lib.jv_exact_search.restype = C.c_int
     lib.jv_merge_topk_device.argtypes = [i32, vp, vp, i32, i32, i32, vp, vp, vp]
     lib.jv_merge_topk_device.restype = C.c_int
+    lib.jv_encode_blocks_device.argtypes = [i32, vp, i32, i64, i32, i32, vp, vp, vp]
+    lib.jv_encode_blocks_device.restype = C.c_int
+    lib.jv_decode_blocks_device.argtypes = [i32, vp, vp, i32, i32, i32, vp, i64, vp]
+    lib.jv_decode_blocks_device.restype = C.c_int
+    lib.jv_score_blocks_device.argtypes = [i32, vp, vp, i32, vp, vp, i32, i32, i32, vp, i64, vp]
+    lib.jv_score_blocks_device.restype = C.c_int
+    lib.jv_softmax_workspace.argtypes = [C.POINTER(JvSoftmaxParams), C.c_uint32, C.POINTER(i64)]
+    lib.jv_softmax_workspace.restype = C.c_int
+    lib.jv_softmax_loss_device.argtypes = [C.POINTER(JvSoftmaxParams), vp, vp, vp]
+    lib.jv_softmax_loss_device.restype = C.c_int
+    lib.jv_softmax_grad_device.argtypes = [C.POINTER(JvSoftmaxParams), vp, vp, vp, i64, vp, i64, vp]
+    lib.jv_softmax_grad_device.restype = C.c_int
     lib.jv_index_get_info.argtypes = [vp, C.POINTER(JvIndexInfo)]
     lib.jv_index_get_info.restype = C.c_int
     lib.jv_set_option.argtypes = [C.c_char_p, i64]
@@ -572,3 +597,46 @@ def merge_topk_device(device: int, d_docs: int, d_scores: int, nq: int, lists: i
                       d_out_scores: int, stream: int = 0):
     lib = load_library()
     _check(lib, lib.jv_merge_topk_device(device, d_docs, d_scores, nq, lists, k, d_out_docs, d_out_scores, stream or None))
+
+
+def encode_blocks_device(device: int, d_vectors: int, dtype: int, row_stride: int, n: int, d: int, d_out_codes: int, d_out_scales: int, stream: int = 0):
+    lib = load_library()
+    _check(lib, lib.jv_encode_blocks_device(device, d_vectors, dtype, row_stride, n, d, d_out_codes, d_out_scales, stream or None))
+
+
+def decode_blocks_device(device: int, d_codes: int, d_scales: int, n: int, d: int, dtype: int, d_out_vectors: int, row_stride: int, stream: int = 0):
+    lib = load_library()
+    _check(lib, lib.jv_decode_blocks_device(device, d_codes, d_scales, n, d, dtype, d_out_vectors, row_stride, stream or None))
+
+
+def score_blocks_device(device: int, d_query_codes: int, d_query_scales: int, nq: int, d_codes: int, d_scales: int, n: int, d: int, dtype: int,
+                        d_out_scores: int, row_stride: int, stream: int = 0):
+    lib = load_library()
+    _check(lib, lib.jv_score_blocks_device(device, d_query_codes, d_query_scales, nq, d_codes, d_scales, n, d, dtype, d_out_scores, row_stride,
+                                           stream or None))
+
+
+def softmax_params(device: int, dtype: int, nq: int, n: int, d: int, scale: float, d_queries: int = 0, query_stride: int = 0, d_vectors: int = 0,
+                   vector_stride: int = 0, d_targets: int = 0) -> JvSoftmaxParams:
+    """jv_softmax_params without a workspace (softmax_workspace says how large it has to be)."""
+    return JvSoftmaxParams(C.sizeof(JvSoftmaxParams), device, dtype, nq, n, d, scale, 0, d_queries or None, query_stride, d_vectors or None,
+                           vector_stride, d_targets or None, None, 0)
+
+
+def softmax_workspace(params: JvSoftmaxParams, what: int) -> int:
+    lib = load_library()
+    need = C.c_int64()
+    _check(lib, lib.jv_softmax_workspace(C.byref(params), what, C.byref(need)))
+    return need.value
+
+
+def softmax_loss_device(params: JvSoftmaxParams, d_out_loss: int, d_out_lse: int, stream: int = 0):
+    lib = load_library()
+    _check(lib, lib.jv_softmax_loss_device(C.byref(params), d_out_loss, d_out_lse, stream or None))
+
+
+def softmax_grad_device(params: JvSoftmaxParams, d_lse: int, d_loss_grad: int, d_out_query_grad: int, query_grad_stride: int, d_out_vector_grad: int,
+                        vector_grad_stride: int, stream: int = 0):
+    lib = load_library()
+    _check(lib, lib.jv_softmax_grad_device(C.byref(params), d_lse, d_loss_grad or None, d_out_query_grad or None, query_grad_stride,
+                                           d_out_vector_grad or None, vector_grad_stride, stream or None))

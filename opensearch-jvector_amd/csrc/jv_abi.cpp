@@ -1698,6 +1698,15 @@ int check_common(jv_index* index, const void* q, int nq, int topK, int rk, float
 
 }  // namespace
 
+__attribute__((visibility("hidden"))) int jvi_fail(int code, const char* fmt, ...) {   // fail() for jv_abi_ops.cpp
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof(buf), fmt, ap);
+    va_end(ap);
+    return fail(code, "%s", buf);
+}
+
 extern "C" {
 
 int jv_abi_version(void) { return JVGPU_ABI_VERSION; }

@@ -1,0 +1,331 @@
+// jv_abi_ops.cpp — C ABI of the training and 8-bit scoring operators (include/jvgpu.h): argument checks, plans, launches.
+// No handle, no allocation, no host round trip: a call only enqueues kernels on the caller's stream, so it can be captured.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+
+#include "../../include/jvgpu.h"
+#include "jv_ops.h"
+
+#define CHK(expr)                                                                                                                    \
+    do {                                                                                                                             \
+        hipError_t e_ = (expr);                                                                                                      \
+        if (e_ != hipSuccess)                                                                                                        \
+            return jvi_fail(e_ == hipErrorOutOfMemory ? JV_ENOMEM : JV_EDEVICE, "%s failed: %s", #expr, hipGetErrorString(e_));      \
+    } while (0)
+
+namespace {
+
+constexpr int64_t kMaxRows = 0x7fffffffll - 65536;   // a tile behind the last row still has an int32 number
+constexpr int64_t kMaxStride = 1ll << 31;
+
+// the caller's current device comes back on every way out
+class OnDevice {
+public:
+    explicit OnDevice(int device) {
+        if ((err_ = hipGetDevice(&before_)) != hipSuccess) return;
+        if (before_ != device && (err_ = hipSetDevice(device)) == hipSuccess) moved_ = true;
+    }
+    ~OnDevice() {
+        if (moved_) (void)hipSetDevice(before_);
+    }
+    hipError_t error() const { return err_; }
+
+private:
+    int before_ = 0;
+    bool moved_ = false;
+    hipError_t err_ = hipSuccess;
+};
+
+int done(void* stream) {   // NULL: the legacy default stream, synchronous
+    if (!stream) CHK(hipStreamSynchronize(nullptr));
+    return JV_OK;
+}
+
+int size_of(int dtype) { return dtype == JV_DTYPE_F32 ? 4 : 2; }
+
+int check_dtype(int dtype, const char* what) {
+    if (dtype != JV_DTYPE_F32 && dtype != JV_DTYPE_BF16) return jvi_fail(JV_EINVAL, "%s: dtype %d is neither JV_DTYPE_F32 nor JV_DTYPE_BF16", what, dtype);
+    return JV_OK;
+}
+// a matrix of the caller's: rows of d components, `stride` components apart
+int check_rows(const void* p, int64_t rows, int64_t stride, int d, int dtype, const char* what) {
+    if (rows > 0 && !p) return jvi_fail(JV_EINVAL, "%s is NULL", what);
+    if ((uintptr_t)p % size_of(dtype)) return jvi_fail(JV_EINVAL, "%s is not aligned to its %d-byte components", what, size_of(dtype));
+    if (stride < d || stride > kMaxStride) return jvi_fail(JV_EINVAL, "%s: row stride %lld not in [d = %d, 2^31]", what, (long long)stride, d);
+    return JV_OK;
+}
+int check_codes(const void* codes, const void* scales, int64_t rows, const char* what) {
+    if (rows > 0 && (!codes || !scales)) return jvi_fail(JV_EINVAL, "%s: codes / scales are NULL", what);
+    if ((uintptr_t)codes % 16) return jvi_fail(JV_EINVAL, "%s: codes are not 16-byte aligned", what);
+    return JV_OK;
+}
+int check_shape(int64_t n, int d, const char* what) {
+    if (n < 0 || d <= 0) return jvi_fail(JV_EINVAL, "%s: bad shape n=%lld d=%d", what, (long long)n, d);
+    if (n > kMaxRows || d > JV_OPS_MAX_D) return jvi_fail(JV_EUNSUPPORTED, "%s: n=%lld d=%d beyond %lld rows / %d components", what, (long long)n, d, (long long)kMaxRows, JV_OPS_MAX_D);
+    return JV_OK;
+}
+
+#define TRY(x)                        \
+    do {                              \
+        const int rc_ = (x);          \
+        if (rc_ != JV_OK) return rc_; \
+    } while (0)
+
+// ---- the softmax loss: what a call needs, from its shape alone ----
+struct Plan {
+    int P, segs, dp, nk, kq;          // planes, segments; d padded to 64, in 128-B steps; nq padded to 64
+    int64_t rows_f, rows_b;           // rows of one piece, forward (only if the vectors have to be laid out) / backward
+    int splits_f, splits_q;
+    int64_t off_q, off_v, off_vt, off_qt, off_g, off_gt, off_slab, off_part, bytes;
+};
+
+int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+// n cut into equal pieces of at most `most` rows, whole tiles
+int64_t piece(int64_t n, int64_t most) {
+    most = std::max<int64_t>(up(most, 128), 128);
+    const int64_t pieces = std::max<int64_t>((n + most - 1) / most, 1);
+    return std::max<int64_t>(up((n + pieces - 1) / pieces, 128), 128);
+}
+
+Plan make_plan(int dtype, int nq, int64_t n, int d, uint32_t what) {
+    Plan p{};
+    p.P = dtype == JV_DTYPE_F32 ? 3 : 1;
+    p.segs = dtype == JV_DTYPE_F32 ? 6 : 1;
+    p.dp = (int)up(d, 64);
+    p.nk = p.dp / 64;
+    p.kq = (int)up(std::max(nq, 1), 64);
+    const int64_t panels = (nq + 127) / 128, row = (int64_t)p.P * p.dp * 2;
+    const int64_t fill = 128 * ((1024 + panels - 1) / std::max<int64_t>(panels, 1));   // rows that fill the chip once
+    p.rows_f = piece(n, std::max<int64_t>((64ll << 20) / row, fill));
+    p.rows_b = piece(n, std::max<int64_t>((64ll << 20) / ((int64_t)p.P * 2 * p.kq), fill));
+    const int64_t panel = std::max<int64_t>(panels, 1);
+    p.splits_f = (int)std::min<int64_t>((1024 + panel - 1) / panel, std::max<int64_t>((n + 127) / 128, 1));
+    int64_t at = 0;
+    auto take = [&](int64_t bytes) {
+        const int64_t o = at;
+        at += up(bytes, 256);
+        return o;
+    };
+    p.off_q = take((int64_t)nq * row);
+    if (what & JV_SOFTMAX_LOSS) {
+        p.off_part = take((int64_t)p.splits_f * nq * 8);
+        p.off_v = take(std::min<int64_t>(p.rows_f, n) * row);
+    }
+    if (what & (JV_SOFTMAX_QUERY_GRAD | JV_SOFTMAX_VECTOR_GRAD)) {
+        p.off_v = take(p.rows_b * row);
+        if (what & JV_SOFTMAX_QUERY_GRAD) {
+            const int64_t tiles = panel * ((d + 127) / 128), steps = p.rows_b / 64 * p.segs;
+            p.splits_q = (int)std::max<int64_t>(std::min<int64_t>((512 + tiles - 1) / tiles, steps / 8), 1);
+            p.off_vt = take((int64_t)d * p.P * p.rows_b * 2);
+            p.off_g = take((int64_t)nq * p.P * p.rows_b * 2);
+            p.off_slab = take((int64_t)p.splits_q * nq * d * 4);
+        }
+        if (what & JV_SOFTMAX_VECTOR_GRAD) {
+            p.off_qt = take((int64_t)d * p.P * p.kq * 2);
+            p.off_gt = take(p.rows_b * p.P * p.kq * 2);
+        }
+    }
+    p.bytes = at;
+    return p;
+}
+
+// rows as the matrix cores take them: the caller's own where they are bf16, 16-B aligned and whole steps
+struct Rows {
+    const char* p;
+    int64_t stride;
+    bool ready;
+};
+Rows rows_of(const void* p, int64_t stride, int d, int dtype) {
+    return {(const char*)p, stride * 2, dtype == JV_DTYPE_BF16 && (uintptr_t)p % 16 == 0 && stride % 8 == 0 && d % 64 == 0};
+}
+
+int check_softmax(const jv_softmax_params* p) {
+    if (!p) return jvi_fail(JV_EINVAL, "softmax: params is NULL");
+    if (p->struct_size != sizeof(jv_softmax_params))
+        return jvi_fail(JV_EINVAL, "jv_softmax_params.struct_size %u != %zu (ABI mismatch)", p->struct_size, sizeof(jv_softmax_params));
+    TRY(check_dtype(p->dtype, "softmax"));
+    TRY(check_shape(p->n, p->d, "softmax: vectors"));
+    TRY(check_shape(p->nq, p->d, "softmax: queries"));
+    if (p->nq > JV_SOFTMAX_MAX_QUERIES) return jvi_fail(JV_EUNSUPPORTED, "softmax: %d queries (> %d)", p->nq, JV_SOFTMAX_MAX_QUERIES);
+    if (!std::isfinite(p->scale)) return jvi_fail(JV_EINVAL, "softmax: scale is not finite");
+    return JV_OK;
+}
+int check_softmax_call(const jv_softmax_params* p, const Plan& plan) {
+    TRY(check_rows(p->queries, p->nq, p->query_stride, p->d, p->dtype, "softmax: queries"));
+    TRY(check_rows(p->vectors, p->n, p->vector_stride, p->d, p->dtype, "softmax: vectors"));
+    if (!p->workspace || (uintptr_t)p->workspace % 256) return jvi_fail(JV_EINVAL, "softmax: workspace is NULL or not 256-byte aligned");
+    if (p->workspace_bytes < plan.bytes)
+        return jvi_fail(JV_EINVAL, "softmax: workspace of %lld bytes, %lld needed", (long long)p->workspace_bytes, (long long)plan.bytes);
+    return JV_OK;
+}
+
+// the rows [at, at + rows) of a matrix, laid out in the workspace unless they are ready
+int lay_out(const Rows& r, const void* p, int64_t stride, int dtype, int64_t at, int64_t rows, const Plan& plan, int d, char* to, hipStream_t s, const char** out,
+            int64_t* ld) {
+    if (r.ready) {
+        *out = r.p + at * r.stride;
+        *ld = r.stride;
+        return JV_OK;
+    }
+    CHK(jvk_sx_pack((const char*)p + at * stride * size_of(dtype), dtype, stride, rows, d, plan.dp, (uint16_t*)to, s));
+    *out = to;
+    *ld = (int64_t)plan.P * plan.dp * 2;
+    return JV_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int jv_encode_blocks_device(int32_t device, const void* d_vectors, int32_t dtype, int64_t row_stride, int32_t n, int32_t d, uint8_t* d_out_codes,
+                            uint8_t* d_out_scales, void* hip_stream) {
+    TRY(check_dtype(dtype, "encode"));
+    TRY(check_shape(n, d, "encode"));
+    TRY(check_rows(d_vectors, n, row_stride, d, dtype, "encode: vectors"));
+    TRY(check_codes(d_out_codes, d_out_scales, n, "encode"));
+    OnDevice on(device);
+    CHK(on.error());
+    CHK(jvk_f8_encode(d_vectors, dtype, row_stride, n, d, d_out_codes, d_out_scales, (hipStream_t)hip_stream));
+    return done(hip_stream);
+}
+
+int jv_decode_blocks_device(int32_t device, const uint8_t* d_codes, const uint8_t* d_scales, int32_t n, int32_t d, int32_t dtype, void* d_out_vectors,
+                            int64_t row_stride, void* hip_stream) {
+    TRY(check_dtype(dtype, "decode"));
+    TRY(check_shape(n, d, "decode"));
+    TRY(check_rows(d_out_vectors, n, row_stride, d, dtype, "decode: vectors"));
+    TRY(check_codes(d_codes, d_scales, n, "decode"));
+    OnDevice on(device);
+    CHK(on.error());
+    CHK(jvk_f8_decode(d_codes, d_scales, n, d, d_out_vectors, dtype, row_stride, (hipStream_t)hip_stream));
+    return done(hip_stream);
+}
+
+int jv_score_blocks_device(int32_t device, const uint8_t* d_query_codes, const uint8_t* d_query_scales, int32_t nq, const uint8_t* d_codes,
+                           const uint8_t* d_scales, int32_t n, int32_t d, int32_t dtype, void* d_out_scores, int64_t row_stride, void* hip_stream) {
+    TRY(check_dtype(dtype, "score"));
+    TRY(check_shape(nq, d, "score: queries"));
+    TRY(check_shape(n, d, "score: rows"));
+    TRY(check_codes(d_query_codes, d_query_scales, nq, "score: queries"));
+    TRY(check_codes(d_codes, d_scales, n, "score: rows"));
+    if (nq > 0) TRY(check_rows(d_out_scores, n, row_stride, n, dtype, "score: scores"));
+    OnDevice on(device);
+    CHK(on.error());
+    JvMmOut a{};
+    a.mm.nk = (d + 127) / 128;
+    a.mm.a = (const char*)d_query_codes, a.mm.b = (const char*)d_codes;
+    a.mm.lda = a.mm.ldb = (int64_t)a.mm.nk * 128;
+    a.mm.M = nq, a.mm.N = n, a.mm.segs = 1;
+    a.mm.sa = d_query_scales, a.mm.sb = d_scales;
+    a.dtype = dtype, a.out = d_out_scores, a.ldo = row_stride, a.splits = 1;
+    CHK(jvk_f8_score(&a, (hipStream_t)hip_stream));
+    return done(hip_stream);
+}
+
+int jv_softmax_workspace(const jv_softmax_params* params, uint32_t what, int64_t* out_bytes) {
+    TRY(check_softmax(params));
+    if (!out_bytes || !what || (what & ~7u)) return jvi_fail(JV_EINVAL, "softmax: out_bytes is NULL or unknown flags %#x", what);
+    int64_t need = 256;   // (the loss and its gradient are separate calls: the larger of the two)
+    for (uint32_t part : {what & JV_SOFTMAX_LOSS, what & (JV_SOFTMAX_QUERY_GRAD | JV_SOFTMAX_VECTOR_GRAD)})
+        if (part) need = std::max(need, make_plan(params->dtype, params->nq, params->n, params->d, part).bytes);
+    *out_bytes = need;
+    return JV_OK;
+}
+
+int jv_softmax_loss_device(const jv_softmax_params* p, float* d_out_loss, float* d_out_lse, void* hip_stream) {
+    TRY(check_softmax(p));
+    const Plan plan = make_plan(p->dtype, p->nq, p->n, p->d, JV_SOFTMAX_LOSS);
+    TRY(check_softmax_call(p, plan));
+    if (p->nq > 0 && (!d_out_loss || !d_out_lse)) return jvi_fail(JV_EINVAL, "softmax: output pointer is NULL");
+    OnDevice on(p->device);
+    CHK(on.error());
+    hipStream_t s = (hipStream_t)hip_stream;
+    if (p->nq > 0) {
+        char* ws = (char*)p->workspace;
+        const Rows rq = rows_of(p->queries, p->query_stride, p->d, p->dtype), rv = rows_of(p->vectors, p->vector_stride, p->d, p->dtype);
+        const int64_t step = rv.ready ? std::max<int64_t>(p->n, 1) : plan.rows_f;
+        JvSxLoss a{};
+        a.mm.nk = plan.nk, a.mm.segs = plan.segs, a.mm.N = p->nq;
+        a.c = p->scale * 1.44269504088896341f;
+        a.splits = p->n > 0 ? plan.splits_f : 0, a.part = (float*)(ws + plan.off_part);
+        if (p->n > 0) TRY(lay_out(rq, p->queries, p->query_stride, p->dtype, 0, p->nq, plan, p->d, ws + plan.off_q, s, &a.mm.b, &a.mm.ldb));
+        for (int64_t at = 0; at < p->n; at += step) {
+            a.mm.M = (int)std::min<int64_t>(step, p->n - at);
+            a.first = at == 0;
+            TRY(lay_out(rv, p->vectors, p->vector_stride, p->dtype, at, a.mm.M, plan, p->d, ws + plan.off_v, s, &a.mm.a, &a.mm.lda));
+            CHK(jvk_sx_loss(&a, s));
+        }
+        CHK(jvk_sx_join(a.part, a.splits, p->nq, p->queries, p->query_stride, p->vectors, p->vector_stride, p->dtype, p->d, p->targets, p->n, p->scale, d_out_loss,
+                        d_out_lse, s));
+    }
+    return done(hip_stream);
+}
+
+int jv_softmax_grad_device(const jv_softmax_params* p, const float* d_lse, const float* d_loss_grad, void* d_out_query_grad, int64_t query_grad_stride,
+                           void* d_out_vector_grad, int64_t vector_grad_stride, void* hip_stream) {
+    TRY(check_softmax(p));
+    const uint32_t what = (d_out_query_grad ? JV_SOFTMAX_QUERY_GRAD : 0) | (d_out_vector_grad ? JV_SOFTMAX_VECTOR_GRAD : 0);
+    if (!what) return jvi_fail(JV_EINVAL, "softmax: no gradient asked for");
+    const Plan plan = make_plan(p->dtype, p->nq, p->n, p->d, what);
+    TRY(check_softmax_call(p, plan));
+    if (p->nq > 0 && !d_lse) return jvi_fail(JV_EINVAL, "softmax: lse is NULL");
+    if (d_out_query_grad) TRY(check_rows(d_out_query_grad, p->nq, query_grad_stride, p->d, p->dtype, "softmax: query gradient"));
+    if (d_out_vector_grad) TRY(check_rows(d_out_vector_grad, p->n, vector_grad_stride, p->d, p->dtype, "softmax: vector gradient"));
+    OnDevice on(p->device);
+    CHK(on.error());
+    hipStream_t s = (hipStream_t)hip_stream;
+    if (p->nq == 0 || p->n == 0 || !p->targets) {   // nothing was asked of the rows: gradients of zero
+        if (d_out_query_grad) CHK(jvk_sx_fill(d_out_query_grad, p->dtype, query_grad_stride, p->nq, p->d, 0.0f, s));
+        if (d_out_vector_grad) CHK(jvk_sx_fill(d_out_vector_grad, p->dtype, vector_grad_stride, p->n, p->d, 0.0f, s));
+        return done(hip_stream);
+    }
+    char* ws = (char*)p->workspace;
+    const Rows rq = rows_of(p->queries, p->query_stride, p->d, p->dtype), rv = rows_of(p->vectors, p->vector_stride, p->d, p->dtype);
+    JvSxWeights w{};
+    w.mm.nk = plan.nk, w.mm.segs = plan.segs, w.mm.N = p->nq;
+    w.c = p->scale * 1.44269504088896341f, w.scale = p->scale;
+    w.lse = d_lse, w.w = d_loss_grad, w.targets = p->targets, w.n = p->n;
+    w.planes = plan.P, w.kq = plan.kq;
+    w.g = d_out_query_grad ? (uint16_t*)(ws + plan.off_g) : nullptr;
+    w.gt = d_out_vector_grad ? (uint16_t*)(ws + plan.off_gt) : nullptr;
+    uint16_t *vt = (uint16_t*)(ws + plan.off_vt), *qt = (uint16_t*)(ws + plan.off_qt);
+    TRY(lay_out(rq, p->queries, p->query_stride, p->dtype, 0, p->nq, plan, p->d, ws + plan.off_q, s, &w.mm.b, &w.mm.ldb));
+    if (w.gt) CHK(jvk_sx_pack_t(p->queries, p->dtype, p->query_stride, p->nq, p->d, plan.kq, qt, s));
+    for (int64_t at = 0; at < p->n; at += plan.rows_b) {
+        const int rows = (int)std::min<int64_t>(plan.rows_b, p->n - at);
+        w.mm.M = rows, w.row0 = at, w.kv = (int)up(rows, 64);
+        TRY(lay_out(rv, p->vectors, p->vector_stride, p->dtype, at, rows, plan, p->d, ws + plan.off_v, s, &w.mm.a, &w.mm.lda));
+        CHK(jvk_sx_weights(&w, s));
+        const char* v = (const char*)p->vectors + at * p->vector_stride * size_of(p->dtype);
+        JvMmOut o{};
+        o.mm.segs = plan.segs, o.dtype = p->dtype;
+        if (w.g) {
+            CHK(jvk_sx_pack_t(v, p->dtype, p->vector_stride, rows, p->d, w.kv, vt, s));
+            o.mm.a = (const char*)w.g, o.mm.b = (const char*)vt;
+            o.mm.lda = o.mm.ldb = (int64_t)plan.P * w.kv * 2;
+            o.mm.M = p->nq, o.mm.N = p->d, o.mm.nk = w.kv / 64;
+            o.slab = (float*)(ws + plan.off_slab), o.add = at > 0;
+            o.splits = std::min(plan.splits_q, o.mm.nk * plan.segs);   // (only the last piece can be that short: it adds to the first splits)
+            CHK(jvk_sx_mm(&o, s));
+        }
+        if (w.gt) {
+            o.mm.a = (const char*)w.gt, o.mm.b = (const char*)qt;
+            o.mm.lda = o.mm.ldb = (int64_t)plan.P * plan.kq * 2;
+            o.mm.M = rows, o.mm.N = p->d, o.mm.nk = plan.kq / 64;
+            o.slab = nullptr, o.splits = 1;
+            o.out = (char*)d_out_vector_grad + at * vector_grad_stride * size_of(p->dtype), o.ldo = vector_grad_stride;
+            CHK(jvk_sx_mm(&o, s));
+        }
+    }
+    if (w.g) {
+        const int splits = std::min<int64_t>(plan.splits_q, up(std::min<int64_t>(plan.rows_b, p->n), 64) / 64 * plan.segs);
+        CHK(jvk_sx_finish((const float*)(ws + plan.off_slab), splits, p->nq, p->d, d_out_query_grad, p->dtype, query_grad_stride, s));
+    }
+    return done(hip_stream);
+}
+
+}  // extern "C"

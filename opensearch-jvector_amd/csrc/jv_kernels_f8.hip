@@ -1,0 +1,141 @@
+// jv_kernels_f8.hip — rows of 8-bit floats with one scale for each block of 128 components: encode, decode, and the product of a batch of
+// queries with such rows (gfx950).
+//
+// A block of x is held as e4m3 codes c and one exponent byte b:  x ~ c 2^(b - 127),  2^(b - 127) the least power of two with
+// max|x| <= 448 * 2^(b - 127)  (448: the largest e4m3 value).  A power of two, because the matrix instruction takes such a scale as an
+// operand and because it makes both directions exact but for the one rounding to e4m3.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "jv_mm.h"
+#include "jv_mm_out.h"
+
+using namespace jvmm;
+
+#define F8_CHUNK 128   // blocks of one workgroup: 16 for each of its 8 half-waves
+
+// ---------------------------------------------------------------------------------------------
+// A half-wave holds one block, four components a lane: the block's maximum is five exchanges, a store is 4 B of codes.
+// ---------------------------------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ f32x4 load4(const T* row, int at, int d, bool wide) {
+    f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (wide && at + 3 < d) {
+        if constexpr (sizeof(T) == 4) {
+            x = *(const f32x4*)(row + at);
+        } else {
+            const bf16x4 v = *(const bf16x4*)(row + at);
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[e] = (float)v[e];
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (at + e < d) x[e] = (float)row[at + e];
+    }
+    return x;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void jvf_encode_kernel(const T* __restrict__ x, int64_t stride, int64_t blocks, int d, int nb, int wide,
+                                                         uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+    const int hw = threadIdx.x >> 5, l = threadIdx.x & 31;
+    const int64_t first = (int64_t)blockIdx.x * F8_CHUNK;
+    const int64_t row0 = first / nb;
+    const uint32_t b0 = (uint32_t)(first - row0 * nb);
+    for (int i = 0; i < F8_CHUNK / 8; i++) {
+        const int64_t blk = first + i * 8 + hw;
+        if (blk >= blocks) break;   // (whole half-waves: the exchanges below stay inside one)
+        const uint32_t at = b0 + (uint32_t)(i * 8 + hw), up = at / (uint32_t)nb, b = at - up * (uint32_t)nb;
+        const f32x4 v = load4(x + (row0 + up) * stride, (int)b * 128 + l * 4, d, wide);
+        // the largest finite magnitude, compared as bits
+        uint32_t top = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const uint32_t bits = __float_as_uint(v[e]) & 0x7fffffffu;
+            top = bits < 0x7f800000u && bits > top ? bits : top;
+        }
+#pragma unroll
+        for (int off = 16; off >= 1; off >>= 1) {
+            const uint32_t other = (uint32_t)__shfl_xor((int)top, off, 64);
+            top = other > top ? other : top;
+        }
+        // top = 1.m 2^(e - 127): 2^(e - 135) reaches 1.75 2^8 = 448, the next one the rest (a subnormal maximum ends at byte 0)
+        int byte = (int)(top >> 23) - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
+        byte = byte < 0 ? 0 : byte;
+        byte = top == 0 ? 127 : byte;
+        const float inv = __uint_as_float((uint32_t)(254 - byte) << 23);
+        int c = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * inv, v[1] * inv, 0, false);
+        c = __builtin_amdgcn_cvt_pk_fp8_f32(v[2] * inv, v[3] * inv, c, true);
+        uint32_t code = (uint32_t)c;
+#pragma unroll
+        for (int e = 0; e < 4; e++)   // e4m3 has no infinity: what is not finite becomes its NaN
+            if ((__float_as_uint(v[e]) & 0x7f800000u) == 0x7f800000u) code = (code & ~(0xffu << (8 * e))) | (0x7fu << (8 * e));
+        *(uint32_t*)(codes + blk * 128 + l * 4) = code;
+        if (l == 0) scales[blk] = (uint8_t)byte;
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void jvf_decode_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t blocks,
+                                                         int d, int nb, int wide, T* __restrict__ x, int64_t stride) {
+    const int hw = threadIdx.x >> 5, l = threadIdx.x & 31;
+    const int64_t first = (int64_t)blockIdx.x * F8_CHUNK;
+    const int64_t row0 = first / nb;
+    const uint32_t b0 = (uint32_t)(first - row0 * nb);
+    for (int i = 0; i < F8_CHUNK / 8; i++) {
+        const int64_t blk = first + i * 8 + hw;
+        if (blk >= blocks) break;
+        const uint32_t p = b0 + (uint32_t)(i * 8 + hw), up = p / (uint32_t)nb, b = p - up * (uint32_t)nb;
+        const int code = *(const int*)(codes + blk * 128 + l * 4);
+        const uint32_t byte = scales[blk];
+        const float s = byte == 0 ? __uint_as_float(0x00400000u) : byte == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float(byte << 23);
+        const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(code, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(code, true);
+        const float v[4] = {lo[0] * s, lo[1] * s, hi[0] * s, hi[1] * s};
+        const int at = (int)b * 128 + l * 4;
+        T* out = x + (row0 + up) * stride + at;
+        if (wide && at + 3 < d) {
+            if constexpr (sizeof(T) == 4) {
+                *(f32x4*)out = (f32x4){v[0], v[1], v[2], v[3]};
+            } else {
+                *(bf16x4*)out = (bf16x4){(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (at + e < d) out[e] = (T)v[e];
+        }
+    }
+}
+
+static bool wide4(const void* p, int64_t stride, int dtype) {
+    const int size = dtype == 0 ? 4 : 2;
+    return ((uintptr_t)p % (4 * size)) == 0 && stride % 4 == 0;
+}
+
+extern "C" hipError_t jvk_f8_encode(const void* x, int dtype, int64_t stride, int64_t n, int d, uint8_t* codes, uint8_t* scales, hipStream_t s) {
+    const int nb = (d + 127) / 128;
+    const int64_t blocks = n * nb, grid = (blocks + F8_CHUNK - 1) / F8_CHUNK;
+    if (grid <= 0) return hipSuccess;
+    if (grid > 0x7fffffffll) return hipErrorInvalidValue;
+    const int wide = wide4(x, stride, dtype);
+    if (dtype == 0) jvf_encode_kernel<float><<<(unsigned)grid, 256, 0, s>>>((const float*)x, stride, blocks, d, nb, wide, codes, scales);
+    else jvf_encode_kernel<__bf16><<<(unsigned)grid, 256, 0, s>>>((const __bf16*)x, stride, blocks, d, nb, wide, codes, scales);
+    return hipGetLastError();
+}
+
+extern "C" hipError_t jvk_f8_decode(const uint8_t* codes, const uint8_t* scales, int64_t n, int d, void* x, int dtype, int64_t stride, hipStream_t s) {
+    const int nb = (d + 127) / 128;
+    const int64_t blocks = n * nb, grid = (blocks + F8_CHUNK - 1) / F8_CHUNK;
+    if (grid <= 0) return hipSuccess;
+    if (grid > 0x7fffffffll) return hipErrorInvalidValue;
+    const int wide = wide4(x, stride, dtype);
+    if (dtype == 0) jvf_decode_kernel<float><<<(unsigned)grid, 256, 0, s>>>(codes, scales, blocks, d, nb, wide, (float*)x, stride);
+    else jvf_decode_kernel<__bf16><<<(unsigned)grid, 256, 0, s>>>(codes, scales, blocks, d, nb, wide, (__bf16*)x, stride);
+    return hipGetLastError();
+}
+
+// bf16 scores keep 8 bits: the 8-bit unit's sums are enough.  float32 scores take the bf16 unit (jv_mm.h).
+extern "C" hipError_t jvk_f8_score(const JvMmOut* a, hipStream_t s) {
+    return a->dtype == 0 ? mm_out<F8W, 2, 2, 2, 2>(*a, s) : mm_out<F8, 2, 2, 2, 2>(*a, s);
+}

@@ -1,0 +1,192 @@
+// jv_mm.h — the matrix-core product of rows with rows that the training and 8-bit scoring kernels share (see JvMm).
+//
+// A workgroup owns a tile of C and walks k in steps of 128 bytes a row, in one of three kinds of arithmetic:
+//   BF16  64 bf16 (v_mfma_f32_32x32x16_bf16: exact products, float32 sums);
+//   F8    128 e4m3 as they are (v_mfma_scale_f32_32x32x64_f8f6f4, whose operands take the block's power-of-two scale as an exponent byte:
+//         the scale costs no vector instruction).  This unit adds a group's products with about 12 bits below the largest of them
+//         (measured: off by up to 2^-11.7 of the largest product, 1.4e-5 of the result's norm), so it serves results of 8 bits;
+//   F8W   128 e4m3 widened to bf16 with their scale on the way into the bf16 unit (exact: 4 significant bits): float32 sums (5e-8 of the
+//         result's norm) at half the rate and one conversion for every two components.
+// Both operands are staged with 16-B copies straight into LDS; a copy's 64 lanes fill an 8-row group of 1 024 B in
+// order, so the swizzle (16-B piece p of row r at p ^ (r & 7)) is on the source address.  Groups are 1 152 B apart: a 16-B fragment
+// read serves 16 consecutive rows at a time, the pad puts the two groups of such a pair on opposite halves of the 256-B bank row.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "jv_ops.h"
+
+namespace jvmm {
+
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(4))) int i32x4;
+typedef __attribute__((ext_vector_type(8))) int i32x8;
+
+enum { BF16 = 0, F8 = 1, F8W = 2 };
+constexpr int GROUP = 1152;
+
+__device__ __forceinline__ void glds16(const char* g, unsigned char* l) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g, (__attribute__((address_space(3))) void*)l, 16, 0, 0);
+}
+
+// plane of segment g (see JvMm): pairs (2,0) (0,2) (1,1) (1,0) (0,1) (0,0), the smallest products first
+__device__ __forceinline__ int plane_a(int g) { return (0x052 >> (2 * g)) & 3; }
+__device__ __forceinline__ int plane_b(int g) { return (0x118 >> (2 * g)) & 3; }
+
+// eight e4m3 codes times 2^(byte - 127), as bf16
+__device__ __forceinline__ bf16x8 widen(int lo, int hi, int byte) {
+    const float s = __int_as_float(byte << 23);
+    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, true);
+    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, true);
+    const bf16x4 x = __builtin_shufflevector(a, b, 0, 1, 2, 3), y = __builtin_shufflevector(c, d, 0, 1, 2, 3);
+    return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// MT x NT accumulators of 32 x 32 for each of WM x WN waves
+template <int TY, int MT, int NT, int WM, int WN>
+struct Tile {
+    static constexpr int TM = 32 * MT * WM, TN = 32 * NT * WN, WAVES = WM * WN, THREADS = 64 * WAVES;
+    static constexpr int GA = TM / 8, GB = TN / 8, PER = (GA + GB) / WAVES;   // 8-row groups; copies of one wave a step
+    static constexpr int BUF = (GA + GB) * GROUP, LDS = 2 * BUF;
+    static_assert((GA + GB) % WAVES == 0 && GA % PER == 0, "a wave's groups lie in one operand");
+
+    // C tile at (m0, n0), steps [k0, k1) of the segs * nk in all.  Rows behind the operands' last are read as their last.
+    static __device__ __forceinline__ void run(const JvMm& a, int m0, int n0, int k0, int k1, unsigned char* smem, f32x16 (&acc)[MT][NT]) {
+        const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+        const int lr = lane >> 3, lp = (lane & 7) ^ lr;
+        const bool isb = w * PER >= GA;
+        const char* src[PER];
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            const int row = 8 * (w * PER + i) + lr;
+            int r = isb ? n0 + row - TM : m0 + row;
+            const int last = (isb ? a.N : a.M) - 1;
+            if (r > last) r = last;
+            src[i] = (isb ? a.b + (int64_t)r * a.ldb : a.a + (int64_t)r * a.lda) + lp * 16;
+        }
+        const int wm = w % WM, wn = w / WM, h = lane >> 5, r31 = lane & 31;
+        int aoff[MT], boff[NT], ax, bx;
+#pragma unroll
+        for (int t = 0; t < MT; t++) {
+            const int r = (wm * MT + t) * 32 + r31;
+            aoff[t] = (r >> 3) * GROUP + (r & 7) * 128;
+        }
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            const int r = (wn * NT + t) * 32 + r31;
+            boff[t] = (GA + (r >> 3)) * GROUP + (r & 7) * 128;
+        }
+        ax = bx = r31 & 7;
+        const uint8_t *pa[MT], *pb[NT];
+        if constexpr (TY != BF16) {
+#pragma unroll
+            for (int t = 0; t < MT; t++) pa[t] = a.sa + (int64_t)min(m0 + (wm * MT + t) * 32 + r31, a.M - 1) * a.nk;
+#pragma unroll
+            for (int t = 0; t < NT; t++) pb[t] = a.sb + (int64_t)min(n0 + (wn * NT + t) * 32 + r31, a.N - 1) * a.nk;
+        }
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) acc[m][n][e] = 0.0f;
+
+        int seg = k0 / a.nk, kin = k0 - seg * a.nk;   // of the next step to be staged
+        auto stage = [&](int buf) {
+            int64_t off = (int64_t)kin * 128;
+            if (a.segs > 1) off += (int64_t)(isb ? plane_b(seg) : plane_a(seg)) * a.nk * 128;
+            unsigned char* dst = smem + buf * BUF + w * PER * GROUP;
+#pragma unroll
+            for (int i = 0; i < PER; i++) glds16(src[i] + off, dst + i * GROUP);
+            if (++kin == a.nk) kin = 0, seg++;
+        };
+        stage(0);
+        for (int s = k0; s < k1; s++) {
+            const int buf = (s - k0) & 1;
+            int fa[MT], fb[NT];
+            if constexpr (TY != BF16) {
+#pragma unroll
+                for (int t = 0; t < MT; t++) fa[t] = pa[t][s];
+#pragma unroll
+                for (int t = 0; t < NT; t++) fb[t] = pb[t][s];
+            }
+            if (s + 1 < k1) {
+                stage(buf ^ 1);
+                asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(PER) : "memory");
+            } else {
+                asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+            }
+            const unsigned char* base = smem + buf * BUF;
+            if constexpr (TY == BF16) {
+#pragma unroll
+                for (int kk = 0; kk < 4; kk++) {
+                    bf16x8 va[MT], vb[NT];
+#pragma unroll
+                    for (int t = 0; t < MT; t++) va[t] = *(const bf16x8*)(base + aoff[t] + (((2 * kk + h) ^ ax) << 4));
+#pragma unroll
+                    for (int t = 0; t < NT; t++) vb[t] = *(const bf16x8*)(base + boff[t] + (((2 * kk + h) ^ bx) << 4));
+#pragma unroll
+                    for (int m = 0; m < MT; m++)
+#pragma unroll
+                        for (int n = 0; n < NT; n++) acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va[m], vb[n], acc[m][n], 0, 0, 0);
+                }
+            } else if constexpr (TY == F8W) {
+                // (16 components a lane and step: which of the block's 128 does not matter as long as both operands agree)
+#pragma unroll
+                for (int kk = 0; kk < 4; kk++) {
+                    i32x4 ra[MT], rb[NT];
+#pragma unroll
+                    for (int t = 0; t < MT; t++) ra[t] = *(const i32x4*)(base + aoff[t] + (((2 * kk + h) ^ ax) << 4));
+#pragma unroll
+                    for (int t = 0; t < NT; t++) rb[t] = *(const i32x4*)(base + boff[t] + (((2 * kk + h) ^ bx) << 4));
+#pragma unroll
+                    for (int half = 0; half < 2; half++) {
+                        bf16x8 va[MT], vb[NT];
+#pragma unroll
+                        for (int t = 0; t < MT; t++) va[t] = widen(ra[t][2 * half], ra[t][2 * half + 1], fa[t]);
+#pragma unroll
+                        for (int t = 0; t < NT; t++) vb[t] = widen(rb[t][2 * half], rb[t][2 * half + 1], fb[t]);
+#pragma unroll
+                        for (int m = 0; m < MT; m++)
+#pragma unroll
+                            for (int n = 0; n < NT; n++) acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va[m], vb[n], acc[m][n], 0, 0, 0);
+                    }
+                }
+            } else {
+                // (which 32 of the block's 128 components a lane holds does not matter as long as both operands agree: one scale for all)
+#pragma unroll
+                for (int kk = 0; kk < 2; kk++) {
+                    i32x8 va[MT], vb[NT];
+                    auto frag = [&](int off, int x) -> i32x8 {
+                        const i32x4 lo = *(const i32x4*)(base + off + (((4 * kk + 2 * h) ^ x) << 4));
+                        const i32x4 hi = *(const i32x4*)(base + off + (((4 * kk + 2 * h + 1) ^ x) << 4));
+                        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                    };
+#pragma unroll
+                    for (int t = 0; t < MT; t++) va[t] = frag(aoff[t], ax);
+#pragma unroll
+                    for (int t = 0; t < NT; t++) vb[t] = frag(boff[t], bx);
+#pragma unroll
+                    for (int m = 0; m < MT; m++)
+#pragma unroll
+                        for (int n = 0; n < NT; n++)
+                            acc[m][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(va[m], vb[n], acc[m][n], 0, 0, 0, fa[m], 0, fb[n]);
+                }
+            }
+            // every fragment read of this buffer has returned before any wave stages into it again
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        }
+    }
+    // row of accumulator register e of tile m, column of tile n, inside the workgroup's tile
+    static __device__ __forceinline__ int row_of(int m, int e) {
+        const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+        return ((w % WM) * MT + m) * 32 + (e & 3) + 8 * (e >> 2) + 4 * (lane >> 5);
+    }
+    static __device__ __forceinline__ int col_of(int n) { return (((threadIdx.x >> 6) / WM) * NT + n) * 32 + (threadIdx.x & 31); }
+};
+
+}  // namespace jvmm
