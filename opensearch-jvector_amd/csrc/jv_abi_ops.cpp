@@ -76,19 +76,19 @@ int check_shape(int64_t n, int d, const char* what) {
 
 // ---- the softmax loss: what a call needs, from its shape alone ----
 struct Plan {
-    int P, segs, dp, nk, kq;          // planes, segments; d padded to 64, in 128-B steps; nq padded to 64
+    int P, segs, dp, kq;              // planes, segments; d and nq padded to 64
     int64_t rows_f, rows_b;           // rows of one piece, forward (only if the vectors have to be laid out) / backward
-    int splits_f, splits_q;
-    int64_t off_q, off_v, off_vt, off_qt, off_g, off_gt, off_slab, off_part, bytes;
+    int tile, splits_f, splits_q;
+    int64_t off_q, off_v, off_part, off_query, off_norm, off_rest, off_g, off_slab, bytes;
 };
 
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
 // n cut into equal pieces of at most `most` rows, whole tiles
 int64_t piece(int64_t n, int64_t most) {
-    most = std::max<int64_t>(up(most, 128), 128);
+    most = std::max<int64_t>(up(most, 256), 256);
     const int64_t pieces = std::max<int64_t>((n + most - 1) / most, 1);
-    return std::max<int64_t>(up((n + pieces - 1) / pieces, 128), 128);
+    return std::max<int64_t>(up((n + pieces - 1) / pieces, 256), 256);
 }
 
 Plan make_plan(int dtype, int nq, int64_t n, int d, uint32_t what) {
@@ -96,14 +96,11 @@ Plan make_plan(int dtype, int nq, int64_t n, int d, uint32_t what) {
     p.P = dtype == JV_DTYPE_F32 ? 3 : 1;
     p.segs = dtype == JV_DTYPE_F32 ? 6 : 1;
     p.dp = (int)up(d, 64);
-    p.nk = p.dp / 64;
     p.kq = (int)up(std::max(nq, 1), 64);
-    const int64_t panels = (nq + 127) / 128, row = (int64_t)p.P * p.dp * 2;
-    const int64_t fill = 128 * ((1024 + panels - 1) / std::max<int64_t>(panels, 1));   // rows that fill the chip once
-    p.rows_f = piece(n, std::max<int64_t>((64ll << 20) / row, fill));
-    p.rows_b = piece(n, std::max<int64_t>((64ll << 20) / ((int64_t)p.P * 2 * p.kq), fill));
-    const int64_t panel = std::max<int64_t>(panels, 1);
-    p.splits_f = (int)std::min<int64_t>((1024 + panel - 1) / panel, std::max<int64_t>((n + 127) / 128, 1));
+    const int64_t panels = std::max((nq + 255) / 256, 1), row = (int64_t)p.P * p.dp * 2;
+    const int64_t fill = 256 * ((1024 + panels - 1) / panels);   // rows whose tiles fill the chip four times
+    p.rows_f = piece(n, std::max<int64_t>((128ll << 20) / row, fill));
+    p.rows_b = piece(n, std::max<int64_t>((128ll << 20) / ((int64_t)p.P * 2 * p.kq), fill));
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
         const int64_t o = at;
@@ -112,21 +109,21 @@ Plan make_plan(int dtype, int nq, int64_t n, int d, uint32_t what) {
     };
     p.off_q = take((int64_t)nq * row);
     if (what & JV_SOFTMAX_LOSS) {
+        p.splits_f = jvk_sx_loss_plan(nq, n, &p.tile);
         p.off_part = take((int64_t)p.splits_f * nq * 8);
         p.off_v = take(std::min<int64_t>(p.rows_f, n) * row);
     }
     if (what & (JV_SOFTMAX_QUERY_GRAD | JV_SOFTMAX_VECTOR_GRAD)) {
-        p.off_v = take(p.rows_b * row);
+        p.off_v = take(std::min<int64_t>(p.rows_b, n) * row);
+        p.off_query = take((int64_t)nq * sizeof(JvSxQuery));
+        p.off_norm = take(4);
+        p.off_rest = take((int64_t)nq * 4);
+        p.off_g = take((int64_t)p.kq * p.P * p.rows_b * 2);
         if (what & JV_SOFTMAX_QUERY_GRAD) {
-            const int64_t tiles = panel * ((d + 127) / 128), steps = p.rows_b / 64 * p.segs;
-            p.splits_q = (int)std::max<int64_t>(std::min<int64_t>((512 + tiles - 1) / tiles, steps / 8), 1);
-            p.off_vt = take((int64_t)d * p.P * p.rows_b * 2);
-            p.off_g = take((int64_t)nq * p.P * p.rows_b * 2);
-            p.off_slab = take((int64_t)p.splits_q * nq * d * 4);
-        }
-        if (what & JV_SOFTMAX_VECTOR_GRAD) {
-            p.off_qt = take((int64_t)d * p.P * p.kq * 2);
-            p.off_gt = take(p.rows_b * p.P * p.kq * 2);
+            // k ranges: all tiles of all ranges once around the CUs, eight phases in each at least
+            const int64_t tiles = panels * ((d + 255) / 256), phases = p.rows_b / 32 * p.segs;
+            p.splits_q = (int)std::max<int64_t>(std::min<int64_t>(256 / tiles, phases / 8), 1);
+            p.off_slab = take((int64_t)p.splits_q * nq * p.dp * 4);
         }
     }
     p.bytes = at;
@@ -161,6 +158,14 @@ int check_softmax_call(const jv_softmax_params* p, const Plan& plan) {
     if (p->workspace_bytes < plan.bytes)
         return jvi_fail(JV_EINVAL, "softmax: workspace of %lld bytes, %lld needed", (long long)p->workspace_bytes, (long long)plan.bytes);
     return JV_OK;
+}
+
+// queries times vectors, but for where the vectors lie and how many they are
+JvMm logits(const Plan& plan, int nq) {
+    JvMm mm{};
+    mm.M = nq, mm.kph = plan.dp / 32, mm.segs = plan.segs;
+    mm.plane_a = mm.plane_b = (int64_t)plan.dp * 2;
+    return mm;
 }
 
 // the rows [at, at + rows) of a matrix, laid out in the workspace unless they are ready
@@ -216,12 +221,13 @@ int jv_score_blocks_device(int32_t device, const uint8_t* d_query_codes, const u
     OnDevice on(device);
     CHK(on.error());
     JvMmOut a{};
-    a.mm.nk = (d + 127) / 128;
+    const int blocks = (d + 127) / 128;
+    a.mm.kph = 2 * blocks;
     a.mm.a = (const char*)d_query_codes, a.mm.b = (const char*)d_codes;
-    a.mm.lda = a.mm.ldb = (int64_t)a.mm.nk * 128;
+    a.mm.lda = a.mm.ldb = (int64_t)blocks * 128;
     a.mm.M = nq, a.mm.N = n, a.mm.segs = 1;
     a.mm.sa = d_query_scales, a.mm.sb = d_scales;
-    a.dtype = dtype, a.out = d_out_scores, a.ldo = row_stride, a.splits = 1;
+    a.mul = 1.0f, a.dtype = dtype, a.out = d_out_scores, a.ldo = row_stride, a.splits = 1;
     CHK(jvk_f8_score(&a, (hipStream_t)hip_stream));
     return done(hip_stream);
 }
@@ -249,14 +255,14 @@ int jv_softmax_loss_device(const jv_softmax_params* p, float* d_out_loss, float*
         const Rows rq = rows_of(p->queries, p->query_stride, p->d, p->dtype), rv = rows_of(p->vectors, p->vector_stride, p->d, p->dtype);
         const int64_t step = rv.ready ? std::max<int64_t>(p->n, 1) : plan.rows_f;
         JvSxLoss a{};
-        a.mm.nk = plan.nk, a.mm.segs = plan.segs, a.mm.N = p->nq;
+        a.mm = logits(plan, p->nq);
         a.c = p->scale * 1.44269504088896341f;
-        a.splits = p->n > 0 ? plan.splits_f : 0, a.part = (float*)(ws + plan.off_part);
-        if (p->n > 0) TRY(lay_out(rq, p->queries, p->query_stride, p->dtype, 0, p->nq, plan, p->d, ws + plan.off_q, s, &a.mm.b, &a.mm.ldb));
+        a.tile = plan.tile, a.splits = p->n > 0 ? plan.splits_f : 0, a.part = (float*)(ws + plan.off_part);
+        if (p->n > 0) TRY(lay_out(rq, p->queries, p->query_stride, p->dtype, 0, p->nq, plan, p->d, ws + plan.off_q, s, &a.mm.a, &a.mm.lda));
         for (int64_t at = 0; at < p->n; at += step) {
-            a.mm.M = (int)std::min<int64_t>(step, p->n - at);
+            a.mm.N = (int)std::min<int64_t>(step, p->n - at);
             a.first = at == 0;
-            TRY(lay_out(rv, p->vectors, p->vector_stride, p->dtype, at, a.mm.M, plan, p->d, ws + plan.off_v, s, &a.mm.a, &a.mm.lda));
+            TRY(lay_out(rv, p->vectors, p->vector_stride, p->dtype, at, a.mm.N, plan, p->d, ws + plan.off_v, s, &a.mm.b, &a.mm.ldb));
             CHK(jvk_sx_loss(&a, s));
         }
         CHK(jvk_sx_join(a.part, a.splits, p->nq, p->queries, p->query_stride, p->vectors, p->vector_stride, p->dtype, p->d, p->targets, p->n, p->scale, d_out_loss,
@@ -286,44 +292,42 @@ int jv_softmax_grad_device(const jv_softmax_params* p, const float* d_lse, const
     char* ws = (char*)p->workspace;
     const Rows rq = rows_of(p->queries, p->query_stride, p->d, p->dtype), rv = rows_of(p->vectors, p->vector_stride, p->d, p->dtype);
     JvSxWeights w{};
-    w.mm.nk = plan.nk, w.mm.segs = plan.segs, w.mm.N = p->nq;
-    w.c = p->scale * 1.44269504088896341f, w.scale = p->scale;
-    w.lse = d_lse, w.w = d_loss_grad, w.targets = p->targets, w.n = p->n;
-    w.planes = plan.P, w.kq = plan.kq;
-    w.g = d_out_query_grad ? (uint16_t*)(ws + plan.off_g) : nullptr;
-    w.gt = d_out_vector_grad ? (uint16_t*)(ws + plan.off_gt) : nullptr;
-    uint16_t *vt = (uint16_t*)(ws + plan.off_vt), *qt = (uint16_t*)(ws + plan.off_qt);
-    TRY(lay_out(rq, p->queries, p->query_stride, p->dtype, 0, p->nq, plan, p->d, ws + plan.off_q, s, &w.mm.b, &w.mm.ldb));
-    if (w.gt) CHK(jvk_sx_pack_t(p->queries, p->dtype, p->query_stride, p->nq, p->d, plan.kq, qt, s));
+    w.mm = logits(plan, p->nq);
+    w.c = p->scale * 1.44269504088896341f;
+    w.planes = plan.P, w.g = (uint16_t*)(ws + plan.off_g), w.rest = (float*)(ws + plan.off_rest);
+    JvSxQuery* query = (JvSxQuery*)(ws + plan.off_query);
+    w.query = query;
+    float* norm = (float*)(ws + plan.off_norm);
+    CHK(jvk_sx_queries(d_lse, d_loss_grad, p->targets, p->nq, p->n, query, norm, w.rest, s));
+    TRY(lay_out(rq, p->queries, p->query_stride, p->dtype, 0, p->nq, plan, p->d, ws + plan.off_q, s, &w.mm.a, &w.mm.lda));
     for (int64_t at = 0; at < p->n; at += plan.rows_b) {
         const int rows = (int)std::min<int64_t>(plan.rows_b, p->n - at);
-        w.mm.M = rows, w.row0 = at, w.kv = (int)up(rows, 64);
-        TRY(lay_out(rv, p->vectors, p->vector_stride, p->dtype, at, rows, plan, p->d, ws + plan.off_v, s, &w.mm.a, &w.mm.lda));
+        w.mm.N = rows, w.row0 = at, w.kv = (int)up(rows, 64);
+        TRY(lay_out(rv, p->vectors, p->vector_stride, p->dtype, at, rows, plan, p->d, ws + plan.off_v, s, &w.mm.b, &w.mm.ldb));
         CHK(jvk_sx_weights(&w, s));
-        const char* v = (const char*)p->vectors + at * p->vector_stride * size_of(p->dtype);
         JvMmOut o{};
-        o.mm.segs = plan.segs, o.dtype = p->dtype;
-        if (w.g) {
-            CHK(jvk_sx_pack_t(v, p->dtype, p->vector_stride, rows, p->d, w.kv, vt, s));
-            o.mm.a = (const char*)w.g, o.mm.b = (const char*)vt;
-            o.mm.lda = o.mm.ldb = (int64_t)plan.P * w.kv * 2;
-            o.mm.M = p->nq, o.mm.N = p->d, o.mm.nk = w.kv / 64;
-            o.slab = (float*)(ws + plan.off_slab), o.add = at > 0;
-            o.splits = std::min(plan.splits_q, o.mm.nk * plan.segs);   // (only the last piece can be that short: it adds to the first splits)
-            CHK(jvk_sx_mm(&o, s));
+        o.mm.segs = plan.segs;
+        o.mm.a = (const char*)w.g, o.mm.lda = (int64_t)plan.P * w.kv * 2, o.mm.plane_a = (int64_t)w.kv * 2;
+        o.mm.N = p->d, o.mm.plane_b = (int64_t)plan.dp * 2, o.mm.cb = plan.dp;
+        if (d_out_query_grad) {   // G times the piece's vectors: k = its rows
+            o.mm.M = p->nq, o.mm.kph = w.kv / 32;
+            o.mm.b = w.mm.b, o.mm.ldb = w.mm.ldb, o.mm.kb = rows;
+            o.mul = 1.0f, o.out = ws + plan.off_slab, o.ldo = plan.dp, o.add = at > 0;
+            o.splits = std::min(plan.splits_q, o.mm.kph * plan.segs);   // (only the last piece can be that short: it adds to the first ranges)
+            CHK(jvk_sx_query_grad(&o, s));
         }
-        if (w.gt) {
-            o.mm.a = (const char*)w.gt, o.mm.b = (const char*)qt;
-            o.mm.lda = o.mm.ldb = (int64_t)plan.P * plan.kq * 2;
-            o.mm.M = rows, o.mm.N = p->d, o.mm.nk = plan.kq / 64;
-            o.slab = nullptr, o.splits = 1;
+        if (d_out_vector_grad) {   // G across times the queries: k = the queries
+            o.mm.M = rows, o.mm.kph = plan.kq / 32, o.mm.ka = plan.kq, o.mm.ca = w.kv;
+            o.mm.b = w.mm.a, o.mm.ldb = w.mm.lda, o.mm.kb = p->nq;
+            o.mul = p->scale, o.norm = norm, o.dtype = p->dtype, o.splits = 1, o.add = 0;
             o.out = (char*)d_out_vector_grad + at * vector_grad_stride * size_of(p->dtype), o.ldo = vector_grad_stride;
-            CHK(jvk_sx_mm(&o, s));
+            CHK(jvk_sx_vector_grad(&o, s));
         }
     }
-    if (w.g) {
-        const int splits = std::min<int64_t>(plan.splits_q, up(std::min<int64_t>(plan.rows_b, p->n), 64) / 64 * plan.segs);
-        CHK(jvk_sx_finish((const float*)(ws + plan.off_slab), splits, p->nq, p->d, d_out_query_grad, p->dtype, query_grad_stride, s));
+    if (d_out_query_grad) {
+        const int splits = (int)std::min<int64_t>(plan.splits_q, up(std::min<int64_t>(plan.rows_b, p->n), 64) / 32 * plan.segs);
+        CHK(jvk_sx_finish((const float*)(ws + plan.off_slab), splits, p->nq, p->d, plan.dp, w.rest, query, p->vectors, p->vector_stride, p->scale, norm, d_out_query_grad,
+                          p->dtype, query_grad_stride, s));
     }
     return done(hip_stream);
 }

@@ -14,6 +14,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 #include "jv_mm.h"
 #include "jv_mm_out.h"
 
@@ -70,42 +72,6 @@ __global__ __launch_bounds__(256) void jvs_pack_kernel(const T* __restrict__ x, 
     }
 }
 
-// rows [rows][d] -> columns as rows [d][P][kr], zeros behind `rows`: 64 x 64 blocks through LDS
-template <typename T>
-__global__ __launch_bounds__(256) void jvs_pack_t_kernel(const T* __restrict__ x, int64_t stride, int rows, int d, int kr, uint16_t* __restrict__ out) {
-    constexpr int P = sizeof(T) == 4 ? 3 : 1;
-    __shared__ T tile[64][65];
-    const int r0 = blockIdx.x * 64, c0 = blockIdx.y * 64;
-    for (int i = threadIdx.x; i < 4096; i += 256) {
-        const int r = i >> 6, c = i & 63;
-        tile[r][c] = r0 + r < rows && c0 + c < d ? x[(int64_t)(r0 + r) * stride + c0 + c] : (T)0.0f;
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < 512; i += 256) {
-        const int c = i >> 3, r = (i & 7) * 8;
-        if (c0 + c >= d) continue;
-        uint16_t p[3][8];
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            if constexpr (P == 1) {
-                p[0][e] = __builtin_bit_cast(uint16_t, tile[r + e][c]);
-            } else {
-                uint16_t q[3];
-                planes3(tile[r + e][c], q);
-#pragma unroll
-                for (int k = 0; k < 3; k++) p[k][e] = q[k];
-            }
-        }
-#pragma unroll
-        for (int k = 0; k < P; k++) {
-            i32x4 o;
-#pragma unroll
-            for (int e = 0; e < 4; e++) o[e] = (int)((uint32_t)p[k][2 * e] | ((uint32_t)p[k][2 * e + 1] << 16));
-            *(i32x4*)(out + ((int64_t)(c0 + c) * P + k) * kr + r0 + r) = o;
-        }
-    }
-}
-
 extern "C" hipError_t jvk_sx_pack(const void* x, int dtype, int64_t stride, int64_t rows, int d, int kp, uint16_t* out, hipStream_t s) {
     const int64_t want = (rows * (kp / 8) + 255) / 256;
     if (want <= 0) return hipSuccess;
@@ -114,14 +80,6 @@ extern "C" hipError_t jvk_sx_pack(const void* x, int dtype, int64_t stride, int6
     else jvs_pack_kernel<__bf16><<<grid, 256, 0, s>>>((const __bf16*)x, stride, rows, d, kp, out);
     return hipGetLastError();
 }
-extern "C" hipError_t jvk_sx_pack_t(const void* x, int dtype, int64_t stride, int rows, int d, int kr, uint16_t* out, hipStream_t s) {
-    if (kr <= 0 || d <= 0) return hipSuccess;
-    const dim3 grid((unsigned)(kr / 64), (unsigned)((d + 63) / 64));
-    if (dtype == 0) jvs_pack_t_kernel<float><<<grid, 256, 0, s>>>((const float*)x, stride, rows, d, kr, out);
-    else jvs_pack_t_kernel<__bf16><<<grid, 256, 0, s>>>((const __bf16*)x, stride, rows, d, kr, out);
-    return hipGetLastError();
-}
-
 // ---------------------------------------------------------------------------------------------
 // forward: running maximum and sum over this workgroup's tiles of rows
 // ---------------------------------------------------------------------------------------------
@@ -133,73 +91,138 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
     m = top;
 }
 
-template <int MT, int NT, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN) void jvs_loss_kernel(const JvSxLoss a) {
-    using T = Tile<BF16, MT, NT, WM, WN>;
-    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    const int tiles = (a.mm.M + T::TM - 1) / T::TM;
-    const int split = blockIdx.x, n0 = blockIdx.y * T::TN;
-    float top[NT], sum[NT];
+// a lane's part of a tile: MT queries, NT * 16 rows each.  `rows`: how many rows the tile has in all (NT * 16 of them are not this lane's)
+template <class Core, int MT, int NT>
+__device__ __forceinline__ void add_tile(const f32x16 (&acc)[MT][NT], float c, int rows, float (&top)[MT], float (&sum)[MT]) {
+    const bool full = rows >= Core::TN;
 #pragma unroll
-    for (int n = 0; n < NT; n++) top[n] = -__builtin_inff(), sum[n] = 0.0f;
-    for (int t = split; t < tiles; t += a.splits) {
-        f32x16 acc[MT][NT];
-        T::run(a.mm, t * T::TM, n0, 0, a.mm.nk * a.mm.segs, smem, acc);
+    for (int m = 0; m < MT; m++) {
+        float best = -__builtin_inff();
+        float z[NT][16];
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
-            float best = -__builtin_inff();
+        for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int m = 0; m < MT; m++)
+            for (int e = 0; e < 16; e++) {
+                z[n][e] = full || Core::col(n, e) < rows ? acc[m][n][e] * c : -__builtin_inff();
+                best = fmaxf(best, z[n][e]);
+            }
+        const float now = fmaxf(top[m], best), ref = now == -__builtin_inff() ? 0.0f : now;
+        float s = sum[m] * exp2_(top[m] - ref);
 #pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    const float z = t * T::TM + T::row_of(m, e) < a.mm.M ? acc[m][n][e] * a.c : -__builtin_inff();
-                    acc[m][n][e] = z;
-                    best = fmaxf(best, z);
-                }
-            const float now = fmaxf(top[n], best), ref = now == -__builtin_inff() ? 0.0f : now;
-            float s = sum[n] * exp2_(top[n] - ref);
+        for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int m = 0; m < MT; m++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) s += exp2_(acc[m][n][e] - ref);
-            top[n] = now;
-            sum[n] = s;
-        }
+            for (int e = 0; e < 16; e++) s += exp2_(z[n][e] - ref);
+        top[m] = now;
+        sum[m] = s;
     }
-    // the two halves of a wave hold different rows of the same query, and so do the WM waves of a column
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, wm = w % WM;
-    float* sh = (float*)smem;   // [WM][TN][2]
+}
+
+// joins what the lanes and waves of a workgroup hold of the same queries and writes one partial for each of the panel's queries
+template <int TM, int MT, int WN, class Row>
+__device__ __forceinline__ void write_partials(const JvSxLoss& a, unsigned char* smem, int m0, int split, int wn, Row&& row, float (&top)[MT], float (&sum)[MT]) {
+    float* sh = (float*)smem;   // [WN][TM][2]
     __syncthreads();
 #pragma unroll
-    for (int n = 0; n < NT; n++) {
-        join(top[n], sum[n], __shfl_xor(top[n], 32, 64), __shfl_xor(sum[n], 32, 64));
-        if (lane < 32) {
-            sh[(wm * T::TN + T::col_of(n)) * 2] = top[n];
-            sh[(wm * T::TN + T::col_of(n)) * 2 + 1] = sum[n];
+    for (int m = 0; m < MT; m++) {
+        join(top[m], sum[m], __shfl_xor(top[m], 32, 64), __shfl_xor(sum[m], 32, 64));
+        if ((threadIdx.x & 63) < 32) {
+            sh[(wn * TM + row(m)) * 2] = top[m];
+            sh[(wn * TM + row(m)) * 2 + 1] = sum[m];
         }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < T::TN; i += T::THREADS) {
-        if (n0 + i >= a.mm.N) continue;
+    for (int i = threadIdx.x; i < TM; i += blockDim.x) {
+        if (m0 + i >= a.mm.M) continue;
         float m = sh[i * 2], s = sh[i * 2 + 1];
 #pragma unroll
-        for (int k = 1; k < WM; k++) join(m, s, sh[(k * T::TN + i) * 2], sh[(k * T::TN + i) * 2 + 1]);
-        float* pm = a.part + (int64_t)split * a.mm.N + n0 + i;
-        float* ps = pm + (int64_t)a.splits * a.mm.N;
+        for (int k = 1; k < WN; k++) join(m, s, sh[(k * TM + i) * 2], sh[(k * TM + i) * 2 + 1]);
+        float* pm = a.part + (int64_t)split * a.mm.M + m0 + i;
+        float* ps = pm + (int64_t)a.splits * a.mm.M;
         if (!a.first) join(m, s, *pm, *ps);
         *pm = m;
         *ps = s;
     }
 }
 
-extern "C" hipError_t jvk_sx_loss(const JvSxLoss* a, hipStream_t s) {
-    using T = Tile<BF16, 2, 2, 2, 2>;
-    const int panels = (a->mm.N + T::TN - 1) / T::TN;
-    if (panels <= 0 || a->mm.M <= 0) return hipSuccess;
-    if (panels > 65535 || a->splits < 1) return hipErrorInvalidValue;
-    hipError_t e = hipFuncSetAttribute((const void*)jvs_loss_kernel<2, 2, 2, 2>, hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS);
+__global__ __launch_bounds__(512) void jvs_loss_pipe_kernel(const JvSxLoss a) {
+    using P = Pipe<BF16>;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    // one panel of queries and every `splits`-th tile of rows; the panels of a split side by side: they share its rows
+    const int panels = (a.mm.M + P::TM - 1) / P::TM, tiles = (a.mm.N + P::TN - 1) / P::TN;
+    const Share share(panels * a.splits);
+    int L;
+    if (!share.at(0, L)) return;
+    const int split = L / panels, m0 = (L - split * panels) * P::TM;
+    float top[4], sum[4];
+#pragma unroll
+    for (int m = 0; m < 4; m++) top[m] = -__builtin_inff(), sum[m] = 0.0f;
+    if (split < tiles)
+        P::run(
+            a.mm, smem,
+            [&](int i, Work& w) {
+                const int t = split + i * a.splits;
+                if (t >= tiles) return false;
+                w.m0 = m0, w.n0 = t * P::TN, w.k0 = 0, w.k1 = a.mm.kph * a.mm.segs;
+                return true;
+            },
+            [&](const Work& w, f32x16 (&acc)[4][2]) -> int {
+                add_tile<P>(acc, a.c, a.mm.N - w.n0, top, sum);
+                return 0;
+            });
+    write_partials<P::TM, 4, 4>(a, smem, m0, split, threadIdx.x >> 7, [](int m) { return P::row(m); }, top, sum);
+}
+
+template <int MT, int NT, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void jvs_loss_tile_kernel(const JvSxLoss a) {
+    using T = Tile<BF16, MT, NT, WM, WN>;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    const int panels = (a.mm.M + T::TM - 1) / T::TM, tiles = (a.mm.N + T::TN - 1) / T::TN;
+    const Share share(panels * a.splits);
+    int L;
+    if (!share.at(0, L)) return;
+    const int split = L / panels, m0 = (L - split * panels) * T::TM;
+    float top[MT], sum[MT];
+#pragma unroll
+    for (int m = 0; m < MT; m++) top[m] = -__builtin_inff(), sum[m] = 0.0f;
+    for (int t = split; t < tiles; t += a.splits) {
+        f32x16 acc[MT][NT];
+        T::run(a.mm, m0, t * T::TN, smem, acc);
+        add_tile<T>(acc, a.c, a.mm.N - t * T::TN, top, sum);
+    }
+    write_partials<T::TM, MT, WN>(a, smem, m0, split, (threadIdx.x >> 6) / WM, [](int m) { return T::row(m); }, top, sum);
+}
+
+// the large tiles where they fill the chip
+static bool large(int nq, int64_t rows) { return nq > 64 && ((nq + 255) / 256) * ((rows + 255) / 256) >= 192; }
+
+// workgroups that share a panel's rows: one for each CU with the large tiles, two or three with the small ones
+extern "C" int jvk_sx_loss_plan(int nq, int64_t rows, int* tile) {
+    const int tm = large(nq, rows) ? 256 : nq > 64 ? 128 : nq > 32 ? 64 : 32, tn = tm == 256 ? 256 : 128, full = tm == 256 ? 256 : tm == 128 ? 512 : 768;
+    const int64_t panels = std::max((nq + tm - 1) / tm, 1), tiles = std::max<int64_t>((rows + tn - 1) / tn, 1);
+    *tile = tm;
+    return (int)std::min(std::max<int64_t>(full / panels, 1), tiles);
+}
+
+template <int MT, int NT, int WM, int WN>
+static hipError_t loss_tile(const JvSxLoss& a, hipStream_t s) {
+    using T = Tile<BF16, MT, NT, WM, WN>;
+    hipError_t e = hipFuncSetAttribute((const void*)jvs_loss_tile_kernel<MT, NT, WM, WN>, hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS);
     if (e != hipSuccess) return e;
-    jvs_loss_kernel<2, 2, 2, 2><<<dim3((unsigned)a->splits, (unsigned)panels), T::THREADS, T::LDS, s>>>(*a);
+    const int64_t all = (int64_t)((a.mm.M + T::TM - 1) / T::TM) * a.splits;
+    jvs_loss_tile_kernel<MT, NT, WM, WN><<<(unsigned)((all + 7) / 8 * 8), T::THREADS, T::LDS, s>>>(a);
+    return hipGetLastError();
+}
+extern "C" hipError_t jvk_sx_loss(const JvSxLoss* a, hipStream_t s) {
+    using P = Pipe<BF16>;
+    if (a->mm.N <= 0 || a->mm.M <= 0) return hipSuccess;
+    if (a->splits < 1) return hipErrorInvalidValue;
+    if (a->tile == 128) return loss_tile<2, 2, 2, 2>(*a, s);
+    if (a->tile == 64) return loss_tile<2, 1, 1, 4>(*a, s);
+    if (a->tile == 32) return loss_tile<1, 1, 1, 4>(*a, s);
+    hipError_t e = hipFuncSetAttribute((const void*)jvs_loss_pipe_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, P::LDS);
+    if (e != hipSuccess) return e;
+    const int64_t all = (int64_t)((a->mm.M + P::TM - 1) / P::TM) * a->splits;
+    jvs_loss_pipe_kernel<<<(unsigned)((all + 7) / 8 * 8), P::THREADS, P::LDS, s>>>(*a);
     return hipGetLastError();
 }
 
@@ -239,73 +262,122 @@ extern "C" hipError_t jvk_sx_join(const float* part, int splits, int nq, const v
 // ---------------------------------------------------------------------------------------------
 // backward: the logits again, as weights g
 // ---------------------------------------------------------------------------------------------
-template <int MT, int NT, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN) void jvs_weights_kernel(const JvSxWeights a) {
-    using T = Tile<BF16, MT, NT, WM, WN>;
-    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    const int m0 = blockIdx.x * T::TM, n0 = blockIdx.y * T::TN;
-    f32x16 acc[MT][NT];
-    T::run(a.mm, m0, n0, 0, a.mm.nk * a.mm.segs, smem, acc);
+// What the gradient needs of each query.  The weights are divided by the largest of them (`norm`, multiplied back in float32 at the end): an
+// entry at a target is then just below 1 for the largest weight, where bf16's step is finest in relation.
+__global__ __launch_bounds__(1024) void jvs_queries_kernel(const float* __restrict__ lse, const float* __restrict__ w, const int32_t* __restrict__ targets,
+                                                           int nq, int64_t n, JvSxQuery* __restrict__ query, float* __restrict__ norm,
+                                                           float* __restrict__ rest) {
+    __shared__ float part[16];
+    float top = 0.0f;
+    if (w)
+        for (int i = threadIdx.x; i < nq; i += 1024)
+            if (targets[i] >= 0 && targets[i] < n) top = fmaxf(top, fabsf(w[i]));
 #pragma unroll
-    for (int n = 0; n < NT; n++) {
-        const int col = n0 + T::col_of(n);
-        const bool live = col < a.mm.N;
-        const int t = live ? a.targets[col] : -1;
-        const bool known = t >= 0 && t < a.n;
-        const float w = known ? (a.w ? a.w[col] : 1.0f) * a.scale : 0.0f;
-        const float lse2 = known ? a.lse[col] * 1.44269504088896341f : 0.0f;
-        const int at = known && t >= a.row0 && t - a.row0 < a.mm.M ? (int)(t - a.row0) : -1;
+    for (int off = 32; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
+    __syncthreads();
 #pragma unroll
-        for (int m = 0; m < MT; m++) {
-#pragma unroll
-            for (int e4 = 0; e4 < 4; e4++) {
-                uint16_t p[4][3];
-                const int row = m0 + T::row_of(m, e4 * 4);
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    float g = exp2_(fmaf(acc[m][n][e4 * 4 + e], a.c, -lse2)) - (row + e == at ? 1.0f : 0.0f);
-                    g = known && row + e < a.mm.M ? g * w : 0.0f;
-                    planes3(g, p[e]);
-                }
-#pragma unroll
-                for (int k = 0; k < 3; k++) {
-                    if (k >= a.planes) break;
-                    if (a.g && live && row < a.kv)   // (kv is a multiple of 64: four rows are in or out together)
-                        *(uint2*)(a.g + ((int64_t)col * a.planes + k) * a.kv + row) =
-                            make_uint2((uint32_t)p[0][k] | ((uint32_t)p[1][k] << 16), (uint32_t)p[2][k] | ((uint32_t)p[3][k] << 16));
-                    if (a.gt && col < a.kq) {
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            if (row + e < a.mm.M) a.gt[((int64_t)(row + e) * a.planes + k) * a.kq + col] = p[e][k];
-                    }
-                }
-            }
-        }
+    for (int k = 0; k < 16; k++) top = fmaxf(top, part[k]);
+    // (no weights, none but zeros, or one that is not finite: 1, so that what is not finite shows in the gradient)
+    const float unit = w && top > 0.0f && top < __builtin_inff() ? top : 1.0f;
+    if (threadIdx.x == 0) *norm = unit;
+    for (int i = threadIdx.x; i < nq; i += 1024) {
+        const int t = targets[i];
+        const bool known = t >= 0 && t < n;
+        JvSxQuery q;
+        q.lse2 = known ? lse[i] * 1.44269504088896341f : 0.0f;
+        q.w = known ? (w ? w[i] : 1.0f) / unit : 0.0f;
+        q.target = known ? t : -1;
+        q.pad = 0;
+        query[i] = q;
+        rest[i] = 0.0f;
     }
 }
-
-extern "C" hipError_t jvk_sx_weights(const JvSxWeights* a, hipStream_t s) {
-    using T = Tile<BF16, 2, 2, 2, 2>;
-    if (a->mm.M <= 0 || a->mm.N <= 0) return hipSuccess;
-    const int panels = (a->mm.N + T::TN - 1) / T::TN;
-    if (panels > 65535) return hipErrorInvalidValue;
-    hipError_t e = hipFuncSetAttribute((const void*)jvs_weights_kernel<2, 2, 2, 2>, hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS);
-    if (e != hipSuccess) return e;
-    jvs_weights_kernel<2, 2, 2, 2><<<dim3((unsigned)((a->mm.M + T::TM - 1) / T::TM), (unsigned)panels), T::THREADS, T::LDS, s>>>(*a);
+extern "C" hipError_t jvk_sx_queries(const float* lse, const float* w, const int32_t* targets, int nq, int64_t n, JvSxQuery* query, float* norm, float* rest,
+                                     hipStream_t s) {
+    jvs_queries_kernel<<<1, 1024, 0, s>>>(lse, w, targets, nq, n, query, norm, rest);
     return hipGetLastError();
 }
 
-extern "C" hipError_t jvk_sx_mm(const JvMmOut* a, hipStream_t s) { return mm_out<BF16, 2, 2, 2, 2>(*a, s); }
+__global__ __launch_bounds__(512) void jvs_weights_kernel(const JvSxWeights a) {
+    using P = Pipe<BF16>;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    const int tm = (a.mm.M + P::TM - 1) / P::TM, tn = (a.mm.N + P::TN - 1) / P::TN;
+    const Share share(tm * tn);
+    if (!share.mine()) return;
+    const int padded = (a.mm.M + 63) / 64 * 64;
+    P::run(
+        a.mm, smem,
+        [&](int i, Work& w) {
+            int L, m, n;
+            if (!share.at(i, L)) return false;
+            band_order(L, tm, tn, m, n);
+            w.m0 = m * P::TM, w.n0 = n * P::TN, w.k0 = 0, w.k1 = a.mm.kph * a.mm.segs;
+            return true;
+        },
+        [&](const Work& w, f32x16 (&acc)[4][2]) -> int {
+#pragma unroll
+            for (int m = 0; m < 4; m++) {
+                const int r = w.m0 + P::row(m);
+                JvSxQuery q = {0.0f, 0.0f, -1, 0};
+                if (r < a.mm.M) q = a.query[r];
+                const int at = q.target >= 0 && q.target >= a.row0 && q.target - a.row0 < a.mm.N ? (int)(q.target - a.row0) - w.n0 : -1;
+#pragma unroll
+                for (int n = 0; n < 2; n++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        const int c = P::col(n, e);
+                        float g = exp2_(fmaf(acc[m][n][e], a.c, -q.lse2));
+                        if (c == at) g -= 1.0f;
+                        g = q.target >= 0 && w.n0 + c < a.mm.N ? g * q.w : 0.0f;
+                        acc[m][n][e] = g;
+                        if (a.planes == 1 && c == at) a.rest[r] = g - (float)(__bf16)g;
+                    }
+            }
+            int stores = 0;
+            for (int k = 0; k < a.planes; k++) {
+                stores = P::write_bf16(smem, a.g + (int64_t)k * a.kv, (int64_t)a.planes * a.kv, true, w, padded, a.kv, [&](int m, int n, int e) { return acc[m][n][e]; });
+                if (a.planes > 1) {
+#pragma unroll
+                    for (int m = 0; m < 4; m++)
+#pragma unroll
+                        for (int n = 0; n < 2; n++)
+#pragma unroll
+                            for (int e = 0; e < 16; e++) acc[m][n][e] -= (float)(__bf16)acc[m][n][e];
+                }
+            }
+            return stores;
+        });
+}
 
-// partial sums -> the gradient's rows
+extern "C" hipError_t jvk_sx_weights(const JvSxWeights* a, hipStream_t s) {
+    using P = Pipe<BF16>;
+    if (a->mm.M <= 0 || a->mm.N <= 0) return hipSuccess;
+    const int64_t all = (int64_t)((a->mm.M + P::TM - 1) / P::TM) * ((a->mm.N + P::TN - 1) / P::TN);
+    if (all > 0x7fffffffll) return hipErrorInvalidValue;
+    hipError_t e = hipFuncSetAttribute((const void*)jvs_weights_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, P::LDS);
+    if (e != hipSuccess) return e;
+    jvs_weights_kernel<<<(unsigned)(all < 256 ? (all + 7) / 8 * 8 : 256), P::THREADS, P::LDS, s>>>(*a);
+    return hipGetLastError();
+}
+
+// dq = G V: G's rows are queries, V's rows are k.  dv = G^T Q: the rows of both are k.
+extern "C" hipError_t jvk_sx_query_grad(const JvMmOut* a, hipStream_t s) { return mm_out_pipe<BF16, false, true>(*a, s); }
+extern "C" hipError_t jvk_sx_vector_grad(const JvMmOut* a, hipStream_t s) { return mm_out_pipe<BF16, true, true>(*a, s); }
+
+// partial sums -> the queries' gradient, and what G lacked at the target
 template <typename T>
-__global__ __launch_bounds__(256) void jvs_finish_kernel(const float* __restrict__ slab, int splits, int64_t rows, int d, T* __restrict__ out, int64_t ldo) {
+__global__ __launch_bounds__(256) void jvs_finish_kernel(const float* __restrict__ slab, int splits, int64_t rows, int d, int64_t lds, const float* __restrict__ rest,
+                                                         const JvSxQuery* __restrict__ query, const T* __restrict__ v, int64_t v_stride, float mul,
+                                                         const float* __restrict__ norm, T* __restrict__ out, int64_t ldo) {
     const int64_t all = rows * d;
+    const float by = mul * *norm;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
-        float v = 0.0f;
-        for (int k = 0; k < splits; k++) v += slab[k * all + i];
-        const int64_t r = i / d;
-        out[r * ldo + (i - r * d)] = (T)v;
+        const int64_t r = i / d, c = i - r * d;
+        float x = 0.0f;
+        for (int k = 0; k < splits; k++) x += slab[(k * rows + r) * lds + c];
+        if (const float lack = rest[r]; lack != 0.0f) x = fmaf(lack, (float)v[query[r].target * v_stride + c], x);
+        out[r * ldo + c] = (T)(x * by);
     }
 }
 template <typename T>
@@ -319,10 +391,13 @@ static unsigned grid_for(int64_t items) {
     const int64_t want = (items + 255) / 256;
     return (unsigned)(want < 16384 ? want : 16384);
 }
-extern "C" hipError_t jvk_sx_finish(const float* slab, int splits, int64_t rows, int d, void* out, int dtype, int64_t ldo, hipStream_t s) {
+extern "C" hipError_t jvk_sx_finish(const float* slab, int splits, int64_t rows, int d, int64_t lds, const float* rest, const JvSxQuery* query, const void* v,
+                                    int64_t v_stride, float mul, const float* norm, void* out, int dtype, int64_t ldo, hipStream_t s) {
     if (rows <= 0 || d <= 0) return hipSuccess;
-    if (dtype == 0) jvs_finish_kernel<float><<<grid_for(rows * d), 256, 0, s>>>(slab, splits, rows, d, (float*)out, ldo);
-    else jvs_finish_kernel<__bf16><<<grid_for(rows * d), 256, 0, s>>>(slab, splits, rows, d, (__bf16*)out, ldo);
+    if (dtype == 0)
+        jvs_finish_kernel<float><<<grid_for(rows * d), 256, 0, s>>>(slab, splits, rows, d, lds, rest, query, (const float*)v, v_stride, mul, norm, (float*)out, ldo);
+    else
+        jvs_finish_kernel<__bf16><<<grid_for(rows * d), 256, 0, s>>>(slab, splits, rows, d, lds, rest, query, (const __bf16*)v, v_stride, mul, norm, (__bf16*)out, ldo);
     return hipGetLastError();
 }
 extern "C" hipError_t jvk_sx_fill(void* out, int dtype, int64_t stride, int64_t rows, int d, float value, hipStream_t s) {

@@ -46,28 +46,25 @@ __device__ __forceinline__ bf16x8 widen(int lo, int hi, int byte) {
     return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-// MT x NT accumulators of 32 x 32 for each of WM x WN waves
+// The product for small shapes: MT x NT accumulators of 32 x 32 for each of WM x WN waves, two steps of k in LDS, several workgroups a CU.
 template <int TY, int MT, int NT, int WM, int WN>
 struct Tile {
     static constexpr int TM = 32 * MT * WM, TN = 32 * NT * WN, WAVES = WM * WN, THREADS = 64 * WAVES;
-    static constexpr int GA = TM / 8, GB = TN / 8, PER = (GA + GB) / WAVES;   // 8-row groups; copies of one wave a step
+    static constexpr int GA = TM / 8, GB = TN / 8;                               // 8-row groups
+    static constexpr int CA = GA / WAVES, CB = GB / WAVES, PER = CA + CB;        // copies of one wave a step
     static constexpr int BUF = (GA + GB) * GROUP, LDS = 2 * BUF;
-    static_assert((GA + GB) % WAVES == 0 && GA % PER == 0, "a wave's groups lie in one operand");
+    static_assert(GA % WAVES == 0 && GB % WAVES == 0, "every wave copies the same number of groups of each operand");
 
-    // C tile at (m0, n0), steps [k0, k1) of the segs * nk in all.  Rows behind the operands' last are read as their last.
-    static __device__ __forceinline__ void run(const JvMm& a, int m0, int n0, int k0, int k1, unsigned char* smem, f32x16 (&acc)[MT][NT]) {
+    // C tile at (m0, n0).  Rows behind the operands' last are read as their last.
+    static __device__ __forceinline__ void run(const JvMm& a, int m0, int n0, unsigned char* smem, f32x16 (&acc)[MT][NT]) {
+        const int nk = a.kph >> 1, k1 = nk * a.segs;   // steps: two phases each
         const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
         const int lr = lane >> 3, lp = (lane & 7) ^ lr;
-        const bool isb = w * PER >= GA;
-        const char* src[PER];
+        const char* src[PER];   // group i * WAVES + w of A, then of B
 #pragma unroll
-        for (int i = 0; i < PER; i++) {
-            const int row = 8 * (w * PER + i) + lr;
-            int r = isb ? n0 + row - TM : m0 + row;
-            const int last = (isb ? a.N : a.M) - 1;
-            if (r > last) r = last;
-            src[i] = (isb ? a.b + (int64_t)r * a.ldb : a.a + (int64_t)r * a.lda) + lp * 16;
-        }
+        for (int i = 0; i < CA; i++) src[i] = a.a + (int64_t)min(m0 + 8 * (i * WAVES + w) + lr, a.M - 1) * a.lda + lp * 16;
+#pragma unroll
+        for (int i = 0; i < CB; i++) src[CA + i] = a.b + (int64_t)min(n0 + 8 * (i * WAVES + w) + lr, a.N - 1) * a.ldb + lp * 16;
         const int wm = w % WM, wn = w / WM, h = lane >> 5, r31 = lane & 31;
         int aoff[MT], boff[NT], ax, bx;
 #pragma unroll
@@ -84,9 +81,9 @@ struct Tile {
         const uint8_t *pa[MT], *pb[NT];
         if constexpr (TY != BF16) {
 #pragma unroll
-            for (int t = 0; t < MT; t++) pa[t] = a.sa + (int64_t)min(m0 + (wm * MT + t) * 32 + r31, a.M - 1) * a.nk;
+            for (int t = 0; t < MT; t++) pa[t] = a.sa + (int64_t)min(m0 + (wm * MT + t) * 32 + r31, a.M - 1) * nk;
 #pragma unroll
-            for (int t = 0; t < NT; t++) pb[t] = a.sb + (int64_t)min(n0 + (wn * NT + t) * 32 + r31, a.N - 1) * a.nk;
+            for (int t = 0; t < NT; t++) pb[t] = a.sb + (int64_t)min(n0 + (wn * NT + t) * 32 + r31, a.N - 1) * nk;
         }
 #pragma unroll
         for (int m = 0; m < MT; m++)
@@ -95,18 +92,20 @@ struct Tile {
 #pragma unroll
                 for (int e = 0; e < 16; e++) acc[m][n][e] = 0.0f;
 
-        int seg = k0 / a.nk, kin = k0 - seg * a.nk;   // of the next step to be staged
+        int seg = 0, kin = 0;   // of the next step to be staged
         auto stage = [&](int buf) {
-            int64_t off = (int64_t)kin * 128;
-            if (a.segs > 1) off += (int64_t)(isb ? plane_b(seg) : plane_a(seg)) * a.nk * 128;
-            unsigned char* dst = smem + buf * BUF + w * PER * GROUP;
+            int64_t offa = (int64_t)kin * 128, offb = offa;
+            if (a.segs > 1) offa += plane_a(seg) * a.plane_a, offb += plane_b(seg) * a.plane_b;
+            unsigned char* dst = smem + buf * BUF + w * GROUP;
 #pragma unroll
-            for (int i = 0; i < PER; i++) glds16(src[i] + off, dst + i * GROUP);
-            if (++kin == a.nk) kin = 0, seg++;
+            for (int i = 0; i < CA; i++) glds16(src[i] + offa, dst + i * WAVES * GROUP);
+#pragma unroll
+            for (int i = 0; i < CB; i++) glds16(src[CA + i] + offb, dst + (GA + i * WAVES) * GROUP);
+            if (++kin == nk) kin = 0, seg++;
         };
         stage(0);
-        for (int s = k0; s < k1; s++) {
-            const int buf = (s - k0) & 1;
+        for (int s = 0; s < k1; s++) {
+            const int buf = s & 1;
             int fa[MT], fb[NT];
             if constexpr (TY != BF16) {
 #pragma unroll
@@ -122,17 +121,21 @@ struct Tile {
             }
             const unsigned char* base = smem + buf * BUF;
             if constexpr (TY == BF16) {
+                bf16x8 va[2][MT], vb[2][NT];
+                auto frag = [&](int kk) {
+#pragma unroll
+                    for (int t = 0; t < MT; t++) va[kk & 1][t] = *(const bf16x8*)(base + aoff[t] + (((2 * kk + h) ^ ax) << 4));
+#pragma unroll
+                    for (int t = 0; t < NT; t++) vb[kk & 1][t] = *(const bf16x8*)(base + boff[t] + (((2 * kk + h) ^ bx) << 4));
+                };
+                frag(0);
 #pragma unroll
                 for (int kk = 0; kk < 4; kk++) {
-                    bf16x8 va[MT], vb[NT];
-#pragma unroll
-                    for (int t = 0; t < MT; t++) va[t] = *(const bf16x8*)(base + aoff[t] + (((2 * kk + h) ^ ax) << 4));
-#pragma unroll
-                    for (int t = 0; t < NT; t++) vb[t] = *(const bf16x8*)(base + boff[t] + (((2 * kk + h) ^ bx) << 4));
+                    if (kk < 3) frag(kk + 1);
 #pragma unroll
                     for (int m = 0; m < MT; m++)
 #pragma unroll
-                        for (int n = 0; n < NT; n++) acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va[m], vb[n], acc[m][n], 0, 0, 0);
+                        for (int n = 0; n < NT; n++) acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vb[kk & 1][n], va[kk & 1][m], acc[m][n], 0, 0, 0);
                 }
             } else if constexpr (TY == F8W) {
                 // (16 components a lane and step: which of the block's 128 does not matter as long as both operands agree)
@@ -153,7 +156,7 @@ struct Tile {
 #pragma unroll
                         for (int m = 0; m < MT; m++)
 #pragma unroll
-                            for (int n = 0; n < NT; n++) acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va[m], vb[n], acc[m][n], 0, 0, 0);
+                            for (int n = 0; n < NT; n++) acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vb[n], va[m], acc[m][n], 0, 0, 0);
                     }
                 }
             } else {
@@ -174,19 +177,18 @@ struct Tile {
                     for (int m = 0; m < MT; m++)
 #pragma unroll
                         for (int n = 0; n < NT; n++)
-                            acc[m][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(va[m], vb[n], acc[m][n], 0, 0, 0, fa[m], 0, fb[n]);
+                            acc[m][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(vb[n], va[m], acc[m][n], 0, 0, 0, fb[n], 0, fa[m]);
                 }
             }
             // every fragment read of this buffer has returned before any wave stages into it again
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         }
     }
-    // row of accumulator register e of tile m, column of tile n, inside the workgroup's tile
-    static __device__ __forceinline__ int row_of(int m, int e) {
-        const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-        return ((w % WM) * MT + m) * 32 + (e & 3) + 8 * (e >> 2) + 4 * (lane >> 5);
+    // acc[m][n][e] is C[row(m)][col(n, e)] of the tile, four consecutive e are four consecutive columns
+    static __device__ __forceinline__ int row(int m) { return (((threadIdx.x >> 6) % WM) * MT + m) * 32 + (threadIdx.x & 31); }
+    static __device__ __forceinline__ int col(int n, int e) {
+        return (((threadIdx.x >> 6) / WM) * NT + n) * 32 + (e & 3) + 8 * (e >> 2) + 4 * ((threadIdx.x >> 5) & 1);
     }
-    static __device__ __forceinline__ int col_of(int n) { return (((threadIdx.x >> 6) / WM) * NT + n) * 32 + (threadIdx.x & 31); }
 };
 
 }  // namespace jvmm

@@ -1,60 +1,109 @@
-// jv_mm_out.h — the product of jv_mm.h written as it is: rows of float32 or bf16, or float32 partial sums of a split k range.
+// jv_mm_out.h — matrix products written as they are, on the tiles of jv_mm.h (small) and jv_pipe.h (large).
 #pragma once
-#include "jv_mm.h"
+#include "jv_pipe.h"
 
 namespace jvmm {
 
-// The workgroups of one XCD (blockIdx % 8 of the grid) take a contiguous run of tiles, A's tiles innermost: what they share of B meets
-// in one L2 (bijective for any grid size).
-__device__ __forceinline__ int xcd_order(int i, int n) {
-    const int xcd = i & 7, slot = i >> 3, q = n >> 3, r = n & 7;
-    return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + slot;
+// Tile L of tm x tn in bands of 8 tiles of A: the 32 workgroups that an XCD runs at a time share 8 tiles of A and 4 of B.
+__device__ __forceinline__ void band_order(int L, int tm, int tn, int& m, int& n) {
+    const int band = L / (8 * tn), in = L - band * 8 * tn, high = min(8, tm - band * 8);
+    n = in / high;
+    m = band * 8 + in - n * high;
+}
+
+template <int TY, bool TA, bool TB>
+__global__ __launch_bounds__(512) void jvm_out_pipe_kernel(const JvMmOut a) {
+    using P = Pipe<TY, TA, TB>;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    const int tm = (a.mm.M + P::TM - 1) / P::TM, tn = (a.mm.N + P::TN - 1) / P::TN, tiles = tm * tn;
+    const Share share(tiles * a.splits);
+    if (!share.mine()) return;
+    const int phases = a.mm.kph * a.mm.segs;
+    auto work = [&](int i, Work& w) {
+        int L;
+        if (!share.at(i, L)) return false;
+        int m, n;
+        w.part = 0;
+        if (a.splits > 1) w.part = L / tiles, L -= w.part * tiles;   // (the tiles of one k range side by side: they share both operands)
+        band_order(L, tm, tn, m, n);
+        w.m0 = m * P::TM, w.n0 = n * P::TN;
+        w.k0 = (int)((int64_t)phases * w.part / a.splits), w.k1 = (int)((int64_t)phases * (w.part + 1) / a.splits);
+        return true;
+    };
+    const float mul = a.norm ? a.mul * *a.norm : a.mul;
+    const bool wide = (uintptr_t)a.out % 16 == 0 && a.ldo % (a.dtype == 0 ? 4 : 8) == 0;
+    P::run(a.mm, smem, work, [&](const Work& w, f32x16 (&acc)[4][2]) -> int {
+        auto value = [&](int m, int n, int e) { return acc[m][n][e] * mul; };
+        if (a.dtype != 0) return P::write_bf16(smem, (uint16_t*)a.out, a.ldo, wide, w, a.mm.M, a.mm.N, value);
+        return P::write_f32(smem, (float*)a.out + (int64_t)w.part * a.mm.M * a.ldo, a.ldo, wide, a.add, w, a.mm.M, a.mm.N, value);
+    });
+}
+
+template <int TY, bool TA = false, bool TB = false>
+static hipError_t mm_out_pipe(const JvMmOut& a, hipStream_t s) {
+    using P = Pipe<TY, TA, TB>;
+    if (a.mm.M <= 0 || a.mm.N <= 0) return hipSuccess;
+    const int64_t all = (int64_t)((a.mm.M + P::TM - 1) / P::TM) * ((a.mm.N + P::TN - 1) / P::TN) * a.splits;
+    if (all > 0x7fffffffll || a.splits < 1 || a.splits > a.mm.kph * a.mm.segs) return hipErrorInvalidValue;
+    hipError_t e = hipFuncSetAttribute((const void*)jvm_out_pipe_kernel<TY, TA, TB>, hipFuncAttributeMaxDynamicSharedMemorySize, P::LDS);
+    if (e != hipSuccess) return e;
+    jvm_out_pipe_kernel<TY, TA, TB><<<(unsigned)(all < 256 ? (all + 7) / 8 * 8 : 256), P::THREADS, P::LDS, s>>>(a);
+    return hipGetLastError();
 }
 
 template <int TY, int MT, int NT, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN) void jvm_out_kernel(const JvMmOut a) {
+__global__ __launch_bounds__(64 * WM * WN) void jvm_out_tile_kernel(const JvMmOut a) {
     using T = Tile<TY, MT, NT, WM, WN>;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    const int tm = (a.mm.M + T::TM - 1) / T::TM;
-    const int L = xcd_order(blockIdx.x, gridDim.x);
-    const int m0 = (L % tm) * T::TM, n0 = (L / tm) * T::TN;
-    const int steps = a.mm.nk * a.mm.segs;
-    const int k0 = (int)((int64_t)steps * blockIdx.y / a.splits), k1 = (int)((int64_t)steps * (blockIdx.y + 1) / a.splits);
+    const int tm = (a.mm.M + T::TM - 1) / T::TM, tn = (a.mm.N + T::TN - 1) / T::TN;
+    const Share share(tm * tn);   // (a grid of one workgroup for each tile, rounded up to 8)
+    int L, m0, n0;
+    if (!share.at(0, L)) return;
+    band_order(L, tm, tn, m0, n0);
+    m0 *= T::TM, n0 *= T::TN;
     f32x16 acc[MT][NT];
-    T::run(a.mm, m0, n0, k0, k1, smem, acc);
+    T::run(a.mm, m0, n0, smem, acc);
+    const bool wide = (uintptr_t)a.out % 16 == 0 && a.ldo % (a.dtype == 0 ? 4 : 8) == 0;
 #pragma unroll
-    for (int n = 0; n < NT; n++) {
-        const int col = n0 + T::col_of(n);
-        if (col >= a.mm.N) continue;
+    for (int m = 0; m < MT; m++) {
+        const int row = m0 + T::row(m);
+        if (row >= a.mm.M) continue;
 #pragma unroll
-        for (int m = 0; m < MT; m++) {
+        for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int e = 0; e < 16; e++) {
-                const int row = m0 + T::row_of(m, e);
-                if (row >= a.mm.M) continue;
-                const float v = acc[m][n][e];
-                if (a.slab) {
-                    float* p = a.slab + ((int64_t)blockIdx.y * a.mm.M + row) * a.mm.N + col;
-                    *p = a.add ? *p + v : v;
-                } else if (a.dtype == 0) {
-                    ((float*)a.out)[(int64_t)row * a.ldo + col] = v;
+            for (int g = 0; g < 4; g++) {
+                const int col = n0 + T::col(n, 4 * g);
+                f32x4 v;
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] = acc[m][n][4 * g + e] * a.mul;
+                if (a.dtype == 0) {
+                    float* p = (float*)a.out + (int64_t)row * a.ldo + col;
+                    if (wide && col + 4 <= a.mm.N) *(f32x4*)p = v;
+                    else
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            if (col + e < a.mm.N) p[e] = v[e];
                 } else {
-                    ((__bf16*)a.out)[(int64_t)row * a.ldo + col] = (__bf16)v;
+                    __bf16* p = (__bf16*)a.out + (int64_t)row * a.ldo + col;
+                    if (wide && col + 4 <= a.mm.N) *(bf16x4*)p = (bf16x4){(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+                    else
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            if (col + e < a.mm.N) p[e] = (__bf16)v[e];
                 }
             }
-        }
     }
 }
 
 template <int TY, int MT, int NT, int WM, int WN>
-static hipError_t mm_out(const JvMmOut& a, hipStream_t s) {
+static hipError_t mm_out_tile(const JvMmOut& a, hipStream_t s) {
     using T = Tile<TY, MT, NT, WM, WN>;
     if (a.mm.M <= 0 || a.mm.N <= 0) return hipSuccess;
     const int64_t tiles = (int64_t)((a.mm.M + T::TM - 1) / T::TM) * ((a.mm.N + T::TN - 1) / T::TN);
-    if (tiles > 0x7fffffffll || a.splits < 1 || a.splits > 65535 || a.splits > a.mm.nk * a.mm.segs) return hipErrorInvalidValue;
-    hipError_t e = hipFuncSetAttribute((const void*)jvm_out_kernel<TY, MT, NT, WM, WN>, hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS);
+    if (tiles > 0x7ffffff0ll || a.splits != 1 || a.add) return hipErrorInvalidValue;
+    hipError_t e = hipFuncSetAttribute((const void*)jvm_out_tile_kernel<TY, MT, NT, WM, WN>, hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS);
     if (e != hipSuccess) return e;
-    jvm_out_kernel<TY, MT, NT, WM, WN><<<dim3((unsigned)tiles, (unsigned)a.splits), T::THREADS, T::LDS, s>>>(a);
+    jvm_out_tile_kernel<TY, MT, NT, WM, WN><<<(unsigned)((tiles + 7) / 8 * 8), T::THREADS, T::LDS, s>>>(a);
     return hipGetLastError();
 }
 

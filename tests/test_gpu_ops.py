@@ -379,3 +379,47 @@ def test_refusals_of_the_torch_view(torch, ops, pkg):
             call()
         assert e.value.code == pkg.binding.JV_EINVAL
     assert ops.softmax_loss_grad(q, v, t, 1.0, torch.zeros(4, device="cuda"), queries_grad=False, vectors_grad=False) == (None, None)
+
+
+# ------------------------------------------------------------------------------------------------ the large tiles
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+@pytest.mark.parametrize("nq,n,d", [(300, 33000, 200), (257, 24700, 1000), (2050, 6500, 128), (3100, 5000, 640), (70, 50001, 2200), (49153, 20, 64)])
+def test_scores_on_the_large_tiles(torch, ops, out, nq, n, d):
+    """Sizes that fill the chip with 256 x 256 tiles, none of them whole: scales of several windows, odd ends, rows that are not 16-B aligned."""
+    g = torch.Generator(device="cuda").manual_seed(nq + n + d)
+    q, v = (torch.randn((k, d), generator=g, device="cuda") * torch.exp2(torch.randint(-9, 9, (k, 1), generator=g, device="cuda")) for k in (nq, n))
+    (qc, qs), (vc, vs) = ops.encode_blocks(q), ops.encode_blocks(v)
+    a, b = (ops.decode_blocks(c, s, d).double() for c, s in ((qc, qs), (vc, vs)))
+    want, off = a @ b.t(), (d + 2) * 2.0 ** -23 * (a.abs() @ b.abs().t())
+    if out == "bf16":
+        for k in range(0, d, 64):   # 2^-11 of a group's largest product: at most of the product of the two largest components
+            off += 2.0 ** -11 * a[:, k:k + 64].abs().amax(1)[:, None] * b[:, k:k + 64].abs().amax(1)[None]
+        off += 2.0 ** -8 * (want.abs() + off)
+    got = ops.score_blocks(qc, qs, vc, vs, d, dtype_of(torch, out))
+    assert got.dtype == dtype_of(torch, out) and ((got.double() - want).abs() <= off).all()
+    again = ops.score_blocks(qc, qs, vc, vs, d, dtype_of(torch, out))
+    assert torch.equal(got, again)
+
+
+@pytest.mark.parametrize("dtype,nq,n,d,pad", [("bf16", 300, 30011, 200, 0), ("f32", 257, 26000, 70, 3), ("bf16", 1030, 10001, 384, 8), ("bf16", 80, 60000, 64, 0),
+                                              ("f32", 600, 17000, 128, 0)])
+def test_softmax_on_the_large_tiles(torch, ops, dtype, nq, n, d, pad):
+    q, v, t, w, _, _, t64, _ = loss_case(torch, nq, n, d, dtype, pad)
+    scale = 15.0
+    loss, lse = ops.softmax_loss(q, v, t, scale)
+    z = scale * (q.double() @ v.double().t())
+    lse64 = torch.logsumexp(z, 1)
+    known = (t >= 0) & (t < n)
+    at = t.long().clamp(0, n - 1)
+    # (terms + 2) 2^-23 of a logit's reach (rows have length about 1: scale), the logits' roundings, a sum of n terms
+    de = (6 * d + 2) * 2.0 ** -23 * scale * 1.1 + 8 * 2.0 ** -24 * 2 * scale + n * 2.0 ** -24
+    assert (lse - lse64).abs().max().item() <= de
+    assert (loss - torch.where(known, lse64 - z[torch.arange(nq, device="cuda"), at], torch.zeros_like(lse64))).abs().max().item() <= 2 * de
+    g = torch.exp(z - lse64[:, None])
+    g[torch.arange(nq, device="cuda"), at] -= 1
+    g *= (known * w * scale).double()[:, None]
+    dq, dv = ops.softmax_loss_grad(q, v, t, scale, lse, w)
+    r = 2.0 ** -8 if dtype == "bf16" else 2.0 ** -23
+    for got, a, b, k in ((dq, g, v.double(), n), (dv, g.t(), q.double(), nq)):
+        want, reach = a @ b, a.abs() @ b.abs()
+        assert ((got.double() - want).abs() <= (r + 4 * de + 6 * k * 2.0 ** -23) * reach + 2 * ref.half_step(dtype) * want.abs() + 1e-30).all()
