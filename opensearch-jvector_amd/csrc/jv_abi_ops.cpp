@@ -78,7 +78,7 @@ int check_shape(int64_t n, int d, const char* what) {
 struct Plan {
     int P, segs, dp, kq;              // planes, segments; d and nq padded to 64
     int64_t rows_f, rows_b;           // rows of one piece, forward (only if the vectors have to be laid out) / backward
-    int tile, splits_f, splits_q;
+    int tile, splits_f, splits_q, large;
     int64_t off_q, off_v, off_part, off_query, off_norm, off_rest, off_g, off_slab, bytes;
 };
 
@@ -114,15 +114,14 @@ Plan make_plan(int dtype, int nq, int64_t n, int d, uint32_t what) {
         p.off_v = take(std::min<int64_t>(p.rows_f, n) * row);
     }
     if (what & (JV_SOFTMAX_QUERY_GRAD | JV_SOFTMAX_VECTOR_GRAD)) {
+        p.large = jvk_sx_large(nq, std::min<int64_t>(p.rows_b, n));
         p.off_v = take(std::min<int64_t>(p.rows_b, n) * row);
         p.off_query = take((int64_t)nq * sizeof(JvSxQuery));
         p.off_norm = take(4);
         p.off_rest = take((int64_t)nq * 4);
         p.off_g = take((int64_t)p.kq * p.P * p.rows_b * 2);
         if (what & JV_SOFTMAX_QUERY_GRAD) {
-            // k ranges: all tiles of all ranges once around the CUs, eight phases in each at least
-            const int64_t tiles = panels * ((d + 255) / 256), phases = p.rows_b / 32 * p.segs;
-            p.splits_q = (int)std::max<int64_t>(std::min<int64_t>(256 / tiles, phases / 8), 1);
+            p.splits_q = jvk_sx_grad_splits(nq, d, p.rows_b, p.segs, p.large);
             p.off_slab = take((int64_t)p.splits_q * nq * p.dp * 4);
         }
     }
@@ -168,18 +167,19 @@ JvMm logits(const Plan& plan, int nq) {
     return mm;
 }
 
-// the rows [at, at + rows) of a matrix, laid out in the workspace unless they are ready
-int lay_out(const Rows& r, const void* p, int64_t stride, int dtype, int64_t at, int64_t rows, const Plan& plan, int d, char* to, hipStream_t s, const char** out,
-            int64_t* ld) {
+// The rows [at, at + rows) of a matrix as a product reads them: the caller's own, or where the next jvk_sx_prepare lays them out.
+void take_rows(const Rows& r, const void* p, int64_t stride, int dtype, int64_t at, int64_t rows, const Plan& plan, char* to, JvSxPrepare::Matrix* m, const char** out,
+               int64_t* ld) {
     if (r.ready) {
         *out = r.p + at * r.stride;
         *ld = r.stride;
-        return JV_OK;
+        m->rows = 0;
+        return;
     }
-    CHK(jvk_sx_pack((const char*)p + at * stride * size_of(dtype), dtype, stride, rows, d, plan.dp, (uint16_t*)to, s));
+    m->x = (const char*)p + at * stride * size_of(dtype);
+    m->stride = stride, m->rows = rows, m->out = (uint16_t*)to;
     *out = to;
     *ld = (int64_t)plan.P * plan.dp * 2;
-    return JV_OK;
 }
 
 }  // namespace
@@ -258,11 +258,15 @@ int jv_softmax_loss_device(const jv_softmax_params* p, float* d_out_loss, float*
         a.mm = logits(plan, p->nq);
         a.c = p->scale * 1.44269504088896341f;
         a.tile = plan.tile, a.splits = p->n > 0 ? plan.splits_f : 0, a.part = (float*)(ws + plan.off_part);
-        if (p->n > 0) TRY(lay_out(rq, p->queries, p->query_stride, p->dtype, 0, p->nq, plan, p->d, ws + plan.off_q, s, &a.mm.a, &a.mm.lda));
+        JvSxPrepare pre{};
+        pre.dtype = p->dtype, pre.d = p->d, pre.kp = plan.dp;
+        take_rows(rq, p->queries, p->query_stride, p->dtype, 0, p->nq, plan, ws + plan.off_q, &pre.m[0], &a.mm.a, &a.mm.lda);
         for (int64_t at = 0; at < p->n; at += step) {
             a.mm.N = (int)std::min<int64_t>(step, p->n - at);
             a.first = at == 0;
-            TRY(lay_out(rv, p->vectors, p->vector_stride, p->dtype, at, a.mm.N, plan, p->d, ws + plan.off_v, s, &a.mm.b, &a.mm.ldb));
+            take_rows(rv, p->vectors, p->vector_stride, p->dtype, at, a.mm.N, plan, ws + plan.off_v, &pre.m[1], &a.mm.b, &a.mm.ldb);
+            CHK(jvk_sx_prepare(&pre, s));
+            pre.m[0].rows = 0;
             CHK(jvk_sx_loss(&a, s));
         }
         CHK(jvk_sx_join(a.part, a.splits, p->nq, p->queries, p->query_stride, p->vectors, p->vector_stride, p->dtype, p->d, p->targets, p->n, p->scale, d_out_loss,
@@ -298,14 +302,18 @@ int jv_softmax_grad_device(const jv_softmax_params* p, const float* d_lse, const
     JvSxQuery* query = (JvSxQuery*)(ws + plan.off_query);
     w.query = query;
     float* norm = (float*)(ws + plan.off_norm);
-    CHK(jvk_sx_queries(d_lse, d_loss_grad, p->targets, p->nq, p->n, query, norm, w.rest, s));
-    TRY(lay_out(rq, p->queries, p->query_stride, p->dtype, 0, p->nq, plan, p->d, ws + plan.off_q, s, &w.mm.a, &w.mm.lda));
+    JvSxPrepare pre{};
+    pre.dtype = p->dtype, pre.d = p->d, pre.kp = plan.dp;
+    pre.lse = d_lse, pre.w = d_loss_grad, pre.targets = p->targets, pre.nq = p->nq, pre.n = p->n, pre.query = query, pre.norm = norm, pre.rest = w.rest;
+    take_rows(rq, p->queries, p->query_stride, p->dtype, 0, p->nq, plan, ws + plan.off_q, &pre.m[0], &w.mm.a, &w.mm.lda);
     for (int64_t at = 0; at < p->n; at += plan.rows_b) {
         const int rows = (int)std::min<int64_t>(plan.rows_b, p->n - at);
         w.mm.N = rows, w.row0 = at, w.kv = (int)up(rows, 64);
-        TRY(lay_out(rv, p->vectors, p->vector_stride, p->dtype, at, rows, plan, p->d, ws + plan.off_v, s, &w.mm.b, &w.mm.ldb));
-        CHK(jvk_sx_weights(&w, s));
-        JvMmOut o{};
+        take_rows(rv, p->vectors, p->vector_stride, p->dtype, at, rows, plan, ws + plan.off_v, &pre.m[1], &w.mm.b, &w.mm.ldb);
+        CHK(jvk_sx_prepare(&pre, s));
+        pre.m[0].rows = 0, pre.query = nullptr;
+        CHK(jvk_sx_weights(&w, plan.large, s));
+        JvMmOut o{}, q;
         o.mm.segs = plan.segs;
         o.mm.a = (const char*)w.g, o.mm.lda = (int64_t)plan.P * w.kv * 2, o.mm.plane_a = (int64_t)w.kv * 2;
         o.mm.N = p->d, o.mm.plane_b = (int64_t)plan.dp * 2, o.mm.cb = plan.dp;
@@ -313,19 +321,19 @@ int jv_softmax_grad_device(const jv_softmax_params* p, const float* d_lse, const
             o.mm.M = p->nq, o.mm.kph = w.kv / 32;
             o.mm.b = w.mm.b, o.mm.ldb = w.mm.ldb, o.mm.kb = rows;
             o.mul = 1.0f, o.out = ws + plan.off_slab, o.ldo = plan.dp, o.add = at > 0;
-            o.splits = std::min(plan.splits_q, o.mm.kph * plan.segs);   // (only the last piece can be that short: it adds to the first ranges)
-            CHK(jvk_sx_query_grad(&o, s));
+            o.splits = std::min(plan.splits_q, o.mm.kph / 2 * plan.segs);   // (only the last piece can be that short: it adds to the first ranges)
+            q = o;
         }
         if (d_out_vector_grad) {   // G across times the queries: k = the queries
             o.mm.M = rows, o.mm.kph = plan.kq / 32, o.mm.ka = plan.kq, o.mm.ca = w.kv;
             o.mm.b = w.mm.a, o.mm.ldb = w.mm.lda, o.mm.kb = p->nq;
             o.mul = p->scale, o.norm = norm, o.dtype = p->dtype, o.splits = 1, o.add = 0;
             o.out = (char*)d_out_vector_grad + at * vector_grad_stride * size_of(p->dtype), o.ldo = vector_grad_stride;
-            CHK(jvk_sx_vector_grad(&o, s));
         }
+        CHK(jvk_sx_grads(d_out_query_grad ? &q : nullptr, d_out_vector_grad ? &o : nullptr, plan.large, s));
     }
     if (d_out_query_grad) {
-        const int splits = (int)std::min<int64_t>(plan.splits_q, up(std::min<int64_t>(plan.rows_b, p->n), 64) / 32 * plan.segs);
+        const int splits = (int)std::min<int64_t>(plan.splits_q, up(std::min<int64_t>(plan.rows_b, p->n), 64) / 64 * plan.segs);
         CHK(jvk_sx_finish((const float*)(ws + plan.off_slab), splits, p->nq, p->d, plan.dp, w.rest, query, p->vectors, p->vector_stride, p->scale, norm, d_out_query_grad,
                           p->dtype, query_grad_stride, s));
     }

@@ -39,25 +39,33 @@ __device__ __forceinline__ void planes3(float x, uint16_t (&p)[3]) {
 }
 
 // ---------------------------------------------------------------------------------------------
-// rows -> padded bf16 planes [rows][P][kp], eight components a thread
+// what has to be laid out: rows as padded bf16 planes [rows][planes][kp], and what the gradient needs of each query
 // ---------------------------------------------------------------------------------------------
 template <typename T>
-__global__ __launch_bounds__(256) void jvs_pack_kernel(const T* __restrict__ x, int64_t stride, int64_t rows, int d, int kp, uint16_t* __restrict__ out) {
+__device__ __forceinline__ void pack(const JvSxPrepare::Matrix& m, int d, int kp, int64_t first, int64_t step) {   // eight components a thread
     constexpr int P = sizeof(T) == 4 ? 3 : 1;
     const int per = kp / 8;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * per; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / per;
+    const int wide = (uintptr_t)m.x % 16 == 0 && m.stride % (16 / sizeof(T)) == 0;
+    for (int64_t i = first; i < m.rows * per; i += step) {
+        const int64_t r = i < 0x100000000ll ? (int64_t)((uint32_t)i / (uint32_t)per) : i / per;
         const int at = (int)(i - r * per) * 8;
-        const T* row = x + r * stride;
+        const T* row = (const T*)m.x + r * m.stride;
+        T x[8];
+        if (wide && at + 8 <= d) {
+#pragma unroll
+            for (int k = 0; k < (int)sizeof(T) / 2; k++) ((i32x4*)x)[k] = ((const i32x4*)(row + at))[k];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = at + e < d ? row[at + e] : (T)0.0f;
+        }
         uint16_t p[3][8];
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            const T v = at + e < d ? row[at + e] : (T)0.0f;
             if constexpr (P == 1) {
-                p[0][e] = __builtin_bit_cast(uint16_t, v);
+                p[0][e] = __builtin_bit_cast(uint16_t, x[e]);
             } else {
                 uint16_t q[3];
-                planes3(v, q);
+                planes3(x[e], q);
 #pragma unroll
                 for (int k = 0; k < 3; k++) p[k][e] = q[k];
             }
@@ -67,19 +75,56 @@ __global__ __launch_bounds__(256) void jvs_pack_kernel(const T* __restrict__ x, 
             i32x4 o;
 #pragma unroll
             for (int e = 0; e < 4; e++) o[e] = (int)((uint32_t)p[k][2 * e] | ((uint32_t)p[k][2 * e + 1] << 16));
-            *(i32x4*)(out + (r * P + k) * kp + at) = o;
+            *(i32x4*)(m.out + (r * P + k) * kp + at) = o;
         }
     }
 }
 
-extern "C" hipError_t jvk_sx_pack(const void* x, int dtype, int64_t stride, int64_t rows, int d, int kp, uint16_t* out, hipStream_t s) {
-    const int64_t want = (rows * (kp / 8) + 255) / 256;
-    if (want <= 0) return hipSuccess;
-    const unsigned grid = (unsigned)(want < 65536 ? want : 65536);
-    if (dtype == 0) jvs_pack_kernel<float><<<grid, 256, 0, s>>>((const float*)x, stride, rows, d, kp, out);
-    else jvs_pack_kernel<__bf16><<<grid, 256, 0, s>>>((const __bf16*)x, stride, rows, d, kp, out);
+// The weights are divided by the largest of them (`norm`, multiplied back in float32 at the end): an entry of g at a target is then just
+// below 1 for the largest weight, where bf16's step is finest in relation.
+__device__ __forceinline__ void queries(const JvSxPrepare& a) {
+    __shared__ float part[4];
+    float top = 0.0f;
+    if (a.w)
+        for (int i = threadIdx.x; i < a.nq; i += 256)
+            if (a.targets[i] >= 0 && a.targets[i] < a.n) top = fmaxf(top, fabsf(a.w[i]));
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+    // (no weights, none but zeros, or one that is not finite: 1, so that what is not finite shows in the gradient)
+    const float unit = a.w && top > 0.0f && top < __builtin_inff() ? top : 1.0f;
+    if (threadIdx.x == 0) *a.norm = unit;
+    for (int i = threadIdx.x; i < a.nq; i += 256) {
+        const int t = a.targets[i];
+        const bool known = t >= 0 && t < a.n;
+        JvSxQuery q;
+        q.lse2 = known ? a.lse[i] * 1.44269504088896341f : 0.0f;
+        q.w = known ? (a.w ? a.w[i] : 1.0f) / unit : 0.0f;
+        q.target = known ? t : -1;
+        q.pad = 0;
+        a.query[i] = q;
+        a.rest[i] = 0.0f;
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void jvs_prepare_kernel(const JvSxPrepare a, int g0, int g1) {   // g0 + g1 workgroups for the matrices
+    if ((int)blockIdx.x < g0) pack<T>(a.m[0], a.d, a.kp, (int64_t)blockIdx.x * 256 + threadIdx.x, (int64_t)g0 * 256);
+    else if ((int)blockIdx.x < g0 + g1) pack<T>(a.m[1], a.d, a.kp, (int64_t)((int)blockIdx.x - g0) * 256 + threadIdx.x, (int64_t)g1 * 256);
+    else queries(a);
+}
+extern "C" hipError_t jvk_sx_prepare(const JvSxPrepare* a, hipStream_t s) {
+    int g[2];
+    for (int k = 0; k < 2; k++) g[k] = (int)std::min<int64_t>((a->m[k].rows * (a->kp / 8) + 255) / 256, 32768);
+    const unsigned grid = (unsigned)(g[0] + g[1] + (a->query ? 1 : 0));
+    if (grid == 0) return hipSuccess;
+    if (a->dtype == 0) jvs_prepare_kernel<float><<<grid, 256, 0, s>>>(*a, g[0], g[1]);
+    else jvs_prepare_kernel<__bf16><<<grid, 256, 0, s>>>(*a, g[0], g[1]);
     return hipGetLastError();
 }
+
 // ---------------------------------------------------------------------------------------------
 // forward: running maximum and sum over this workgroup's tiles of rows
 // ---------------------------------------------------------------------------------------------
@@ -186,7 +231,7 @@ __global__ __launch_bounds__(64 * WM * WN) void jvs_loss_tile_kernel(const JvSxL
     for (int m = 0; m < MT; m++) top[m] = -__builtin_inff(), sum[m] = 0.0f;
     for (int t = split; t < tiles; t += a.splits) {
         f32x16 acc[MT][NT];
-        T::run(a.mm, m0, t * T::TN, smem, acc);
+        T::run(a.mm, m0, t * T::TN, 0, (a.mm.kph >> 1) * a.mm.segs, smem, acc);
         add_tile<T>(acc, a.c, a.mm.N - t * T::TN, top, sum);
     }
     write_partials<T::TM, MT, WN>(a, smem, m0, split, (threadIdx.x >> 6) / WM, [](int m) { return T::row(m); }, top, sum);
@@ -194,6 +239,7 @@ __global__ __launch_bounds__(64 * WM * WN) void jvs_loss_tile_kernel(const JvSxL
 
 // the large tiles where they fill the chip
 static bool large(int nq, int64_t rows) { return nq > 64 && ((nq + 255) / 256) * ((rows + 255) / 256) >= 192; }
+extern "C" int jvk_sx_large(int nq, int64_t rows) { return large(nq, rows); }
 
 // workgroups that share a panel's rows: one for each CU with the large tiles, two or three with the small ones
 extern "C" int jvk_sx_loss_plan(int nq, int64_t rows, int* tile) {
@@ -262,41 +308,20 @@ extern "C" hipError_t jvk_sx_join(const float* part, int splits, int nq, const v
 // ---------------------------------------------------------------------------------------------
 // backward: the logits again, as weights g
 // ---------------------------------------------------------------------------------------------
-// What the gradient needs of each query.  The weights are divided by the largest of them (`norm`, multiplied back in float32 at the end): an
-// entry at a target is then just below 1 for the largest weight, where bf16's step is finest in relation.
-__global__ __launch_bounds__(1024) void jvs_queries_kernel(const float* __restrict__ lse, const float* __restrict__ w, const int32_t* __restrict__ targets,
-                                                           int nq, int64_t n, JvSxQuery* __restrict__ query, float* __restrict__ norm,
-                                                           float* __restrict__ rest) {
-    __shared__ float part[16];
-    float top = 0.0f;
-    if (w)
-        for (int i = threadIdx.x; i < nq; i += 1024)
-            if (targets[i] >= 0 && targets[i] < n) top = fmaxf(top, fabsf(w[i]));
+// g of a lane's columns of one query, in place of the logits; `cols`: how many of the tile's columns are rows of the piece; `hit`: the target's column
+template <class Core, int NT>
+__device__ __forceinline__ void weigh(f32x16 (&acc)[NT], const JvSxQuery& q, float c, int cols, int hit, bool lossy, float* rest) {
 #pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
-    __syncthreads();
+    for (int n = 0; n < NT; n++)
 #pragma unroll
-    for (int k = 0; k < 16; k++) top = fmaxf(top, part[k]);
-    // (no weights, none but zeros, or one that is not finite: 1, so that what is not finite shows in the gradient)
-    const float unit = w && top > 0.0f && top < __builtin_inff() ? top : 1.0f;
-    if (threadIdx.x == 0) *norm = unit;
-    for (int i = threadIdx.x; i < nq; i += 1024) {
-        const int t = targets[i];
-        const bool known = t >= 0 && t < n;
-        JvSxQuery q;
-        q.lse2 = known ? lse[i] * 1.44269504088896341f : 0.0f;
-        q.w = known ? (w ? w[i] : 1.0f) / unit : 0.0f;
-        q.target = known ? t : -1;
-        q.pad = 0;
-        query[i] = q;
-        rest[i] = 0.0f;
-    }
-}
-extern "C" hipError_t jvk_sx_queries(const float* lse, const float* w, const int32_t* targets, int nq, int64_t n, JvSxQuery* query, float* norm, float* rest,
-                                     hipStream_t s) {
-    jvs_queries_kernel<<<1, 1024, 0, s>>>(lse, w, targets, nq, n, query, norm, rest);
-    return hipGetLastError();
+        for (int e = 0; e < 16; e++) {
+            const int at = Core::col(n, e);
+            float g = exp2_(fmaf(acc[n][e], c, -q.lse2));
+            if (at == hit) g -= 1.0f;
+            g = q.target >= 0 && at < cols ? g * q.w : 0.0f;
+            acc[n][e] = g;
+            if (at == hit && lossy) *rest = g - (float)(__bf16)g;   // (one lane holds it; three planes lack nothing)
+        }
 }
 
 __global__ __launch_bounds__(512) void jvs_weights_kernel(const JvSxWeights a) {
@@ -321,18 +346,7 @@ __global__ __launch_bounds__(512) void jvs_weights_kernel(const JvSxWeights a) {
                 const int r = w.m0 + P::row(m);
                 JvSxQuery q = {0.0f, 0.0f, -1, 0};
                 if (r < a.mm.M) q = a.query[r];
-                const int at = q.target >= 0 && q.target >= a.row0 && q.target - a.row0 < a.mm.N ? (int)(q.target - a.row0) - w.n0 : -1;
-#pragma unroll
-                for (int n = 0; n < 2; n++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        const int c = P::col(n, e);
-                        float g = exp2_(fmaf(acc[m][n][e], a.c, -q.lse2));
-                        if (c == at) g -= 1.0f;
-                        g = q.target >= 0 && w.n0 + c < a.mm.N ? g * q.w : 0.0f;
-                        acc[m][n][e] = g;
-                        if (a.planes == 1 && c == at) a.rest[r] = g - (float)(__bf16)g;
-                    }
+                weigh<P>(acc[m], q, a.c, a.mm.N - w.n0, q.target >= 0 ? (int)(q.target - a.row0) - w.n0 : -1, a.planes == 1, a.rest + r);
             }
             int stores = 0;
             for (int k = 0; k < a.planes; k++) {
@@ -350,9 +364,60 @@ __global__ __launch_bounds__(512) void jvs_weights_kernel(const JvSxWeights a) {
         });
 }
 
-extern "C" hipError_t jvk_sx_weights(const JvSxWeights* a, hipStream_t s) {
+// the same on small tiles, one a workgroup
+template <int MT, int NT, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void jvs_weights_tile_kernel(const JvSxWeights a) {
+    using T = Tile<BF16, MT, NT, WM, WN>;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    const int tm = (a.mm.M + T::TM - 1) / T::TM, tn = (a.mm.N + T::TN - 1) / T::TN;
+    const int padded = (a.mm.M + 63) / 64 * 64;
+    int m0, n0;
+    band_order(xcd_order(blockIdx.x, gridDim.x), tm, tn, m0, n0);
+    m0 *= T::TM, n0 *= T::TN;
+    f32x16 acc[MT][NT];
+    T::run(a.mm, m0, n0, 0, (a.mm.kph >> 1) * a.mm.segs, smem, acc);
+#pragma unroll
+    for (int m = 0; m < MT; m++) {
+        const int r = m0 + T::row(m);
+        JvSxQuery q = {0.0f, 0.0f, -1, 0};
+        if (r < a.mm.M) q = a.query[r];
+        weigh<T>(acc[m], q, a.c, a.mm.N - n0, q.target >= 0 ? (int)(q.target - a.row0) - n0 : -1, a.planes == 1, a.rest + r);
+        // (rows of 32: those behind the padded ones only where one tile has more rows than there are)
+        for (int k = 0; k < a.planes; k++) {
+            uint16_t* row = a.g + ((int64_t)r * a.planes + k) * a.kv;
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int g = 0; g < 4; g++) {
+                    const int col = n0 + T::col(n, 4 * g);
+                    bf16x4 v;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        v[e] = (__bf16)acc[m][n][4 * g + e];
+                        acc[m][n][4 * g + e] -= (float)v[e];
+                    }
+                    if (r < padded && col < a.kv) *(bf16x4*)(row + col) = v;   // (kv is a multiple of 64)
+                }
+        }
+    }
+}
+
+template <int MT, int NT, int WM, int WN>
+static hipError_t weights_tile(const JvSxWeights& a, hipStream_t s) {
+    using T = Tile<BF16, MT, NT, WM, WN>;
+    // (tiles cover the 64 padded queries: a tile of 32 needs two of them)
+    const int64_t all = (int64_t)(((a.mm.M + 63) / 64 * 64 + T::TM - 1) / T::TM) * ((a.mm.N + T::TN - 1) / T::TN);
+    if (all > 0x7fffffffll) return hipErrorInvalidValue;
+    hipError_t e = hipFuncSetAttribute((const void*)jvs_weights_tile_kernel<MT, NT, WM, WN>, hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS);
+    if (e != hipSuccess) return e;
+    jvs_weights_tile_kernel<MT, NT, WM, WN><<<(unsigned)all, T::THREADS, T::LDS, s>>>(a);
+    return hipGetLastError();
+}
+
+extern "C" hipError_t jvk_sx_weights(const JvSxWeights* a, int large, hipStream_t s) {
     using P = Pipe<BF16>;
     if (a->mm.M <= 0 || a->mm.N <= 0) return hipSuccess;
+    if (!large) return a->mm.M > 64 ? weights_tile<2, 2, 2, 2>(*a, s) : weights_tile<2, 1, 1, 4>(*a, s);
     const int64_t all = (int64_t)((a->mm.M + P::TM - 1) / P::TM) * ((a->mm.N + P::TN - 1) / P::TN);
     if (all > 0x7fffffffll) return hipErrorInvalidValue;
     hipError_t e = hipFuncSetAttribute((const void*)jvs_weights_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, P::LDS);
@@ -361,23 +426,56 @@ extern "C" hipError_t jvk_sx_weights(const JvSxWeights* a, hipStream_t s) {
     return hipGetLastError();
 }
 
-// dq = G V: G's rows are queries, V's rows are k.  dv = G^T Q: the rows of both are k.
-extern "C" hipError_t jvk_sx_query_grad(const JvMmOut* a, hipStream_t s) { return mm_out_pipe<BF16, false, true>(*a, s); }
-extern "C" hipError_t jvk_sx_vector_grad(const JvMmOut* a, hipStream_t s) { return mm_out_pipe<BF16, true, true>(*a, s); }
+// dq = G V: G's rows are queries, V's rows are k.  dv = G^T Q: the rows of both are k.  On small tiles both share a launch.
+__global__ __launch_bounds__(256) void jvs_grads_tile_kernel(const JvMmOut q, const JvMmOut v, int first) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    if ((int)blockIdx.x < first) out_tile<BF16, 2, 2, 2, 2, false, true>(q, blockIdx.x, smem);
+    else out_tile<BF16, 2, 2, 2, 2, true, true>(v, blockIdx.x - first, smem);
+}
 
-// partial sums -> the queries' gradient, and what G lacked at the target
+// k ranges of dq: with the large tiles once around the CUs, eight phases in each at least; with the small ones twice, four steps at least
+extern "C" int jvk_sx_grad_splits(int nq, int d, int64_t rows, int segs, int large) {
+    const int t = large ? 256 : 128, full = large ? 256 : 512;
+    const int64_t tiles = std::max<int64_t>((nq + t - 1) / t, 1) * ((d + t - 1) / t), steps = (rows + 63) / 64 * segs;
+    return (int)std::max<int64_t>(std::min<int64_t>(full / tiles, steps / 4), 1);
+}
+extern "C" hipError_t jvk_sx_grads(const JvMmOut* q, const JvMmOut* v, int large, hipStream_t s) {
+    if (large) {
+        hipError_t e = hipSuccess;
+        if (q) e = mm_out_pipe<BF16, false, true>(*q, s);
+        if (v && e == hipSuccess) e = mm_out_pipe<BF16, true, true>(*v, s);
+        return e;
+    }
+    using T = Tile<BF16, 2, 2, 2, 2>;
+    const int64_t nq = q ? tile_count(*q, T::TM, T::TN) : 0, nv = v ? tile_count(*v, T::TM, T::TN) : 0;
+    if (nq < 0 || nv < 0 || nq + nv > 0x7fffffffll) return hipErrorInvalidValue;
+    if (nq + nv == 0) return hipSuccess;
+    hipError_t e = hipFuncSetAttribute((const void*)jvs_grads_tile_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS);
+    if (e != hipSuccess) return e;
+    jvs_grads_tile_kernel<<<(unsigned)(nq + nv), T::THREADS, T::LDS, s>>>(q ? *q : JvMmOut{}, v ? *v : JvMmOut{}, (int)nq);
+    return hipGetLastError();
+}
+
+// partial sums -> the queries' gradient, and what G lacked at the target: one wave a row, four columns a lane
 template <typename T>
 __global__ __launch_bounds__(256) void jvs_finish_kernel(const float* __restrict__ slab, int splits, int64_t rows, int d, int64_t lds, const float* __restrict__ rest,
                                                          const JvSxQuery* __restrict__ query, const T* __restrict__ v, int64_t v_stride, float mul,
                                                          const float* __restrict__ norm, T* __restrict__ out, int64_t ldo) {
-    const int64_t all = rows * d;
-    const float by = mul * *norm;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / d, c = i - r * d;
-        float x = 0.0f;
-        for (int k = 0; k < splits; k++) x += slab[(k * rows + r) * lds + c];
-        if (const float lack = rest[r]; lack != 0.0f) x = fmaf(lack, (float)v[query[r].target * v_stride + c], x);
-        out[r * ldo + c] = (T)(x * by);
+    const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (r >= rows) return;
+    const float by = mul * *norm, lack = rest[r];
+    const int64_t target = lack != 0.0f ? query[r].target : 0;
+    for (int c = (threadIdx.x & 63) * 4 + blockIdx.y * 256; c < d; c += gridDim.y * 256) {   // (lds is a multiple of 64)
+        const float* p = slab + r * lds + c;
+        f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+        for (int k = 0; k < splits; k++) x += *(const f32x4*)(p + k * rows * lds);
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (c + e < d) {
+                const float y = lack != 0.0f ? fmaf(lack, (float)v[target * v_stride + c + e], x[e]) : x[e];
+                out[r * ldo + c + e] = (T)(y * by);
+            }
     }
 }
 template <typename T>
@@ -394,10 +492,11 @@ static unsigned grid_for(int64_t items) {
 extern "C" hipError_t jvk_sx_finish(const float* slab, int splits, int64_t rows, int d, int64_t lds, const float* rest, const JvSxQuery* query, const void* v,
                                     int64_t v_stride, float mul, const float* norm, void* out, int dtype, int64_t ldo, hipStream_t s) {
     if (rows <= 0 || d <= 0) return hipSuccess;
+    const dim3 grid((unsigned)((rows + 3) / 4), (unsigned)std::min((d + 255) / 256, 16));
     if (dtype == 0)
-        jvs_finish_kernel<float><<<grid_for(rows * d), 256, 0, s>>>(slab, splits, rows, d, lds, rest, query, (const float*)v, v_stride, mul, norm, (float*)out, ldo);
+        jvs_finish_kernel<float><<<grid, 256, 0, s>>>(slab, splits, rows, d, lds, rest, query, (const float*)v, v_stride, mul, norm, (float*)out, ldo);
     else
-        jvs_finish_kernel<__bf16><<<grid_for(rows * d), 256, 0, s>>>(slab, splits, rows, d, lds, rest, query, (const __bf16*)v, v_stride, mul, norm, (__bf16*)out, ldo);
+        jvs_finish_kernel<__bf16><<<grid, 256, 0, s>>>(slab, splits, rows, d, lds, rest, query, (const __bf16*)v, v_stride, mul, norm, (__bf16*)out, ldo);
     return hipGetLastError();
 }
 extern "C" hipError_t jvk_sx_fill(void* out, int dtype, int64_t stride, int64_t rows, int d, float value, hipStream_t s) {

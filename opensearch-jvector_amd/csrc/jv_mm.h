@@ -46,25 +46,54 @@ __device__ __forceinline__ bf16x8 widen(int lo, int hi, int byte) {
     return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+__device__ __forceinline__ s16x4 read_across(const unsigned char* p) {   // 16 lanes give four rows of 16 columns, and take a column's four rows
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
+}
+
 // The product for small shapes: MT x NT accumulators of 32 x 32 for each of WM x WN waves, two steps of k in LDS, several workgroups a CU.
-template <int TY, int MT, int NT, int WM, int WN>
+// TA / TB: an operand with k across its rows (bf16): 64 rows of TM / TN columns a step.  Four rows of 64 B are read at a time: piece p of row k
+// lies at p ^ (swirl << 2) so that they are the four quarters of a 256-B bank row.
+template <int TY, int MT, int NT, int WM, int WN, bool TA = false, bool TB = false>
 struct Tile {
     static constexpr int TM = 32 * MT * WM, TN = 32 * NT * WN, WAVES = WM * WN, THREADS = 64 * WAVES;
     static constexpr int GA = TM / 8, GB = TN / 8;                               // 8-row groups
     static constexpr int CA = GA / WAVES, CB = GB / WAVES, PER = CA + CB;        // copies of one wave a step
     static constexpr int BUF = (GA + GB) * GROUP, LDS = 2 * BUF;
     static_assert(GA % WAVES == 0 && GB % WAVES == 0, "every wave copies the same number of groups of each operand");
+    static_assert(TY == BF16 || (!TA && !TB), "8-bit operands have k along their rows");
 
-    // C tile at (m0, n0).  Rows behind the operands' last are read as their last.
-    static __device__ __forceinline__ void run(const JvMm& a, int m0, int n0, unsigned char* smem, f32x16 (&acc)[MT][NT]) {
-        const int nk = a.kph >> 1, k1 = nk * a.segs;   // steps: two phases each
+    template <int PIECES>   // 16-B pieces of a row
+    static __device__ __forceinline__ int swirl(int k) {
+        return PIECES >= 16 ? k & 3 : PIECES == 8 ? (k >> 1) & 1 : 0;
+    }
+    // 32 columns from `first` on, rows 16 kk + 8 h + (0 .. 7)
+    template <int PIECES>
+    static __device__ __forceinline__ bf16x8 across(const unsigned char* base, int first, int kk) {
+        const int lane = threadIdx.x & 63, c = first + ((lane >> 4) & 1) * 16 + (lane & 3) * 4, k = 16 * kk + 8 * (lane >> 5) + ((lane & 15) >> 2);
+        auto at = [&](int row) { return base + (row * PIECES + ((c >> 3) ^ (swirl<PIECES>(row) << 2))) * 16 + (c & 4) * 2; };
+        return __builtin_bit_cast(bf16x8, __builtin_shufflevector(read_across(at(k)), read_across(at(k + 4)), 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+
+    // C tile at (m0, n0), steps [k0, k1) of the segs * kph / 2 in all.  Rows behind the operands' last are read as their last.
+    static __device__ __forceinline__ void run(const JvMm& a, int m0, int n0, int k0, int k1, unsigned char* smem, f32x16 (&acc)[MT][NT]) {
+        const int nk = a.kph >> 1;   // steps of a segment
         const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
         const int lr = lane >> 3, lp = (lane & 7) ^ lr;
-        const char* src[PER];   // group i * WAVES + w of A, then of B
+        const char* src[PER];   // k along rows: the row's piece; k across: the column's piece of row 0
+        int krow[PER];          // k across: the row inside a step
 #pragma unroll
-        for (int i = 0; i < CA; i++) src[i] = a.a + (int64_t)min(m0 + 8 * (i * WAVES + w) + lr, a.M - 1) * a.lda + lp * 16;
+        for (int i = 0; i < CA; i++) {
+            krow[i] = (i * WAVES + w) * (64 / GA) + lane / GA;   // (a row of TM columns is GA pieces)
+            if constexpr (!TA) src[i] = a.a + (int64_t)min(m0 + 8 * (i * WAVES + w) + lr, a.M - 1) * a.lda + lp * 16;
+            else src[i] = a.a + (int64_t)min(m0 + 8 * ((lane % GA) ^ (swirl<GA>(krow[i]) << 2)), a.ca - 8) * 2;
+        }
 #pragma unroll
-        for (int i = 0; i < CB; i++) src[CA + i] = a.b + (int64_t)min(n0 + 8 * (i * WAVES + w) + lr, a.N - 1) * a.ldb + lp * 16;
+        for (int i = 0; i < CB; i++) {
+            krow[CA + i] = (i * WAVES + w) * (64 / GB) + lane / GB;
+            if constexpr (!TB) src[CA + i] = a.b + (int64_t)min(n0 + 8 * (i * WAVES + w) + lr, a.N - 1) * a.ldb + lp * 16;
+            else src[CA + i] = a.b + (int64_t)min(n0 + 8 * ((lane % GB) ^ (swirl<GB>(krow[CA + i]) << 2)), a.cb - 8) * 2;
+        }
         const int wm = w % WM, wn = w / WM, h = lane >> 5, r31 = lane & 31;
         int aoff[MT], boff[NT], ax, bx;
 #pragma unroll
@@ -92,20 +121,22 @@ struct Tile {
 #pragma unroll
                 for (int e = 0; e < 16; e++) acc[m][n][e] = 0.0f;
 
-        int seg = 0, kin = 0;   // of the next step to be staged
+        int seg = k0 / nk, kin = k0 - seg * nk;   // of the next step to be staged
         auto stage = [&](int buf) {
-            int64_t offa = (int64_t)kin * 128, offb = offa;
+            int64_t offa = TA ? 0 : (int64_t)kin * 128, offb = TB ? 0 : (int64_t)kin * 128;
             if (a.segs > 1) offa += plane_a(seg) * a.plane_a, offb += plane_b(seg) * a.plane_b;
-            unsigned char* dst = smem + buf * BUF + w * GROUP;
+            unsigned char* dst = smem + buf * BUF;
 #pragma unroll
-            for (int i = 0; i < CA; i++) glds16(src[i] + offa, dst + i * WAVES * GROUP);
+            for (int i = 0; i < CA; i++)
+                glds16(src[i] + offa + (TA ? (int64_t)min(kin * 64 + krow[i], a.ka - 1) * a.lda : 0), dst + (i * WAVES + w) * (TA ? 1024 : GROUP));
 #pragma unroll
-            for (int i = 0; i < CB; i++) glds16(src[CA + i] + offb, dst + (GA + i * WAVES) * GROUP);
+            for (int i = 0; i < CB; i++)
+                glds16(src[CA + i] + offb + (TB ? (int64_t)min(kin * 64 + krow[CA + i], a.kb - 1) * a.ldb : 0), dst + GA * GROUP + (i * WAVES + w) * (TB ? 1024 : GROUP));
             if (++kin == nk) kin = 0, seg++;
         };
         stage(0);
-        for (int s = 0; s < k1; s++) {
-            const int buf = s & 1;
+        for (int s = k0; s < k1; s++) {
+            const int buf = (s - k0) & 1;
             int fa[MT], fb[NT];
             if constexpr (TY != BF16) {
 #pragma unroll
@@ -121,21 +152,23 @@ struct Tile {
             }
             const unsigned char* base = smem + buf * BUF;
             if constexpr (TY == BF16) {
-                bf16x8 va[2][MT], vb[2][NT];
-                auto frag = [&](int kk) {
-#pragma unroll
-                    for (int t = 0; t < MT; t++) va[kk & 1][t] = *(const bf16x8*)(base + aoff[t] + (((2 * kk + h) ^ ax) << 4));
-#pragma unroll
-                    for (int t = 0; t < NT; t++) vb[kk & 1][t] = *(const bf16x8*)(base + boff[t] + (((2 * kk + h) ^ bx) << 4));
-                };
-                frag(0);
 #pragma unroll
                 for (int kk = 0; kk < 4; kk++) {
-                    if (kk < 3) frag(kk + 1);
+                    bf16x8 va[MT], vb[NT];
+#pragma unroll
+                    for (int t = 0; t < MT; t++) {
+                        if constexpr (TA) va[t] = across<GA>(base, (wm * MT + t) * 32, kk);
+                        else va[t] = *(const bf16x8*)(base + aoff[t] + (((2 * kk + h) ^ ax) << 4));
+                    }
+#pragma unroll
+                    for (int t = 0; t < NT; t++) {
+                        if constexpr (TB) vb[t] = across<GB>(base + GA * GROUP, (wn * NT + t) * 32, kk);
+                        else vb[t] = *(const bf16x8*)(base + boff[t] + (((2 * kk + h) ^ bx) << 4));
+                    }
 #pragma unroll
                     for (int m = 0; m < MT; m++)
 #pragma unroll
-                        for (int n = 0; n < NT; n++) acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vb[kk & 1][n], va[kk & 1][m], acc[m][n], 0, 0, 0);
+                        for (int n = 0; n < NT; n++) acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vb[n], va[m], acc[m][n], 0, 0, 0);
                 }
             } else if constexpr (TY == F8W) {
                 // (16 components a lane and step: which of the block's 128 does not matter as long as both operands agree)

@@ -51,19 +51,27 @@ static hipError_t mm_out_pipe(const JvMmOut& a, hipStream_t s) {
     return hipGetLastError();
 }
 
-template <int TY, int MT, int NT, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN) void jvm_out_tile_kernel(const JvMmOut a) {
-    using T = Tile<TY, MT, NT, WM, WN>;
-    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    const int tm = (a.mm.M + T::TM - 1) / T::TM, tn = (a.mm.N + T::TN - 1) / T::TN;
-    const Share share(tm * tn);   // (a grid of one workgroup for each tile, rounded up to 8)
-    int L, m0, n0;
-    if (!share.at(0, L)) return;
+// Tile `i` of `n` when every workgroup has one: those of an XCD (i & 7) take a contiguous run (bijective for any n).
+__device__ __forceinline__ int xcd_order(int i, int n) {
+    const int xcd = i & 7, slot = i >> 3, q = n >> 3, r = n & 7;
+    return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + slot;
+}
+
+// workgroup `i` of tiles * splits: one tile over one k range
+template <int TY, int MT, int NT, int WM, int WN, bool TA, bool TB>
+__device__ __forceinline__ void out_tile(const JvMmOut& a, int i, unsigned char* smem) {
+    using T = Tile<TY, MT, NT, WM, WN, TA, TB>;
+    const int tm = (a.mm.M + T::TM - 1) / T::TM, tn = (a.mm.N + T::TN - 1) / T::TN, tiles = tm * tn;
+    int L = xcd_order(i, tiles * a.splits), part = 0, m0, n0;
+    if (a.splits > 1) part = L / tiles, L -= part * tiles;
     band_order(L, tm, tn, m0, n0);
     m0 *= T::TM, n0 *= T::TN;
+    const int steps = (a.mm.kph >> 1) * a.mm.segs;
     f32x16 acc[MT][NT];
-    T::run(a.mm, m0, n0, smem, acc);
+    T::run(a.mm, m0, n0, (int)((int64_t)steps * part / a.splits), (int)((int64_t)steps * (part + 1) / a.splits), smem, acc);
+    const float mul = a.norm ? a.mul * *a.norm : a.mul;
     const bool wide = (uintptr_t)a.out % 16 == 0 && a.ldo % (a.dtype == 0 ? 4 : 8) == 0;
+    const int64_t slab = (int64_t)part * a.mm.M * a.ldo;
 #pragma unroll
     for (int m = 0; m < MT; m++) {
         const int row = m0 + T::row(m);
@@ -75,35 +83,53 @@ __global__ __launch_bounds__(64 * WM * WN) void jvm_out_tile_kernel(const JvMmOu
                 const int col = n0 + T::col(n, 4 * g);
                 f32x4 v;
 #pragma unroll
-                for (int e = 0; e < 4; e++) v[e] = acc[m][n][4 * g + e] * a.mul;
+                for (int e = 0; e < 4; e++) v[e] = acc[m][n][4 * g + e] * mul;
                 if (a.dtype == 0) {
-                    float* p = (float*)a.out + (int64_t)row * a.ldo + col;
-                    if (wide && col + 4 <= a.mm.N) *(f32x4*)p = v;
-                    else
+                    float* p = (float*)a.out + slab + (int64_t)row * a.ldo + col;
+                    if (wide && col + 4 <= a.mm.N) {
+                        if (a.add) v += *(const f32x4*)p;
+                        *(f32x4*)p = v;
+                    } else {
 #pragma unroll
                         for (int e = 0; e < 4; e++)
-                            if (col + e < a.mm.N) p[e] = v[e];
+                            if (col + e < a.mm.N) p[e] = a.add ? p[e] + v[e] : v[e];
+                    }
                 } else {
                     __bf16* p = (__bf16*)a.out + (int64_t)row * a.ldo + col;
-                    if (wide && col + 4 <= a.mm.N) *(bf16x4*)p = (bf16x4){(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
-                    else
+                    if (wide && col + 4 <= a.mm.N) {
+                        *(bf16x4*)p = (bf16x4){(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+                    } else {
 #pragma unroll
                         for (int e = 0; e < 4; e++)
                             if (col + e < a.mm.N) p[e] = (__bf16)v[e];
+                    }
                 }
             }
     }
 }
 
 template <int TY, int MT, int NT, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void jvm_out_tile_kernel(const JvMmOut a) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    out_tile<TY, MT, NT, WM, WN, false, false>(a, blockIdx.x, smem);
+}
+
+// workgroups of a product on tiles of TM x TN, 0 = none, negative = more than a launch takes
+static inline int64_t tile_count(const JvMmOut& a, int TM, int TN) {
+    if (a.mm.M <= 0 || a.mm.N <= 0) return 0;
+    if (a.splits < 1 || a.splits > (a.mm.kph >> 1) * a.mm.segs || (a.dtype != 0 && a.splits > 1)) return -1;
+    const int64_t all = (int64_t)((a.mm.M + TM - 1) / TM) * ((a.mm.N + TN - 1) / TN) * a.splits;
+    return all > 0x7fffffffll ? -1 : all;
+}
+
+template <int TY, int MT, int NT, int WM, int WN>
 static hipError_t mm_out_tile(const JvMmOut& a, hipStream_t s) {
     using T = Tile<TY, MT, NT, WM, WN>;
-    if (a.mm.M <= 0 || a.mm.N <= 0) return hipSuccess;
-    const int64_t tiles = (int64_t)((a.mm.M + T::TM - 1) / T::TM) * ((a.mm.N + T::TN - 1) / T::TN);
-    if (tiles > 0x7ffffff0ll || a.splits != 1 || a.add) return hipErrorInvalidValue;
+    const int64_t all = tile_count(a, T::TM, T::TN);
+    if (all <= 0) return all ? hipErrorInvalidValue : hipSuccess;
     hipError_t e = hipFuncSetAttribute((const void*)jvm_out_tile_kernel<TY, MT, NT, WM, WN>, hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS);
     if (e != hipSuccess) return e;
-    jvm_out_tile_kernel<TY, MT, NT, WM, WN><<<(unsigned)((tiles + 7) / 8 * 8), T::THREADS, T::LDS, s>>>(a);
+    jvm_out_tile_kernel<TY, MT, NT, WM, WN><<<(unsigned)all, T::THREADS, T::LDS, s>>>(a);
     return hipGetLastError();
 }
 

@@ -58,6 +58,23 @@ struct JvSxWeights {
     float* rest;           // [M] bf16: what G's entry at the target lacks of its float32 value
 };
 
+// what has to be laid out before a product: up to two matrices (rows -> bf16 planes [rows][planes][kp]) and the queries' constants, one launch
+struct JvSxPrepare {
+    struct Matrix {
+        const void* x;
+        int64_t stride, rows;   // rows = 0: none
+        uint16_t* out;
+    } m[2];
+    int32_t dtype, d, kp;
+    // the gradient's queries (query == nullptr: none)
+    const float *lse, *w;
+    const int32_t* targets;
+    int32_t nq;
+    int64_t n;
+    JvSxQuery* query;
+    float *norm, *rest;
+};
+
 // sets jv_last_error() and returns `code` (jv_abi.cpp)
 __attribute__((visibility("hidden"))) int jvi_fail(int code, const char* fmt, ...);
 
@@ -66,15 +83,16 @@ hipError_t jvk_f8_encode(const void* x, int dtype, int64_t stride, int64_t n, in
 hipError_t jvk_f8_decode(const uint8_t* codes, const uint8_t* scales, int64_t n, int d, void* x, int dtype, int64_t stride, hipStream_t s);
 hipError_t jvk_f8_score(const JvMmOut* a, hipStream_t s);
 
-hipError_t jvk_sx_pack(const void* x, int dtype, int64_t stride, int64_t rows, int d, int kp, uint16_t* out, hipStream_t s);
+hipError_t jvk_sx_prepare(const JvSxPrepare* a, hipStream_t s);
 int jvk_sx_loss_plan(int nq, int64_t rows, int* tile);   // splits, and the queries of a tile
 hipError_t jvk_sx_loss(const JvSxLoss* a, hipStream_t s);
 hipError_t jvk_sx_join(const float* part, int splits, int nq, const void* q, int64_t q_stride, const void* v, int64_t v_stride, int dtype, int d,
                        const int32_t* targets, int64_t n, float scale, float* loss, float* lse, hipStream_t s);
-hipError_t jvk_sx_queries(const float* lse, const float* w, const int32_t* targets, int nq, int64_t n, JvSxQuery* query, float* norm, float* rest, hipStream_t s);
-hipError_t jvk_sx_weights(const JvSxWeights* a, hipStream_t s);
-hipError_t jvk_sx_query_grad(const JvMmOut* a, hipStream_t s);
-hipError_t jvk_sx_vector_grad(const JvMmOut* a, hipStream_t s);
+hipError_t jvk_sx_weights(const JvSxWeights* a, int large, hipStream_t s);
+// dq = G V and dv = G^T Q (nullptr: not asked for)
+int jvk_sx_grad_splits(int nq, int d, int64_t rows, int segs, int large);
+hipError_t jvk_sx_grads(const JvMmOut* q, const JvMmOut* v, int large, hipStream_t s);
+int jvk_sx_large(int nq, int64_t rows);   // whether a piece of the rows takes the large tiles
 hipError_t jvk_sx_finish(const float* slab, int splits, int64_t rows, int d, int64_t lds, const float* rest, const JvSxQuery* query, const void* v, int64_t v_stride,
                          float mul, const float* norm, void* out, int dtype, int64_t ldo, hipStream_t s);
 hipError_t jvk_sx_fill(void* out, int dtype, int64_t stride, int64_t rows, int d, float value, hipStream_t s);

@@ -20,8 +20,6 @@
 
 namespace jvmm {
 
-typedef __attribute__((ext_vector_type(4))) short s16x4;
-
 struct Work {
     int m0, n0;      // first row and column of the tile
     int k0, k1;      // phases of the segs * kph in all
@@ -111,9 +109,7 @@ struct Pipe {
         auto across = [&](const unsigned char* base, int first, int j) -> i32x4 {   // 32 columns from `first` on
             const int c = first + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
             const unsigned char* p = base + (16 * j + 8 * h + tk) * 512 + (((c >> 3) ^ (tk << 2)) << 4) + (c & 4) * 2;
-            auto get = [](const unsigned char* q) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)q); };
-            const s16x4 lo = get(p), hi = get(p + 4 * 512);
-            return __builtin_bit_cast(i32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+            return __builtin_bit_cast(i32x4, __builtin_shufflevector(read_across(p), read_across(p + 4 * 512), 0, 1, 2, 3, 4, 5, 6, 7));
         };
 
         // ---- scales: thread t keeps row t of the two tiles; a window of 16 blocks (32 phases) goes from global memory to LDS while the one
