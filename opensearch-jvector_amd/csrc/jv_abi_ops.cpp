@@ -121,7 +121,7 @@ Plan make_plan(int dtype, int nq, int64_t n, int d, uint32_t what) {
         p.off_rest = take((int64_t)nq * 4);
         p.off_g = take((int64_t)p.kq * p.P * p.rows_b * 2);
         if (what & JV_SOFTMAX_QUERY_GRAD) {
-            p.splits_q = jvk_sx_grad_splits(nq, d, p.rows_b, p.segs, p.large);
+            p.splits_q = jvk_sx_grad_splits(nq, d, std::min<int64_t>(p.rows_b, n), p.P == 3, p.large);
             p.off_slab = take((int64_t)p.splits_q * nq * p.dp * 4);
         }
     }
@@ -129,14 +129,15 @@ Plan make_plan(int dtype, int nq, int64_t n, int d, uint32_t what) {
     return p;
 }
 
-// rows as the matrix cores take them: the caller's own where they are bf16, 16-B aligned and whole steps
+// rows as a product takes them: the caller's own where they are bf16, 16-B aligned and whole steps, or float32 and the tiles small
 struct Rows {
     const char* p;
-    int64_t stride;
+    int64_t stride;   // bytes
     bool ready;
 };
-Rows rows_of(const void* p, int64_t stride, int d, int dtype) {
-    return {(const char*)p, stride * 2, dtype == JV_DTYPE_BF16 && (uintptr_t)p % 16 == 0 && stride % 8 == 0 && d % 64 == 0};
+Rows rows_of(const void* p, int64_t stride, int d, int dtype, bool large) {
+    const bool ready = dtype == JV_DTYPE_F32 ? !large : (uintptr_t)p % 16 == 0 && stride % 8 == 0 && d % 64 == 0;
+    return {(const char*)p, stride * size_of(dtype), ready};
 }
 
 int check_softmax(const jv_softmax_params* p) {
@@ -159,10 +160,13 @@ int check_softmax_call(const jv_softmax_params* p, const Plan& plan) {
     return JV_OK;
 }
 
+// k ranges that a piece of `rows` rows has at most: its steps
+int splits_of(const Plan& plan, int64_t rows, bool f32) { return (int)(up(rows, 64) / (f32 ? 32 : 64) * (f32 ? 1 : plan.segs)); }
+
 // queries times vectors, but for where the vectors lie and how many they are
-JvMm logits(const Plan& plan, int nq) {
+JvMm logits(const Plan& plan, int nq, int d) {
     JvMm mm{};
-    mm.M = nq, mm.kph = plan.dp / 32, mm.segs = plan.segs;
+    mm.M = nq, mm.k = d, mm.kph = plan.dp / 32, mm.segs = plan.segs;
     mm.plane_a = mm.plane_b = (int64_t)plan.dp * 2;
     return mm;
 }
@@ -252,10 +256,11 @@ int jv_softmax_loss_device(const jv_softmax_params* p, float* d_out_loss, float*
     hipStream_t s = (hipStream_t)hip_stream;
     if (p->nq > 0) {
         char* ws = (char*)p->workspace;
-        const Rows rq = rows_of(p->queries, p->query_stride, p->d, p->dtype), rv = rows_of(p->vectors, p->vector_stride, p->d, p->dtype);
+        const bool large = plan.tile == 256, f32 = p->dtype == JV_DTYPE_F32 && !large;
+        const Rows rq = rows_of(p->queries, p->query_stride, p->d, p->dtype, large), rv = rows_of(p->vectors, p->vector_stride, p->d, p->dtype, large);
         const int64_t step = rv.ready ? std::max<int64_t>(p->n, 1) : plan.rows_f;
         JvSxLoss a{};
-        a.mm = logits(plan, p->nq);
+        a.mm = logits(plan, p->nq, p->d);
         a.c = p->scale * 1.44269504088896341f;
         a.tile = plan.tile, a.splits = p->n > 0 ? plan.splits_f : 0, a.part = (float*)(ws + plan.off_part);
         JvSxPrepare pre{};
@@ -267,7 +272,7 @@ int jv_softmax_loss_device(const jv_softmax_params* p, float* d_out_loss, float*
             take_rows(rv, p->vectors, p->vector_stride, p->dtype, at, a.mm.N, plan, ws + plan.off_v, &pre.m[1], &a.mm.b, &a.mm.ldb);
             CHK(jvk_sx_prepare(&pre, s));
             pre.m[0].rows = 0;
-            CHK(jvk_sx_loss(&a, s));
+            CHK(jvk_sx_loss(&a, f32, s));
         }
         CHK(jvk_sx_join(a.part, a.splits, p->nq, p->queries, p->query_stride, p->vectors, p->vector_stride, p->dtype, p->d, p->targets, p->n, p->scale, d_out_loss,
                         d_out_lse, s));
@@ -294,11 +299,12 @@ int jv_softmax_grad_device(const jv_softmax_params* p, const float* d_lse, const
         return done(hip_stream);
     }
     char* ws = (char*)p->workspace;
-    const Rows rq = rows_of(p->queries, p->query_stride, p->d, p->dtype), rv = rows_of(p->vectors, p->vector_stride, p->d, p->dtype);
+    const bool f32 = p->dtype == JV_DTYPE_F32 && !plan.large;
+    const Rows rq = rows_of(p->queries, p->query_stride, p->d, p->dtype, plan.large), rv = rows_of(p->vectors, p->vector_stride, p->d, p->dtype, plan.large);
     JvSxWeights w{};
-    w.mm = logits(plan, p->nq);
+    w.mm = logits(plan, p->nq, p->d);
     w.c = p->scale * 1.44269504088896341f;
-    w.planes = plan.P, w.g = (uint16_t*)(ws + plan.off_g), w.rest = (float*)(ws + plan.off_rest);
+    w.planes = f32 ? 0 : plan.P, w.g = ws + plan.off_g, w.rest = (float*)(ws + plan.off_rest);
     JvSxQuery* query = (JvSxQuery*)(ws + plan.off_query);
     w.query = query;
     float* norm = (float*)(ws + plan.off_norm);
@@ -315,25 +321,25 @@ int jv_softmax_grad_device(const jv_softmax_params* p, const float* d_lse, const
         CHK(jvk_sx_weights(&w, plan.large, s));
         JvMmOut o{}, q;
         o.mm.segs = plan.segs;
-        o.mm.a = (const char*)w.g, o.mm.lda = (int64_t)plan.P * w.kv * 2, o.mm.plane_a = (int64_t)w.kv * 2;
-        o.mm.N = p->d, o.mm.plane_b = (int64_t)plan.dp * 2, o.mm.cb = plan.dp;
+        o.mm.a = (const char*)w.g, o.mm.lda = f32 ? (int64_t)w.kv * 4 : (int64_t)plan.P * w.kv * 2, o.mm.plane_a = (int64_t)w.kv * 2;
+        o.mm.N = p->d, o.mm.plane_b = (int64_t)plan.dp * 2, o.mm.cb = f32 ? p->d : plan.dp;
         if (d_out_query_grad) {   // G times the piece's vectors: k = its rows
-            o.mm.M = p->nq, o.mm.kph = w.kv / 32;
+            o.mm.M = p->nq, o.mm.k = w.kv, o.mm.kph = w.kv / 32;
             o.mm.b = w.mm.b, o.mm.ldb = w.mm.ldb, o.mm.kb = rows;
             o.mul = 1.0f, o.out = ws + plan.off_slab, o.ldo = plan.dp, o.add = at > 0;
-            o.splits = std::min(plan.splits_q, o.mm.kph / 2 * plan.segs);   // (only the last piece can be that short: it adds to the first ranges)
+            o.splits = std::min(plan.splits_q, splits_of(plan, rows, f32));   // (only the last piece can be that short: it adds to the first ranges)
             q = o;
         }
         if (d_out_vector_grad) {   // G across times the queries: k = the queries
-            o.mm.M = rows, o.mm.kph = plan.kq / 32, o.mm.ka = plan.kq, o.mm.ca = w.kv;
+            o.mm.M = rows, o.mm.k = plan.kq, o.mm.kph = plan.kq / 32, o.mm.ka = plan.kq, o.mm.ca = w.kv;
             o.mm.b = w.mm.a, o.mm.ldb = w.mm.lda, o.mm.kb = p->nq;
             o.mul = p->scale, o.norm = norm, o.dtype = p->dtype, o.splits = 1, o.add = 0;
             o.out = (char*)d_out_vector_grad + at * vector_grad_stride * size_of(p->dtype), o.ldo = vector_grad_stride;
         }
-        CHK(jvk_sx_grads(d_out_query_grad ? &q : nullptr, d_out_vector_grad ? &o : nullptr, plan.large, s));
+        CHK(jvk_sx_grads(d_out_query_grad ? &q : nullptr, d_out_vector_grad ? &o : nullptr, f32, plan.large, s));
     }
     if (d_out_query_grad) {
-        const int splits = (int)std::min<int64_t>(plan.splits_q, up(std::min<int64_t>(plan.rows_b, p->n), 64) / 64 * plan.segs);
+        const int splits = std::min(plan.splits_q, splits_of(plan, std::min<int64_t>(plan.rows_b, p->n), f32));
         CHK(jvk_sx_finish((const float*)(ws + plan.off_slab), splits, p->nq, p->d, plan.dp, w.rest, query, p->vectors, p->vector_stride, p->scale, norm, d_out_query_grad,
                           p->dtype, query_grad_stride, s));
     }

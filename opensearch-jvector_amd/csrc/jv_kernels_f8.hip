@@ -141,7 +141,7 @@ template <int TY>
 static hipError_t score(const JvMmOut& a, hipStream_t s) {
     const int64_t large = (int64_t)((a.mm.M + 255) / 256) * ((a.mm.N + 255) / 256);
     if (a.mm.M > 64 && large >= 192 && a.mm.N >= 16) return mm_out_pipe<TY>(a, s);
-    if (a.mm.M > 64) return mm_out_tile<TY, 2, 2, 2, 2>(a, s);
-    return a.mm.M > 32 ? mm_out_tile<TY, 2, 1, 1, 4>(a, s) : mm_out_tile<TY, 1, 1, 1, 4>(a, s);
+    if (a.mm.M > 64) return mm_out_tile<Tile<TY, 2, 2, 2, 2>>(a, s);
+    return a.mm.M > 32 ? mm_out_tile<Tile<TY, 2, 1, 1, 4>>(a, s) : mm_out_tile<Tile<TY, 1, 1, 1, 4>>(a, s);
 }
 extern "C" hipError_t jvk_f8_score(const JvMmOut* a, hipStream_t s) { return a->dtype == 0 ? score<F8W>(*a, s) : score<F8>(*a, s); }

@@ -217,9 +217,9 @@ __global__ __launch_bounds__(512) void jvs_loss_pipe_kernel(const JvSxLoss a) {
     write_partials<P::TM, 4, 4>(a, smem, m0, split, threadIdx.x >> 7, [](int m) { return P::row(m); }, top, sum);
 }
 
-template <int MT, int NT, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN) void jvs_loss_tile_kernel(const JvSxLoss a) {
-    using T = Tile<BF16, MT, NT, WM, WN>;
+template <class T, int WM, int WN>
+__global__ __launch_bounds__(T::THREADS) void jvs_loss_tile_kernel(const JvSxLoss a) {
+    constexpr int MT = T::MT, NT = T::NT;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int panels = (a.mm.M + T::TM - 1) / T::TM, tiles = (a.mm.N + T::TN - 1) / T::TN;
     const Share share(panels * a.splits);
@@ -231,7 +231,7 @@ __global__ __launch_bounds__(64 * WM * WN) void jvs_loss_tile_kernel(const JvSxL
     for (int m = 0; m < MT; m++) top[m] = -__builtin_inff(), sum[m] = 0.0f;
     for (int t = split; t < tiles; t += a.splits) {
         f32x16 acc[MT][NT];
-        T::run(a.mm, m0, t * T::TN, 0, (a.mm.kph >> 1) * a.mm.segs, smem, acc);
+        T::run(a.mm, m0, t * T::TN, 0, T::steps(a.mm), smem, acc);
         add_tile<T>(acc, a.c, a.mm.N - t * T::TN, top, sum);
     }
     write_partials<T::TM, MT, WN>(a, smem, m0, split, (threadIdx.x >> 6) / WM, [](int m) { return T::row(m); }, top, sum);
@@ -249,25 +249,39 @@ extern "C" int jvk_sx_loss_plan(int nq, int64_t rows, int* tile) {
     return (int)std::min(std::max<int64_t>(full / panels, 1), tiles);
 }
 
-template <int MT, int NT, int WM, int WN>
+template <class T, int WM, int WN>
 static hipError_t loss_tile(const JvSxLoss& a, hipStream_t s) {
-    using T = Tile<BF16, MT, NT, WM, WN>;
-    hipError_t e = hipFuncSetAttribute((const void*)jvs_loss_tile_kernel<MT, NT, WM, WN>, hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS);
+    hipError_t e = lds_of(jvs_loss_tile_kernel<T, WM, WN>, T::LDS);
     if (e != hipSuccess) return e;
     const int64_t all = (int64_t)((a.mm.M + T::TM - 1) / T::TM) * a.splits;
-    jvs_loss_tile_kernel<MT, NT, WM, WN><<<(unsigned)((all + 7) / 8 * 8), T::THREADS, T::LDS, s>>>(a);
+    if (all > 0x7ffffff0ll) return hipErrorInvalidValue;
+    jvs_loss_tile_kernel<T, WM, WN><<<(unsigned)((all + 7) / 8 * 8), T::THREADS, T::LDS, s>>>(a);
     return hipGetLastError();
 }
-extern "C" hipError_t jvk_sx_loss(const JvSxLoss* a, hipStream_t s) {
+// rows that copies of 16 B a lane can take: aligned, and ending with 16 B
+static bool wide32(const void* p, int64_t ld, int cols) { return (uintptr_t)p % 16 == 0 && ld % 16 == 0 && cols % 4 == 0; }
+
+extern "C" hipError_t jvk_sx_loss(const JvSxLoss* a, int f32, hipStream_t s) {
     using P = Pipe<BF16>;
     if (a->mm.N <= 0 || a->mm.M <= 0) return hipSuccess;
     if (a->splits < 1) return hipErrorInvalidValue;
-    if (a->tile == 128) return loss_tile<2, 2, 2, 2>(*a, s);
-    if (a->tile == 64) return loss_tile<2, 1, 1, 4>(*a, s);
-    if (a->tile == 32) return loss_tile<1, 1, 1, 4>(*a, s);
-    hipError_t e = hipFuncSetAttribute((const void*)jvs_loss_pipe_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, P::LDS);
+    if (f32) {
+        if (wide32(a->mm.a, a->mm.lda, a->mm.k) && wide32(a->mm.b, a->mm.ldb, a->mm.k)) {
+            if (a->tile == 128) return loss_tile<Tile32<2, 2, 2, 2, false, false, false, false>, 2, 2>(*a, s);
+            if (a->tile == 64) return loss_tile<Tile32<2, 1, 1, 4, false, false, false, false>, 1, 4>(*a, s);
+            return loss_tile<Tile32<1, 1, 1, 4, false, false, false, false>, 1, 4>(*a, s);
+        }
+        if (a->tile == 128) return loss_tile<Tile32<2, 2, 2, 2, false, false, true, true>, 2, 2>(*a, s);
+        if (a->tile == 64) return loss_tile<Tile32<2, 1, 1, 4, false, false, true, true>, 1, 4>(*a, s);
+        return loss_tile<Tile32<1, 1, 1, 4, false, false, true, true>, 1, 4>(*a, s);
+    }
+    if (a->tile == 128) return loss_tile<Tile<BF16, 2, 2, 2, 2>, 2, 2>(*a, s);
+    if (a->tile == 64) return loss_tile<Tile<BF16, 2, 1, 1, 4>, 1, 4>(*a, s);
+    if (a->tile == 32) return loss_tile<Tile<BF16, 1, 1, 1, 4>, 1, 4>(*a, s);
+    hipError_t e = lds_of(jvs_loss_pipe_kernel, P::LDS);
     if (e != hipSuccess) return e;
     const int64_t all = (int64_t)((a->mm.M + P::TM - 1) / P::TM) * a->splits;
+    if (all > 0x7ffffff0ll) return hipErrorInvalidValue;
     jvs_loss_pipe_kernel<<<(unsigned)((all + 7) / 8 * 8), P::THREADS, P::LDS, s>>>(*a);
     return hipGetLastError();
 }
@@ -350,7 +364,7 @@ __global__ __launch_bounds__(512) void jvs_weights_kernel(const JvSxWeights a) {
             }
             int stores = 0;
             for (int k = 0; k < a.planes; k++) {
-                stores = P::write_bf16(smem, a.g + (int64_t)k * a.kv, (int64_t)a.planes * a.kv, true, w, padded, a.kv, [&](int m, int n, int e) { return acc[m][n][e]; });
+                stores = P::write_bf16(smem, (uint16_t*)a.g + (int64_t)k * a.kv, (int64_t)a.planes * a.kv, true, w, padded, a.kv, [&](int m, int n, int e) { return acc[m][n][e]; });
                 if (a.planes > 1) {
 #pragma unroll
                     for (int m = 0; m < 4; m++)
@@ -365,26 +379,32 @@ __global__ __launch_bounds__(512) void jvs_weights_kernel(const JvSxWeights a) {
 }
 
 // the same on small tiles, one a workgroup
-template <int MT, int NT, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN) void jvs_weights_tile_kernel(const JvSxWeights a) {
-    using T = Tile<BF16, MT, NT, WM, WN>;
+template <class T>
+__global__ __launch_bounds__(T::THREADS) void jvs_weights_tile_kernel(const JvSxWeights a) {
+    constexpr int MT = T::MT, NT = T::NT;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    const int tm = (a.mm.M + T::TM - 1) / T::TM, tn = (a.mm.N + T::TN - 1) / T::TN;
     const int padded = (a.mm.M + 63) / 64 * 64;
     int m0, n0;
-    band_order(xcd_order(blockIdx.x, gridDim.x), tm, tn, m0, n0);
+    band_order(xcd_order(blockIdx.x, gridDim.x), (padded + T::TM - 1) / T::TM, (a.mm.N + T::TN - 1) / T::TN, m0, n0);
     m0 *= T::TM, n0 *= T::TN;
     f32x16 acc[MT][NT];
-    T::run(a.mm, m0, n0, 0, (a.mm.kph >> 1) * a.mm.segs, smem, acc);
+    T::run(a.mm, m0, n0, 0, T::steps(a.mm), smem, acc);
 #pragma unroll
     for (int m = 0; m < MT; m++) {
         const int r = m0 + T::row(m);
         JvSxQuery q = {0.0f, 0.0f, -1, 0};
         if (r < a.mm.M) q = a.query[r];
         weigh<T>(acc[m], q, a.c, a.mm.N - n0, q.target >= 0 ? (int)(q.target - a.row0) - n0 : -1, a.planes == 1, a.rest + r);
-        // (rows of 32: those behind the padded ones only where one tile has more rows than there are)
-        for (int k = 0; k < a.planes; k++) {
-            uint16_t* row = a.g + ((int64_t)r * a.planes + k) * a.kv;
+        if (a.planes == 0) {
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int g = 0; g < 4; g++) {
+                    const int col = n0 + T::col(n, 4 * g);
+                    if (r < padded && col < a.kv)   // (kv is a multiple of 64)
+                        *(f32x4*)((float*)a.g + (int64_t)r * a.kv + col) = (f32x4){acc[m][n][4 * g], acc[m][n][4 * g + 1], acc[m][n][4 * g + 2], acc[m][n][4 * g + 3]};
+                }
+        } else {   // (one plane: three only come with the large tiles)
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -392,68 +412,77 @@ __global__ __launch_bounds__(64 * WM * WN) void jvs_weights_tile_kernel(const Jv
                     const int col = n0 + T::col(n, 4 * g);
                     bf16x4 v;
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        v[e] = (__bf16)acc[m][n][4 * g + e];
-                        acc[m][n][4 * g + e] -= (float)v[e];
-                    }
-                    if (r < padded && col < a.kv) *(bf16x4*)(row + col) = v;   // (kv is a multiple of 64)
+                    for (int e = 0; e < 4; e++) v[e] = (__bf16)acc[m][n][4 * g + e];
+                    if (r < padded && col < a.kv) *(bf16x4*)((uint16_t*)a.g + (int64_t)r * a.kv + col) = v;
                 }
         }
     }
 }
 
-template <int MT, int NT, int WM, int WN>
+template <class T>
 static hipError_t weights_tile(const JvSxWeights& a, hipStream_t s) {
-    using T = Tile<BF16, MT, NT, WM, WN>;
-    // (tiles cover the 64 padded queries: a tile of 32 needs two of them)
     const int64_t all = (int64_t)(((a.mm.M + 63) / 64 * 64 + T::TM - 1) / T::TM) * ((a.mm.N + T::TN - 1) / T::TN);
     if (all > 0x7fffffffll) return hipErrorInvalidValue;
-    hipError_t e = hipFuncSetAttribute((const void*)jvs_weights_tile_kernel<MT, NT, WM, WN>, hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS);
+    hipError_t e = lds_of(jvs_weights_tile_kernel<T>, T::LDS);
     if (e != hipSuccess) return e;
-    jvs_weights_tile_kernel<MT, NT, WM, WN><<<(unsigned)all, T::THREADS, T::LDS, s>>>(a);
+    jvs_weights_tile_kernel<T><<<(unsigned)all, T::THREADS, T::LDS, s>>>(a);
     return hipGetLastError();
 }
 
 extern "C" hipError_t jvk_sx_weights(const JvSxWeights* a, int large, hipStream_t s) {
     using P = Pipe<BF16>;
     if (a->mm.M <= 0 || a->mm.N <= 0) return hipSuccess;
-    if (!large) return a->mm.M > 64 ? weights_tile<2, 2, 2, 2>(*a, s) : weights_tile<2, 1, 1, 4>(*a, s);
+    if (a->planes == 0) {
+        if (wide32(a->mm.a, a->mm.lda, a->mm.k) && wide32(a->mm.b, a->mm.ldb, a->mm.k))
+            return a->mm.M > 64 ? weights_tile<Tile32<2, 2, 2, 2, false, false, false, false>>(*a, s) : weights_tile<Tile32<2, 1, 1, 4, false, false, false, false>>(*a, s);
+        return a->mm.M > 64 ? weights_tile<Tile32<2, 2, 2, 2, false, false, true, true>>(*a, s) : weights_tile<Tile32<2, 1, 1, 4, false, false, true, true>>(*a, s);
+    }
+    if (!large) return a->mm.M > 64 ? weights_tile<Tile<BF16, 2, 2, 2, 2>>(*a, s) : weights_tile<Tile<BF16, 2, 1, 1, 4>>(*a, s);
     const int64_t all = (int64_t)((a->mm.M + P::TM - 1) / P::TM) * ((a->mm.N + P::TN - 1) / P::TN);
     if (all > 0x7fffffffll) return hipErrorInvalidValue;
-    hipError_t e = hipFuncSetAttribute((const void*)jvs_weights_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, P::LDS);
+    hipError_t e = lds_of(jvs_weights_kernel, P::LDS);
     if (e != hipSuccess) return e;
     jvs_weights_kernel<<<(unsigned)(all < 256 ? (all + 7) / 8 * 8 : 256), P::THREADS, P::LDS, s>>>(*a);
     return hipGetLastError();
 }
 
 // dq = G V: G's rows are queries, V's rows are k.  dv = G^T Q: the rows of both are k.  On small tiles both share a launch.
+template <class TQ, class TV>
 __global__ __launch_bounds__(256) void jvs_grads_tile_kernel(const JvMmOut q, const JvMmOut v, int first) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    if ((int)blockIdx.x < first) out_tile<BF16, 2, 2, 2, 2, false, true>(q, blockIdx.x, smem);
-    else out_tile<BF16, 2, 2, 2, 2, true, true>(v, blockIdx.x - first, smem);
+    if ((int)blockIdx.x < first) out_tile<TQ>(q, blockIdx.x, smem);
+    else out_tile<TV>(v, blockIdx.x - first, smem);
+}
+template <class TQ, class TV>
+static hipError_t grads_tile(const JvMmOut* q, const JvMmOut* v, bool f32, hipStream_t s) {
+    static_assert(TQ::LDS == TV::LDS && TQ::THREADS == 256 && TV::THREADS == 256);
+    auto steps = [&](const JvMmOut& a) { return f32 ? (a.mm.k + 31) / 32 : (a.mm.kph >> 1) * a.mm.segs; };
+    const int64_t nq = q ? tile_count(*q, TQ::TM, TQ::TN, steps(*q)) : 0, nv = v ? tile_count(*v, TV::TM, TV::TN, steps(*v)) : 0;
+    if (nq < 0 || nv < 0 || nq + nv > 0x7fffffffll) return hipErrorInvalidValue;
+    if (nq + nv == 0) return hipSuccess;
+    hipError_t e = lds_of(jvs_grads_tile_kernel<TQ, TV>, TQ::LDS);
+    if (e != hipSuccess) return e;
+    jvs_grads_tile_kernel<TQ, TV><<<(unsigned)(nq + nv), 256, TQ::LDS, s>>>(q ? *q : JvMmOut{}, v ? *v : JvMmOut{}, (int)nq);
+    return hipGetLastError();
 }
 
-// k ranges of dq: with the large tiles once around the CUs, eight phases in each at least; with the small ones twice, four steps at least
-extern "C" int jvk_sx_grad_splits(int nq, int d, int64_t rows, int segs, int large) {
+// k ranges of dq: with the large tiles once around the CUs, with the small ones twice; four steps in each at least
+extern "C" int jvk_sx_grad_splits(int nq, int d, int64_t rows, int f32, int large) {
     const int t = large ? 256 : 128, full = large ? 256 : 512;
-    const int64_t tiles = std::max<int64_t>((nq + t - 1) / t, 1) * ((d + t - 1) / t), steps = (rows + 63) / 64 * segs;
+    const int64_t tiles = std::max<int64_t>((nq + t - 1) / t, 1) * ((d + t - 1) / t), steps = (rows + 63) / 64 * (f32 ? large ? 6 : 2 : 1);
     return (int)std::max<int64_t>(std::min<int64_t>(full / tiles, steps / 4), 1);
 }
-extern "C" hipError_t jvk_sx_grads(const JvMmOut* q, const JvMmOut* v, int large, hipStream_t s) {
+extern "C" hipError_t jvk_sx_grads(const JvMmOut* q, const JvMmOut* v, int f32, int large, hipStream_t s) {
     if (large) {
         hipError_t e = hipSuccess;
         if (q) e = mm_out_pipe<BF16, false, true>(*q, s);
         if (v && e == hipSuccess) e = mm_out_pipe<BF16, true, true>(*v, s);
         return e;
     }
-    using T = Tile<BF16, 2, 2, 2, 2>;
-    const int64_t nq = q ? tile_count(*q, T::TM, T::TN) : 0, nv = v ? tile_count(*v, T::TM, T::TN) : 0;
-    if (nq < 0 || nv < 0 || nq + nv > 0x7fffffffll) return hipErrorInvalidValue;
-    if (nq + nv == 0) return hipSuccess;
-    hipError_t e = hipFuncSetAttribute((const void*)jvs_grads_tile_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS);
-    if (e != hipSuccess) return e;
-    jvs_grads_tile_kernel<<<(unsigned)(nq + nv), T::THREADS, T::LDS, s>>>(q ? *q : JvMmOut{}, v ? *v : JvMmOut{}, (int)nq);
-    return hipGetLastError();
+    if (!f32) return grads_tile<Tile<BF16, 2, 2, 2, 2, false, true>, Tile<BF16, 2, 2, 2, 2, true, true>>(q, v, false, s);
+    if ((!q || wide32(q->mm.b, q->mm.ldb, q->mm.cb)) && (!v || wide32(v->mm.b, v->mm.ldb, v->mm.cb)))
+        return grads_tile<Tile32<2, 2, 2, 2, false, true, false, false>, Tile32<2, 2, 2, 2, true, true, false, false>>(q, v, true, s);
+    return grads_tile<Tile32<2, 2, 2, 2, false, true, false, true>, Tile32<2, 2, 2, 2, true, true, false, true>>(q, v, true, s);
 }
 
 // partial sums -> the queries' gradient, and what G lacked at the target: one wave a row, four columns a lane

@@ -54,14 +54,16 @@ __device__ __forceinline__ s16x4 read_across(const unsigned char* p) {   // 16 l
 // The product for small shapes: MT x NT accumulators of 32 x 32 for each of WM x WN waves, two steps of k in LDS, several workgroups a CU.
 // TA / TB: an operand with k across its rows (bf16): 64 rows of TM / TN columns a step.  Four rows of 64 B are read at a time: piece p of row k
 // lies at p ^ (swirl << 2) so that they are the four quarters of a 256-B bank row.
-template <int TY, int MT, int NT, int WM, int WN, bool TA = false, bool TB = false>
+template <int TY, int MT_, int NT_, int WM, int WN, bool TA = false, bool TB = false>
 struct Tile {
+    static constexpr int MT = MT_, NT = NT_;
     static constexpr int TM = 32 * MT * WM, TN = 32 * NT * WN, WAVES = WM * WN, THREADS = 64 * WAVES;
     static constexpr int GA = TM / 8, GB = TN / 8;                               // 8-row groups
     static constexpr int CA = GA / WAVES, CB = GB / WAVES, PER = CA + CB;        // copies of one wave a step
     static constexpr int BUF = (GA + GB) * GROUP, LDS = 2 * BUF;
     static_assert(GA % WAVES == 0 && GB % WAVES == 0, "every wave copies the same number of groups of each operand");
     static_assert(TY == BF16 || (!TA && !TB), "8-bit operands have k along their rows");
+    static __device__ __forceinline__ int steps(const JvMm& a) { return (a.kph >> 1) * a.segs; }
 
     template <int PIECES>   // 16-B pieces of a row
     static __device__ __forceinline__ int swirl(int k) {
@@ -75,7 +77,7 @@ struct Tile {
         return __builtin_bit_cast(bf16x8, __builtin_shufflevector(read_across(at(k)), read_across(at(k + 4)), 0, 1, 2, 3, 4, 5, 6, 7));
     }
 
-    // C tile at (m0, n0), steps [k0, k1) of the segs * kph / 2 in all.  Rows behind the operands' last are read as their last.
+    // C tile at (m0, n0), steps [k0, k1).  Rows behind the operands' last are read as their last.
     static __device__ __forceinline__ void run(const JvMm& a, int m0, int n0, int k0, int k1, unsigned char* smem, f32x16 (&acc)[MT][NT]) {
         const int nk = a.kph >> 1;   // steps of a segment
         const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;

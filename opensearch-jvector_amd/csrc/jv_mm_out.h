@@ -1,6 +1,11 @@
 // jv_mm_out.h — matrix products written as they are, on the tiles of jv_mm.h (small) and jv_pipe.h (large).
 #pragma once
+#include <mutex>
+#include <set>
+#include <utility>
+
 #include "jv_pipe.h"
+#include "jv_tile32.h"
 
 namespace jvmm {
 
@@ -9,6 +14,21 @@ __device__ __forceinline__ void band_order(int L, int tm, int tn, int& m, int& n
     const int band = L / (8 * tn), in = L - band * 8 * tn, high = min(8, tm - band * 8);
     n = in / high;
     m = band * 8 + in - n * high;
+}
+
+// Lets a kernel have that much LDS, once for each device (a second thread that gets here meanwhile does the same again).
+template <class... Args>
+static hipError_t lds_of(void (*kernel)(Args...), int bytes) {
+    static std::mutex lock;
+    static std::set<std::pair<const void*, int>> known;
+    int device = 0;
+    hipError_t e = hipGetDevice(&device);
+    if (e != hipSuccess) return e;
+    std::lock_guard<std::mutex> hold(lock);
+    if (known.count({(const void*)kernel, device})) return hipSuccess;
+    e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == hipSuccess) known.insert({(const void*)kernel, device});
+    return e;
 }
 
 template <int TY, bool TA, bool TB>
@@ -45,7 +65,7 @@ static hipError_t mm_out_pipe(const JvMmOut& a, hipStream_t s) {
     if (a.mm.M <= 0 || a.mm.N <= 0) return hipSuccess;
     const int64_t all = (int64_t)((a.mm.M + P::TM - 1) / P::TM) * ((a.mm.N + P::TN - 1) / P::TN) * a.splits;
     if (all > 0x7fffffffll || a.splits < 1 || a.splits > a.mm.kph * a.mm.segs) return hipErrorInvalidValue;
-    hipError_t e = hipFuncSetAttribute((const void*)jvm_out_pipe_kernel<TY, TA, TB>, hipFuncAttributeMaxDynamicSharedMemorySize, P::LDS);
+    hipError_t e = lds_of(jvm_out_pipe_kernel<TY, TA, TB>, P::LDS);
     if (e != hipSuccess) return e;
     jvm_out_pipe_kernel<TY, TA, TB><<<(unsigned)(all < 256 ? (all + 7) / 8 * 8 : 256), P::THREADS, P::LDS, s>>>(a);
     return hipGetLastError();
@@ -58,15 +78,15 @@ __device__ __forceinline__ int xcd_order(int i, int n) {
 }
 
 // workgroup `i` of tiles * splits: one tile over one k range
-template <int TY, int MT, int NT, int WM, int WN, bool TA, bool TB>
+template <class T>
 __device__ __forceinline__ void out_tile(const JvMmOut& a, int i, unsigned char* smem) {
-    using T = Tile<TY, MT, NT, WM, WN, TA, TB>;
+    constexpr int MT = T::MT, NT = T::NT;
     const int tm = (a.mm.M + T::TM - 1) / T::TM, tn = (a.mm.N + T::TN - 1) / T::TN, tiles = tm * tn;
     int L = xcd_order(i, tiles * a.splits), part = 0, m0, n0;
     if (a.splits > 1) part = L / tiles, L -= part * tiles;
     band_order(L, tm, tn, m0, n0);
     m0 *= T::TM, n0 *= T::TN;
-    const int steps = (a.mm.kph >> 1) * a.mm.segs;
+    const int steps = T::steps(a.mm);
     f32x16 acc[MT][NT];
     T::run(a.mm, m0, n0, (int)((int64_t)steps * part / a.splits), (int)((int64_t)steps * (part + 1) / a.splits), smem, acc);
     const float mul = a.norm ? a.mul * *a.norm : a.mul;
@@ -108,28 +128,27 @@ __device__ __forceinline__ void out_tile(const JvMmOut& a, int i, unsigned char*
     }
 }
 
-template <int TY, int MT, int NT, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN) void jvm_out_tile_kernel(const JvMmOut a) {
+template <class T>
+__global__ __launch_bounds__(T::THREADS) void jvm_out_tile_kernel(const JvMmOut a) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    out_tile<TY, MT, NT, WM, WN, false, false>(a, blockIdx.x, smem);
+    out_tile<T>(a, blockIdx.x, smem);
 }
 
 // workgroups of a product on tiles of TM x TN, 0 = none, negative = more than a launch takes
-static inline int64_t tile_count(const JvMmOut& a, int TM, int TN) {
+static inline int64_t tile_count(const JvMmOut& a, int TM, int TN, int steps) {
     if (a.mm.M <= 0 || a.mm.N <= 0) return 0;
-    if (a.splits < 1 || a.splits > (a.mm.kph >> 1) * a.mm.segs || (a.dtype != 0 && a.splits > 1)) return -1;
+    if (a.splits < 1 || a.splits > steps || (a.dtype != 0 && a.splits > 1)) return -1;
     const int64_t all = (int64_t)((a.mm.M + TM - 1) / TM) * ((a.mm.N + TN - 1) / TN) * a.splits;
     return all > 0x7fffffffll ? -1 : all;
 }
 
-template <int TY, int MT, int NT, int WM, int WN>
+template <class T>
 static hipError_t mm_out_tile(const JvMmOut& a, hipStream_t s) {
-    using T = Tile<TY, MT, NT, WM, WN>;
-    const int64_t all = tile_count(a, T::TM, T::TN);
+    const int64_t all = tile_count(a, T::TM, T::TN, (a.mm.kph >> 1) * a.mm.segs);
     if (all <= 0) return all ? hipErrorInvalidValue : hipSuccess;
-    hipError_t e = hipFuncSetAttribute((const void*)jvm_out_tile_kernel<TY, MT, NT, WM, WN>, hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS);
+    hipError_t e = lds_of(jvm_out_tile_kernel<T>, T::LDS);
     if (e != hipSuccess) return e;
-    jvm_out_tile_kernel<TY, MT, NT, WM, WN><<<(unsigned)all, T::THREADS, T::LDS, s>>>(a);
+    jvm_out_tile_kernel<T><<<(unsigned)all, T::THREADS, T::LDS, s>>>(a);
     return hipGetLastError();
 }
 

@@ -12,6 +12,7 @@ struct JvMm {
     const char *a, *b;
     int64_t lda, ldb;
     int32_t M, N;
+    int32_t k;               // components (float32 as it lies, jv_tile32.h: nothing is padded there, and planes and segments do not count)
     int32_t kph;             // phases of one segment
     int32_t segs;            // 1 (bf16, e4m3) or 6 (float32)
     int64_t plane_a, plane_b;  // bytes from plane to plane
@@ -52,8 +53,8 @@ struct JvSxWeights {
     float c;
     int64_t row0;          // first row of this piece
     const JvSxQuery* query;
-    int32_t planes;        // 1 or 3
-    uint16_t* g;
+    int32_t planes;        // 1 or 3, or 0: float32 as it is
+    void* g;                 // (planes = 0: float32)
     int32_t kv;            // N padded to 64
     float* rest;           // [M] bf16: what G's entry at the target lacks of its float32 value
 };
@@ -85,13 +86,13 @@ hipError_t jvk_f8_score(const JvMmOut* a, hipStream_t s);
 
 hipError_t jvk_sx_prepare(const JvSxPrepare* a, hipStream_t s);
 int jvk_sx_loss_plan(int nq, int64_t rows, int* tile);   // splits, and the queries of a tile
-hipError_t jvk_sx_loss(const JvSxLoss* a, hipStream_t s);
+hipError_t jvk_sx_loss(const JvSxLoss* a, int f32, hipStream_t s);   // f32: operands are float32 as they lie
 hipError_t jvk_sx_join(const float* part, int splits, int nq, const void* q, int64_t q_stride, const void* v, int64_t v_stride, int dtype, int d,
                        const int32_t* targets, int64_t n, float scale, float* loss, float* lse, hipStream_t s);
-hipError_t jvk_sx_weights(const JvSxWeights* a, int large, hipStream_t s);
+hipError_t jvk_sx_weights(const JvSxWeights* a, int large, hipStream_t s);   // (planes = 0: float32 as it lies)
 // dq = G V and dv = G^T Q (nullptr: not asked for)
-int jvk_sx_grad_splits(int nq, int d, int64_t rows, int segs, int large);
-hipError_t jvk_sx_grads(const JvMmOut* q, const JvMmOut* v, int large, hipStream_t s);
+int jvk_sx_grad_splits(int nq, int d, int64_t rows, int f32, int large);
+hipError_t jvk_sx_grads(const JvMmOut* q, const JvMmOut* v, int f32, int large, hipStream_t s);
 int jvk_sx_large(int nq, int64_t rows);   // whether a piece of the rows takes the large tiles
 hipError_t jvk_sx_finish(const float* slab, int splits, int64_t rows, int d, int64_t lds, const float* rest, const JvSxQuery* query, const void* v, int64_t v_stride,
                          float mul, const float* norm, void* out, int dtype, int64_t ldo, hipStream_t s);
