@@ -137,11 +137,15 @@ extern "C" hipError_t jvk_f8_decode(const uint8_t* codes, const uint8_t* scales,
 
 // bf16 scores keep 8 bits: the 8-bit unit's sums are enough.  float32 scores take the bf16 unit (jv_mm.h).  The large tiles where they fill the
 // chip, else tiles of as few queries as there are.
+template <int TY, int NS>
+static hipError_t score_small(const JvMmOut& a, hipStream_t s) {
+    if (a.mm.M > 64) return mm_out_tile<Tile<TY, 2, 2, 2, 2, NS>>(a, s);
+    return a.mm.M > 32 ? mm_out_tile<Tile<TY, 2, 1, 1, 4, NS>>(a, s) : mm_out_tile<Tile<TY, 1, 1, 1, 4, NS>>(a, s);
+}
 template <int TY>
 static hipError_t score(const JvMmOut& a, hipStream_t s) {
-    const int64_t large = (int64_t)((a.mm.M + 255) / 256) * ((a.mm.N + 255) / 256);
-    if (a.mm.M > 64 && large >= 192 && a.mm.N >= 16) return mm_out_pipe<TY>(a, s);
-    if (a.mm.M > 64) return mm_out_tile<Tile<TY, 2, 2, 2, 2>>(a, s);
-    return a.mm.M > 32 ? mm_out_tile<Tile<TY, 2, 1, 1, 4>>(a, s) : mm_out_tile<Tile<TY, 1, 1, 1, 4>>(a, s);
+    if (a.mm.M > 64 && (int64_t)((a.mm.M + 255) / 256) * ((a.mm.N + 255) / 256) >= 192 && a.mm.N >= 16) return mm_out_pipe<TY>(a, s);
+    const int64_t small = (int64_t)(a.mm.M > 64 ? (a.mm.M + 127) / 128 : 1) * ((a.mm.N + 127) / 128);
+    return small <= 256 ? score_small<TY, 4>(a, s) : score_small<TY, 2>(a, s);
 }
 extern "C" hipError_t jvk_f8_score(const JvMmOut* a, hipStream_t s) { return a->dtype == 0 ? score<F8W>(*a, s) : score<F8>(*a, s); }

@@ -261,23 +261,31 @@ static hipError_t loss_tile(const JvSxLoss& a, hipStream_t s) {
 // rows that copies of 16 B a lane can take: aligned, and ending with 16 B
 static bool wide32(const void* p, int64_t ld, int cols) { return (uintptr_t)p % 16 == 0 && ld % 16 == 0 && cols % 4 == 0; }
 
+template <int NS>
+static hipError_t loss_small(const JvSxLoss& a, bool f32, bool wide, hipStream_t s) {
+    if (!f32) {
+        if (a.tile == 128) return loss_tile<Tile<BF16, 2, 2, 2, 2, NS>, 2, 2>(a, s);
+        return a.tile == 64 ? loss_tile<Tile<BF16, 2, 1, 1, 4, NS>, 1, 4>(a, s) : loss_tile<Tile<BF16, 1, 1, 1, 4, NS>, 1, 4>(a, s);
+    }
+    if (wide) {
+        if (a.tile == 128) return loss_tile<Tile32<2, 2, 2, 2, NS, false, false, false, false>, 2, 2>(a, s);
+        if (a.tile == 64) return loss_tile<Tile32<2, 1, 1, 4, NS, false, false, false, false>, 1, 4>(a, s);
+        return loss_tile<Tile32<1, 1, 1, 4, NS, false, false, false, false>, 1, 4>(a, s);
+    }
+    if (a.tile == 128) return loss_tile<Tile32<2, 2, 2, 2, NS, false, false, true, true>, 2, 2>(a, s);
+    if (a.tile == 64) return loss_tile<Tile32<2, 1, 1, 4, NS, false, false, true, true>, 1, 4>(a, s);
+    return loss_tile<Tile32<1, 1, 1, 4, NS, false, false, true, true>, 1, 4>(a, s);
+}
+
 extern "C" hipError_t jvk_sx_loss(const JvSxLoss* a, int f32, hipStream_t s) {
     using P = Pipe<BF16>;
     if (a->mm.N <= 0 || a->mm.M <= 0) return hipSuccess;
     if (a->splits < 1) return hipErrorInvalidValue;
-    if (f32) {
-        if (wide32(a->mm.a, a->mm.lda, a->mm.k) && wide32(a->mm.b, a->mm.ldb, a->mm.k)) {
-            if (a->tile == 128) return loss_tile<Tile32<2, 2, 2, 2, false, false, false, false>, 2, 2>(*a, s);
-            if (a->tile == 64) return loss_tile<Tile32<2, 1, 1, 4, false, false, false, false>, 1, 4>(*a, s);
-            return loss_tile<Tile32<1, 1, 1, 4, false, false, false, false>, 1, 4>(*a, s);
-        }
-        if (a->tile == 128) return loss_tile<Tile32<2, 2, 2, 2, false, false, true, true>, 2, 2>(*a, s);
-        if (a->tile == 64) return loss_tile<Tile32<2, 1, 1, 4, false, false, true, true>, 1, 4>(*a, s);
-        return loss_tile<Tile32<1, 1, 1, 4, false, false, true, true>, 1, 4>(*a, s);
+    if (f32 || a->tile != 256) {
+        const bool wide = f32 && wide32(a->mm.a, a->mm.lda, a->mm.k) && wide32(a->mm.b, a->mm.ldb, a->mm.k);
+        const bool few = (int64_t)((a->mm.M + a->tile - 1) / a->tile) * a->splits <= 256;
+        return few ? loss_small<4>(*a, f32, wide, s) : loss_small<2>(*a, f32, wide, s);
     }
-    if (a->tile == 128) return loss_tile<Tile<BF16, 2, 2, 2, 2>, 2, 2>(*a, s);
-    if (a->tile == 64) return loss_tile<Tile<BF16, 2, 1, 1, 4>, 1, 4>(*a, s);
-    if (a->tile == 32) return loss_tile<Tile<BF16, 1, 1, 1, 4>, 1, 4>(*a, s);
     hipError_t e = lds_of(jvs_loss_pipe_kernel, P::LDS);
     if (e != hipSuccess) return e;
     const int64_t all = (int64_t)((a->mm.M + P::TM - 1) / P::TM) * a->splits;
@@ -429,15 +437,22 @@ static hipError_t weights_tile(const JvSxWeights& a, hipStream_t s) {
     return hipGetLastError();
 }
 
+template <int NS>
+static hipError_t weights_small(const JvSxWeights& a, hipStream_t s) {
+    const bool tall = a.mm.M > 64;
+    if (a.planes != 0) return tall ? weights_tile<Tile<BF16, 2, 2, 2, 2, NS>>(a, s) : weights_tile<Tile<BF16, 2, 1, 1, 4, NS>>(a, s);
+    if (wide32(a.mm.a, a.mm.lda, a.mm.k) && wide32(a.mm.b, a.mm.ldb, a.mm.k))
+        return tall ? weights_tile<Tile32<2, 2, 2, 2, NS, false, false, false, false>>(a, s) : weights_tile<Tile32<2, 1, 1, 4, NS, false, false, false, false>>(a, s);
+    return tall ? weights_tile<Tile32<2, 2, 2, 2, NS, false, false, true, true>>(a, s) : weights_tile<Tile32<2, 1, 1, 4, NS, false, false, true, true>>(a, s);
+}
+
 extern "C" hipError_t jvk_sx_weights(const JvSxWeights* a, int large, hipStream_t s) {
     using P = Pipe<BF16>;
     if (a->mm.M <= 0 || a->mm.N <= 0) return hipSuccess;
-    if (a->planes == 0) {
-        if (wide32(a->mm.a, a->mm.lda, a->mm.k) && wide32(a->mm.b, a->mm.ldb, a->mm.k))
-            return a->mm.M > 64 ? weights_tile<Tile32<2, 2, 2, 2, false, false, false, false>>(*a, s) : weights_tile<Tile32<2, 1, 1, 4, false, false, false, false>>(*a, s);
-        return a->mm.M > 64 ? weights_tile<Tile32<2, 2, 2, 2, false, false, true, true>>(*a, s) : weights_tile<Tile32<2, 1, 1, 4, false, false, true, true>>(*a, s);
+    if (a->planes == 0 || !large) {
+        const int64_t tiles = (int64_t)(a->mm.M > 64 ? (a->mm.M + 127) / 128 : 1) * ((a->mm.N + 127) / 128);
+        return tiles <= 256 ? weights_small<4>(*a, s) : weights_small<2>(*a, s);
     }
-    if (!large) return a->mm.M > 64 ? weights_tile<Tile<BF16, 2, 2, 2, 2>>(*a, s) : weights_tile<Tile<BF16, 2, 1, 1, 4>>(*a, s);
     const int64_t all = (int64_t)((a->mm.M + P::TM - 1) / P::TM) * ((a->mm.N + P::TN - 1) / P::TN);
     if (all > 0x7fffffffll) return hipErrorInvalidValue;
     hipError_t e = lds_of(jvs_weights_kernel, P::LDS);
@@ -472,6 +487,13 @@ extern "C" int jvk_sx_grad_splits(int nq, int d, int64_t rows, int f32, int larg
     const int64_t tiles = std::max<int64_t>((nq + t - 1) / t, 1) * ((d + t - 1) / t), steps = (rows + 63) / 64 * (f32 ? large ? 6 : 2 : 1);
     return (int)std::max<int64_t>(std::min<int64_t>(full / tiles, steps / 4), 1);
 }
+template <int NS>
+static hipError_t grads_small(const JvMmOut* q, const JvMmOut* v, bool f32, hipStream_t s) {
+    if (!f32) return grads_tile<Tile<BF16, 2, 2, 2, 2, NS, false, true>, Tile<BF16, 2, 2, 2, 2, NS, true, true>>(q, v, false, s);
+    if ((!q || wide32(q->mm.b, q->mm.ldb, q->mm.cb)) && (!v || wide32(v->mm.b, v->mm.ldb, v->mm.cb)))
+        return grads_tile<Tile32<2, 2, 2, 2, NS, false, true, false, false>, Tile32<2, 2, 2, 2, NS, true, true, false, false>>(q, v, true, s);
+    return grads_tile<Tile32<2, 2, 2, 2, NS, false, true, false, true>, Tile32<2, 2, 2, 2, NS, true, true, false, true>>(q, v, true, s);
+}
 extern "C" hipError_t jvk_sx_grads(const JvMmOut* q, const JvMmOut* v, int f32, int large, hipStream_t s) {
     if (large) {
         hipError_t e = hipSuccess;
@@ -479,10 +501,10 @@ extern "C" hipError_t jvk_sx_grads(const JvMmOut* q, const JvMmOut* v, int f32, 
         if (v && e == hipSuccess) e = mm_out_pipe<BF16, true, true>(*v, s);
         return e;
     }
-    if (!f32) return grads_tile<Tile<BF16, 2, 2, 2, 2, false, true>, Tile<BF16, 2, 2, 2, 2, true, true>>(q, v, false, s);
-    if ((!q || wide32(q->mm.b, q->mm.ldb, q->mm.cb)) && (!v || wide32(v->mm.b, v->mm.ldb, v->mm.cb)))
-        return grads_tile<Tile32<2, 2, 2, 2, false, true, false, false>, Tile32<2, 2, 2, 2, true, true, false, false>>(q, v, true, s);
-    return grads_tile<Tile32<2, 2, 2, 2, false, true, false, true>, Tile32<2, 2, 2, 2, true, true, false, true>>(q, v, true, s);
+    int64_t tiles = 0;
+    for (const JvMmOut* o : {q, v})
+        if (o) tiles += (int64_t)((o->mm.M + 127) / 128) * ((o->mm.N + 127) / 128) * o->splits;
+    return tiles <= 256 ? grads_small<4>(q, v, f32, s) : grads_small<2>(q, v, f32, s);
 }
 
 // partial sums -> the queries' gradient, and what G lacked at the target: one wave a row, four columns a lane

@@ -3,7 +3,7 @@
 // A float32 product on the bf16 matrix unit: each operand is split into three bf16 parts (x = h + m + l, 24 bits) on the way from LDS into the
 // fragments, and the six pairs of parts that reach 2^-24 are multiplied, the smallest first.  Nothing is laid out beforehand: a value is read
 // from memory once for each tile that needs it, as 4 bytes, where planes in memory would be written as 6 and read as 12.  k goes by in steps
-// of 32; LDS holds two.  An operand with k along its rows (d components, any number: what lies behind is masked in the last step) is
+// of 32; LDS holds NS of them (Tile).  An operand with k along its rows (d components, any number: what lies behind is masked in the last step) is
 // staged in 8-row groups of 128 B a row as in Tile; one with k across its rows as 32 rows of TM / TN columns, where the rows 8 .. 15 and
 // 24 .. 31 have their 128-B halves of 256 B swapped, so that the two halves of a wave, eight rows apart, read different banks.
 // Copies are 16 B a lane, or 4 B (NA / NB) where a row is not 16-B aligned or ends inside 16 B.
@@ -12,13 +12,13 @@
 
 namespace jvmm {
 
-template <int MT_, int NT_, int WM, int WN, bool TA, bool TB, bool NA, bool NB>
+template <int MT_, int NT_, int WM, int WN, int NS, bool TA, bool TB, bool NA, bool NB>
 struct Tile32 {
     static constexpr int MT = MT_, NT = NT_;
     static constexpr int TM = 32 * MT * WM, TN = 32 * NT * WN, WAVES = WM * WN, THREADS = 64 * WAVES;
     static constexpr int GA = TM / 8, GB = TN / 8;                       // KB of a step
     static constexpr int CA = GA / WAVES * (NA ? 4 : 1), CB = GB / WAVES * (NB ? 4 : 1), PER = CA + CB;   // copies of one wave a step
-    static constexpr int BUF = (GA + GB) * GROUP, LDS = 2 * BUF;
+    static constexpr int BUF = (GA + GB) * GROUP, LDS = NS * BUF, AHEAD = (NS - 1) * PER < 63 ? (NS - 1) * PER : 63;
     static_assert(GA % WAVES == 0 && GB % WAVES == 0, "every wave copies the same number of groups of each operand");
     static_assert((!TA || GA >= 8) && (!TB || GB >= 8), "the swapped halves are 32 columns each");
     static __device__ __forceinline__ int steps(const JvMm& a) { return (a.k + 31) / 32; }
@@ -117,20 +117,19 @@ struct Tile32 {
             for (int n = 0; n < NT; n++)
 #pragma unroll
                 for (int e = 0; e < 16; e++) acc[m][n][e] = 0.0f;
+        // (behind the last step the last one is copied again, into a buffer that nobody reads: the number of copies under way stays the same)
         auto stage = [&](int s) {
-            unsigned char* dst = smem + (s & 1) * BUF;
+            unsigned char* dst = smem + (s - k0) % NS * BUF;
+            s = min(s, k1 - 1);
             sa.copy(a.lda, s, TA ? a.ka : a.k, dst);
             sb.copy(a.ldb, s, TB ? a.kb : a.k, dst + GA * GROUP);
         };
-        stage(k0);
+#pragma unroll
+        for (int i = 0; i < NS - 1; i++) stage(k0 + i);
         for (int s = k0; s < k1; s++) {
-            if (s + 1 < k1) {
-                stage(s + 1);
-                asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(PER) : "memory");
-            } else {
-                asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-            }
-            const unsigned char* base = smem + (s & 1) * BUF;
+            stage(s + NS - 1);
+            asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(AHEAD) : "memory");
+            const unsigned char* base = smem + (s - k0) % NS * BUF;
             const int valid = a.k - s * 32;
 #pragma unroll
             for (int kk = 0; kk < 2; kk++) {
@@ -151,6 +150,7 @@ struct Tile32 {
             // every fragment read of this buffer has returned before any wave stages into it again
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         }
+        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");   // nothing is on its way into LDS any more
     }
     // acc[m][n][e] is C[row(m)][col(n, e)] of the tile, four consecutive e are four consecutive columns
     static __device__ __forceinline__ int row(int m) { return (((threadIdx.x >> 6) % WM) * MT + m) * 32 + (threadIdx.x & 31); }

@@ -12,6 +12,8 @@ contiguous; the rows may lie any distance apart.  Not differentiable by autograd
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import binding
@@ -22,7 +24,12 @@ _LEGACY_STREAM = 1   # hipStreamLegacy: the default stream's handle (0) would ma
 
 
 def _stream(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream or _LEGACY_STREAM
+    return torch._C._cuda_getCurrentRawStream(device.index) or _LEGACY_STREAM   # (what current_stream(device).cuda_stream is, without its objects)
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(dtype: int, nq: int, n: int, d: int, flags: int) -> int:
+    return binding.softmax_workspace(binding.softmax_params(0, dtype, nq, n, d, 1.0), flags)   # (the shape alone decides)
 
 
 def _matrix(x: torch.Tensor, what: str):
@@ -95,7 +102,7 @@ def _softmax(queries, vectors, targets, scale, what, flags):
         _like(targets, queries, (nq,), torch.int32, f"{what}: targets")
     params = binding.softmax_params(queries.device.index, dtype, nq, n, d, scale, queries.data_ptr(), q_stride, vectors.data_ptr(), v_stride,
                                     0 if targets is None else targets.data_ptr())
-    params.workspace_bytes = binding.softmax_workspace(params, flags)
+    params.workspace_bytes = _workspace_bytes(dtype, nq, n, d, flags)
     workspace = torch.empty(params.workspace_bytes, dtype=torch.uint8, device=queries.device)
     params.workspace = workspace.data_ptr()
     return params, workspace
