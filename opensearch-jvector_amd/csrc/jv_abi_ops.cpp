@@ -129,14 +129,15 @@ Plan make_plan(int dtype, int nq, int64_t n, int d, uint32_t what) {
     return p;
 }
 
-// rows as a product takes them: the caller's own where they are bf16, 16-B aligned and whole steps, or float32 and the tiles small
+// rows as a product takes them: the caller's own where they are bf16, 4-B aligned and whole steps, or float32
+// of at least four components and the tiles small
 struct Rows {
     const char* p;
     int64_t stride;   // bytes
     bool ready;
 };
 Rows rows_of(const void* p, int64_t stride, int d, int dtype, bool large) {
-    const bool ready = dtype == JV_DTYPE_F32 ? !large : (uintptr_t)p % 16 == 0 && stride % 8 == 0 && d % 64 == 0;
+    const bool ready = dtype == JV_DTYPE_F32 ? !large && d >= 4 : (uintptr_t)p % 4 == 0 && stride % 2 == 0 && d % 64 == 0;
     return {(const char*)p, stride * size_of(dtype), ready};
 }
 
@@ -172,8 +173,8 @@ JvMm logits(const Plan& plan, int nq, int d) {
 }
 
 // The rows [at, at + rows) of a matrix as a product reads them: the caller's own, or where the next jvk_sx_prepare lays them out.
-void take_rows(const Rows& r, const void* p, int64_t stride, int dtype, int64_t at, int64_t rows, const Plan& plan, char* to, JvSxPrepare::Matrix* m, const char** out,
-               int64_t* ld) {
+void take_rows(const Rows& r, const void* p, int64_t stride, int dtype, int64_t at, int64_t rows, const Plan& plan, int kp, char* to,
+               JvSxPrepare::Matrix* m, const char** out, int64_t* ld) {
     if (r.ready) {
         *out = r.p + at * r.stride;
         *ld = r.stride;
@@ -183,7 +184,7 @@ void take_rows(const Rows& r, const void* p, int64_t stride, int dtype, int64_t 
     m->x = (const char*)p + at * stride * size_of(dtype);
     m->stride = stride, m->rows = rows, m->out = (uint16_t*)to;
     *out = to;
-    *ld = (int64_t)plan.P * plan.dp * 2;
+    *ld = kp == 4 ? 16 : (int64_t)plan.P * plan.dp * 2;
 }
 
 }  // namespace
@@ -264,12 +265,12 @@ int jv_softmax_loss_device(const jv_softmax_params* p, float* d_out_loss, float*
         a.c = p->scale * 1.44269504088896341f;
         a.tile = plan.tile, a.splits = p->n > 0 ? plan.splits_f : 0, a.part = (float*)(ws + plan.off_part);
         JvSxPrepare pre{};
-        pre.dtype = p->dtype, pre.d = p->d, pre.kp = plan.dp;
-        take_rows(rq, p->queries, p->query_stride, p->dtype, 0, p->nq, plan, ws + plan.off_q, &pre.m[0], &a.mm.a, &a.mm.lda);
+        pre.dtype = p->dtype, pre.d = p->d, pre.kp = f32 ? 4 : plan.dp;   // (float32 as it lies: only rows of fewer than four are laid out)
+        take_rows(rq, p->queries, p->query_stride, p->dtype, 0, p->nq, plan, pre.kp, ws + plan.off_q, &pre.m[0], &a.mm.a, &a.mm.lda);
         for (int64_t at = 0; at < p->n; at += step) {
             a.mm.N = (int)std::min<int64_t>(step, p->n - at);
             a.first = at == 0;
-            take_rows(rv, p->vectors, p->vector_stride, p->dtype, at, a.mm.N, plan, ws + plan.off_v, &pre.m[1], &a.mm.b, &a.mm.ldb);
+            take_rows(rv, p->vectors, p->vector_stride, p->dtype, at, a.mm.N, plan, pre.kp, ws + plan.off_v, &pre.m[1], &a.mm.b, &a.mm.ldb);
             CHK(jvk_sx_prepare(&pre, s));
             pre.m[0].rows = 0;
             CHK(jvk_sx_loss(&a, f32, s));
@@ -304,18 +305,20 @@ int jv_softmax_grad_device(const jv_softmax_params* p, const float* d_lse, const
     JvSxWeights w{};
     w.mm = logits(plan, p->nq, p->d);
     w.c = p->scale * 1.44269504088896341f;
-    w.planes = f32 ? 0 : plan.P, w.g = ws + plan.off_g, w.rest = (float*)(ws + plan.off_rest);
+    w.planes = f32 ? 0 : plan.P, w.g = ws + plan.off_g;
     JvSxQuery* query = (JvSxQuery*)(ws + plan.off_query);
-    w.query = query;
-    float* norm = (float*)(ws + plan.off_norm);
+    float* norm = f32 ? nullptr : (float*)(ws + plan.off_norm);   // (float32 g needs no common unit and lacks nothing at a target)
+    if (f32) w.lse = d_lse, w.w = d_loss_grad, w.targets = p->targets, w.n = p->n;
+    else w.query = query, w.rest = (float*)(ws + plan.off_rest);
+    const bool direct = f32 && plan.splits_q == 1 && plan.rows_b >= p->n;   // dq is complete at once
     JvSxPrepare pre{};
-    pre.dtype = p->dtype, pre.d = p->d, pre.kp = plan.dp;
-    pre.lse = d_lse, pre.w = d_loss_grad, pre.targets = p->targets, pre.nq = p->nq, pre.n = p->n, pre.query = query, pre.norm = norm, pre.rest = w.rest;
-    take_rows(rq, p->queries, p->query_stride, p->dtype, 0, p->nq, plan, ws + plan.off_q, &pre.m[0], &w.mm.a, &w.mm.lda);
+    pre.dtype = p->dtype, pre.d = p->d, pre.kp = f32 ? 4 : plan.dp;   // (float32 as it lies: only rows of fewer than four are laid out)
+    pre.lse = d_lse, pre.w = d_loss_grad, pre.targets = p->targets, pre.nq = p->nq, pre.n = p->n, pre.query = f32 ? nullptr : query, pre.norm = norm, pre.rest = w.rest;
+    take_rows(rq, p->queries, p->query_stride, p->dtype, 0, p->nq, plan, pre.kp, ws + plan.off_q, &pre.m[0], &w.mm.a, &w.mm.lda);
     for (int64_t at = 0; at < p->n; at += plan.rows_b) {
         const int rows = (int)std::min<int64_t>(plan.rows_b, p->n - at);
         w.mm.N = rows, w.row0 = at, w.kv = (int)up(rows, 64);
-        take_rows(rv, p->vectors, p->vector_stride, p->dtype, at, rows, plan, ws + plan.off_v, &pre.m[1], &w.mm.b, &w.mm.ldb);
+        take_rows(rv, p->vectors, p->vector_stride, p->dtype, at, rows, plan, pre.kp, ws + plan.off_v, &pre.m[1], &w.mm.b, &w.mm.ldb);
         CHK(jvk_sx_prepare(&pre, s));
         pre.m[0].rows = 0, pre.query = nullptr;
         CHK(jvk_sx_weights(&w, plan.large, s));
@@ -328,6 +331,7 @@ int jv_softmax_grad_device(const jv_softmax_params* p, const float* d_lse, const
             o.mm.b = w.mm.b, o.mm.ldb = w.mm.ldb, o.mm.kb = rows;
             o.mul = 1.0f, o.out = ws + plan.off_slab, o.ldo = plan.dp, o.add = at > 0;
             o.splits = std::min(plan.splits_q, splits_of(plan, rows, f32));   // (only the last piece can be that short: it adds to the first ranges)
+            if (direct) o.mul = p->scale, o.out = d_out_query_grad, o.ldo = query_grad_stride;
             q = o;
         }
         if (d_out_vector_grad) {   // G across times the queries: k = the queries
@@ -338,7 +342,7 @@ int jv_softmax_grad_device(const jv_softmax_params* p, const float* d_lse, const
         }
         CHK(jvk_sx_grads(d_out_query_grad ? &q : nullptr, d_out_vector_grad ? &o : nullptr, f32, plan.large, s));
     }
-    if (d_out_query_grad) {
+    if (d_out_query_grad && !direct) {
         const int splits = std::min(plan.splits_q, splits_of(plan, std::min<int64_t>(plan.rows_b, p->n), f32));
         CHK(jvk_sx_finish((const float*)(ws + plan.off_slab), splits, p->nq, p->d, plan.dp, w.rest, query, p->vectors, p->vector_stride, p->scale, norm, d_out_query_grad,
                           p->dtype, query_grad_stride, s));

@@ -80,6 +80,12 @@ __device__ __forceinline__ void pack(const JvSxPrepare::Matrix& m, int d, int kp
     }
 }
 
+__device__ __forceinline__ JvSxQuery query_of(const float* lse, const float* w, const int32_t* targets, int64_t n, int i) {
+    const int t = targets[i];
+    const bool known = t >= 0 && t < n;
+    return {known ? lse[i] * 1.44269504088896341f : 0.0f, known ? (w ? w[i] : 1.0f) : 0.0f, known ? t : -1, 0};
+}
+
 // The weights are divided by the largest of them (`norm`, multiplied back in float32 at the end): an entry of g at a target is then just
 // below 1 for the largest weight, where bf16's step is finest in relation.
 __device__ __forceinline__ void queries(const JvSxPrepare& a) {
@@ -97,13 +103,8 @@ __device__ __forceinline__ void queries(const JvSxPrepare& a) {
     const float unit = a.w && top > 0.0f && top < __builtin_inff() ? top : 1.0f;
     if (threadIdx.x == 0) *a.norm = unit;
     for (int i = threadIdx.x; i < a.nq; i += 256) {
-        const int t = a.targets[i];
-        const bool known = t >= 0 && t < a.n;
-        JvSxQuery q;
-        q.lse2 = known ? a.lse[i] * 1.44269504088896341f : 0.0f;
-        q.w = known ? (a.w ? a.w[i] : 1.0f) / unit : 0.0f;
-        q.target = known ? t : -1;
-        q.pad = 0;
+        JvSxQuery q = query_of(a.lse, a.w, a.targets, a.n, i);
+        q.w /= unit;
         a.query[i] = q;
         a.rest[i] = 0.0f;
     }
@@ -111,13 +112,20 @@ __device__ __forceinline__ void queries(const JvSxPrepare& a) {
 
 template <typename T>
 __global__ __launch_bounds__(256) void jvs_prepare_kernel(const JvSxPrepare a, int g0, int g1) {   // g0 + g1 workgroups for the matrices
+    if (a.kp == 4) {   // float32 rows of fewer than four components, as rows of four
+        for (int k = 0; k < 2; k++)
+            for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.m[k].rows * 4; i += (int64_t)gridDim.x * 256)
+                ((float*)a.m[k].out)[i] = (i & 3) < a.d ? (float)((const T*)a.m[k].x)[(i >> 2) * a.m[k].stride + (i & 3)] : 0.0f;
+        if (a.query && blockIdx.x == 0) queries(a);
+        return;
+    }
     if ((int)blockIdx.x < g0) pack<T>(a.m[0], a.d, a.kp, (int64_t)blockIdx.x * 256 + threadIdx.x, (int64_t)g0 * 256);
     else if ((int)blockIdx.x < g0 + g1) pack<T>(a.m[1], a.d, a.kp, (int64_t)((int)blockIdx.x - g0) * 256 + threadIdx.x, (int64_t)g1 * 256);
     else queries(a);
 }
 extern "C" hipError_t jvk_sx_prepare(const JvSxPrepare* a, hipStream_t s) {
     int g[2];
-    for (int k = 0; k < 2; k++) g[k] = (int)std::min<int64_t>((a->m[k].rows * (a->kp / 8) + 255) / 256, 32768);
+    for (int k = 0; k < 2; k++) g[k] = (int)std::min<int64_t>((a->m[k].rows * std::max(a->kp / 8, 1) + 255) / 256, 32768);
     const unsigned grid = (unsigned)(g[0] + g[1] + (a->query ? 1 : 0));
     if (grid == 0) return hipSuccess;
     if (a->dtype == 0) jvs_prepare_kernel<float><<<grid, 256, 0, s>>>(*a, g[0], g[1]);
@@ -241,11 +249,25 @@ __global__ __launch_bounds__(T::THREADS) void jvs_loss_tile_kernel(const JvSxLos
 static bool large(int nq, int64_t rows) { return nq > 64 && ((nq + 255) / 256) * ((rows + 255) / 256) >= 192; }
 extern "C" int jvk_sx_large(int nq, int64_t rows) { return large(nq, rows); }
 
+// Queries and rows of the tiles that a product of nq queries with `rows` rows takes:
+//   256 x 256  where they fill the chip (large);
+//   32 x 128 and 64 x 128 for up to 32 and 64 queries: the rows are streamed, and as little as possible is multiplied for nothing;
+//   128 x 128 otherwise, but where that is no more than one tile a CU 64 x 64, with four steps of k under way: the way to memory and the
+//   multiplications of one tile's steps are what counts then (float32, 118 x 18 x 843: 66 -> 24 us)
+static int tile_of(int nq, int64_t rows) {
+    if (large(nq, rows)) return 256;
+    if (nq <= 32) return 32;
+    const int64_t tiles = (int64_t)((nq + 127) / 128) * ((rows + 127) / 128);
+    return tiles <= 256 ? 65 : nq <= 64 ? 64 : 128;   // (65: 64 x 64)
+}
+static int rows_of_tile(int tile) { return tile == 256 ? 256 : tile == 65 ? 64 : 128; }
+static int queries_of_tile(int tile) { return tile == 65 ? 64 : tile; }
+
 // workgroups that share a panel's rows: one for each CU with the large tiles, two or three with the small ones
 extern "C" int jvk_sx_loss_plan(int nq, int64_t rows, int* tile) {
-    const int tm = large(nq, rows) ? 256 : nq > 64 ? 128 : nq > 32 ? 64 : 32, tn = tm == 256 ? 256 : 128, full = tm == 256 ? 256 : tm == 128 ? 512 : 768;
+    const int t = tile_of(nq, rows), tm = queries_of_tile(t), tn = rows_of_tile(t), full = t == 256 ? 256 : t == 128 || t == 65 ? 512 : 768;
     const int64_t panels = std::max((nq + tm - 1) / tm, 1), tiles = std::max<int64_t>((rows + tn - 1) / tn, 1);
-    *tile = tm;
+    *tile = t;
     return (int)std::min(std::max<int64_t>(full / panels, 1), tiles);
 }
 
@@ -258,34 +280,25 @@ static hipError_t loss_tile(const JvSxLoss& a, hipStream_t s) {
     jvs_loss_tile_kernel<T, WM, WN><<<(unsigned)((all + 7) / 8 * 8), T::THREADS, T::LDS, s>>>(a);
     return hipGetLastError();
 }
-// rows that copies of 16 B a lane can take: aligned, and ending with 16 B
-static bool wide32(const void* p, int64_t ld, int cols) { return (uintptr_t)p % 16 == 0 && ld % 16 == 0 && cols % 4 == 0; }
-
-template <int NS>
-static hipError_t loss_small(const JvSxLoss& a, bool f32, bool wide, hipStream_t s) {
-    if (!f32) {
-        if (a.tile == 128) return loss_tile<Tile<BF16, 2, 2, 2, 2, NS>, 2, 2>(a, s);
-        return a.tile == 64 ? loss_tile<Tile<BF16, 2, 1, 1, 4, NS>, 1, 4>(a, s) : loss_tile<Tile<BF16, 1, 1, 1, 4, NS>, 1, 4>(a, s);
+static hipError_t loss_small(const JvSxLoss& a, bool f32, hipStream_t s) {
+    const bool few = (int64_t)((a.mm.M + 31) / 32) * a.splits <= 256;   // (32 queries)
+    if (f32) {
+        if (a.tile == 128) return loss_tile<Tile32<2, 2, 2, 2, 2, false, false>, 2, 2>(a, s);
+        if (a.tile == 65) return loss_tile<Tile32<1, 1, 2, 2, 4, false, false>, 2, 2>(a, s);
+        if (a.tile == 64) return loss_tile<Tile32<2, 1, 1, 4, 2, false, false>, 1, 4>(a, s);
+        return few ? loss_tile<Tile32<1, 1, 1, 4, 4, false, false>, 1, 4>(a, s) : loss_tile<Tile32<1, 1, 1, 4, 2, false, false>, 1, 4>(a, s);
     }
-    if (wide) {
-        if (a.tile == 128) return loss_tile<Tile32<2, 2, 2, 2, NS, false, false, false, false>, 2, 2>(a, s);
-        if (a.tile == 64) return loss_tile<Tile32<2, 1, 1, 4, NS, false, false, false, false>, 1, 4>(a, s);
-        return loss_tile<Tile32<1, 1, 1, 4, NS, false, false, false, false>, 1, 4>(a, s);
-    }
-    if (a.tile == 128) return loss_tile<Tile32<2, 2, 2, 2, NS, false, false, true, true>, 2, 2>(a, s);
-    if (a.tile == 64) return loss_tile<Tile32<2, 1, 1, 4, NS, false, false, true, true>, 1, 4>(a, s);
-    return loss_tile<Tile32<1, 1, 1, 4, NS, false, false, true, true>, 1, 4>(a, s);
+    if (a.tile == 128) return loss_tile<Tile<BF16, 2, 2, 2, 2, 2>, 2, 2>(a, s);
+    if (a.tile == 65) return loss_tile<Tile<BF16, 1, 1, 2, 2, 4>, 2, 2>(a, s);
+    if (a.tile == 64) return loss_tile<Tile<BF16, 2, 1, 1, 4, 2>, 1, 4>(a, s);
+    return few ? loss_tile<Tile<BF16, 1, 1, 1, 4, 4>, 1, 4>(a, s) : loss_tile<Tile<BF16, 1, 1, 1, 4, 2>, 1, 4>(a, s);
 }
 
 extern "C" hipError_t jvk_sx_loss(const JvSxLoss* a, int f32, hipStream_t s) {
     using P = Pipe<BF16>;
     if (a->mm.N <= 0 || a->mm.M <= 0) return hipSuccess;
     if (a->splits < 1) return hipErrorInvalidValue;
-    if (f32 || a->tile != 256) {
-        const bool wide = f32 && wide32(a->mm.a, a->mm.lda, a->mm.k) && wide32(a->mm.b, a->mm.ldb, a->mm.k);
-        const bool few = (int64_t)((a->mm.M + a->tile - 1) / a->tile) * a->splits <= 256;
-        return few ? loss_small<4>(*a, f32, wide, s) : loss_small<2>(*a, f32, wide, s);
-    }
+    if (a->tile != 256) return loss_small(*a, f32, s);
     hipError_t e = lds_of(jvs_loss_pipe_kernel, P::LDS);
     if (e != hipSuccess) return e;
     const int64_t all = (int64_t)((a->mm.M + P::TM - 1) / P::TM) * a->splits;
@@ -401,7 +414,7 @@ __global__ __launch_bounds__(T::THREADS) void jvs_weights_tile_kernel(const JvSx
     for (int m = 0; m < MT; m++) {
         const int r = m0 + T::row(m);
         JvSxQuery q = {0.0f, 0.0f, -1, 0};
-        if (r < a.mm.M) q = a.query[r];
+        if (r < a.mm.M) q = a.query ? a.query[r] : query_of(a.lse, a.w, a.targets, a.n, r);
         weigh<T>(acc[m], q, a.c, a.mm.N - n0, q.target >= 0 ? (int)(q.target - a.row0) - n0 : -1, a.planes == 1, a.rest + r);
         if (a.planes == 0) {
 #pragma unroll
@@ -437,22 +450,21 @@ static hipError_t weights_tile(const JvSxWeights& a, hipStream_t s) {
     return hipGetLastError();
 }
 
-template <int NS>
-static hipError_t weights_small(const JvSxWeights& a, hipStream_t s) {
-    const bool tall = a.mm.M > 64;
-    if (a.planes != 0) return tall ? weights_tile<Tile<BF16, 2, 2, 2, 2, NS>>(a, s) : weights_tile<Tile<BF16, 2, 1, 1, 4, NS>>(a, s);
-    if (wide32(a.mm.a, a.mm.lda, a.mm.k) && wide32(a.mm.b, a.mm.ldb, a.mm.k))
-        return tall ? weights_tile<Tile32<2, 2, 2, 2, NS, false, false, false, false>>(a, s) : weights_tile<Tile32<2, 1, 1, 4, NS, false, false, false, false>>(a, s);
-    return tall ? weights_tile<Tile32<2, 2, 2, 2, NS, false, false, true, true>>(a, s) : weights_tile<Tile32<2, 1, 1, 4, NS, false, false, true, true>>(a, s);
+static hipError_t weights_small(const JvSxWeights& a, hipStream_t s) {   // (G's padded queries are a multiple of 64: no tile of 32)
+    const int t = tile_of(a.mm.M, a.mm.N);
+    const bool few = t == 65 || (t == 32 && (a.mm.N + 127) / 128 <= 256);
+    if (a.planes == 0) {
+        if (few) return weights_tile<Tile32<1, 1, 2, 2, 4, false, false>>(a, s);
+        return a.mm.M > 64 ? weights_tile<Tile32<2, 2, 2, 2, 2, false, false>>(a, s) : weights_tile<Tile32<2, 1, 1, 4, 2, false, false>>(a, s);
+    }
+    if (few) return weights_tile<Tile<BF16, 1, 1, 2, 2, 4>>(a, s);
+    return a.mm.M > 64 ? weights_tile<Tile<BF16, 2, 2, 2, 2, 2>>(a, s) : weights_tile<Tile<BF16, 2, 1, 1, 4, 2>>(a, s);
 }
 
 extern "C" hipError_t jvk_sx_weights(const JvSxWeights* a, int large, hipStream_t s) {
     using P = Pipe<BF16>;
     if (a->mm.M <= 0 || a->mm.N <= 0) return hipSuccess;
-    if (a->planes == 0 || !large) {
-        const int64_t tiles = (int64_t)(a->mm.M > 64 ? (a->mm.M + 127) / 128 : 1) * ((a->mm.N + 127) / 128);
-        return tiles <= 256 ? weights_small<4>(*a, s) : weights_small<2>(*a, s);
-    }
+    if (!large) return weights_small(*a, s);
     const int64_t all = (int64_t)((a->mm.M + P::TM - 1) / P::TM) * ((a->mm.N + P::TN - 1) / P::TN);
     if (all > 0x7fffffffll) return hipErrorInvalidValue;
     hipError_t e = lds_of(jvs_weights_kernel, P::LDS);
@@ -481,18 +493,16 @@ static hipError_t grads_tile(const JvMmOut* q, const JvMmOut* v, bool f32, hipSt
     return hipGetLastError();
 }
 
-// k ranges of dq: with the large tiles once around the CUs, with the small ones twice; four steps in each at least
+// Tiles of the gradients' products: 256 x 256 (large), else 128 x 128, or 64 x 64 where that would be no more than one tile a CU.
+static bool few_grads(int64_t tiles) { return tiles <= 256; }
+static int64_t tiles128(int64_t rows, int64_t cols) { return std::max<int64_t>((rows + 127) / 128, 1) * ((cols + 127) / 128); }
+
+// k ranges of dq: once around the CUs with the large tiles, twice with the small ones; at least four and eight steps in each (a range that is
+// joined costs a launch more)
 extern "C" int jvk_sx_grad_splits(int nq, int d, int64_t rows, int f32, int large) {
-    const int t = large ? 256 : 128, full = large ? 256 : 512;
-    const int64_t tiles = std::max<int64_t>((nq + t - 1) / t, 1) * ((d + t - 1) / t), steps = (rows + 63) / 64 * (f32 ? large ? 6 : 2 : 1);
-    return (int)std::max<int64_t>(std::min<int64_t>(full / tiles, steps / 4), 1);
-}
-template <int NS>
-static hipError_t grads_small(const JvMmOut* q, const JvMmOut* v, bool f32, hipStream_t s) {
-    if (!f32) return grads_tile<Tile<BF16, 2, 2, 2, 2, NS, false, true>, Tile<BF16, 2, 2, 2, 2, NS, true, true>>(q, v, false, s);
-    if ((!q || wide32(q->mm.b, q->mm.ldb, q->mm.cb)) && (!v || wide32(v->mm.b, v->mm.ldb, v->mm.cb)))
-        return grads_tile<Tile32<2, 2, 2, 2, NS, false, true, false, false>, Tile32<2, 2, 2, 2, NS, true, true, false, false>>(q, v, true, s);
-    return grads_tile<Tile32<2, 2, 2, 2, NS, false, true, false, true>, Tile32<2, 2, 2, 2, NS, true, true, false, true>>(q, v, true, s);
+    const int64_t tiles = large ? std::max<int64_t>((nq + 255) / 256, 1) * ((d + 255) / 256) : tiles128(nq, d);
+    const int64_t steps = (rows + 63) / 64 * (f32 ? large ? 6 : 2 : 1);
+    return (int)std::max<int64_t>(std::min<int64_t>((large ? 256 : 512) / tiles, steps / (large ? 4 : 8)), 1);
 }
 extern "C" hipError_t jvk_sx_grads(const JvMmOut* q, const JvMmOut* v, int f32, int large, hipStream_t s) {
     if (large) {
@@ -503,8 +513,13 @@ extern "C" hipError_t jvk_sx_grads(const JvMmOut* q, const JvMmOut* v, int f32, 
     }
     int64_t tiles = 0;
     for (const JvMmOut* o : {q, v})
-        if (o) tiles += (int64_t)((o->mm.M + 127) / 128) * ((o->mm.N + 127) / 128) * o->splits;
-    return tiles <= 256 ? grads_small<4>(q, v, f32, s) : grads_small<2>(q, v, f32, s);
+        if (o) tiles += tiles128(o->mm.M, o->mm.N) * o->splits;
+    if (few_grads(tiles)) {
+        if (f32) return grads_tile<Tile32<1, 1, 2, 2, 4, false, true>, Tile32<1, 1, 2, 2, 4, true, true>>(q, v, true, s);
+        return grads_tile<Tile<BF16, 1, 1, 2, 2, 4, false, true>, Tile<BF16, 1, 1, 2, 2, 4, true, true>>(q, v, false, s);
+    }
+    if (f32) return grads_tile<Tile32<2, 2, 2, 2, 2, false, true>, Tile32<2, 2, 2, 2, 2, true, true>>(q, v, true, s);
+    return grads_tile<Tile<BF16, 2, 2, 2, 2, 2, false, true>, Tile<BF16, 2, 2, 2, 2, 2, true, true>>(q, v, false, s);
 }
 
 // partial sums -> the queries' gradient, and what G lacked at the target: one wave a row, four columns a lane
@@ -514,7 +529,7 @@ __global__ __launch_bounds__(256) void jvs_finish_kernel(const float* __restrict
                                                          const float* __restrict__ norm, T* __restrict__ out, int64_t ldo) {
     const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (r >= rows) return;
-    const float by = mul * *norm, lack = rest[r];
+    const float by = norm ? mul * *norm : mul, lack = rest ? rest[r] : 0.0f;
     const int64_t target = lack != 0.0f ? query[r].target : 0;
     for (int c = (threadIdx.x & 63) * 4 + blockIdx.y * 256; c < d; c += gridDim.y * 256) {   // (lds is a multiple of 64)
         const float* p = slab + r * lds + c;

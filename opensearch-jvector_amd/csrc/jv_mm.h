@@ -51,6 +51,17 @@ __device__ __forceinline__ s16x4 read_across(const unsigned char* p) {   // 16 l
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
 }
 
+// This wave's copies of a step have landed and everybody's have, `left` steps (PER copies each, NS - 1 at most) being under way behind it.
+template <int NS, int PER>
+__device__ __forceinline__ void wait_step(int left) {
+    static_assert(NS >= 2 && NS <= 4);
+    constexpr int most = 63;   // (what the counter holds)
+    if (left >= NS - 1) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((NS - 1) * PER < most ? (NS - 1) * PER : most) : "memory");
+    else if (NS > 3 && left == 2) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * PER < most ? 2 * PER : most) : "memory");
+    else if (NS > 2 && left == 1) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(PER < most ? PER : most) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
 // The product for small shapes: MT x NT accumulators of 32 x 32 for each of WM x WN waves, NS steps of k in LDS: two and
 // several workgroups a CU, or four where there are no more workgroups than CUs and the way to memory is what counts.
 // TA / TB: an operand with k across its rows (bf16): 64 rows of TM / TN columns a step.  Four rows of 64 B are read at a time: piece p of row k
@@ -61,7 +72,7 @@ struct Tile {
     static constexpr int TM = 32 * MT * WM, TN = 32 * NT * WN, WAVES = WM * WN, THREADS = 64 * WAVES;
     static constexpr int GA = TM / 8, GB = TN / 8;                               // 8-row groups
     static constexpr int CA = GA / WAVES, CB = GB / WAVES, PER = CA + CB;        // copies of one wave a step
-    static constexpr int BUF = (GA + GB) * GROUP, LDS = NS * BUF, AHEAD = (NS - 1) * PER < 63 ? (NS - 1) * PER : 63;
+    static constexpr int BUF = (GA + GB) * GROUP, LDS = NS * BUF;
     static_assert(GA % WAVES == 0 && GB % WAVES == 0, "every wave copies the same number of groups of each operand");
     static_assert(TY == BF16 || (!TA && !TB), "8-bit operands have k along their rows");
     static __device__ __forceinline__ int steps(const JvMm& a) { return (a.kph >> 1) * a.segs; }
@@ -125,7 +136,6 @@ struct Tile {
                 for (int e = 0; e < 16; e++) acc[m][n][e] = 0.0f;
 
         int seg = k0 / nk, kin = k0 - seg * nk;   // of the next step to be staged
-        const int last_seg = (k1 - 1) / nk, last_kin = k1 - 1 - last_seg * nk;
         auto stage = [&](int buf) {
             int64_t offa = TA ? 0 : (int64_t)kin * 128, offb = TB ? 0 : (int64_t)kin * 128;
             if (a.segs > 1) offa += plane_a(seg) * a.plane_a, offb += plane_b(seg) * a.plane_b;
@@ -138,12 +148,9 @@ struct Tile {
                 glds16(src[CA + i] + offb + (TB ? (int64_t)min(kin * 64 + krow[CA + i], a.kb - 1) * a.ldb : 0), dst + GA * GROUP + (i * WAVES + w) * (TB ? 1024 : GROUP));
             if (++kin == nk) kin = 0, seg++;
         };
-        // (behind the last step the last one is copied again, into a buffer that nobody reads: the number of copies under way stays the same)
 #pragma unroll
-        for (int i = 0; i < NS - 1; i++) {
-            stage(i);
-            if (k0 + i + 1 >= k1) kin = last_kin, seg = last_seg;
-        }
+        for (int i = 0; i < NS - 1; i++)
+            if (k0 + i < k1) stage(i);
         for (int s = k0; s < k1; s++) {
             const int buf = (s - k0) % NS;
             int fa[MT], fb[NT];
@@ -153,9 +160,8 @@ struct Tile {
 #pragma unroll
                 for (int t = 0; t < NT; t++) fb[t] = pb[t][s];
             }
-            stage((s - k0 + NS - 1) % NS);
-            if (s + NS >= k1) kin = last_kin, seg = last_seg;
-            asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(AHEAD) : "memory");
+            if (s + NS - 1 < k1) stage((s - k0 + NS - 1) % NS);
+            wait_step<NS, PER>(k1 - 1 - s);
             const unsigned char* base = smem + buf * BUF;
             if constexpr (TY == BF16) {
 #pragma unroll
@@ -222,7 +228,6 @@ struct Tile {
             // every fragment read of this buffer has returned before any wave stages into it again
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         }
-        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");   // nothing is on its way into LDS any more
     }
     // acc[m][n][e] is C[row(m)][col(n, e)] of the tile, four consecutive e are four consecutive columns
     static __device__ __forceinline__ int row(int m) { return (((threadIdx.x >> 6) % WM) * MT + m) * 32 + (threadIdx.x & 31); }

@@ -52,7 +52,10 @@ struct JvSxWeights {
     JvMm mm;               // A = queries, B = vectors of this piece
     float c;
     int64_t row0;          // first row of this piece
-    const JvSxQuery* query;
+    const JvSxQuery* query;   // nullptr: from lse, w (nullptr = 1) and targets as they are
+    const float *lse, *w;
+    const int32_t* targets;
+    int64_t n;             // rows in all
     int32_t planes;        // 1 or 3, or 0: float32 as it is
     void* g;                 // (planes = 0: float32)
     int32_t kv;            // N padded to 64

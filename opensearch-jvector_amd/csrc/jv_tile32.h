@@ -6,19 +6,20 @@
 // of 32; LDS holds NS of them (Tile).  An operand with k along its rows (d components, any number: what lies behind is masked in the last step) is
 // staged in 8-row groups of 128 B a row as in Tile; one with k across its rows as 32 rows of TM / TN columns, where the rows 8 .. 15 and
 // 24 .. 31 have their 128-B halves of 256 B swapped, so that the two halves of a wave, eight rows apart, read different banks.
-// Copies are 16 B a lane, or 4 B (NA / NB) where a row is not 16-B aligned or ends inside 16 B.
+// Copies are 16 B a lane from addresses that need 4-B alignment only.  The 16 B that would pass the end of a row start so much earlier that
+// they end with it, and their components are taken from so much further back (rows of fewer than four are laid out with four beforehand).
 #pragma once
 #include "jv_mm.h"
 
 namespace jvmm {
 
-template <int MT_, int NT_, int WM, int WN, int NS, bool TA, bool TB, bool NA, bool NB>
+template <int MT_, int NT_, int WM, int WN, int NS, bool TA, bool TB>
 struct Tile32 {
     static constexpr int MT = MT_, NT = NT_;
     static constexpr int TM = 32 * MT * WM, TN = 32 * NT * WN, WAVES = WM * WN, THREADS = 64 * WAVES;
     static constexpr int GA = TM / 8, GB = TN / 8;                       // KB of a step
-    static constexpr int CA = GA / WAVES * (NA ? 4 : 1), CB = GB / WAVES * (NB ? 4 : 1), PER = CA + CB;   // copies of one wave a step
-    static constexpr int BUF = (GA + GB) * GROUP, LDS = NS * BUF, AHEAD = (NS - 1) * PER < 63 ? (NS - 1) * PER : 63;
+    static constexpr int PER = (GA + GB) / WAVES;                        // copies of one wave a step
+    static constexpr int BUF = (GA + GB) * GROUP, LDS = NS * BUF;
     static_assert(GA % WAVES == 0 && GB % WAVES == 0, "every wave copies the same number of groups of each operand");
     static_assert((!TA || GA >= 8) && (!TB || GB >= 8), "the swapped halves are 32 columns each");
     static __device__ __forceinline__ int steps(const JvMm& a) { return (a.k + 31) / 32; }
@@ -36,26 +37,24 @@ struct Tile32 {
             }
     }
 
-    // One operand of `rows` rows (k along) or columns (k across), ROWS = TM / TN of them from `first` on.
-    template <bool ACROSS, bool NARROW, int GROUPS>
+    // One operand of `rows` rows of k components (k along) or k rows of `cols` columns (k across); GROUPS * 8 rows or columns from `first` on.
+    template <bool ACROSS, int GROUPS>
     struct Side {
-        static constexpr int COPIES = GROUPS / WAVES * (NARROW ? 4 : 1);
-        static constexpr int STRIDE = ACROSS ? 1024 : GROUP;   // LDS bytes of a KB of the operand
+        static constexpr int COPIES = GROUPS / WAVES;
         const char* src[COPIES];
 
-        // copy i of this wave is number c = i * WAVES + w of its KB (wide) or 256 B (narrow)
+        // copy i of this wave is KB number i * WAVES + w: eight rows of 128 B (k along), or rows of GROUPS * 32 B (k across)
         __device__ __forceinline__ void init(const char* base, int64_t ld, int first, int rows, int cols) {
             const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
 #pragma unroll
             for (int i = 0; i < COPIES; i++) {
                 const int c = i * WAVES + w;
                 if constexpr (!ACROSS) {
-                    const int row = NARROW ? 2 * c + (lane >> 5) : 8 * c + (lane >> 3);
-                    src[i] = base + (int64_t)min(first + row, rows - 1) * ld;
+                    src[i] = base + (int64_t)min(first + 8 * c + (lane >> 3), rows - 1) * ld;
                 } else {
-                    const int byte = NARROW ? c * 256 + lane * 4 : c * 1024 + lane * 16, k = byte / (GROUPS * 32);
+                    const int byte = c * 1024 + lane * 16, k = byte / (GROUPS * 32);
                     const int col = ((byte % (GROUPS * 32)) >> 2) ^ (((k >> 3) & 1) << 5);
-                    src[i] = base + (int64_t)min(first + col, cols - (NARROW ? 1 : 4)) * 4;
+                    src[i] = base + (int64_t)min(first + col, max(cols, 4) - 4) * 4;
                 }
             }
         }
@@ -65,35 +64,35 @@ struct Tile32 {
             for (int i = 0; i < COPIES; i++) {
                 const int c = i * WAVES + w;
                 const char* p = src[i];
-                if constexpr (!ACROSS) {
-                    // piece (16 B) or component inside the 128 B of a row; what lies behind the last component reads as the first (and is masked)
-                    const int row = NARROW ? 2 * c + (lane >> 5) : 8 * c + (lane >> 3);
-                    const int at = NARROW ? ((((lane & 31) >> 2) ^ (row & 7)) << 2) + (lane & 3) : ((lane & 7) ^ (row & 7)) << 2;
-                    const int col = step * 32 + at;
-                    p += (int64_t)(col < k ? col : 0) * 4;
-                } else {
-                    const int byte = NARROW ? c * 256 + lane * 4 : c * 1024 + lane * 16, row = byte / (GROUPS * 32);
-                    p += (int64_t)min(step * 32 + row, k - 1) * ld;
-                }
-                if constexpr (NARROW) {
-                    unsigned char* to = dst + (ACROSS ? c * 256 : (c >> 2) * GROUP + (c & 3) * 256);
-                    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p, (__attribute__((address_space(3))) void*)to, 4, 0, 0);
-                } else {
-                    glds16(p, dst + c * STRIDE);
-                }
+                if constexpr (!ACROSS) p += (int64_t)min(step * 32 + (((lane & 7) ^ (lane >> 3)) << 2), max(k, 4) - 4) * 4;
+                else p += (int64_t)min(step * 32 + (c * 1024 + lane * 16) / (GROUPS * 32), k - 1) * ld;
+                glds16(p, dst + c * (ACROSS ? 1024 : GROUP));
             }
         }
-        // eight k's (16 kk + 8 h ..) of row or column r; `valid`: components of this step (k along rows)
-        __device__ __forceinline__ void read(const unsigned char* base, int r, int kk, int valid, bf16x8 (&p)[3]) const {
+        // where column r of the tile lies in a row of the step (k across)
+        static __device__ __forceinline__ int place(int r, int first, int cols) {
+            const int back = cols < 4 ? 0 : min(max(first + (r & ~3) + 4 - cols, 0), 3);
+            return (r & ~3) + min((r & 3) + back, 3);
+        }
+        // eight k's (16 kk + 8 h ..) of row r, or of the column at `r` (place); `valid`: components of this step, `k` in all (k along)
+        __device__ __forceinline__ void read(const unsigned char* base, int r, int kk, int valid, int k, bf16x8 (&p)[3]) const {
             const int h = (threadIdx.x >> 5) & 1;
             float x[8];
             if constexpr (!ACROSS) {
                 const unsigned char* row = base + (r >> 3) * GROUP + (r & 7) * 128;
-                *(f32x4*)x = *(const f32x4*)(row + (((4 * kk + 2 * h) ^ (r & 7)) << 4));
-                *(f32x4*)(x + 4) = *(const f32x4*)(row + (((4 * kk + 2 * h + 1) ^ (r & 7)) << 4));
-                if (valid < 32) {
 #pragma unroll
-                    for (int e = 0; e < 8; e++) x[e] = 16 * kk + 8 * h + e < valid ? x[e] : 0.0f;
+                for (int half = 0; half < 2; half++) {
+                    const int piece = 4 * kk + 2 * h + half;
+                    f32x4 v = *(const f32x4*)(row + ((piece ^ (r & 7)) << 4));
+                    if (valid < 32) {
+                        const int back = k < 4 || 4 * piece >= valid ? 0 : max(4 * piece + 4 - valid, 0);
+                        if (back & 1) v = (f32x4){v[1], v[2], v[3], v[3]};
+                        if (back & 2) v = (f32x4){v[2], v[3], v[3], v[3]};
+#pragma unroll
+                        for (int e = 0; e < 4; e++) v[e] = 4 * piece + e < valid ? v[e] : 0.0f;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; e++) x[4 * half + e] = v[e];
                 }
             } else {
                 const int c = r ^ (h << 5);
@@ -107,8 +106,8 @@ struct Tile32 {
     // C tile at (m0, n0), steps [k0, k1) of ceil(k / 32)
     static __device__ __forceinline__ void run(const JvMm& a, int m0, int n0, int k0, int k1, unsigned char* smem, f32x16 (&acc)[MT][NT]) {
         const int w = threadIdx.x >> 6, r31 = threadIdx.x & 31, wm = w % WM, wn = w / WM;
-        Side<TA, NA, GA> sa;
-        Side<TB, NB, GB> sb;
+        Side<TA, GA> sa;
+        Side<TB, GB> sb;
         sa.init(a.a, a.lda, m0, a.M, a.ca);
         sb.init(a.b, a.ldb, n0, a.N, a.cb);
 #pragma unroll
@@ -117,27 +116,31 @@ struct Tile32 {
             for (int n = 0; n < NT; n++)
 #pragma unroll
                 for (int e = 0; e < 16; e++) acc[m][n][e] = 0.0f;
-        // (behind the last step the last one is copied again, into a buffer that nobody reads: the number of copies under way stays the same)
+        int ra[MT], rb[NT];
+#pragma unroll
+        for (int t = 0; t < MT; t++) ra[t] = (wm * MT + t) * 32 + r31, ra[t] = TA ? sa.place(ra[t], m0, a.ca) : ra[t];
+#pragma unroll
+        for (int t = 0; t < NT; t++) rb[t] = (wn * NT + t) * 32 + r31, rb[t] = TB ? sb.place(rb[t], n0, a.cb) : rb[t];
         auto stage = [&](int s) {
             unsigned char* dst = smem + (s - k0) % NS * BUF;
-            s = min(s, k1 - 1);
             sa.copy(a.lda, s, TA ? a.ka : a.k, dst);
             sb.copy(a.ldb, s, TB ? a.kb : a.k, dst + GA * GROUP);
         };
 #pragma unroll
-        for (int i = 0; i < NS - 1; i++) stage(k0 + i);
+        for (int i = 0; i < NS - 1; i++)
+            if (k0 + i < k1) stage(k0 + i);
         for (int s = k0; s < k1; s++) {
-            stage(s + NS - 1);
-            asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(AHEAD) : "memory");
+            if (s + NS - 1 < k1) stage(s + NS - 1);
+            wait_step<NS, PER>(k1 - 1 - s);
             const unsigned char* base = smem + (s - k0) % NS * BUF;
             const int valid = a.k - s * 32;
 #pragma unroll
             for (int kk = 0; kk < 2; kk++) {
                 bf16x8 va[MT][3], vb[NT][3];
 #pragma unroll
-                for (int t = 0; t < MT; t++) sa.read(base, (wm * MT + t) * 32 + r31, kk, valid, va[t]);
+                for (int t = 0; t < MT; t++) sa.read(base, ra[t], kk, valid, a.k, va[t]);
 #pragma unroll
-                for (int t = 0; t < NT; t++) sb.read(base + GA * GROUP, (wn * NT + t) * 32 + r31, kk, valid, vb[t]);
+                for (int t = 0; t < NT; t++) sb.read(base + GA * GROUP, rb[t], kk, valid, a.k, vb[t]);
 #pragma unroll
                 for (int g = 0; g < 6; g++) {
                     const int pa = (0x052 >> (2 * g)) & 3, pb = (0x118 >> (2 * g)) & 3;
@@ -150,7 +153,6 @@ struct Tile32 {
             // every fragment read of this buffer has returned before any wave stages into it again
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         }
-        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");   // nothing is on its way into LDS any more
     }
     // acc[m][n][e] is C[row(m)][col(n, e)] of the tile, four consecutive e are four consecutive columns
     static __device__ __forceinline__ int row(int m) { return (((threadIdx.x >> 6) % WM) * MT + m) * 32 + (threadIdx.x & 31); }
