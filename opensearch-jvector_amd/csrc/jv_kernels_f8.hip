@@ -7,24 +7,27 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 #include "jv_mm.h"
 #include "jv_mm_out.h"
 
 using namespace jvmm;
 
-#define F8_CHUNK 128   // blocks of one workgroup: 16 for each of its 8 half-waves
-
 // ---------------------------------------------------------------------------------------------
-// A half-wave holds one block, four components a lane: the block's maximum is five exchanges, a store is 4 B of codes.
+// A half-wave holds one block, four components a lane: the block's maximum is five exchanges, a store is 4 B of codes.  A workgroup's eight
+// half-waves take `rounds` runs of eight blocks: sixteen in long calls, one where there are few blocks.  Loads and stores need no alignment.
+// 1 000 003 x 1 000 float32: 1.12 ms, 4.5 TB/s (a large copy: 4.7); back: 0.99 ms, 5.1 TB/s.
 // ---------------------------------------------------------------------------------------------
 template <typename T>
-__device__ __forceinline__ f32x4 load4(const T* row, int at, int d, bool wide) {
+__device__ __forceinline__ f32x4 load4(const T* row, int at, int d) {
     f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (wide && at + 3 < d) {
+    if (at + 3 < d) {
         if constexpr (sizeof(T) == 4) {
-            x = *(const f32x4*)(row + at);
+            __builtin_memcpy(&x, row + at, 16);
         } else {
-            const bf16x4 v = *(const bf16x4*)(row + at);
+            bf16x4 v;
+            __builtin_memcpy(&v, row + at, 8);
 #pragma unroll
             for (int e = 0; e < 4; e++) x[e] = (float)v[e];
         }
@@ -37,17 +40,17 @@ __device__ __forceinline__ f32x4 load4(const T* row, int at, int d, bool wide) {
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void jvf_encode_kernel(const T* __restrict__ x, int64_t stride, int64_t blocks, int d, int nb, int wide,
+__global__ __launch_bounds__(256) void jvf_encode_kernel(const T* __restrict__ x, int64_t stride, int64_t blocks, int d, int nb, int rounds,
                                                          uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
     const int hw = threadIdx.x >> 5, l = threadIdx.x & 31;
-    const int64_t first = (int64_t)blockIdx.x * F8_CHUNK;
+    const int64_t first = (int64_t)blockIdx.x * (rounds * 8);
     const int64_t row0 = first / nb;
     const uint32_t b0 = (uint32_t)(first - row0 * nb);
-    for (int i = 0; i < F8_CHUNK / 8; i++) {
+    for (int i = 0; i < rounds; i++) {
         const int64_t blk = first + i * 8 + hw;
         if (blk >= blocks) break;   // (whole half-waves: the exchanges below stay inside one)
         const uint32_t at = b0 + (uint32_t)(i * 8 + hw), up = at / (uint32_t)nb, b = at - up * (uint32_t)nb;
-        const f32x4 v = load4(x + (row0 + up) * stride, (int)b * 128 + l * 4, d, wide);
+        const f32x4 v = load4(x + (row0 + up) * stride, (int)b * 128 + l * 4, d);
         // the largest finite magnitude, compared as bits
         uint32_t top = 0;
 #pragma unroll
@@ -78,12 +81,12 @@ __global__ __launch_bounds__(256) void jvf_encode_kernel(const T* __restrict__ x
 
 template <typename T>
 __global__ __launch_bounds__(256) void jvf_decode_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t blocks,
-                                                         int d, int nb, int wide, T* __restrict__ x, int64_t stride) {
+                                                         int d, int nb, int rounds, T* __restrict__ x, int64_t stride) {
     const int hw = threadIdx.x >> 5, l = threadIdx.x & 31;
-    const int64_t first = (int64_t)blockIdx.x * F8_CHUNK;
+    const int64_t first = (int64_t)blockIdx.x * (rounds * 8);
     const int64_t row0 = first / nb;
     const uint32_t b0 = (uint32_t)(first - row0 * nb);
-    for (int i = 0; i < F8_CHUNK / 8; i++) {
+    for (int i = 0; i < rounds; i++) {
         const int64_t blk = first + i * 8 + hw;
         if (blk >= blocks) break;
         const uint32_t p = b0 + (uint32_t)(i * 8 + hw), up = p / (uint32_t)nb, b = p - up * (uint32_t)nb;
@@ -91,14 +94,15 @@ __global__ __launch_bounds__(256) void jvf_decode_kernel(const uint8_t* __restri
         const uint32_t byte = scales[blk];
         const float s = byte == 0 ? __uint_as_float(0x00400000u) : byte == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float(byte << 23);
         const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(code, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(code, true);
-        const float v[4] = {lo[0] * s, lo[1] * s, hi[0] * s, hi[1] * s};
+        const f32x4 v = {lo[0] * s, lo[1] * s, hi[0] * s, hi[1] * s};
         const int at = (int)b * 128 + l * 4;
         T* out = x + (row0 + up) * stride + at;
-        if (wide && at + 3 < d) {
+        if (at + 3 < d) {
             if constexpr (sizeof(T) == 4) {
-                *(f32x4*)out = (f32x4){v[0], v[1], v[2], v[3]};
+                __builtin_memcpy(out, &v, 16);
             } else {
-                *(bf16x4*)out = (bf16x4){(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+                const bf16x4 h = {(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+                __builtin_memcpy(out, &h, 8);
             }
         } else {
 #pragma unroll
@@ -108,30 +112,30 @@ __global__ __launch_bounds__(256) void jvf_decode_kernel(const uint8_t* __restri
     }
 }
 
-static bool wide4(const void* p, int64_t stride, int dtype) {
-    const int size = dtype == 0 ? 4 : 2;
-    return ((uintptr_t)p % (4 * size)) == 0 && stride % 4 == 0;
-}
+// runs of eight blocks for each workgroup: eight workgroups a CU before a workgroup gets more than one
+static int rounds_of(int64_t blocks) { return (int)std::min<int64_t>(std::max<int64_t>(blocks / (8 * 2048), 1), 16); }
 
 extern "C" hipError_t jvk_f8_encode(const void* x, int dtype, int64_t stride, int64_t n, int d, uint8_t* codes, uint8_t* scales, hipStream_t s) {
     const int nb = (d + 127) / 128;
-    const int64_t blocks = n * nb, grid = (blocks + F8_CHUNK - 1) / F8_CHUNK;
+    const int64_t blocks = n * nb;
+    const int rounds = rounds_of(blocks);
+    const int64_t grid = (blocks + rounds * 8 - 1) / (rounds * 8);
     if (grid <= 0) return hipSuccess;
     if (grid > 0x7fffffffll) return hipErrorInvalidValue;
-    const int wide = wide4(x, stride, dtype);
-    if (dtype == 0) jvf_encode_kernel<float><<<(unsigned)grid, 256, 0, s>>>((const float*)x, stride, blocks, d, nb, wide, codes, scales);
-    else jvf_encode_kernel<__bf16><<<(unsigned)grid, 256, 0, s>>>((const __bf16*)x, stride, blocks, d, nb, wide, codes, scales);
+    if (dtype == 0) jvf_encode_kernel<float><<<(unsigned)grid, 256, 0, s>>>((const float*)x, stride, blocks, d, nb, rounds, codes, scales);
+    else jvf_encode_kernel<__bf16><<<(unsigned)grid, 256, 0, s>>>((const __bf16*)x, stride, blocks, d, nb, rounds, codes, scales);
     return hipGetLastError();
 }
 
 extern "C" hipError_t jvk_f8_decode(const uint8_t* codes, const uint8_t* scales, int64_t n, int d, void* x, int dtype, int64_t stride, hipStream_t s) {
     const int nb = (d + 127) / 128;
-    const int64_t blocks = n * nb, grid = (blocks + F8_CHUNK - 1) / F8_CHUNK;
+    const int64_t blocks = n * nb;
+    const int rounds = rounds_of(blocks);
+    const int64_t grid = (blocks + rounds * 8 - 1) / (rounds * 8);
     if (grid <= 0) return hipSuccess;
     if (grid > 0x7fffffffll) return hipErrorInvalidValue;
-    const int wide = wide4(x, stride, dtype);
-    if (dtype == 0) jvf_decode_kernel<float><<<(unsigned)grid, 256, 0, s>>>(codes, scales, blocks, d, nb, wide, (float*)x, stride);
-    else jvf_decode_kernel<__bf16><<<(unsigned)grid, 256, 0, s>>>(codes, scales, blocks, d, nb, wide, (__bf16*)x, stride);
+    if (dtype == 0) jvf_decode_kernel<float><<<(unsigned)grid, 256, 0, s>>>(codes, scales, blocks, d, nb, rounds, (float*)x, stride);
+    else jvf_decode_kernel<__bf16><<<(unsigned)grid, 256, 0, s>>>(codes, scales, blocks, d, nb, rounds, (__bf16*)x, stride);
     return hipGetLastError();
 }
 

@@ -83,7 +83,7 @@ __device__ __forceinline__ void pack(const JvSxPrepare::Matrix& m, int d, int kp
 __device__ __forceinline__ JvSxQuery query_of(const float* lse, const float* w, const int32_t* targets, int64_t n, int i) {
     const int t = targets[i];
     const bool known = t >= 0 && t < n;
-    return {known ? lse[i] * 1.44269504088896341f : 0.0f, known ? (w ? w[i] : 1.0f) : 0.0f, known ? t : -1, 0};
+    return {known ? lse[i] * 1.44269504088896341f : __builtin_inff(), known ? (w ? w[i] : 1.0f) : 0.0f, known ? t : -1, 0};   // (no target: 2^-inf * 0)
 }
 
 // The weights are divided by the largest of them (`norm`, multiplied back in float32 at the end): an entry of g at a target is then just
@@ -144,27 +144,55 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
     m = top;
 }
 
-// a lane's part of a tile: MT queries, NT * 16 rows each.  `rows`: how many rows the tile has in all (NT * 16 of them are not this lane's)
+// A lane's part of a tile: MT queries, NT * 16 rows each.  `rows`: how many rows the tile has in all.  Four instructions a logit: the maximum, the
+// scaled difference (c <= 0: the smallest product is the largest logit), the exponential, the sum.
 template <class Core, int MT, int NT>
-__device__ __forceinline__ void add_tile(const f32x16 (&acc)[MT][NT], float c, int rows, float (&top)[MT], float (&sum)[MT]) {
-    const bool full = rows >= Core::TN;
+__device__ __forceinline__ void add_tile(f32x16 (&acc)[MT][NT], float c, int rows, float (&top)[MT], float (&sum)[MT]) {
+    const float none = c < 0.0f ? __builtin_inff() : -__builtin_inff();   // (what is behind the last row: its logit is -inf)
+    if (rows < Core::TN) {
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) acc[m][n][e] = Core::col(n, e) < rows ? acc[m][n][e] : none;
+    }
+    float best[MT];
+    if (c < 0.0f) {
+#pragma unroll
+        for (int m = 0; m < MT; m++) {
+            best[m] = none;
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) best[m] = fminf(best[m], acc[m][n][e]);
+        }
+    } else {
+#pragma unroll
+        for (int m = 0; m < MT; m++) {
+            best[m] = none;
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) best[m] = fmaxf(best[m], acc[m][n][e]);
+        }
+    }
 #pragma unroll
     for (int m = 0; m < MT; m++) {
-        float best = -__builtin_inff();
-        float z[NT][16];
-#pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) {
-                z[n][e] = full || Core::col(n, e) < rows ? acc[m][n][e] * c : -__builtin_inff();
-                best = fmaxf(best, z[n][e]);
-            }
-        const float now = fmaxf(top[m], best), ref = now == -__builtin_inff() ? 0.0f : now;
+        // (c = 0: every logit is 0, also that of an infinite product, but those behind the last row are left out)
+        const float now = fmaxf(top[m], best[m] == none ? -__builtin_inff() : best[m] * c), ref = now == -__builtin_inff() ? 0.0f : now;
         float s = sum[m] * exp2_(top[m] - ref);
+        if (c == 0.0f) {
 #pragma unroll
-        for (int n = 0; n < NT; n++)
+            for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int e = 0; e < 16; e++) s += exp2_(z[n][e] - ref);
+                for (int e = 0; e < 16; e++) s += acc[m][n][e] == none ? 0.0f : exp2_(acc[m][n][e] * 0.0f);
+        } else {
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) s += exp2_(fmaf(acc[m][n][e], c, -ref));
+        }
         top[m] = now;
         sum[m] = s;
     }
@@ -189,11 +217,9 @@ __device__ __forceinline__ void write_partials(const JvSxLoss& a, unsigned char*
         float m = sh[i * 2], s = sh[i * 2 + 1];
 #pragma unroll
         for (int k = 1; k < WN; k++) join(m, s, sh[(k * TM + i) * 2], sh[(k * TM + i) * 2 + 1]);
-        float* pm = a.part + (int64_t)split * a.mm.M + m0 + i;
-        float* ps = pm + (int64_t)a.splits * a.mm.M;
-        if (!a.first) join(m, s, *pm, *ps);
-        *pm = m;
-        *ps = s;
+        float2* p = a.part + (int64_t)(m0 + i) * a.splits + split;
+        if (!a.first) join(m, s, p->x, p->y);
+        *p = make_float2(m, s);
     }
 }
 
@@ -309,19 +335,36 @@ extern "C" hipError_t jvk_sx_loss(const JvSxLoss* a, int f32, hipStream_t s) {
 
 // one wave a query: join the partials, take the target's logit in float32 from the rows themselves
 template <typename T>
-__global__ __launch_bounds__(64) void jvs_join_kernel(const float* __restrict__ part, int splits, int nq, const T* __restrict__ q, int64_t q_stride,
+__global__ __launch_bounds__(64) void jvs_join_kernel(const float2* __restrict__ part, int splits, const T* __restrict__ q, int64_t q_stride,
                                                       const T* __restrict__ v, int64_t v_stride, int d, const int32_t* __restrict__ targets,
                                                       int64_t n, float scale, float* __restrict__ loss, float* __restrict__ lse) {
     const int i = blockIdx.x, lane = threadIdx.x;
-    float m = -__builtin_inff(), s = 0.0f;
-    for (int k = lane; k < splits; k += 64) join(m, s, part[(int64_t)k * nq + i], part[(int64_t)(splits + k) * nq + i]);
-    for (int off = 32; off >= 1; off >>= 1) join(m, s, __shfl_xor(m, off, 64), __shfl_xor(s, off, 64));
-    const float total = (m + log2_(s)) * 0.69314718055994531f;
     const int t = targets ? targets[i] : -1;
     const bool known = t >= 0 && t < n;
+    float m = -__builtin_inff(), s = 0.0f;
+#pragma unroll 4
+    for (int k = lane; k < splits; k += 64) {
+        const float2 p = part[(int64_t)i * splits + k];
+        join(m, s, p.x, p.y);
+    }
+    for (int off = 32; off >= 1; off >>= 1) join(m, s, __shfl_xor(m, off, 64), __shfl_xor(s, off, 64));
+    const float total = (m + log2_(s)) * 0.69314718055994531f;
     float dot = 0.0f;
-    if (known)
-        for (int k = lane; k < d; k += 64) dot = fmaf((float)q[(int64_t)i * q_stride + k], (float)v[(int64_t)t * v_stride + k], dot);
+    if (known) {
+        const T *a = q + (int64_t)i * q_stride, *b = v + (int64_t)t * v_stride;
+#pragma unroll 4
+        for (int k = lane * 4; k < d; k += 256) {
+            T x[4] = {(T)0.0f, (T)0.0f, (T)0.0f, (T)0.0f}, y[4] = {(T)0.0f, (T)0.0f, (T)0.0f, (T)0.0f};
+            if (k + 4 <= d) {
+                __builtin_memcpy(x, a + k, sizeof(x));
+                __builtin_memcpy(y, b + k, sizeof(y));
+            } else {
+                for (int e = 0; e < d - k; e++) x[e] = a[k + e], y[e] = b[k + e];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) dot = fmaf((float)x[e], (float)y[e], dot);
+        }
+    }
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) dot += __shfl_xor(dot, off, 64);
     if (lane == 0) {
@@ -330,33 +373,44 @@ __global__ __launch_bounds__(64) void jvs_join_kernel(const float* __restrict__ 
     }
 }
 
-extern "C" hipError_t jvk_sx_join(const float* part, int splits, int nq, const void* q, int64_t q_stride, const void* v, int64_t v_stride, int dtype,
+extern "C" hipError_t jvk_sx_join(const float2* part, int splits, int nq, const void* q, int64_t q_stride, const void* v, int64_t v_stride, int dtype,
                                   int d, const int32_t* targets, int64_t n, float scale, float* loss, float* lse, hipStream_t s) {
     if (nq <= 0) return hipSuccess;
     if (dtype == 0)
-        jvs_join_kernel<float><<<nq, 64, 0, s>>>(part, splits, nq, (const float*)q, q_stride, (const float*)v, v_stride, d, targets, n, scale, loss, lse);
+        jvs_join_kernel<float><<<nq, 64, 0, s>>>(part, splits, (const float*)q, q_stride, (const float*)v, v_stride, d, targets, n, scale, loss, lse);
     else
-        jvs_join_kernel<__bf16><<<nq, 64, 0, s>>>(part, splits, nq, (const __bf16*)q, q_stride, (const __bf16*)v, v_stride, d, targets, n, scale, loss, lse);
+        jvs_join_kernel<__bf16><<<nq, 64, 0, s>>>(part, splits, (const __bf16*)q, q_stride, (const __bf16*)v, v_stride, d, targets, n, scale, loss, lse);
     return hipGetLastError();
 }
 
 // ---------------------------------------------------------------------------------------------
 // backward: the logits again, as weights g
 // ---------------------------------------------------------------------------------------------
-// g of a lane's columns of one query, in place of the logits; `cols`: how many of the tile's columns are rows of the piece; `hit`: the target's column
+// g of a lane's columns of one query, in place of the logits; `cols`: how many of the tile's columns are rows of the piece; `hit`: the target's
+// column.  Three instructions a value; the target, which few tiles hold, and the last tile's end are seen to apart.
 template <class Core, int NT>
 __device__ __forceinline__ void weigh(f32x16 (&acc)[NT], const JvSxQuery& q, float c, int cols, int hit, bool lossy, float* rest) {
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-            const int at = Core::col(n, e);
-            float g = exp2_(fmaf(acc[n][e], c, -q.lse2));
-            if (at == hit) g -= 1.0f;
-            g = q.target >= 0 && at < cols ? g * q.w : 0.0f;
-            acc[n][e] = g;
-            if (at == hit && lossy) *rest = g - (float)(__bf16)g;   // (one lane holds it; three planes lack nothing)
-        }
+        for (int e = 0; e < 16; e++) acc[n][e] = exp2_(fmaf(acc[n][e], c, -q.lse2)) * q.w;
+    const int first = Core::col(0, 0) & ~31;   // this wave's columns
+    if (__any(hit >= first && hit < first + 32 * NT)) {
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int e = 0; e < 16; e++)
+                if (Core::col(n, e) == hit) {
+                    acc[n][e] -= q.w;
+                    if (lossy) *rest = acc[n][e] - (float)(__bf16)acc[n][e];   // (one lane holds it; three planes lack nothing)
+                }
+    }
+    if (cols < Core::TN) {
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) acc[n][e] = Core::col(n, e) < cols ? acc[n][e] : 0.0f;
+    }
 }
 
 __global__ __launch_bounds__(512) void jvs_weights_kernel(const JvSxWeights a) {
@@ -379,7 +433,7 @@ __global__ __launch_bounds__(512) void jvs_weights_kernel(const JvSxWeights a) {
 #pragma unroll
             for (int m = 0; m < 4; m++) {
                 const int r = w.m0 + P::row(m);
-                JvSxQuery q = {0.0f, 0.0f, -1, 0};
+                JvSxQuery q = {__builtin_inff(), 0.0f, -1, 0};
                 if (r < a.mm.M) q = a.query[r];
                 weigh<P>(acc[m], q, a.c, a.mm.N - w.n0, q.target >= 0 ? (int)(q.target - a.row0) - w.n0 : -1, a.planes == 1, a.rest + r);
             }
@@ -413,7 +467,7 @@ __global__ __launch_bounds__(T::THREADS) void jvs_weights_tile_kernel(const JvSx
 #pragma unroll
     for (int m = 0; m < MT; m++) {
         const int r = m0 + T::row(m);
-        JvSxQuery q = {0.0f, 0.0f, -1, 0};
+        JvSxQuery q = {__builtin_inff(), 0.0f, -1, 0};
         if (r < a.mm.M) q = a.query ? a.query[r] : query_of(a.lse, a.w, a.targets, a.n, r);
         weigh<T>(acc[m], q, a.c, a.mm.N - n0, q.target >= 0 ? (int)(q.target - a.row0) - n0 : -1, a.planes == 1, a.rest + r);
         if (a.planes == 0) {

@@ -37,7 +37,7 @@ struct JvSxLoss {
     float c;               // scale * log2(e)
     int32_t tile;          // jvk_sx_loss_plan's
     int32_t splits;        // workgroups that share a panel of queries
-    float* part;           // [2][splits][M]: maxima, then sums (log2 domain)
+    float2* part;          // [M][splits]: maximum and sum (log2 domain)
     int32_t first;         // 0: partials of an earlier piece of the rows are in `part` already, join them
 };
 // what the gradient needs of a query
@@ -90,7 +90,7 @@ hipError_t jvk_f8_score(const JvMmOut* a, hipStream_t s);
 hipError_t jvk_sx_prepare(const JvSxPrepare* a, hipStream_t s);
 int jvk_sx_loss_plan(int nq, int64_t rows, int* tile);   // splits, and the queries of a tile
 hipError_t jvk_sx_loss(const JvSxLoss* a, int f32, hipStream_t s);   // f32: operands are float32 as they lie
-hipError_t jvk_sx_join(const float* part, int splits, int nq, const void* q, int64_t q_stride, const void* v, int64_t v_stride, int dtype, int d,
+hipError_t jvk_sx_join(const float2* part, int splits, int nq, const void* q, int64_t q_stride, const void* v, int64_t v_stride, int dtype, int d,
                        const int32_t* targets, int64_t n, float scale, float* loss, float* lse, hipStream_t s);
 hipError_t jvk_sx_weights(const JvSxWeights* a, int large, hipStream_t s);   // (planes = 0: float32 as it lies)
 // dq = G V and dv = G^T Q (nullptr: not asked for)

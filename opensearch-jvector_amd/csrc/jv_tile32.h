@@ -74,8 +74,9 @@ struct Tile32 {
             const int back = cols < 4 ? 0 : min(max(first + (r & ~3) + 4 - cols, 0), 3);
             return (r & ~3) + min((r & 3) + back, 3);
         }
-        // eight k's (16 kk + 8 h ..) of row r, or of the column at `r` (place); `valid`: components of this step, `k` in all (k along)
-        __device__ __forceinline__ void read(const unsigned char* base, int r, int kk, int valid, int k, bf16x8 (&p)[3]) const {
+        // eight k's (16 kk + 8 h ..) of row r, or of the column at `r` (place); LAST: the step has `valid` of 32 components, `k` in all (k along)
+        template <bool LAST>
+        static __device__ __forceinline__ void read(const unsigned char* base, int r, int kk, int valid, int k, bf16x8 (&p)[3]) {
             const int h = (threadIdx.x >> 5) & 1;
             float x[8];
             if constexpr (!ACROSS) {
@@ -84,7 +85,7 @@ struct Tile32 {
                 for (int half = 0; half < 2; half++) {
                     const int piece = 4 * kk + 2 * h + half;
                     f32x4 v = *(const f32x4*)(row + ((piece ^ (r & 7)) << 4));
-                    if (valid < 32) {
+                    if constexpr (LAST) {
                         const int back = k < 4 || 4 * piece >= valid ? 0 : max(4 * piece + 4 - valid, 0);
                         if (back & 1) v = (f32x4){v[1], v[2], v[3], v[3]};
                         if (back & 2) v = (f32x4){v[2], v[3], v[3], v[3]};
@@ -103,6 +104,26 @@ struct Tile32 {
         }
     };
 
+    // one step
+    template <bool LAST>
+    static __device__ __forceinline__ void multiply(const JvMm& a, const unsigned char* base, const int (&ra)[MT], const int (&rb)[NT], int valid, f32x16 (&acc)[MT][NT]) {
+#pragma unroll
+        for (int kk = 0; kk < 2; kk++) {
+            bf16x8 va[MT][3], vb[NT][3];
+#pragma unroll
+            for (int t = 0; t < MT; t++) Side<TA, GA>::template read<LAST>(base, ra[t], kk, valid, a.k, va[t]);
+#pragma unroll
+            for (int t = 0; t < NT; t++) Side<TB, GB>::template read<LAST>(base + GA * GROUP, rb[t], kk, valid, a.k, vb[t]);
+#pragma unroll
+            for (int g = 0; g < 6; g++) {
+                const int pa = (0x052 >> (2 * g)) & 3, pb = (0x118 >> (2 * g)) & 3;
+#pragma unroll
+                for (int m = 0; m < MT; m++)
+#pragma unroll
+                    for (int n = 0; n < NT; n++) acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vb[n][pb], va[m][pa], acc[m][n], 0, 0, 0);
+            }
+        }
+    }
     // C tile at (m0, n0), steps [k0, k1) of ceil(k / 32)
     static __device__ __forceinline__ void run(const JvMm& a, int m0, int n0, int k0, int k1, unsigned char* smem, f32x16 (&acc)[MT][NT]) {
         const int w = threadIdx.x >> 6, r31 = threadIdx.x & 31, wm = w % WM, wn = w / WM;
@@ -133,23 +154,8 @@ struct Tile32 {
             if (s + NS - 1 < k1) stage(s + NS - 1);
             wait_step<NS, PER>(k1 - 1 - s);
             const unsigned char* base = smem + (s - k0) % NS * BUF;
-            const int valid = a.k - s * 32;
-#pragma unroll
-            for (int kk = 0; kk < 2; kk++) {
-                bf16x8 va[MT][3], vb[NT][3];
-#pragma unroll
-                for (int t = 0; t < MT; t++) sa.read(base, ra[t], kk, valid, a.k, va[t]);
-#pragma unroll
-                for (int t = 0; t < NT; t++) sb.read(base + GA * GROUP, rb[t], kk, valid, a.k, vb[t]);
-#pragma unroll
-                for (int g = 0; g < 6; g++) {
-                    const int pa = (0x052 >> (2 * g)) & 3, pb = (0x118 >> (2 * g)) & 3;
-#pragma unroll
-                    for (int m = 0; m < MT; m++)
-#pragma unroll
-                        for (int n = 0; n < NT; n++) acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vb[n][pb], va[m][pa], acc[m][n], 0, 0, 0);
-                }
-            }
+            if ((s + 1) * 32 <= a.k) multiply<false>(a, base, ra, rb, 32, acc);
+            else multiply<true>(a, base, ra, rb, a.k - s * 32, acc);   // (apart: the masks would cost every step a third more)
             // every fragment read of this buffer has returned before any wave stages into it again
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         }
