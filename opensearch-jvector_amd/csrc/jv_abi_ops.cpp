@@ -78,7 +78,7 @@ int check_shape(int64_t n, int d, const char* what) {
 struct Plan {
     int P, segs, dp, kq;              // planes, segments; d and nq padded to 64
     int64_t rows_f, rows_b;           // rows of one piece, forward (only if the vectors have to be laid out) / backward
-    int tile, splits_f, splits_q, large;
+    int tile, splits_f, splits_q, large, large_grads;
     int64_t off_q, off_v, off_part, off_query, off_norm, off_rest, off_g, off_slab, bytes;
 };
 
@@ -113,19 +113,20 @@ Plan make_plan(int dtype, int nq, int64_t n, int d, uint32_t what) {
     };
     p.off_q = take((int64_t)nq * row);
     if (what & JV_SOFTMAX_LOSS) {
-        p.splits_f = jvk_sx_loss_plan(nq, n, &p.tile);
+        p.splits_f = jvk_sx_loss_plan(nq, n, d, dtype == JV_DTYPE_F32, &p.tile);
         p.off_part = take((int64_t)p.splits_f * nq * 8);
         p.off_v = take(std::min<int64_t>(p.rows_f, n) * row);
     }
     if (what & (JV_SOFTMAX_QUERY_GRAD | JV_SOFTMAX_VECTOR_GRAD)) {
-        p.large = jvk_sx_large(nq, std::min<int64_t>(p.rows_b, n));
+        p.large = jvk_sx_large(nq, std::min<int64_t>(p.rows_b, n), d, dtype == JV_DTYPE_F32);
+        p.large_grads = jvk_sx_large_grads(p.large, d);
         p.off_v = take(std::min<int64_t>(p.rows_b, n) * row);
         p.off_query = take((int64_t)nq * sizeof(JvSxQuery));
         p.off_norm = take(4);
         p.off_rest = take((int64_t)nq * 4);
         p.off_g = take((int64_t)p.kq * p.P * p.rows_b * 2);
         if (what & JV_SOFTMAX_QUERY_GRAD) {
-            p.splits_q = jvk_sx_grad_splits(nq, d, std::min<int64_t>(p.rows_b, n), p.P == 3, p.large);
+            p.splits_q = jvk_sx_grad_splits(nq, d, std::min<int64_t>(p.rows_b, n), p.P == 3, p.large_grads);
             p.off_slab = take((int64_t)p.splits_q * nq * p.dp * 4);
         }
     }
@@ -344,7 +345,7 @@ int jv_softmax_grad_device(const jv_softmax_params* p, const float* d_lse, const
             o.mul = p->scale, o.norm = norm, o.dtype = p->dtype, o.splits = 1, o.add = 0;
             o.out = (char*)d_out_vector_grad + at * vector_grad_stride * size_of(p->dtype), o.ldo = vector_grad_stride;
         }
-        CHK(jvk_sx_grads(d_out_query_grad ? &q : nullptr, d_out_vector_grad ? &o : nullptr, f32, plan.large, s));
+        CHK(jvk_sx_grads(d_out_query_grad ? &q : nullptr, d_out_vector_grad ? &o : nullptr, f32, plan.large_grads, s));
     }
     if (d_out_query_grad && !direct) {
         const int splits = std::min(plan.splits_q, splits_of(plan, std::min<int64_t>(plan.rows_b, p->n), f32));

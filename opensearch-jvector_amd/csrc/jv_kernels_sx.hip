@@ -271,17 +271,22 @@ __global__ __launch_bounds__(T::THREADS) void jvs_loss_tile_kernel(const JvSxLos
     write_partials<T::TM, MT, WN>(a, smem, m0, split, (threadIdx.x >> 6) / WM, [](int m) { return T::row(m); }, top, sum);
 }
 
-// the large tiles where they fill the chip
-static bool large(int nq, int64_t rows) { return nq > 64 && ((nq + 255) / 256) * ((rows + 255) / 256) >= 192; }
-extern "C" int jvk_sx_large(int nq, int64_t rows) { return large(nq, rows); }
+// The large tiles where they fill the chip.  float32 only with more than 128 components: its planes are worth laying out when they are read often
+// enough (step 300 x 100 000 x 128: 618 us so, 417 us as it lies; step 777 x 30 011 x 381: 730 and 799 us).
+static bool large(int nq, int64_t rows, int d, bool f32) {
+    return nq > 64 && ((nq + 255) / 256) * ((rows + 255) / 256) >= 192 && (!f32 || d > 128);
+}
+extern "C" int jvk_sx_large(int nq, int64_t rows, int d, int f32) { return large(nq, rows, d, f32); }
+// The gradients' products have d columns: with up to 128 half a large tile would be multiplied for nothing.
+extern "C" int jvk_sx_large_grads(int large, int d) { return large && d > 128; }
 
 // Queries and rows of the tiles that a product of nq queries with `rows` rows takes:
 //   256 x 256  where they fill the chip (large);
 //   32 x 128 and 64 x 128 for up to 32 and 64 queries: the rows are streamed, and as little as possible is multiplied for nothing;
 //   128 x 128 otherwise, but where that is no more than one tile a CU 64 x 64, with four steps of k under way: the way to memory and the
 //   multiplications of one tile's steps are what counts then (float32, 118 x 18 x 843: 66 -> 24 us)
-static int tile_of(int nq, int64_t rows) {
-    if (large(nq, rows)) return 256;
+static int tile_of(int nq, int64_t rows, int d, bool f32) {
+    if (large(nq, rows, d, f32)) return 256;
     if (nq <= 32) return 32;
     const int64_t tiles = (int64_t)((nq + 127) / 128) * ((rows + 127) / 128);
     return tiles <= 256 ? 65 : nq <= 64 ? 64 : 128;   // (65: 64 x 64)
@@ -290,8 +295,8 @@ static int rows_of_tile(int tile) { return tile == 256 ? 256 : tile == 65 ? 64 :
 static int queries_of_tile(int tile) { return tile == 65 ? 64 : tile; }
 
 // workgroups that share a panel's rows: one for each CU with the large tiles, two or three with the small ones
-extern "C" int jvk_sx_loss_plan(int nq, int64_t rows, int* tile) {
-    const int t = tile_of(nq, rows), tm = queries_of_tile(t), tn = rows_of_tile(t), full = t == 256 ? 256 : t == 128 || t == 65 ? 512 : 768;
+extern "C" int jvk_sx_loss_plan(int nq, int64_t rows, int d, int f32, int* tile) {
+    const int t = tile_of(nq, rows, d, f32), tm = queries_of_tile(t), tn = rows_of_tile(t), full = t == 256 ? 256 : t == 128 || t == 65 ? 512 : 768;
     const int64_t panels = std::max((nq + tm - 1) / tm, 1), tiles = std::max<int64_t>((rows + tn - 1) / tn, 1);
     *tile = t;
     return (int)std::min(std::max<int64_t>(full / panels, 1), tiles);
@@ -505,7 +510,7 @@ static hipError_t weights_tile(const JvSxWeights& a, hipStream_t s) {
 }
 
 static hipError_t weights_small(const JvSxWeights& a, hipStream_t s) {   // (G's padded queries are a multiple of 64: no tile of 32)
-    const int t = tile_of(a.mm.M, a.mm.N);
+    const int t = tile_of(a.mm.M, a.mm.N, a.mm.k, a.planes == 0);
     const bool few = t == 65 || (t == 32 && (a.mm.N + 127) / 128 <= 256);
     if (a.planes == 0) {
         if (few) return weights_tile<Tile32<1, 1, 2, 2, 4, false, false>>(a, s);

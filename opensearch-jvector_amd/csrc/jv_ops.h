@@ -88,15 +88,16 @@ hipError_t jvk_f8_decode(const uint8_t* codes, const uint8_t* scales, int64_t n,
 hipError_t jvk_f8_score(const JvMmOut* a, hipStream_t s);
 
 hipError_t jvk_sx_prepare(const JvSxPrepare* a, hipStream_t s);
-int jvk_sx_loss_plan(int nq, int64_t rows, int* tile);   // splits, and the queries of a tile
+int jvk_sx_loss_plan(int nq, int64_t rows, int d, int f32, int* tile);   // splits, and the queries of a tile
 hipError_t jvk_sx_loss(const JvSxLoss* a, int f32, hipStream_t s);   // f32: operands are float32 as they lie
 hipError_t jvk_sx_join(const float2* part, int splits, int nq, const void* q, int64_t q_stride, const void* v, int64_t v_stride, int dtype, int d,
                        const int32_t* targets, int64_t n, float scale, float* loss, float* lse, hipStream_t s);
 hipError_t jvk_sx_weights(const JvSxWeights* a, int large, hipStream_t s);   // (planes = 0: float32 as it lies)
 // dq = G V and dv = G^T Q (nullptr: not asked for)
 int jvk_sx_grad_splits(int nq, int d, int64_t rows, int f32, int large);
-hipError_t jvk_sx_grads(const JvMmOut* q, const JvMmOut* v, int f32, int large, hipStream_t s);
-int jvk_sx_large(int nq, int64_t rows);   // whether a piece of the rows takes the large tiles
+hipError_t jvk_sx_grads(const JvMmOut* q, const JvMmOut* v, int f32, int large, hipStream_t s);   // large: of jvk_sx_large_grads
+int jvk_sx_large_grads(int large, int d);   // and whether the gradients' products do
+int jvk_sx_large(int nq, int64_t rows, int d, int f32);   // whether a piece of the rows takes the large tiles for g
 hipError_t jvk_sx_finish(const float* slab, int splits, int64_t rows, int d, int64_t lds, const float* rest, const JvSxQuery* query, const void* v, int64_t v_stride,
                          float mul, const float* norm, void* out, int dtype, int64_t ldo, hipStream_t s);
 hipError_t jvk_sx_fill(void* out, int dtype, int64_t stride, int64_t rows, int d, float value, hipStream_t s);

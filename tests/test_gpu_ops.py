@@ -404,7 +404,7 @@ def test_scores_on_the_large_tiles(torch, ops, out, nq, n, d):
 
 
 @pytest.mark.parametrize("dtype,nq,n,d,pad", [("bf16", 300, 30011, 200, 0), ("f32", 257, 26000, 70, 3), ("bf16", 1030, 10001, 384, 8), ("bf16", 80, 60000, 64, 0),
-                                              ("f32", 600, 17000, 128, 0)])
+                                              ("f32", 600, 17000, 128, 0), ("f32", 600, 17000, 132, 0), ("bf16", 600, 17000, 128, 0), ("f32", 500, 25000, 129, 2)])
 def test_softmax_on_the_large_tiles(torch, ops, dtype, nq, n, d, pad):
     q, v, t, w, _, _, t64, _ = loss_case(torch, nq, n, d, dtype, pad)
     scale = 15.0
