@@ -20,6 +20,7 @@ namespace {
 
 constexpr int64_t kMaxRows = 0x7fffffffll - 65536;   // a tile behind the last row still has an int32 number
 constexpr int64_t kMaxStride = 1ll << 31;
+constexpr int32_t kNoEnd = 0x7fffff00;          // JvMm.end_b of rows that have all of k
 
 // the caller's current device comes back on every way out
 class OnDevice {
@@ -79,7 +80,7 @@ struct Plan {
     int P, segs, dp, kq;              // planes, segments; d and nq padded to 64
     int64_t rows_f, rows_b;           // rows of one piece, forward (only if the vectors have to be laid out) / backward
     int tile, splits_f, splits_q, large, large_grads;
-    int64_t off_q, off_v, off_part, off_query, off_norm, off_rest, off_g, off_slab, bytes;
+    int64_t off_q, off_v, off_part, off_hit, off_query, off_norm, off_rest, off_g, off_slab, bytes;
 };
 
 // MB of one piece's weights g: few large pieces, for every piece writes and reads dq's partial sums again and starts its tiles anew (step
@@ -115,6 +116,7 @@ Plan make_plan(int dtype, int nq, int64_t n, int d, uint32_t what) {
     if (what & JV_SOFTMAX_LOSS) {
         p.splits_f = jvk_sx_loss_plan(nq, n, d, dtype == JV_DTYPE_F32, &p.tile);
         p.off_part = take((int64_t)p.splits_f * nq * 8);
+        p.off_hit = take((int64_t)nq * 4);
         p.off_v = take(std::min<int64_t>(p.rows_f, n) * row);
     }
     if (what & (JV_SOFTMAX_QUERY_GRAD | JV_SOFTMAX_VECTOR_GRAD)) {
@@ -134,15 +136,15 @@ Plan make_plan(int dtype, int nq, int64_t n, int d, uint32_t what) {
     return p;
 }
 
-// rows as a product takes them: the caller's own where they are bf16, 4-B aligned and whole steps, or float32
-// of at least four components and the tiles small
+// Rows as a product takes them: the caller's own where they are 4-B aligned and bf16 with whole 16 B of components (the queries, whose padding
+// stands for zeros behind the vectors', with whole steps of them), or float32 of at least four components where the tiles are small.
 struct Rows {
     const char* p;
     int64_t stride;   // bytes
     bool ready;
 };
-Rows rows_of(const void* p, int64_t stride, int d, int dtype, bool large) {
-    const bool ready = dtype == JV_DTYPE_F32 ? !large && d >= 4 : (uintptr_t)p % 4 == 0 && stride % 2 == 0 && d % 64 == 0;
+Rows rows_of(const void* p, int64_t stride, int d, int dtype, bool large, int whole) {
+    const bool ready = dtype == JV_DTYPE_F32 ? !large && d >= 4 : (uintptr_t)p % 4 == 0 && stride % 2 == 0 && d % whole == 0;
     return {(const char*)p, stride * size_of(dtype), ready};
 }
 
@@ -174,6 +176,7 @@ JvMm logits(const Plan& plan, int nq, int d) {
     JvMm mm{};
     mm.M = nq, mm.k = d, mm.kph = plan.dp / 32, mm.segs = plan.segs;
     mm.plane_a = mm.plane_b = (int64_t)plan.dp * 2;
+    mm.end_b = kNoEnd;
     return mm;
 }
 
@@ -235,7 +238,7 @@ int jv_score_blocks_device(int32_t device, const uint8_t* d_query_codes, const u
     a.mm.kph = 2 * blocks;
     a.mm.a = (const char*)d_query_codes, a.mm.b = (const char*)d_codes;
     a.mm.lda = a.mm.ldb = (int64_t)blocks * 128;
-    a.mm.M = nq, a.mm.N = n, a.mm.segs = 1;
+    a.mm.M = nq, a.mm.N = n, a.mm.segs = 1, a.mm.end_b = kNoEnd;
     a.mm.sa = d_query_scales, a.mm.sb = d_scales;
     a.mul = 1.0f, a.dtype = dtype, a.out = d_out_scores, a.ldo = row_stride, a.splits = 1;
     CHK(jvk_f8_score(&a, (hipStream_t)hip_stream));
@@ -263,25 +266,26 @@ int jv_softmax_loss_device(const jv_softmax_params* p, float* d_out_loss, float*
     if (p->nq > 0) {
         char* ws = (char*)p->workspace;
         const bool large = plan.tile == 256, f32 = p->dtype == JV_DTYPE_F32 && !large;
-        const Rows rq = rows_of(p->queries, p->query_stride, p->d, p->dtype, large), rv = rows_of(p->vectors, p->vector_stride, p->d, p->dtype, large);
+        const Rows rq = rows_of(p->queries, p->query_stride, p->d, p->dtype, large, 64), rv = rows_of(p->vectors, p->vector_stride, p->d, p->dtype, large, 8);
         const int64_t step = rv.ready ? std::max<int64_t>(p->n, 1) : plan.rows_f;
         JvSxLoss a{};
         a.mm = logits(plan, p->nq, p->d);
         a.c = p->scale * 1.44269504088896341f;
+        a.targets = p->targets, a.hit = (float*)(ws + plan.off_hit);
+        if (rv.ready && !f32) a.mm.end_b = p->d * 2;
         a.tile = plan.tile, a.splits = p->n > 0 ? plan.splits_f : 0, a.part = (float2*)(ws + plan.off_part);
         JvSxPrepare pre{};
         pre.dtype = p->dtype, pre.d = p->d, pre.kp = f32 ? 4 : plan.dp;   // (float32 as it lies: only rows of fewer than four are laid out)
         take_rows(rq, p->queries, p->query_stride, p->dtype, 0, p->nq, plan, pre.kp, ws + plan.off_q, &pre.m[0], &a.mm.a, &a.mm.lda);
         for (int64_t at = 0; at < p->n; at += step) {
             a.mm.N = (int)std::min<int64_t>(step, p->n - at);
-            a.first = at == 0;
+            a.first = at == 0, a.row0 = at;
             take_rows(rv, p->vectors, p->vector_stride, p->dtype, at, a.mm.N, plan, pre.kp, ws + plan.off_v, &pre.m[1], &a.mm.b, &a.mm.ldb);
             CHK(jvk_sx_prepare(&pre, s));
             pre.m[0].rows = 0;
             CHK(jvk_sx_loss(&a, f32, s));
         }
-        CHK(jvk_sx_join(a.part, a.splits, p->nq, p->queries, p->query_stride, p->vectors, p->vector_stride, p->dtype, p->d, p->targets, p->n, p->scale, d_out_loss,
-                        d_out_lse, s));
+        CHK(jvk_sx_join(a.part, a.splits, p->nq, a.hit, p->targets, p->n, d_out_loss, d_out_lse, s));
     }
     return done(hip_stream);
 }
@@ -306,10 +310,11 @@ int jv_softmax_grad_device(const jv_softmax_params* p, const float* d_lse, const
     }
     char* ws = (char*)p->workspace;
     const bool f32 = p->dtype == JV_DTYPE_F32 && !plan.large;
-    const Rows rq = rows_of(p->queries, p->query_stride, p->d, p->dtype, plan.large), rv = rows_of(p->vectors, p->vector_stride, p->d, p->dtype, plan.large);
+    const Rows rq = rows_of(p->queries, p->query_stride, p->d, p->dtype, plan.large, 64), rv = rows_of(p->vectors, p->vector_stride, p->d, p->dtype, plan.large, 8);
     JvSxWeights w{};
     w.mm = logits(plan, p->nq, p->d);
     w.c = p->scale * 1.44269504088896341f;
+    if (rv.ready && !f32) w.mm.end_b = p->d * 2;
     w.planes = f32 ? 0 : plan.P, w.g = ws + plan.off_g;
     JvSxQuery* query = (JvSxQuery*)(ws + plan.off_query);
     float* norm = f32 ? nullptr : (float*)(ws + plan.off_norm);   // (float32 g needs no common unit and lacks nothing at a target)
@@ -330,10 +335,10 @@ int jv_softmax_grad_device(const jv_softmax_params* p, const float* d_lse, const
         JvMmOut o{}, q;
         o.mm.segs = plan.segs;
         o.mm.a = (const char*)w.g, o.mm.lda = f32 ? (int64_t)w.kv * 4 : (int64_t)plan.P * w.kv * 2, o.mm.plane_a = (int64_t)w.kv * 2;
-        o.mm.N = p->d, o.mm.plane_b = (int64_t)plan.dp * 2, o.mm.cb = f32 ? p->d : plan.dp;
+        o.mm.N = p->d, o.mm.plane_b = (int64_t)plan.dp * 2, o.mm.end_b = kNoEnd;
         if (d_out_query_grad) {   // G times the piece's vectors: k = its rows
             o.mm.M = p->nq, o.mm.k = w.kv, o.mm.kph = w.kv / 32;
-            o.mm.b = w.mm.b, o.mm.ldb = w.mm.ldb, o.mm.kb = rows;
+            o.mm.b = w.mm.b, o.mm.ldb = w.mm.ldb, o.mm.kb = rows, o.mm.cb = rv.ready || f32 ? p->d : plan.dp;
             o.mul = 1.0f, o.out = ws + plan.off_slab, o.ldo = plan.dp, o.add = at > 0;
             o.splits = std::min(plan.splits_q, splits_of(plan, rows, f32));   // (only the last piece can be that short: it adds to the first ranges)
             if (direct) o.mul = p->scale, o.out = d_out_query_grad, o.ldo = query_grad_stride;
@@ -341,7 +346,7 @@ int jv_softmax_grad_device(const jv_softmax_params* p, const float* d_lse, const
         }
         if (d_out_vector_grad) {   // G across times the queries: k = the queries
             o.mm.M = rows, o.mm.k = plan.kq, o.mm.kph = plan.kq / 32, o.mm.ka = plan.kq, o.mm.ca = w.kv;
-            o.mm.b = w.mm.a, o.mm.ldb = w.mm.lda, o.mm.kb = p->nq;
+            o.mm.b = w.mm.a, o.mm.ldb = w.mm.lda, o.mm.kb = p->nq, o.mm.cb = rq.ready || f32 ? p->d : plan.dp;
             o.mul = p->scale, o.norm = norm, o.dtype = p->dtype, o.splits = 1, o.add = 0;
             o.out = (char*)d_out_vector_grad + at * vector_grad_stride * size_of(p->dtype), o.ldo = vector_grad_stride;
         }

@@ -146,8 +146,23 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
 
 // A lane's part of a tile: MT queries, NT * 16 rows each.  `rows`: how many rows the tile has in all.  Four instructions a logit: the maximum, the
 // scaled difference (c <= 0: the smallest product is the largest logit), the exponential, the sum.
+// `m0`, `n0`: where the tile lies; the target's own logit is taken from the same product, so that a loss near 0 keeps its digits.
 template <class Core, int MT, int NT>
-__device__ __forceinline__ void add_tile(f32x16 (&acc)[MT][NT], float c, int rows, float (&top)[MT], float (&sum)[MT]) {
+__device__ __forceinline__ void add_tile(const JvSxLoss& a, f32x16 (&acc)[MT][NT], int m0, int n0, const int (&want)[MT], float (&top)[MT], float (&sum)[MT]) {
+    const float c = a.c;
+    const int rows = a.mm.N - n0;
+    const int first = Core::col(0, 0) & ~31;   // this wave's columns
+#pragma unroll
+    for (int m = 0; m < MT; m++) {
+        const int at = want[m] - n0;
+        if (__any(at >= first && at < first + 32 * NT)) {
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int e = 0; e < 16; e++)
+                    if (Core::col(n, e) == at) a.hit[m0 + Core::row(m)] = acc[m][n][e] * c;
+        }
+    }
     const float none = c < 0.0f ? __builtin_inff() : -__builtin_inff();   // (what is behind the last row: its logit is -inf)
     if (rows < Core::TN) {
 #pragma unroll
@@ -198,6 +213,12 @@ __device__ __forceinline__ void add_tile(f32x16 (&acc)[MT][NT], float c, int row
     }
 }
 
+// the piece's row that is query `q`'s target, far away if there is none
+__device__ __forceinline__ int wanted(const JvSxLoss& a, int q) {
+    const int64_t at = q < a.mm.M && a.targets ? a.targets[q] - a.row0 : -1;
+    return at >= 0 && at < a.mm.N ? (int)at : -0x40000000;
+}
+
 // joins what the lanes and waves of a workgroup hold of the same queries and writes one partial for each of the panel's queries
 template <int TM, int MT, int WN, class Row>
 __device__ __forceinline__ void write_partials(const JvSxLoss& a, unsigned char* smem, int m0, int split, int wn, Row&& row, float (&top)[MT], float (&sum)[MT]) {
@@ -233,8 +254,9 @@ __global__ __launch_bounds__(512) void jvs_loss_pipe_kernel(const JvSxLoss a) {
     if (!share.at(0, L)) return;
     const int split = L / panels, m0 = (L - split * panels) * P::TM;
     float top[4], sum[4];
+    int want[4];
 #pragma unroll
-    for (int m = 0; m < 4; m++) top[m] = -__builtin_inff(), sum[m] = 0.0f;
+    for (int m = 0; m < 4; m++) top[m] = -__builtin_inff(), sum[m] = 0.0f, want[m] = wanted(a, m0 + P::row(m));
     if (split < tiles)
         P::run(
             a.mm, smem,
@@ -245,7 +267,7 @@ __global__ __launch_bounds__(512) void jvs_loss_pipe_kernel(const JvSxLoss a) {
                 return true;
             },
             [&](const Work& w, f32x16 (&acc)[4][2]) -> int {
-                add_tile<P>(acc, a.c, a.mm.N - w.n0, top, sum);
+                add_tile<P>(a, acc, w.m0, w.n0, want, top, sum);
                 return 0;
             });
     write_partials<P::TM, 4, 4>(a, smem, m0, split, threadIdx.x >> 7, [](int m) { return P::row(m); }, top, sum);
@@ -261,20 +283,21 @@ __global__ __launch_bounds__(T::THREADS) void jvs_loss_tile_kernel(const JvSxLos
     if (!share.at(0, L)) return;
     const int split = L / panels, m0 = (L - split * panels) * T::TM;
     float top[MT], sum[MT];
+    int want[MT];
 #pragma unroll
-    for (int m = 0; m < MT; m++) top[m] = -__builtin_inff(), sum[m] = 0.0f;
+    for (int m = 0; m < MT; m++) top[m] = -__builtin_inff(), sum[m] = 0.0f, want[m] = wanted(a, m0 + T::row(m));
     for (int t = split; t < tiles; t += a.splits) {
         f32x16 acc[MT][NT];
         T::run(a.mm, m0, t * T::TN, 0, T::steps(a.mm), smem, acc);
-        add_tile<T>(acc, a.c, a.mm.N - t * T::TN, top, sum);
+        add_tile<T>(a, acc, m0, t * T::TN, want, top, sum);
     }
     write_partials<T::TM, MT, WN>(a, smem, m0, split, (threadIdx.x >> 6) / WM, [](int m) { return T::row(m); }, top, sum);
 }
 
-// The large tiles where they fill the chip.  float32 only with more than 128 components: its planes are worth laying out when they are read often
+// The large tiles where they fill the chip and more than half of one is queries.  float32 only with more than 128 components: its planes are worth laying out when they are read often
 // enough (step 300 x 100 000 x 128: 618 us so, 417 us as it lies; step 777 x 30 011 x 381: 730 and 799 us).
 static bool large(int nq, int64_t rows, int d, bool f32) {
-    return nq > 64 && ((nq + 255) / 256) * ((rows + 255) / 256) >= 192 && (!f32 || d > 128);
+    return nq > 128 && ((nq + 255) / 256) * ((rows + 255) / 256) >= 192 && (!f32 || d > 128);
 }
 extern "C" int jvk_sx_large(int nq, int64_t rows, int d, int f32) { return large(nq, rows, d, f32); }
 // The gradients' products have d columns: with up to 128 half a large tile would be multiplied for nothing.
@@ -338,14 +361,11 @@ extern "C" hipError_t jvk_sx_loss(const JvSxLoss* a, int f32, hipStream_t s) {
     return hipGetLastError();
 }
 
-// one wave a query: join the partials, take the target's logit in float32 from the rows themselves
-template <typename T>
-__global__ __launch_bounds__(64) void jvs_join_kernel(const float2* __restrict__ part, int splits, const T* __restrict__ q, int64_t q_stride,
-                                                      const T* __restrict__ v, int64_t v_stride, int d, const int32_t* __restrict__ targets,
-                                                      int64_t n, float scale, float* __restrict__ loss, float* __restrict__ lse) {
-    const int i = blockIdx.x, lane = threadIdx.x;
-    const int t = targets ? targets[i] : -1;
-    const bool known = t >= 0 && t < n;
+// one wave a query: join the partials
+__global__ __launch_bounds__(256) void jvs_join_kernel(const float2* __restrict__ part, int splits, int nq, const float* __restrict__ hit,
+                                                       const int32_t* __restrict__ targets, int64_t n, float* __restrict__ loss, float* __restrict__ lse) {
+    const int i = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (i >= nq) return;
     float m = -__builtin_inff(), s = 0.0f;
 #pragma unroll 4
     for (int k = lane; k < splits; k += 64) {
@@ -353,38 +373,15 @@ __global__ __launch_bounds__(64) void jvs_join_kernel(const float2* __restrict__
         join(m, s, p.x, p.y);
     }
     for (int off = 32; off >= 1; off >>= 1) join(m, s, __shfl_xor(m, off, 64), __shfl_xor(s, off, 64));
-    const float total = (m + log2_(s)) * 0.69314718055994531f;
-    float dot = 0.0f;
-    if (known) {
-        const T *a = q + (int64_t)i * q_stride, *b = v + (int64_t)t * v_stride;
-#pragma unroll 4
-        for (int k = lane * 4; k < d; k += 256) {
-            T x[4] = {(T)0.0f, (T)0.0f, (T)0.0f, (T)0.0f}, y[4] = {(T)0.0f, (T)0.0f, (T)0.0f, (T)0.0f};
-            if (k + 4 <= d) {
-                __builtin_memcpy(x, a + k, sizeof(x));
-                __builtin_memcpy(y, b + k, sizeof(y));
-            } else {
-                for (int e = 0; e < d - k; e++) x[e] = a[k + e], y[e] = b[k + e];
-            }
-#pragma unroll
-            for (int e = 0; e < 4; e++) dot = fmaf((float)x[e], (float)y[e], dot);
-        }
-    }
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) dot += __shfl_xor(dot, off, 64);
-    if (lane == 0) {
-        lse[i] = total;
-        loss[i] = known ? total - scale * dot : 0.0f;
-    }
+    if (lane != 0) return;
+    const int t = targets ? targets[i] : -1;
+    lse[i] = (m + log2_(s)) * 0.69314718055994531f;
+    loss[i] = t >= 0 && t < n ? ((m - hit[i]) + log2_(s)) * 0.69314718055994531f : 0.0f;
 }
 
-extern "C" hipError_t jvk_sx_join(const float2* part, int splits, int nq, const void* q, int64_t q_stride, const void* v, int64_t v_stride, int dtype,
-                                  int d, const int32_t* targets, int64_t n, float scale, float* loss, float* lse, hipStream_t s) {
+extern "C" hipError_t jvk_sx_join(const float2* part, int splits, int nq, const float* hit, const int32_t* targets, int64_t n, float* loss, float* lse, hipStream_t s) {
     if (nq <= 0) return hipSuccess;
-    if (dtype == 0)
-        jvs_join_kernel<float><<<nq, 64, 0, s>>>(part, splits, (const float*)q, q_stride, (const float*)v, v_stride, d, targets, n, scale, loss, lse);
-    else
-        jvs_join_kernel<__bf16><<<nq, 64, 0, s>>>(part, splits, (const __bf16*)q, q_stride, (const __bf16*)v, v_stride, d, targets, n, scale, loss, lse);
+    jvs_join_kernel<<<(nq + 3) / 4, 256, 0, s>>>(part, splits, nq, hit, targets, n, loss, lse);
     return hipGetLastError();
 }
 

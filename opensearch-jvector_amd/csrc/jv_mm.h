@@ -145,7 +145,7 @@ struct Tile {
                 glds16(src[i] + offa + (TA ? (int64_t)min(kin * 64 + krow[i], a.ka - 1) * a.lda : 0), dst + (i * WAVES + w) * (TA ? 1024 : GROUP));
 #pragma unroll
             for (int i = 0; i < CB; i++)
-                glds16(src[CA + i] + offb + (TB ? (int64_t)min(kin * 64 + krow[CA + i], a.kb - 1) * a.ldb : 0), dst + GA * GROUP + (i * WAVES + w) * (TB ? 1024 : GROUP));
+                glds16(src[CA + i] + (TB ? offb + (int64_t)min(kin * 64 + krow[CA + i], a.kb - 1) * a.ldb : min(offb, (int64_t)(a.end_b - 16 - lp * 16))), dst + GA * GROUP + (i * WAVES + w) * (TB ? 1024 : GROUP));
             if (++kin == nk) kin = 0, seg++;
         };
 #pragma unroll

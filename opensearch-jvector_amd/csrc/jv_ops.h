@@ -17,6 +17,7 @@ struct JvMm {
     int32_t segs;            // 1 (bf16, e4m3) or 6 (float32)
     int64_t plane_a, plane_b;  // bytes from plane to plane
     int32_t ka, kb, ca, cb;  // operands with k across their rows
+    int32_t end_b;           // bytes of k that a row of B has, a multiple of 16 (k along its rows): what lies behind reads as the last 16, A holds zeros there
     const uint8_t *sa, *sb;  // e4m3: scale bytes [M][kph / 2] / [N][kph / 2]
 };
 
@@ -39,6 +40,9 @@ struct JvSxLoss {
     int32_t splits;        // workgroups that share a panel of queries
     float2* part;          // [M][splits]: maximum and sum (log2 domain)
     int32_t first;         // 0: partials of an earlier piece of the rows are in `part` already, join them
+    const int32_t* targets;  // nullptr = none
+    int64_t row0;          // first row of this piece
+    float* hit;            // [M] the target's logit (log2 domain), written by the piece that has it
 };
 // what the gradient needs of a query
 struct JvSxQuery {
@@ -90,8 +94,7 @@ hipError_t jvk_f8_score(const JvMmOut* a, hipStream_t s);
 hipError_t jvk_sx_prepare(const JvSxPrepare* a, hipStream_t s);
 int jvk_sx_loss_plan(int nq, int64_t rows, int d, int f32, int* tile);   // splits, and the queries of a tile
 hipError_t jvk_sx_loss(const JvSxLoss* a, int f32, hipStream_t s);   // f32: operands are float32 as they lie
-hipError_t jvk_sx_join(const float2* part, int splits, int nq, const void* q, int64_t q_stride, const void* v, int64_t v_stride, int dtype, int d,
-                       const int32_t* targets, int64_t n, float scale, float* loss, float* lse, hipStream_t s);
+hipError_t jvk_sx_join(const float2* part, int splits, int nq, const float* hit, const int32_t* targets, int64_t n, float* loss, float* lse, hipStream_t s);
 hipError_t jvk_sx_weights(const JvSxWeights* a, int large, hipStream_t s);   // (planes = 0: float32 as it lies)
 // dq = G V and dv = G^T Q (nullptr: not asked for)
 int jvk_sx_grad_splits(int nq, int d, int64_t rows, int f32, int large);

@@ -78,6 +78,7 @@ struct Pipe {
             }
         };
         rows();
+        const int64_t end_b = a.end_b - 16 - ((lane & 3) ^ ((lane >> 4) & 3)) * 16;
         auto stage = [&]() {
             int64_t offa = TA ? 0 : (int64_t)skin * 64, offb = TB ? 0 : (int64_t)skin * 64;
             if (a.segs > 1) offa += plane_a(sseg) * a.plane_a, offb += plane_b(sseg) * a.plane_b;
@@ -86,7 +87,7 @@ struct Pipe {
             for (int i = 0; i < 2; i++) {
                 const int k = skin * 32 + 16 * i + 2 * w + (lane >> 5);
                 glds16(pa[i] + offa + (TA ? (int64_t)min(k, a.ka - 1) * a.lda : 0), dst + i * 8192);
-                glds16(pb[i] + offb + (TB ? (int64_t)min(k, a.kb - 1) * a.ldb : 0), dst + 16384 + i * 8192);
+                glds16(pb[i] + (TB ? offb + (int64_t)min(k, a.kb - 1) * a.ldb : min(offb, end_b)), dst + 16384 + i * 8192);
             }
             sreg = (sreg + 1) & 3;
             if (++skin == a.kph) skin = 0, sseg++;

@@ -137,7 +137,7 @@ def test_scores_do_not_touch_what_lies_between_rows(torch, ops, pkg):
 LOSS = [(1, 1, 1, 0, 0, 1.0), (1, 5, 3, 0, 0, 2.0), (3, 129, 64, 0, 0, 20.0), (2, 300, 17, 5, 1, 5.0), (129, 127, 65, 1, 3, 20.0), (64, 640, 128, 8, 0, 30.0),
         (130, 3000, 100, 0, 0, 10.0), (257, 1025, 384, 64, 8, 20.0), (31, 2000, 768, 0, 0, 20.0), (512, 260, 200, 0, 0, -3.0), (7, 1000, 1536, 0, 0, 50.0),
         (40, 130, 2, 1, 1, 3.0), (5, 70, 4, 0, 1, 3.0), (35, 77, 31, 0, 2, 9.0), (90, 261, 33, 6, 5, 9.0), (70, 300, 62, 3, 7, 9.0), (118, 18, 843, 24, 0, 10.0),
-        (66, 520, 134, 2, 2, 12.0)]
+        (66, 520, 134, 2, 2, 12.0), (30, 1000, 72, 2, 2, 12.0), (100, 900, 8, 0, 0, 3.0), (61, 40, 200, 8, 6, 12.0)]
 
 
 def loss_case(torch, nq, n, d, dtype, pad=0, shift=0, seed=0):
@@ -404,7 +404,7 @@ def test_scores_on_the_large_tiles(torch, ops, out, nq, n, d):
 
 
 @pytest.mark.parametrize("dtype,nq,n,d,pad", [("bf16", 300, 30011, 200, 0), ("f32", 257, 26000, 70, 3), ("bf16", 1030, 10001, 384, 8), ("bf16", 80, 60000, 64, 0),
-                                              ("f32", 600, 17000, 128, 0), ("f32", 600, 17000, 132, 0), ("bf16", 600, 17000, 128, 0), ("f32", 500, 25000, 129, 2)])
+                                              ("f32", 600, 17000, 128, 0), ("f32", 600, 17000, 132, 0), ("bf16", 600, 17000, 128, 0), ("f32", 500, 25000, 129, 2), ("bf16", 400, 26000, 136, 2), ("bf16", 400, 26000, 8, 2)])
 def test_softmax_on_the_large_tiles(torch, ops, dtype, nq, n, d, pad):
     q, v, t, w, _, _, t64, _ = loss_case(torch, nq, n, d, dtype, pad)
     scale = 15.0
