@@ -79,8 +79,8 @@ int check_shape(int64_t n, int d, const char* what) {
 struct Plan {
     int P, segs, dp, kq;              // planes, segments; d and nq padded to 64
     int64_t rows_f, rows_b;           // rows of one piece, forward (only if the vectors have to be laid out) / backward
-    int tile, splits_f, splits_q, large, large_grads;
-    int64_t off_q, off_v, off_part, off_hit, off_query, off_norm, off_rest, off_g, off_slab, bytes;
+    int path_f, path_b, splits_f, splits_q;   // forward, backward
+    int64_t off_q, off_q4, off_v, off_part, off_hit, off_query, off_norm, off_rest, off_g, off_slab, bytes;
 };
 
 // MB of one piece's weights g: few large pieces, for every piece writes and reads dq's partial sums again and starts its tiles anew (step
@@ -113,22 +113,23 @@ Plan make_plan(int dtype, int nq, int64_t n, int d, uint32_t what) {
         return o;
     };
     p.off_q = take((int64_t)nq * row);
+    p.off_q4 = take((int64_t)(d < 4 ? nq : 0) * 16);   // (float32 rows of fewer than four components, as they lie but with four)
     if (what & JV_SOFTMAX_LOSS) {
-        p.splits_f = jvk_sx_loss_plan(nq, n, d, dtype == JV_DTYPE_F32, &p.tile);
+        p.path_f = jvk_sx_path(nq, n, d, dtype == JV_DTYPE_F32);
+        p.splits_f = jvk_sx_loss_splits(p.path_f, nq, n);
         p.off_part = take((int64_t)p.splits_f * nq * 8);
         p.off_hit = take((int64_t)nq * 4);
         p.off_v = take(std::min<int64_t>(p.rows_f, n) * row);
     }
     if (what & (JV_SOFTMAX_QUERY_GRAD | JV_SOFTMAX_VECTOR_GRAD)) {
-        p.large = jvk_sx_large(nq, std::min<int64_t>(p.rows_b, n), d, dtype == JV_DTYPE_F32);
-        p.large_grads = jvk_sx_large_grads(p.large, d);
+        p.path_b = jvk_sx_path(nq, std::min<int64_t>(p.rows_b, n), d, dtype == JV_DTYPE_F32);
         p.off_v = take(std::min<int64_t>(p.rows_b, n) * row);
         p.off_query = take((int64_t)nq * sizeof(JvSxQuery));
         p.off_norm = take(4);
         p.off_rest = take((int64_t)nq * 4);
         p.off_g = take((int64_t)p.kq * p.P * p.rows_b * 2);
         if (what & JV_SOFTMAX_QUERY_GRAD) {
-            p.splits_q = jvk_sx_grad_splits(nq, d, std::min<int64_t>(p.rows_b, n), p.P == 3, p.large_grads);
+            p.splits_q = jvk_sx_grad_splits(p.path_b, nq, d, std::min<int64_t>(p.rows_b, n));
             p.off_slab = take((int64_t)p.splits_q * nq * p.dp * 4);
         }
     }
@@ -136,16 +137,20 @@ Plan make_plan(int dtype, int nq, int64_t n, int d, uint32_t what) {
     return p;
 }
 
-// Rows as a product takes them: the caller's own where they are 4-B aligned and bf16 with whole 16 B of components (the queries, whose padding
-// stands for zeros behind the vectors', with whole steps of them), or float32 of at least four components where the tiles are small.
+// Rows as a product takes them: the caller's own where they are
+//   bf16, 4-B aligned, with whole 16 B of components (the queries, whose padding stands for zeros behind the vectors', with whole steps of 64), or
+//   float32 with at least four components, and the path takes them as they lie (JV_SX_RAW all of them, JV_SX_PLANES the vectors).
 struct Rows {
     const char* p;
     int64_t stride;   // bytes
     bool ready;
+    int kp;           // components of a row that is laid out instead
 };
-Rows rows_of(const void* p, int64_t stride, int d, int dtype, bool large, int whole) {
-    const bool ready = dtype == JV_DTYPE_F32 ? !large && d >= 4 : (uintptr_t)p % 4 == 0 && stride % 2 == 0 && d % whole == 0;
-    return {(const char*)p, stride * size_of(dtype), ready};
+Rows rows_of(const void* p, int64_t stride, const jv_softmax_params* q, const Plan& plan, int path, bool vectors) {
+    Rows r{(const char*)p, stride * size_of(q->dtype), false, plan.dp};
+    if (q->dtype == JV_DTYPE_BF16) r.ready = (uintptr_t)p % 4 == 0 && stride % 2 == 0 && q->d % (vectors ? 8 : 64) == 0;
+    else if (path == JV_SX_RAW || (path == JV_SX_PLANES && vectors)) r.ready = q->d >= 4, r.kp = 4;
+    return r;
 }
 
 int check_softmax(const jv_softmax_params* p) {
@@ -169,7 +174,9 @@ int check_softmax_call(const jv_softmax_params* p, const Plan& plan) {
 }
 
 // k ranges that a piece of `rows` rows has at most: its steps
-int splits_of(const Plan& plan, int64_t rows, bool f32) { return (int)(up(rows, 64) / (f32 ? 32 : 64) * (f32 ? 1 : plan.segs)); }
+int splits_of(const Plan& plan, int64_t rows) {
+    return (int)(plan.path_b == JV_SX_RAW || plan.path_b == JV_SX_PLANES ? up(rows, 64) / 32 : up(rows, 64) / 64 * plan.segs);
+}
 
 // queries times vectors, but for where the vectors lie and how many they are
 JvMm logits(const Plan& plan, int nq, int d) {
@@ -181,18 +188,16 @@ JvMm logits(const Plan& plan, int nq, int d) {
 }
 
 // The rows [at, at + rows) of a matrix as a product reads them: the caller's own, or where the next jvk_sx_prepare lays them out.
-void take_rows(const Rows& r, const void* p, int64_t stride, int dtype, int64_t at, int64_t rows, const Plan& plan, int kp, char* to,
-               JvSxPrepare::Matrix* m, const char** out, int64_t* ld) {
+void take_rows(const Rows& r, int dtype, int64_t at, int64_t rows, const Plan& plan, char* to, JvSxPrepare::Matrix* m, const char** out, int64_t* ld) {
     if (r.ready) {
         *out = r.p + at * r.stride;
         *ld = r.stride;
         m->rows = 0;
         return;
     }
-    m->x = (const char*)p + at * stride * size_of(dtype);
-    m->stride = stride, m->rows = rows, m->out = (uint16_t*)to;
+    m->x = r.p + at * r.stride, m->stride = r.stride / size_of(dtype), m->rows = rows, m->out = to, m->kp = r.kp;
     *out = to;
-    *ld = kp == 4 ? 16 : (int64_t)plan.P * plan.dp * 2;
+    *ld = r.kp == 4 ? 16 : (int64_t)plan.P * plan.dp * 2;
 }
 
 }  // namespace
@@ -265,25 +270,24 @@ int jv_softmax_loss_device(const jv_softmax_params* p, float* d_out_loss, float*
     hipStream_t s = (hipStream_t)hip_stream;
     if (p->nq > 0) {
         char* ws = (char*)p->workspace;
-        const bool large = plan.tile == 256, f32 = p->dtype == JV_DTYPE_F32 && !large;
-        const Rows rq = rows_of(p->queries, p->query_stride, p->d, p->dtype, large, 64), rv = rows_of(p->vectors, p->vector_stride, p->d, p->dtype, large, 8);
+        const Rows rq = rows_of(p->queries, p->query_stride, p, plan, plan.path_f, false), rv = rows_of(p->vectors, p->vector_stride, p, plan, plan.path_f, true);
         const int64_t step = rv.ready ? std::max<int64_t>(p->n, 1) : plan.rows_f;
         JvSxLoss a{};
         a.mm = logits(plan, p->nq, p->d);
         a.c = p->scale * 1.44269504088896341f;
         a.targets = p->targets, a.hit = (float*)(ws + plan.off_hit);
-        if (rv.ready && !f32) a.mm.end_b = p->d * 2;
-        a.tile = plan.tile, a.splits = p->n > 0 ? plan.splits_f : 0, a.part = (float2*)(ws + plan.off_part);
+        if (rv.ready && p->dtype == JV_DTYPE_BF16) a.mm.end_b = p->d * 2;
+        a.path = plan.path_f, a.splits = p->n > 0 ? plan.splits_f : 0, a.part = (float2*)(ws + plan.off_part);
         JvSxPrepare pre{};
-        pre.dtype = p->dtype, pre.d = p->d, pre.kp = f32 ? 4 : plan.dp;   // (float32 as it lies: only rows of fewer than four are laid out)
-        take_rows(rq, p->queries, p->query_stride, p->dtype, 0, p->nq, plan, pre.kp, ws + plan.off_q, &pre.m[0], &a.mm.a, &a.mm.lda);
+        pre.dtype = p->dtype, pre.d = p->d;
+        take_rows(rq, p->dtype, 0, p->nq, plan, ws + plan.off_q, &pre.m[0], &a.mm.a, &a.mm.lda);
         for (int64_t at = 0; at < p->n; at += step) {
             a.mm.N = (int)std::min<int64_t>(step, p->n - at);
             a.first = at == 0, a.row0 = at;
-            take_rows(rv, p->vectors, p->vector_stride, p->dtype, at, a.mm.N, plan, pre.kp, ws + plan.off_v, &pre.m[1], &a.mm.b, &a.mm.ldb);
+            take_rows(rv, p->dtype, at, a.mm.N, plan, ws + plan.off_v, &pre.m[1], &a.mm.b, &a.mm.ldb);
             CHK(jvk_sx_prepare(&pre, s));
             pre.m[0].rows = 0;
-            CHK(jvk_sx_loss(&a, f32, s));
+            CHK(jvk_sx_loss(&a, s));
         }
         CHK(jvk_sx_join(a.part, a.splits, p->nq, a.hit, p->targets, p->n, d_out_loss, d_out_lse, s));
     }
@@ -309,51 +313,63 @@ int jv_softmax_grad_device(const jv_softmax_params* p, const float* d_lse, const
         return done(hip_stream);
     }
     char* ws = (char*)p->workspace;
-    const bool f32 = p->dtype == JV_DTYPE_F32 && !plan.large;
-    const Rows rq = rows_of(p->queries, p->query_stride, p->d, p->dtype, plan.large, 64), rv = rows_of(p->vectors, p->vector_stride, p->d, p->dtype, plan.large, 8);
+    const Rows rq = rows_of(p->queries, p->query_stride, p, plan, plan.path_b, false), rv = rows_of(p->vectors, p->vector_stride, p, plan, plan.path_b, true);
+    const bool f32 = p->dtype == JV_DTYPE_F32, raw = plan.path_b == JV_SX_RAW;
     JvSxWeights w{};
     w.mm = logits(plan, p->nq, p->d);
     w.c = p->scale * 1.44269504088896341f;
     if (rv.ready && !f32) w.mm.end_b = p->d * 2;
-    w.planes = f32 ? 0 : plan.P, w.g = ws + plan.off_g;
-    JvSxQuery* query = (JvSxQuery*)(ws + plan.off_query);
-    float* norm = f32 ? nullptr : (float*)(ws + plan.off_norm);   // (float32 g needs no common unit and lacks nothing at a target)
-    if (f32) w.lse = d_lse, w.w = d_loss_grad, w.targets = p->targets, w.n = p->n;
-    else w.query = query, w.rest = (float*)(ws + plan.off_rest);
-    const bool direct = f32 && plan.splits_q == 1 && plan.rows_b >= p->n;   // dq is complete at once
+    w.path = plan.path_b, w.g = ws + plan.off_g;
+    // float32 g needs no common unit and lacks nothing at a target
     JvSxPrepare pre{};
-    pre.dtype = p->dtype, pre.d = p->d, pre.kp = f32 ? 4 : plan.dp;   // (float32 as it lies: only rows of fewer than four are laid out)
-    pre.lse = d_lse, pre.w = d_loss_grad, pre.targets = p->targets, pre.nq = p->nq, pre.n = p->n, pre.query = f32 ? nullptr : query, pre.norm = norm, pre.rest = w.rest;
-    take_rows(rq, p->queries, p->query_stride, p->dtype, 0, p->nq, plan, pre.kp, ws + plan.off_q, &pre.m[0], &w.mm.a, &w.mm.lda);
+    pre.dtype = p->dtype, pre.d = p->d;
+    float* norm = nullptr;
+    JvSxQuery* query = nullptr;
+    if (f32) {
+        w.lse = d_lse, w.w = d_loss_grad, w.targets = p->targets, w.n = p->n;
+    } else {
+        w.query = query = (JvSxQuery*)(ws + plan.off_query), w.rest = (float*)(ws + plan.off_rest), norm = (float*)(ws + plan.off_norm);
+        pre.lse = d_lse, pre.w = d_loss_grad, pre.targets = p->targets, pre.nq = p->nq, pre.n = p->n, pre.query = query, pre.norm = norm, pre.rest = w.rest;
+    }
+    const bool direct = raw && plan.splits_q == 1 && plan.rows_b >= p->n;   // dq is complete at once
+    const char* q_rows;   // the queries as dv's product reads them: the same but for planes, which it splits itself
+    int64_t q_ld;
+    take_rows(rq, p->dtype, 0, p->nq, plan, ws + plan.off_q, &pre.m[0], &w.mm.a, &w.mm.lda);
+    const Rows rb = plan.path_b == JV_SX_PLANES ? rows_of(p->queries, p->query_stride, p, plan, JV_SX_RAW, false) : rq;
+    if (plan.path_b == JV_SX_PLANES) {
+        take_rows(rb, p->dtype, 0, p->nq, plan, ws + plan.off_q4, &pre.m[2], &q_rows, &q_ld);
+    } else {
+        q_rows = w.mm.a, q_ld = w.mm.lda;
+    }
     for (int64_t at = 0; at < p->n; at += plan.rows_b) {
         const int rows = (int)std::min<int64_t>(plan.rows_b, p->n - at);
         w.mm.N = rows, w.row0 = at, w.kv = (int)up(rows, 64);
-        take_rows(rv, p->vectors, p->vector_stride, p->dtype, at, rows, plan, pre.kp, ws + plan.off_v, &pre.m[1], &w.mm.b, &w.mm.ldb);
+        take_rows(rv, p->dtype, at, rows, plan, ws + plan.off_v, &pre.m[1], &w.mm.b, &w.mm.ldb);
         CHK(jvk_sx_prepare(&pre, s));
-        pre.m[0].rows = 0, pre.query = nullptr;
-        CHK(jvk_sx_weights(&w, plan.large, s));
+        pre.m[0].rows = pre.m[2].rows = 0, pre.query = nullptr;
+        CHK(jvk_sx_weights(&w, s));
         JvMmOut o{}, q;
         o.mm.segs = plan.segs;
-        o.mm.a = (const char*)w.g, o.mm.lda = f32 ? (int64_t)w.kv * 4 : (int64_t)plan.P * w.kv * 2, o.mm.plane_a = (int64_t)w.kv * 2;
+        o.mm.a = (const char*)w.g, o.mm.lda = raw ? (int64_t)w.kv * 4 : (int64_t)plan.P * w.kv * 2, o.mm.plane_a = (int64_t)w.kv * 2;
         o.mm.N = p->d, o.mm.plane_b = (int64_t)plan.dp * 2, o.mm.end_b = kNoEnd;
         if (d_out_query_grad) {   // G times the piece's vectors: k = its rows
             o.mm.M = p->nq, o.mm.k = w.kv, o.mm.kph = w.kv / 32;
-            o.mm.b = w.mm.b, o.mm.ldb = w.mm.ldb, o.mm.kb = rows, o.mm.cb = rv.ready || f32 ? p->d : plan.dp;
+            o.mm.b = w.mm.b, o.mm.ldb = w.mm.ldb, o.mm.kb = rows, o.mm.cb = rv.ready || rv.kp == 4 ? p->d : plan.dp;
             o.mul = 1.0f, o.out = ws + plan.off_slab, o.ldo = plan.dp, o.add = at > 0;
-            o.splits = std::min(plan.splits_q, splits_of(plan, rows, f32));   // (only the last piece can be that short: it adds to the first ranges)
+            o.splits = std::min(plan.splits_q, splits_of(plan, rows));   // (only the last piece can be that short: it adds to the first ranges)
             if (direct) o.mul = p->scale, o.out = d_out_query_grad, o.ldo = query_grad_stride;
             q = o;
         }
         if (d_out_vector_grad) {   // G across times the queries: k = the queries
-            o.mm.M = rows, o.mm.k = plan.kq, o.mm.kph = plan.kq / 32, o.mm.ka = plan.kq, o.mm.ca = w.kv;
-            o.mm.b = w.mm.a, o.mm.ldb = w.mm.lda, o.mm.kb = p->nq, o.mm.cb = rq.ready || f32 ? p->d : plan.dp;
+            o.mm.M = rows, o.mm.k = (int)up(p->nq, 32), o.mm.kph = plan.kq / 32, o.mm.ka = f32 && plan.path_b != JV_SX_LARGE ? o.mm.k : plan.kq, o.mm.ca = w.kv;
+            o.mm.b = q_rows, o.mm.ldb = q_ld, o.mm.kb = p->nq, o.mm.cb = rb.ready || rb.kp == 4 ? p->d : plan.dp;
             o.mul = p->scale, o.norm = norm, o.dtype = p->dtype, o.splits = 1, o.add = 0;
             o.out = (char*)d_out_vector_grad + at * vector_grad_stride * size_of(p->dtype), o.ldo = vector_grad_stride;
         }
-        CHK(jvk_sx_grads(d_out_query_grad ? &q : nullptr, d_out_vector_grad ? &o : nullptr, f32, plan.large_grads, s));
+        CHK(jvk_sx_grads(d_out_query_grad ? &q : nullptr, d_out_vector_grad ? &o : nullptr, plan.path_b, s));
     }
     if (d_out_query_grad && !direct) {
-        const int splits = std::min(plan.splits_q, splits_of(plan, std::min<int64_t>(plan.rows_b, p->n), f32));
+        const int splits = std::min(plan.splits_q, splits_of(plan, std::min<int64_t>(plan.rows_b, p->n)));
         CHK(jvk_sx_finish((const float*)(ws + plan.off_slab), splits, p->nq, p->d, plan.dp, w.rest, query, p->vectors, p->vector_stride, p->scale, norm, d_out_query_grad,
                           p->dtype, query_grad_stride, s));
     }

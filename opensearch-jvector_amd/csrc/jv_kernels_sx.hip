@@ -42,18 +42,20 @@ __device__ __forceinline__ void planes3(float x, uint16_t (&p)[3]) {
 // what has to be laid out: rows as padded bf16 planes [rows][planes][kp], and what the gradient needs of each query
 // ---------------------------------------------------------------------------------------------
 template <typename T>
-__device__ __forceinline__ void pack(const JvSxPrepare::Matrix& m, int d, int kp, int64_t first, int64_t step) {   // eight components a thread
+__device__ __forceinline__ void pack(const JvSxPrepare::Matrix& m, int d, int64_t first, int64_t step) {   // eight components a thread
     constexpr int P = sizeof(T) == 4 ? 3 : 1;
-    const int per = kp / 8;
-    const int wide = (uintptr_t)m.x % 16 == 0 && m.stride % (16 / sizeof(T)) == 0;
+    const int kp = m.kp, per = kp / 8;
+    if (kp == 4) {
+        for (int64_t i = first; i < m.rows * 4; i += step) ((float*)m.out)[i] = (i & 3) < d ? (float)((const T*)m.x)[(i >> 2) * m.stride + (i & 3)] : 0.0f;
+        return;
+    }
     for (int64_t i = first; i < m.rows * per; i += step) {
         const int64_t r = i < 0x100000000ll ? (int64_t)((uint32_t)i / (uint32_t)per) : i / per;
         const int at = (int)(i - r * per) * 8;
         const T* row = (const T*)m.x + r * m.stride;
         T x[8];
-        if (wide && at + 8 <= d) {
-#pragma unroll
-            for (int k = 0; k < (int)sizeof(T) / 2; k++) ((i32x4*)x)[k] = ((const i32x4*)(row + at))[k];
+        if (at + 8 <= d) {
+            __builtin_memcpy(x, row + at, sizeof(x));   // (no alignment is asked for)
         } else {
 #pragma unroll
             for (int e = 0; e < 8; e++) x[e] = at + e < d ? row[at + e] : (T)0.0f;
@@ -75,7 +77,7 @@ __device__ __forceinline__ void pack(const JvSxPrepare::Matrix& m, int d, int kp
             i32x4 o;
 #pragma unroll
             for (int e = 0; e < 4; e++) o[e] = (int)((uint32_t)p[k][2 * e] | ((uint32_t)p[k][2 * e + 1] << 16));
-            *(i32x4*)(m.out + (r * P + k) * kp + at) = o;
+            *(i32x4*)((uint16_t*)m.out + (r * P + k) * kp + at) = o;
         }
     }
 }
@@ -111,25 +113,22 @@ __device__ __forceinline__ void queries(const JvSxPrepare& a) {
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void jvs_prepare_kernel(const JvSxPrepare a, int g0, int g1) {   // g0 + g1 workgroups for the matrices
-    if (a.kp == 4) {   // float32 rows of fewer than four components, as rows of four
-        for (int k = 0; k < 2; k++)
-            for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.m[k].rows * 4; i += (int64_t)gridDim.x * 256)
-                ((float*)a.m[k].out)[i] = (i & 3) < a.d ? (float)((const T*)a.m[k].x)[(i >> 2) * a.m[k].stride + (i & 3)] : 0.0f;
-        if (a.query && blockIdx.x == 0) queries(a);
-        return;
-    }
-    if ((int)blockIdx.x < g0) pack<T>(a.m[0], a.d, a.kp, (int64_t)blockIdx.x * 256 + threadIdx.x, (int64_t)g0 * 256);
-    else if ((int)blockIdx.x < g0 + g1) pack<T>(a.m[1], a.d, a.kp, (int64_t)((int)blockIdx.x - g0) * 256 + threadIdx.x, (int64_t)g1 * 256);
-    else queries(a);
+__global__ __launch_bounds__(256) void jvs_prepare_kernel(const JvSxPrepare a, int g0, int g1, int g2) {   // workgroups for the matrices, one more for the queries
+    int i = blockIdx.x;
+    if (i < g0) return pack<T>(a.m[0], a.d, (int64_t)i * 256 + threadIdx.x, (int64_t)g0 * 256);
+    i -= g0;
+    if (i < g1) return pack<T>(a.m[1], a.d, (int64_t)i * 256 + threadIdx.x, (int64_t)g1 * 256);
+    i -= g1;
+    if (i < g2) return pack<T>(a.m[2], a.d, (int64_t)i * 256 + threadIdx.x, (int64_t)g2 * 256);
+    queries(a);
 }
 extern "C" hipError_t jvk_sx_prepare(const JvSxPrepare* a, hipStream_t s) {
-    int g[2];
-    for (int k = 0; k < 2; k++) g[k] = (int)std::min<int64_t>((a->m[k].rows * std::max(a->kp / 8, 1) + 255) / 256, 32768);
-    const unsigned grid = (unsigned)(g[0] + g[1] + (a->query ? 1 : 0));
+    int g[3];
+    for (int k = 0; k < 3; k++) g[k] = (int)std::min<int64_t>((a->m[k].rows * std::max(a->m[k].kp / 8, 1) + 255) / 256, 32768);
+    const unsigned grid = (unsigned)(g[0] + g[1] + g[2] + (a->query ? 1 : 0));
     if (grid == 0) return hipSuccess;
-    if (a->dtype == 0) jvs_prepare_kernel<float><<<grid, 256, 0, s>>>(*a, g[0], g[1]);
-    else jvs_prepare_kernel<__bf16><<<grid, 256, 0, s>>>(*a, g[0], g[1]);
+    if (a->dtype == 0) jvs_prepare_kernel<float><<<grid, 256, 0, s>>>(*a, g[0], g[1], g[2]);
+    else jvs_prepare_kernel<__bf16><<<grid, 256, 0, s>>>(*a, g[0], g[1], g[2]);
     return hipGetLastError();
 }
 
@@ -294,34 +293,37 @@ __global__ __launch_bounds__(T::THREADS) void jvs_loss_tile_kernel(const JvSxLos
     write_partials<T::TM, MT, WN>(a, smem, m0, split, (threadIdx.x >> 6) / WM, [](int m) { return T::row(m); }, top, sum);
 }
 
-// The large tiles where they fill the chip and more than half of one is queries.  float32 only with more than 128 components: its planes are worth laying out when they are read often
-// enough (step 300 x 100 000 x 128: 618 us so, 417 us as it lies; step 777 x 30 011 x 381: 730 and 799 us).
-static bool large(int nq, int64_t rows, int d, bool f32) {
-    return nq > 128 && ((nq + 255) / 256) * ((rows + 255) / 256) >= 192 && (!f32 || d > 128);
+// The large tiles where they fill the chip and more than half of one is queries.  float32 only with more than 128 components: both operands'
+// planes are worth laying out when they are read often enough (step 300 x 100 000 x 128: 618 us so, 417 us as it lies; step
+// 777 x 30 011 x 381: 730 and 799 us).  Otherwise smaller tiles; float32 with everything as it lies where that is no more than one of 128 x 128
+// a CU (laying out costs a launch), with the queries as planes above.
+extern "C" int jvk_sx_path(int nq, int64_t rows, int d, int f32) {
+    if (nq > 128 && ((nq + 255) / 256) * ((rows + 255) / 256) >= 192 && (!f32 || d > 128)) return JV_SX_LARGE;
+    if (!f32) return JV_SX_TILES;
+    return (int64_t)((nq + 127) / 128) * ((rows + 127) / 128) <= 256 ? JV_SX_RAW : JV_SX_PLANES;
 }
-extern "C" int jvk_sx_large(int nq, int64_t rows, int d, int f32) { return large(nq, rows, d, f32); }
-// The gradients' products have d columns: with up to 128 half a large tile would be multiplied for nothing.
-extern "C" int jvk_sx_large_grads(int large, int d) { return large && d > 128; }
 
-// Queries and rows of the tiles that a product of nq queries with `rows` rows takes:
-//   256 x 256  where they fill the chip (large);
-//   32 x 128 and 64 x 128 for up to 32 and 64 queries: the rows are streamed, and as little as possible is multiplied for nothing;
-//   128 x 128 otherwise, but where that is no more than one tile a CU 64 x 64, with four steps of k under way: the way to memory and the
-//   multiplications of one tile's steps are what counts then (float32, 118 x 18 x 843: 66 -> 24 us)
-static int tile_of(int nq, int64_t rows, int d, bool f32) {
-    if (large(nq, rows, d, f32)) return 256;
-    if (nq <= 32) return 32;
-    const int64_t tiles = (int64_t)((nq + 127) / 128) * ((rows + 127) / 128);
-    return tiles <= 256 ? 65 : nq <= 64 ? 64 : 128;   // (65: 64 x 64)
+// Queries and rows of the smaller tiles: 32 x 128 and 64 x 128 (float32 also 96 x 128) for up to so many queries, the rows being streamed and as
+// little as possible multiplied for nothing; 128 x 128 otherwise; but where that is no more than one tile a CU 64 x 64, with four steps of k
+// under way: the way to memory and the multiplications of one tile's steps are what counts then (float32, 118 x 18 x 843: 66 -> 36 us)
+struct Shape {
+    int m, n;
+    bool few;
+};
+static Shape shape_of(int path, int nq, int64_t rows) {
+    if (path == JV_SX_LARGE) return {256, 256, false};
+    const bool few = (int64_t)((nq + 127) / 128) * ((rows + 127) / 128) <= 256;
+    if (path == JV_SX_PLANES) return {nq > 96 ? 128 : (nq + 31) / 32 * 32, 128, false};
+    if (nq <= 32) return {32, 128, few};
+    if (few) return {64, 64, true};
+    return {nq <= 64 ? 64 : 128, 128, false};
 }
-static int rows_of_tile(int tile) { return tile == 256 ? 256 : tile == 65 ? 64 : 128; }
-static int queries_of_tile(int tile) { return tile == 65 ? 64 : tile; }
 
-// workgroups that share a panel's rows: one for each CU with the large tiles, two or three with the small ones
-extern "C" int jvk_sx_loss_plan(int nq, int64_t rows, int d, int f32, int* tile) {
-    const int t = tile_of(nq, rows, d, f32), tm = queries_of_tile(t), tn = rows_of_tile(t), full = t == 256 ? 256 : t == 128 || t == 65 ? 512 : 768;
-    const int64_t panels = std::max((nq + tm - 1) / tm, 1), tiles = std::max<int64_t>((rows + tn - 1) / tn, 1);
-    *tile = t;
+// one for each CU with the large tiles, two or three with the small ones
+extern "C" int jvk_sx_loss_splits(int path, int nq, int64_t rows) {
+    const Shape t = shape_of(path, nq, rows);
+    const int full = t.m == 256 ? 256 : t.m == 128 || t.n == 64 || path == JV_SX_PLANES ? 512 : 768;
+    const int64_t panels = std::max((nq + t.m - 1) / t.m, 1), tiles = std::max<int64_t>((rows + t.n - 1) / t.n, 1);
     return (int)std::min(std::max<int64_t>(full / panels, 1), tiles);
 }
 
@@ -334,25 +336,23 @@ static hipError_t loss_tile(const JvSxLoss& a, hipStream_t s) {
     jvs_loss_tile_kernel<T, WM, WN><<<(unsigned)((all + 7) / 8 * 8), T::THREADS, T::LDS, s>>>(a);
     return hipGetLastError();
 }
-static hipError_t loss_small(const JvSxLoss& a, bool f32, hipStream_t s) {
-    const bool few = (int64_t)((a.mm.M + 31) / 32) * a.splits <= 256;   // (32 queries)
-    if (f32) {
-        if (a.tile == 128) return loss_tile<Tile32<2, 2, 2, 2, 2, false, false>, 2, 2>(a, s);
-        if (a.tile == 65) return loss_tile<Tile32<1, 1, 2, 2, 4, false, false>, 2, 2>(a, s);
-        if (a.tile == 64) return loss_tile<Tile32<2, 1, 1, 4, 2, false, false>, 1, 4>(a, s);
-        return few ? loss_tile<Tile32<1, 1, 1, 4, 4, false, false>, 1, 4>(a, s) : loss_tile<Tile32<1, 1, 1, 4, 2, false, false>, 1, 4>(a, s);
-    }
-    if (a.tile == 128) return loss_tile<Tile<BF16, 2, 2, 2, 2, 2>, 2, 2>(a, s);
-    if (a.tile == 65) return loss_tile<Tile<BF16, 1, 1, 2, 2, 4>, 2, 2>(a, s);
-    if (a.tile == 64) return loss_tile<Tile<BF16, 2, 1, 1, 4, 2>, 1, 4>(a, s);
-    return few ? loss_tile<Tile<BF16, 1, 1, 1, 4, 4>, 1, 4>(a, s) : loss_tile<Tile<BF16, 1, 1, 1, 4, 2>, 1, 4>(a, s);
-}
-
-extern "C" hipError_t jvk_sx_loss(const JvSxLoss* a, int f32, hipStream_t s) {
+extern "C" hipError_t jvk_sx_loss(const JvSxLoss* a, hipStream_t s) {
     using P = Pipe<BF16>;
     if (a->mm.N <= 0 || a->mm.M <= 0) return hipSuccess;
     if (a->splits < 1) return hipErrorInvalidValue;
-    if (a->tile != 256) return loss_small(*a, f32, s);
+    const Shape t = shape_of(a->path, a->mm.M, a->mm.N);
+    if (a->path == JV_SX_RAW) return t.m == 32 ? loss_tile<Tile32<1, 1, 1, 4, 4, false, false>, 1, 4>(*a, s) : loss_tile<Tile32<1, 1, 2, 2, 4, false, false>, 2, 2>(*a, s);
+    if (a->path == JV_SX_PLANES) {
+        if (t.m == 32) return loss_tile<Tile3<1, false, false>, 1, 4>(*a, s);
+        if (t.m == 64) return loss_tile<Tile3<2, false, false>, 1, 4>(*a, s);
+        return t.m == 96 ? loss_tile<Tile3<3, false, false>, 1, 4>(*a, s) : loss_tile<Tile3<4, false, false>, 1, 4>(*a, s);
+    }
+    if (a->path == JV_SX_TILES) {
+        if (t.m == 128) return loss_tile<Tile<BF16, 2, 2, 2, 2, 2>, 2, 2>(*a, s);
+        if (t.n == 64) return loss_tile<Tile<BF16, 1, 1, 2, 2, 4>, 2, 2>(*a, s);
+        if (t.m == 64) return loss_tile<Tile<BF16, 2, 1, 1, 4, 2>, 1, 4>(*a, s);
+        return t.few ? loss_tile<Tile<BF16, 1, 1, 1, 4, 4>, 1, 4>(*a, s) : loss_tile<Tile<BF16, 1, 1, 1, 4, 2>, 1, 4>(*a, s);
+    }
     hipError_t e = lds_of(jvs_loss_pipe_kernel, P::LDS);
     if (e != hipSuccess) return e;
     const int64_t all = (int64_t)((a->mm.M + P::TM - 1) / P::TM) * a->splits;
@@ -436,13 +436,14 @@ __global__ __launch_bounds__(512) void jvs_weights_kernel(const JvSxWeights a) {
             for (int m = 0; m < 4; m++) {
                 const int r = w.m0 + P::row(m);
                 JvSxQuery q = {__builtin_inff(), 0.0f, -1, 0};
-                if (r < a.mm.M) q = a.query[r];
-                weigh<P>(acc[m], q, a.c, a.mm.N - w.n0, q.target >= 0 ? (int)(q.target - a.row0) - w.n0 : -1, a.planes == 1, a.rest + r);
+                if (r < a.mm.M) q = a.query ? a.query[r] : query_of(a.lse, a.w, a.targets, a.n, r);
+                weigh<P>(acc[m], q, a.c, a.mm.N - w.n0, q.target >= 0 ? (int)(q.target - a.row0) - w.n0 : -1, a.mm.segs == 1, a.rest + r);
             }
             int stores = 0;
-            for (int k = 0; k < a.planes; k++) {
-                stores = P::write_bf16(smem, (uint16_t*)a.g + (int64_t)k * a.kv, (int64_t)a.planes * a.kv, true, w, padded, a.kv, [&](int m, int n, int e) { return acc[m][n][e]; });
-                if (a.planes > 1) {
+            const int planes = a.mm.segs == 1 ? 1 : 3;
+            for (int k = 0; k < planes; k++) {
+                stores = P::write_bf16(smem, (uint16_t*)a.g + (int64_t)k * a.kv, (int64_t)planes * a.kv, true, w, padded, a.kv, [&](int m, int n, int e) { return acc[m][n][e]; });
+                if (planes > 1) {
 #pragma unroll
                     for (int m = 0; m < 4; m++)
 #pragma unroll
@@ -455,12 +456,18 @@ __global__ __launch_bounds__(512) void jvs_weights_kernel(const JvSxWeights a) {
         });
 }
 
+// rows of G: whole steps of the product that has the queries for k
+static __host__ __device__ __forceinline__ int padded_queries(const JvSxWeights& a) {
+    const int step = a.path == JV_SX_RAW || a.path == JV_SX_PLANES ? 32 : 64;
+    return (a.mm.M + step - 1) / step * step;
+}
+
 // the same on small tiles, one a workgroup
 template <class T>
 __global__ __launch_bounds__(T::THREADS) void jvs_weights_tile_kernel(const JvSxWeights a) {
     constexpr int MT = T::MT, NT = T::NT;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    const int padded = (a.mm.M + 63) / 64 * 64;
+    const int padded = padded_queries(a);
     int m0, n0;
     band_order(xcd_order(blockIdx.x, gridDim.x), (padded + T::TM - 1) / T::TM, (a.mm.N + T::TN - 1) / T::TN, m0, n0);
     m0 *= T::TM, n0 *= T::TN;
@@ -471,34 +478,42 @@ __global__ __launch_bounds__(T::THREADS) void jvs_weights_tile_kernel(const JvSx
         const int r = m0 + T::row(m);
         JvSxQuery q = {__builtin_inff(), 0.0f, -1, 0};
         if (r < a.mm.M) q = a.query ? a.query[r] : query_of(a.lse, a.w, a.targets, a.n, r);
-        weigh<T>(acc[m], q, a.c, a.mm.N - n0, q.target >= 0 ? (int)(q.target - a.row0) - n0 : -1, a.planes == 1, a.rest + r);
-        if (a.planes == 0) {
+        weigh<T>(acc[m], q, a.c, a.mm.N - n0, q.target >= 0 ? (int)(q.target - a.row0) - n0 : -1, a.path == JV_SX_TILES, a.rest + r);
+        // (kv is a multiple of 64: four columns are in or out together)
+        if (a.path == JV_SX_RAW) {
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
                 for (int g = 0; g < 4; g++) {
                     const int col = n0 + T::col(n, 4 * g);
-                    if (r < padded && col < a.kv)   // (kv is a multiple of 64)
+                    if (r < padded && col < a.kv)
                         *(f32x4*)((float*)a.g + (int64_t)r * a.kv + col) = (f32x4){acc[m][n][4 * g], acc[m][n][4 * g + 1], acc[m][n][4 * g + 2], acc[m][n][4 * g + 3]};
                 }
-        } else {   // (one plane: three only come with the large tiles)
+        } else {
+            const int planes = a.path == JV_SX_PLANES ? 3 : 1;
+            for (int k = 0; k < planes; k++) {
+                uint16_t* row = (uint16_t*)a.g + ((int64_t)r * planes + k) * a.kv;
 #pragma unroll
-            for (int n = 0; n < NT; n++)
+                for (int n = 0; n < NT; n++)
 #pragma unroll
-                for (int g = 0; g < 4; g++) {
-                    const int col = n0 + T::col(n, 4 * g);
-                    bf16x4 v;
+                    for (int g = 0; g < 4; g++) {
+                        const int col = n0 + T::col(n, 4 * g);
+                        bf16x4 v;
 #pragma unroll
-                    for (int e = 0; e < 4; e++) v[e] = (__bf16)acc[m][n][4 * g + e];
-                    if (r < padded && col < a.kv) *(bf16x4*)((uint16_t*)a.g + (int64_t)r * a.kv + col) = v;
-                }
+                        for (int e = 0; e < 4; e++) {
+                            v[e] = (__bf16)acc[m][n][4 * g + e];
+                            acc[m][n][4 * g + e] -= (float)v[e];
+                        }
+                        if (r < padded && col < a.kv) *(bf16x4*)(row + col) = v;
+                    }
+            }
         }
     }
 }
 
 template <class T>
 static hipError_t weights_tile(const JvSxWeights& a, hipStream_t s) {
-    const int64_t all = (int64_t)(((a.mm.M + 63) / 64 * 64 + T::TM - 1) / T::TM) * ((a.mm.N + T::TN - 1) / T::TN);
+    const int64_t all = (int64_t)((padded_queries(a) + T::TM - 1) / T::TM) * ((a.mm.N + T::TN - 1) / T::TN);
     if (all > 0x7fffffffll) return hipErrorInvalidValue;
     hipError_t e = lds_of(jvs_weights_tile_kernel<T>, T::LDS);
     if (e != hipSuccess) return e;
@@ -506,21 +521,20 @@ static hipError_t weights_tile(const JvSxWeights& a, hipStream_t s) {
     return hipGetLastError();
 }
 
-static hipError_t weights_small(const JvSxWeights& a, hipStream_t s) {   // (G's padded queries are a multiple of 64: no tile of 32)
-    const int t = tile_of(a.mm.M, a.mm.N, a.mm.k, a.planes == 0);
-    const bool few = t == 65 || (t == 32 && (a.mm.N + 127) / 128 <= 256);
-    if (a.planes == 0) {
-        if (few) return weights_tile<Tile32<1, 1, 2, 2, 4, false, false>>(a, s);
-        return a.mm.M > 64 ? weights_tile<Tile32<2, 2, 2, 2, 2, false, false>>(a, s) : weights_tile<Tile32<2, 1, 1, 4, 2, false, false>>(a, s);
-    }
-    if (few) return weights_tile<Tile<BF16, 1, 1, 2, 2, 4>>(a, s);
-    return a.mm.M > 64 ? weights_tile<Tile<BF16, 2, 2, 2, 2, 2>>(a, s) : weights_tile<Tile<BF16, 2, 1, 1, 4, 2>>(a, s);
-}
-
-extern "C" hipError_t jvk_sx_weights(const JvSxWeights* a, int large, hipStream_t s) {
+extern "C" hipError_t jvk_sx_weights(const JvSxWeights* a, hipStream_t s) {
     using P = Pipe<BF16>;
     if (a->mm.M <= 0 || a->mm.N <= 0) return hipSuccess;
-    if (!large) return weights_small(*a, s);
+    const Shape t = shape_of(a->path, a->mm.M, a->mm.N);
+    if (a->path == JV_SX_RAW) return weights_tile<Tile32<1, 1, 2, 2, 4, false, false>>(*a, s);
+    if (a->path == JV_SX_PLANES) {
+        if (t.m == 32) return weights_tile<Tile3<1, false, false>>(*a, s);
+        if (t.m == 64) return weights_tile<Tile3<2, false, false>>(*a, s);
+        return t.m == 96 ? weights_tile<Tile3<3, false, false>>(*a, s) : weights_tile<Tile3<4, false, false>>(*a, s);
+    }
+    if (a->path == JV_SX_TILES) {   // (G's padded queries are a multiple of 64: no tile of 32)
+        if (t.few) return weights_tile<Tile<BF16, 1, 1, 2, 2, 4>>(*a, s);
+        return t.m == 128 ? weights_tile<Tile<BF16, 2, 2, 2, 2, 2>>(*a, s) : weights_tile<Tile<BF16, 2, 1, 1, 4, 2>>(*a, s);
+    }
     const int64_t all = (int64_t)((a->mm.M + P::TM - 1) / P::TM) * ((a->mm.N + P::TN - 1) / P::TN);
     if (all > 0x7fffffffll) return hipErrorInvalidValue;
     hipError_t e = lds_of(jvs_weights_kernel, P::LDS);
@@ -537,10 +551,9 @@ __global__ __launch_bounds__(256) void jvs_grads_tile_kernel(const JvMmOut q, co
     else out_tile<TV>(v, blockIdx.x - first, smem);
 }
 template <class TQ, class TV>
-static hipError_t grads_tile(const JvMmOut* q, const JvMmOut* v, bool f32, hipStream_t s) {
+static hipError_t grads_tile(const JvMmOut* q, const JvMmOut* v, hipStream_t s) {
     static_assert(TQ::LDS == TV::LDS && TQ::THREADS == 256 && TV::THREADS == 256);
-    auto steps = [&](const JvMmOut& a) { return f32 ? (a.mm.k + 31) / 32 : (a.mm.kph >> 1) * a.mm.segs; };
-    const int64_t nq = q ? tile_count(*q, TQ::TM, TQ::TN, steps(*q)) : 0, nv = v ? tile_count(*v, TV::TM, TV::TN, steps(*v)) : 0;
+    const int64_t nq = q ? tile_count(*q, TQ::TM, TQ::TN, TQ::steps(q->mm)) : 0, nv = v ? tile_count(*v, TV::TM, TV::TN, TV::steps(v->mm)) : 0;
     if (nq < 0 || nv < 0 || nq + nv > 0x7fffffffll) return hipErrorInvalidValue;
     if (nq + nv == 0) return hipSuccess;
     hipError_t e = lds_of(jvs_grads_tile_kernel<TQ, TV>, TQ::LDS);
@@ -549,33 +562,44 @@ static hipError_t grads_tile(const JvMmOut* q, const JvMmOut* v, bool f32, hipSt
     return hipGetLastError();
 }
 
-// Tiles of the gradients' products: 256 x 256 (large), else 128 x 128, or 64 x 64 where that would be no more than one tile a CU.
-static bool few_grads(int64_t tiles) { return tiles <= 256; }
-static int64_t tiles128(int64_t rows, int64_t cols) { return std::max<int64_t>((rows + 127) / 128, 1) * ((cols + 127) / 128); }
+// The gradients' products have d columns: with up to 128 half a large tile would be multiplied for nothing.
+static int grads_path(int path, int d) { return path == JV_SX_LARGE && d <= 128 ? JV_SX_TILES : path; }
 
 // k ranges of dq: once around the CUs with the large tiles, twice with the small ones; at least four and eight steps in each (a range that is
 // joined costs a launch more)
-extern "C" int jvk_sx_grad_splits(int nq, int d, int64_t rows, int f32, int large) {
-    const int64_t tiles = large ? std::max<int64_t>((nq + 255) / 256, 1) * ((d + 255) / 256) : tiles128(nq, d);
-    const int64_t steps = (rows + 63) / 64 * (f32 ? large ? 6 : 2 : 1);
-    return (int)std::max<int64_t>(std::min<int64_t>((large ? 256 : 512) / tiles, steps / (large ? 4 : 8)), 1);
+extern "C" int jvk_sx_grad_splits(int path, int nq, int d, int64_t rows) {
+    path = grads_path(path, d);
+    const int tm = path == JV_SX_LARGE ? 256 : path == JV_SX_PLANES ? shape_of(path, nq, rows).m : 128, tn = path == JV_SX_LARGE ? 256 : 128;
+    const int64_t tiles = std::max<int64_t>((nq + tm - 1) / tm, 1) * ((d + tn - 1) / tn);
+    const int64_t steps = path == JV_SX_RAW || path == JV_SX_PLANES ? (rows + 31) / 32 : (rows + 63) / 64;
+    return (int)std::max<int64_t>(std::min<int64_t>((path == JV_SX_LARGE ? 256 : 512) / tiles, steps / (path == JV_SX_LARGE ? 4 : 8)), 1);
 }
-extern "C" hipError_t jvk_sx_grads(const JvMmOut* q, const JvMmOut* v, int f32, int large, hipStream_t s) {
-    if (large) {
-        hipError_t e = hipSuccess;
+extern "C" hipError_t jvk_sx_grads(const JvMmOut* q, const JvMmOut* v, int path, hipStream_t s) {
+    path = grads_path(path, q ? q->mm.N : v->mm.N);
+    hipError_t e = hipSuccess;
+    if (path == JV_SX_LARGE) {
         if (q) e = mm_out_pipe<BF16, false, true>(*q, s);
         if (v && e == hipSuccess) e = mm_out_pipe<BF16, true, true>(*v, s);
         return e;
     }
+    if (path == JV_SX_PLANES) {
+        if (q) {
+            const int m = shape_of(path, q->mm.M, 0).m;
+            e = m == 32 ? mm_out_tile<Tile3<1, false, true>>(*q, s) : m == 64 ? mm_out_tile<Tile3<2, false, true>>(*q, s) : m == 96 ? mm_out_tile<Tile3<3, false, true>>(*q, s) : mm_out_tile<Tile3<4, false, true>>(*q, s);
+        }
+        if (v && e == hipSuccess) e = mm_out_tile<Tile3<4, true, true>>(*v, s);
+        return e;
+    }
+    // 64 x 64 where 128 x 128 would be no more than one tile a CU
     int64_t tiles = 0;
     for (const JvMmOut* o : {q, v})
-        if (o) tiles += tiles128(o->mm.M, o->mm.N) * o->splits;
-    if (few_grads(tiles)) {
-        if (f32) return grads_tile<Tile32<1, 1, 2, 2, 4, false, true>, Tile32<1, 1, 2, 2, 4, true, true>>(q, v, true, s);
-        return grads_tile<Tile<BF16, 1, 1, 2, 2, 4, false, true>, Tile<BF16, 1, 1, 2, 2, 4, true, true>>(q, v, false, s);
+        if (o) tiles += (int64_t)((o->mm.M + 127) / 128) * ((o->mm.N + 127) / 128) * o->splits;
+    if (path == JV_SX_RAW) {
+        if (tiles <= 256) return grads_tile<Tile32<1, 1, 2, 2, 4, false, true>, Tile32<1, 1, 2, 2, 4, true, true>>(q, v, s);
+        return grads_tile<Tile32<2, 2, 2, 2, 2, false, true>, Tile32<2, 2, 2, 2, 2, true, true>>(q, v, s);
     }
-    if (f32) return grads_tile<Tile32<2, 2, 2, 2, 2, false, true>, Tile32<2, 2, 2, 2, 2, true, true>>(q, v, true, s);
-    return grads_tile<Tile<BF16, 2, 2, 2, 2, 2, false, true>, Tile<BF16, 2, 2, 2, 2, 2, true, true>>(q, v, false, s);
+    if (tiles <= 256) return grads_tile<Tile<BF16, 1, 1, 2, 2, 4, false, true>, Tile<BF16, 1, 1, 2, 2, 4, true, true>>(q, v, s);
+    return grads_tile<Tile<BF16, 2, 2, 2, 2, 2, false, true>, Tile<BF16, 2, 2, 2, 2, 2, true, true>>(q, v, s);
 }
 
 // partial sums -> the queries' gradient, and what G lacked at the target: one wave a row, four columns a lane

@@ -75,7 +75,7 @@ struct Tile {
     static constexpr int BUF = (GA + GB) * GROUP, LDS = NS * BUF;
     static_assert(GA % WAVES == 0 && GB % WAVES == 0, "every wave copies the same number of groups of each operand");
     static_assert(TY == BF16 || (!TA && !TB), "8-bit operands have k along their rows");
-    static __device__ __forceinline__ int steps(const JvMm& a) { return (a.kph >> 1) * a.segs; }
+    static __host__ __device__ __forceinline__ int steps(const JvMm& a) { return (a.kph >> 1) * a.segs; }
 
     template <int PIECES>   // 16-B pieces of a row
     static __device__ __forceinline__ int swirl(int k) {

@@ -5,7 +5,7 @@
 #include <utility>
 
 #include "jv_pipe.h"
-#include "jv_tile32.h"
+#include "jv_tile3.h"
 
 namespace jvmm {
 
@@ -144,7 +144,7 @@ static inline int64_t tile_count(const JvMmOut& a, int TM, int TN, int steps) {
 
 template <class T>
 static hipError_t mm_out_tile(const JvMmOut& a, hipStream_t s) {
-    const int64_t all = tile_count(a, T::TM, T::TN, (a.mm.kph >> 1) * a.mm.segs);
+    const int64_t all = tile_count(a, T::TM, T::TN, T::steps(a.mm));
     if (all <= 0) return all ? hipErrorInvalidValue : hipSuccess;
     hipError_t e = lds_of(jvm_out_tile_kernel<T>, T::LDS);
     if (e != hipSuccess) return e;

@@ -36,8 +36,8 @@ struct JvMmOut {
 struct JvSxLoss {
     JvMm mm;
     float c;               // scale * log2(e)
-    int32_t tile;          // jvk_sx_loss_plan's
-    int32_t splits;        // workgroups that share a panel of queries
+    int32_t path;          // JvSxPath
+    int32_t splits;        // jvk_sx_loss_splits
     float2* part;          // [M][splits]: maximum and sum (log2 domain)
     int32_t first;         // 0: partials of an earlier piece of the rows are in `part` already, join them
     const int32_t* targets;  // nullptr = none
@@ -51,7 +51,8 @@ struct JvSxQuery {
     int32_t target;        // row, -1 = none
     int32_t pad;
 };
-// one piece of the gradient's weights G = w (p - [j = target]), as bf16 planes [up(M, 64)][planes][kv]: zeros behind M and N
+// one piece of the gradient's weights G = w (p - [j = target]): bf16 planes [up(M, 64)][planes][kv], or float32 [up(M, 64)][kv] (JV_SX_RAW), zeros
+// behind M and N; `segs` says float32's three planes (6) from bf16's one (1)
 struct JvSxWeights {
     JvMm mm;               // A = queries, B = vectors of this piece
     float c;
@@ -60,20 +61,21 @@ struct JvSxWeights {
     const float *lse, *w;
     const int32_t* targets;
     int64_t n;             // rows in all
-    int32_t planes;        // 1 or 3, or 0: float32 as it is
-    void* g;                 // (planes = 0: float32)
+    int32_t path;          // JvSxPath
+    void* g;               // one plane of bf16 (JV_SX_RAW: float32, or three planes)
     int32_t kv;            // N padded to 64
     float* rest;           // [M] bf16: what G's entry at the target lacks of its float32 value
 };
 
-// what has to be laid out before a product: up to two matrices (rows -> bf16 planes [rows][planes][kp]) and the queries' constants, one launch
+// what has to be laid out before a product: up to three matrices (rows -> bf16 planes [rows][planes][kp]) and the queries' constants, one launch
 struct JvSxPrepare {
     struct Matrix {
         const void* x;
         int64_t stride, rows;   // rows = 0: none
-        uint16_t* out;
-    } m[2];
-    int32_t dtype, d, kp;
+        void* out;
+        int32_t kp;             // 4: float32 rows of fewer than four components, as rows of four
+    } m[3];
+    int32_t dtype, d;
     // the gradient's queries (query == nullptr: none)
     const float *lse, *w;
     const int32_t* targets;
@@ -92,15 +94,21 @@ hipError_t jvk_f8_decode(const uint8_t* codes, const uint8_t* scales, int64_t n,
 hipError_t jvk_f8_score(const JvMmOut* a, hipStream_t s);
 
 hipError_t jvk_sx_prepare(const JvSxPrepare* a, hipStream_t s);
-int jvk_sx_loss_plan(int nq, int64_t rows, int d, int f32, int* tile);   // splits, and the queries of a tile
-hipError_t jvk_sx_loss(const JvSxLoss* a, int f32, hipStream_t s);   // f32: operands are float32 as they lie
+// How the products of a shape are computed.
+enum JvSxPath {
+    JV_SX_LARGE,    // 256 x 256 tiles (jv_pipe.h); float32 as planes
+    JV_SX_TILES,    // bf16 on smaller tiles (jv_mm.h)
+    JV_SX_PLANES,   // float32: queries and g as planes, vectors as they lie (jv_tile3.h)
+    JV_SX_RAW       // float32, few tiles: everything as it lies (jv_tile32.h)
+};
+int jvk_sx_path(int nq, int64_t rows, int d, int f32);
+int jvk_sx_loss_splits(int path, int nq, int64_t rows);   // workgroups that share a panel of queries
+hipError_t jvk_sx_loss(const JvSxLoss* a, hipStream_t s);
 hipError_t jvk_sx_join(const float2* part, int splits, int nq, const float* hit, const int32_t* targets, int64_t n, float* loss, float* lse, hipStream_t s);
-hipError_t jvk_sx_weights(const JvSxWeights* a, int large, hipStream_t s);   // (planes = 0: float32 as it lies)
+hipError_t jvk_sx_weights(const JvSxWeights* a, hipStream_t s);
 // dq = G V and dv = G^T Q (nullptr: not asked for)
-int jvk_sx_grad_splits(int nq, int d, int64_t rows, int f32, int large);
-hipError_t jvk_sx_grads(const JvMmOut* q, const JvMmOut* v, int f32, int large, hipStream_t s);   // large: of jvk_sx_large_grads
-int jvk_sx_large_grads(int large, int d);   // and whether the gradients' products do
-int jvk_sx_large(int nq, int64_t rows, int d, int f32);   // whether a piece of the rows takes the large tiles for g
+int jvk_sx_grad_splits(int path, int nq, int d, int64_t rows);
+hipError_t jvk_sx_grads(const JvMmOut* q, const JvMmOut* v, int path, hipStream_t s);
 hipError_t jvk_sx_finish(const float* slab, int splits, int64_t rows, int d, int64_t lds, const float* rest, const JvSxQuery* query, const void* v, int64_t v_stride,
                          float mul, const float* norm, void* out, int dtype, int64_t ldo, hipStream_t s);
 hipError_t jvk_sx_fill(void* out, int dtype, int64_t stride, int64_t rows, int d, float value, hipStream_t s);

@@ -22,7 +22,7 @@ struct Tile32 {
     static constexpr int BUF = (GA + GB) * GROUP, LDS = NS * BUF;
     static_assert(GA % WAVES == 0 && GB % WAVES == 0, "every wave copies the same number of groups of each operand");
     static_assert((!TA || GA >= 8) && (!TB || GB >= 8), "the swapped halves are 32 columns each");
-    static __device__ __forceinline__ int steps(const JvMm& a) { return (a.k + 31) / 32; }
+    static __host__ __device__ __forceinline__ int steps(const JvMm& a) { return (a.k + 31) / 32; }
 
     static __device__ __forceinline__ void split(const float (&x)[8], bf16x8 (&p)[3]) {
         float r[8];
@@ -35,6 +35,16 @@ struct Tile32 {
                 p[k][e] = (__bf16)r[e];
                 if (k < 2) r[e] -= (float)p[k][e];
             }
+    }
+
+    // four components of a row's last step: those of the 16 B that started earlier from where they are, what lies behind the row as zeros
+    static __device__ __forceinline__ f32x4 tail(f32x4 v, int piece, int valid, int k) {
+        const int back = k < 4 || 4 * piece >= valid ? 0 : max(4 * piece + 4 - valid, 0);
+        if (back & 1) v = (f32x4){v[1], v[2], v[3], v[3]};
+        if (back & 2) v = (f32x4){v[2], v[3], v[3], v[3]};
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = 4 * piece + e < valid ? v[e] : 0.0f;
+        return v;
     }
 
     // One operand of `rows` rows of k components (k along) or k rows of `cols` columns (k across); GROUPS * 8 rows or columns from `first` on.
@@ -85,13 +95,7 @@ struct Tile32 {
                 for (int half = 0; half < 2; half++) {
                     const int piece = 4 * kk + 2 * h + half;
                     f32x4 v = *(const f32x4*)(row + ((piece ^ (r & 7)) << 4));
-                    if constexpr (LAST) {
-                        const int back = k < 4 || 4 * piece >= valid ? 0 : max(4 * piece + 4 - valid, 0);
-                        if (back & 1) v = (f32x4){v[1], v[2], v[3], v[3]};
-                        if (back & 2) v = (f32x4){v[2], v[3], v[3], v[3]};
-#pragma unroll
-                        for (int e = 0; e < 4; e++) v[e] = 4 * piece + e < valid ? v[e] : 0.0f;
-                    }
+                    if constexpr (LAST) v = tail(v, piece, valid, k);
 #pragma unroll
                     for (int e = 0; e < 4; e++) x[4 * half + e] = v[e];
                 }

@@ -404,7 +404,8 @@ def test_scores_on_the_large_tiles(torch, ops, out, nq, n, d):
 
 
 @pytest.mark.parametrize("dtype,nq,n,d,pad", [("bf16", 300, 30011, 200, 0), ("f32", 257, 26000, 70, 3), ("bf16", 1030, 10001, 384, 8), ("bf16", 80, 60000, 64, 0),
-                                              ("f32", 600, 17000, 128, 0), ("f32", 600, 17000, 132, 0), ("bf16", 600, 17000, 128, 0), ("f32", 500, 25000, 129, 2), ("bf16", 400, 26000, 136, 2), ("bf16", 400, 26000, 8, 2)])
+                                              ("f32", 600, 17000, 128, 0), ("f32", 600, 17000, 132, 0), ("bf16", 600, 17000, 128, 0), ("f32", 500, 25000, 129, 2), ("bf16", 400, 26000, 136, 2), ("bf16", 400, 26000, 8, 2), ("f32", 20, 40001, 70, 1), ("f32", 64, 33000, 3, 0),
+                                              ("f32", 90, 36000, 130, 0), ("f32", 130, 24000, 100, 5), ("f32", 700, 9000, 36, 1)])
 def test_softmax_on_the_large_tiles(torch, ops, dtype, nq, n, d, pad):
     q, v, t, w, _, _, t64, _ = loss_case(torch, nq, n, d, dtype, pad)
     scale = 15.0
