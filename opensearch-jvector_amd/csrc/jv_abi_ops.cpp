@@ -77,8 +77,8 @@ int check_shape(int64_t n, int d, const char* what) {
 
 // ---- the softmax loss: what a call needs, from its shape alone ----
 struct Plan {
-    int P, segs, dp, kq;              // planes, segments; d and nq padded to 64
-    int64_t rows_f, rows_b;           // rows of one piece, forward (only if the vectors have to be laid out) / backward
+    int P, dp, kq;                    // planes; d and nq padded to 64
+    int64_t rows_f, rows_b;           // rows of one piece, forward (where the vectors have to be laid out) / backward
     int path_f, path_b, splits_f, splits_q;   // forward, backward
     int64_t off_q, off_q4, off_v, off_part, off_hit, off_query, off_norm, off_rest, off_g, off_slab, bytes;
 };
@@ -99,7 +99,6 @@ int64_t piece(int64_t n, int64_t most) {
 Plan make_plan(int dtype, int nq, int64_t n, int d, uint32_t what) {
     Plan p{};
     p.P = dtype == JV_DTYPE_F32 ? 3 : 1;
-    p.segs = dtype == JV_DTYPE_F32 ? 6 : 1;
     p.dp = (int)up(d, 64);
     p.kq = (int)up(std::max(nq, 1), 64);
     const int64_t panels = std::max((nq + 255) / 256, 1), row = (int64_t)p.P * p.dp * 2;
@@ -115,14 +114,14 @@ Plan make_plan(int dtype, int nq, int64_t n, int d, uint32_t what) {
     p.off_q = take((int64_t)nq * row);
     p.off_q4 = take((int64_t)(d < 4 ? nq : 0) * 16);   // (float32 rows of fewer than four components, as they lie but with four)
     if (what & JV_SOFTMAX_LOSS) {
-        p.path_f = jvk_sx_path(nq, n, d, dtype == JV_DTYPE_F32);
+        p.path_f = jvk_sx_path(nq, n, dtype == JV_DTYPE_F32);
         p.splits_f = jvk_sx_loss_splits(p.path_f, nq, n);
         p.off_part = take((int64_t)p.splits_f * nq * 8);
         p.off_hit = take((int64_t)nq * 4);
         p.off_v = take(std::min<int64_t>(p.rows_f, n) * row);
     }
     if (what & (JV_SOFTMAX_QUERY_GRAD | JV_SOFTMAX_VECTOR_GRAD)) {
-        p.path_b = jvk_sx_path(nq, std::min<int64_t>(p.rows_b, n), d, dtype == JV_DTYPE_F32);
+        p.path_b = jvk_sx_path(nq, std::min<int64_t>(p.rows_b, n), dtype == JV_DTYPE_F32);
         p.off_v = take(std::min<int64_t>(p.rows_b, n) * row);
         p.off_query = take((int64_t)nq * sizeof(JvSxQuery));
         p.off_norm = take(4);
@@ -175,14 +174,14 @@ int check_softmax_call(const jv_softmax_params* p, const Plan& plan) {
 
 // k ranges that a piece of `rows` rows has at most: its steps
 int splits_of(const Plan& plan, int64_t rows) {
-    return (int)(plan.path_b == JV_SX_RAW || plan.path_b == JV_SX_PLANES ? up(rows, 64) / 32 : up(rows, 64) / 64 * plan.segs);
+    return (int)(up(rows, 64) / (plan.path_b == JV_SX_RAW || plan.path_b == JV_SX_PLANES ? 32 : 64));
 }
 
 // queries times vectors, but for where the vectors lie and how many they are
 JvMm logits(const Plan& plan, int nq, int d) {
     JvMm mm{};
-    mm.M = nq, mm.k = d, mm.kph = plan.dp / 32, mm.segs = plan.segs;
-    mm.plane_a = mm.plane_b = (int64_t)plan.dp * 2;
+    mm.M = nq, mm.k = d, mm.kph = plan.dp / 32;
+    mm.plane_a = (int64_t)plan.dp * 2;
     mm.end_b = kNoEnd;
     return mm;
 }
@@ -243,7 +242,7 @@ int jv_score_blocks_device(int32_t device, const uint8_t* d_query_codes, const u
     a.mm.kph = 2 * blocks;
     a.mm.a = (const char*)d_query_codes, a.mm.b = (const char*)d_codes;
     a.mm.lda = a.mm.ldb = (int64_t)blocks * 128;
-    a.mm.M = nq, a.mm.N = n, a.mm.segs = 1, a.mm.end_b = kNoEnd;
+    a.mm.M = nq, a.mm.N = n, a.mm.end_b = kNoEnd;
     a.mm.sa = d_query_scales, a.mm.sb = d_scales;
     a.mul = 1.0f, a.dtype = dtype, a.out = d_out_scores, a.ldo = row_stride, a.splits = 1;
     CHK(jvk_f8_score(&a, (hipStream_t)hip_stream));
@@ -349,9 +348,8 @@ int jv_softmax_grad_device(const jv_softmax_params* p, const float* d_lse, const
         pre.m[0].rows = pre.m[2].rows = 0, pre.query = nullptr;
         CHK(jvk_sx_weights(&w, s));
         JvMmOut o{}, q;
-        o.mm.segs = plan.segs;
         o.mm.a = (const char*)w.g, o.mm.lda = raw ? (int64_t)w.kv * 4 : (int64_t)plan.P * w.kv * 2, o.mm.plane_a = (int64_t)w.kv * 2;
-        o.mm.N = p->d, o.mm.plane_b = (int64_t)plan.dp * 2, o.mm.end_b = kNoEnd;
+        o.mm.N = p->d, o.mm.end_b = kNoEnd;
         if (d_out_query_grad) {   // G times the piece's vectors: k = its rows
             o.mm.M = p->nq, o.mm.k = w.kv, o.mm.kph = w.kv / 32;
             o.mm.b = w.mm.b, o.mm.ldb = w.mm.ldb, o.mm.kb = rows, o.mm.cb = rv.ready || rv.kp == 4 ? p->d : plan.dp;
@@ -361,7 +359,7 @@ int jv_softmax_grad_device(const jv_softmax_params* p, const float* d_lse, const
             q = o;
         }
         if (d_out_vector_grad) {   // G across times the queries: k = the queries
-            o.mm.M = rows, o.mm.k = (int)up(p->nq, 32), o.mm.kph = plan.kq / 32, o.mm.ka = f32 && plan.path_b != JV_SX_LARGE ? o.mm.k : plan.kq, o.mm.ca = w.kv;
+            o.mm.M = rows, o.mm.k = (int)up(p->nq, 32), o.mm.kph = plan.kq / 32, o.mm.ka = f32 ? o.mm.k : plan.kq, o.mm.ca = w.kv;
             o.mm.b = q_rows, o.mm.ldb = q_ld, o.mm.kb = p->nq, o.mm.cb = rb.ready || rb.kp == 4 ? p->d : plan.dp;
             o.mul = p->scale, o.norm = norm, o.dtype = p->dtype, o.splits = 1, o.add = 0;
             o.out = (char*)d_out_vector_grad + at * vector_grad_stride * size_of(p->dtype), o.ldo = vector_grad_stride;

@@ -262,7 +262,7 @@ __global__ __launch_bounds__(512) void jvs_loss_pipe_kernel(const JvSxLoss a) {
             [&](int i, Work& w) {
                 const int t = split + i * a.splits;
                 if (t >= tiles) return false;
-                w.m0 = m0, w.n0 = t * P::TN, w.k0 = 0, w.k1 = a.mm.kph * a.mm.segs;
+                w.m0 = m0, w.n0 = t * P::TN, w.k0 = 0, w.k1 = a.mm.kph;
                 return true;
             },
             [&](const Work& w, f32x16 (&acc)[4][2]) -> int {
@@ -273,7 +273,7 @@ __global__ __launch_bounds__(512) void jvs_loss_pipe_kernel(const JvSxLoss a) {
 }
 
 template <class T, int WM, int WN>
-__global__ __launch_bounds__(T::THREADS) void jvs_loss_tile_kernel(const JvSxLoss a) {
+__global__ __launch_bounds__(T::THREADS, T::RESIDENT) void jvs_loss_tile_kernel(const JvSxLoss a) {
     constexpr int MT = T::MT, NT = T::NT;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int panels = (a.mm.M + T::TM - 1) / T::TM, tiles = (a.mm.N + T::TN - 1) / T::TN;
@@ -293,13 +293,11 @@ __global__ __launch_bounds__(T::THREADS) void jvs_loss_tile_kernel(const JvSxLos
     write_partials<T::TM, MT, WN>(a, smem, m0, split, (threadIdx.x >> 6) / WM, [](int m) { return T::row(m); }, top, sum);
 }
 
-// The large tiles where they fill the chip and more than half of one is queries.  float32 only with more than 128 components: both operands'
-// planes are worth laying out when they are read often enough (step 300 x 100 000 x 128: 618 us so, 417 us as it lies; step
-// 777 x 30 011 x 381: 730 and 799 us).  Otherwise smaller tiles; float32 with everything as it lies where that is no more than one of 128 x 128
-// a CU (laying out costs a launch), with the queries as planes above.
-extern "C" int jvk_sx_path(int nq, int64_t rows, int d, int f32) {
-    if (nq > 128 && ((nq + 255) / 256) * ((rows + 255) / 256) >= 192 && (!f32 || d > 128)) return JV_SX_LARGE;
-    if (!f32) return JV_SX_TILES;
+// bf16: the large tiles where they fill the chip and more than half of one is queries.  float32: everything as it lies where that is no more than
+// one tile of 128 x 128 a CU (laying out costs a launch), the queries as planes above (step 777 x 30 011 x 381: 555 us; with both operands as
+// planes on the large tiles, every pair of planes a pass over k: 695 us; step 2000 x 30 000 x 1024: 2.82 and 2.90 ms).
+extern "C" int jvk_sx_path(int nq, int64_t rows, int f32) {
+    if (!f32) return nq > 128 && ((nq + 255) / 256) * ((rows + 255) / 256) >= 192 ? JV_SX_LARGE : JV_SX_TILES;
     return (int64_t)((nq + 127) / 128) * ((rows + 127) / 128) <= 256 ? JV_SX_RAW : JV_SX_PLANES;
 }
 
@@ -428,7 +426,7 @@ __global__ __launch_bounds__(512) void jvs_weights_kernel(const JvSxWeights a) {
             int L, m, n;
             if (!share.at(i, L)) return false;
             band_order(L, tm, tn, m, n);
-            w.m0 = m * P::TM, w.n0 = n * P::TN, w.k0 = 0, w.k1 = a.mm.kph * a.mm.segs;
+            w.m0 = m * P::TM, w.n0 = n * P::TN, w.k0 = 0, w.k1 = a.mm.kph;
             return true;
         },
         [&](const Work& w, f32x16 (&acc)[4][2]) -> int {
@@ -436,23 +434,10 @@ __global__ __launch_bounds__(512) void jvs_weights_kernel(const JvSxWeights a) {
             for (int m = 0; m < 4; m++) {
                 const int r = w.m0 + P::row(m);
                 JvSxQuery q = {__builtin_inff(), 0.0f, -1, 0};
-                if (r < a.mm.M) q = a.query ? a.query[r] : query_of(a.lse, a.w, a.targets, a.n, r);
-                weigh<P>(acc[m], q, a.c, a.mm.N - w.n0, q.target >= 0 ? (int)(q.target - a.row0) - w.n0 : -1, a.mm.segs == 1, a.rest + r);
+                if (r < a.mm.M) q = a.query[r];
+                weigh<P>(acc[m], q, a.c, a.mm.N - w.n0, q.target >= 0 ? (int)(q.target - a.row0) - w.n0 : -1, true, a.rest + r);
             }
-            int stores = 0;
-            const int planes = a.mm.segs == 1 ? 1 : 3;
-            for (int k = 0; k < planes; k++) {
-                stores = P::write_bf16(smem, (uint16_t*)a.g + (int64_t)k * a.kv, (int64_t)planes * a.kv, true, w, padded, a.kv, [&](int m, int n, int e) { return acc[m][n][e]; });
-                if (planes > 1) {
-#pragma unroll
-                    for (int m = 0; m < 4; m++)
-#pragma unroll
-                        for (int n = 0; n < 2; n++)
-#pragma unroll
-                            for (int e = 0; e < 16; e++) acc[m][n][e] -= (float)(__bf16)acc[m][n][e];
-                }
-            }
-            return stores;
+            return P::write_bf16(smem, (uint16_t*)a.g, a.kv, true, w, padded, a.kv, [&](int m, int n, int e) { return acc[m][n][e]; });
         });
 }
 
@@ -464,7 +449,7 @@ static __host__ __device__ __forceinline__ int padded_queries(const JvSxWeights&
 
 // the same on small tiles, one a workgroup
 template <class T>
-__global__ __launch_bounds__(T::THREADS) void jvs_weights_tile_kernel(const JvSxWeights a) {
+__global__ __launch_bounds__(T::THREADS, T::RESIDENT) void jvs_weights_tile_kernel(const JvSxWeights a) {
     constexpr int MT = T::MT, NT = T::NT;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int padded = padded_queries(a);

@@ -33,10 +33,6 @@ __device__ __forceinline__ void glds16(const char* g, unsigned char* l) {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g, (__attribute__((address_space(3))) void*)l, 16, 0, 0);
 }
 
-// plane of segment g (see JvMm): pairs (2,0) (0,2) (1,1) (1,0) (0,1) (0,0), the smallest products first
-__device__ __forceinline__ int plane_a(int g) { return (0x052 >> (2 * g)) & 3; }
-__device__ __forceinline__ int plane_b(int g) { return (0x118 >> (2 * g)) & 3; }
-
 // eight e4m3 codes times 2^(byte - 127), as bf16
 __device__ __forceinline__ bf16x8 widen(int lo, int hi, int byte) {
     const float s = __int_as_float(byte << 23);
@@ -68,14 +64,14 @@ __device__ __forceinline__ void wait_step(int left) {
 // lies at p ^ (swirl << 2) so that they are the four quarters of a 256-B bank row.
 template <int TY, int MT_, int NT_, int WM, int WN, int NS, bool TA = false, bool TB = false>
 struct Tile {
-    static constexpr int MT = MT_, NT = NT_;
+    static constexpr int MT = MT_, NT = NT_, RESIDENT = 1;
     static constexpr int TM = 32 * MT * WM, TN = 32 * NT * WN, WAVES = WM * WN, THREADS = 64 * WAVES;
     static constexpr int GA = TM / 8, GB = TN / 8;                               // 8-row groups
     static constexpr int CA = GA / WAVES, CB = GB / WAVES, PER = CA + CB;        // copies of one wave a step
     static constexpr int BUF = (GA + GB) * GROUP, LDS = NS * BUF;
     static_assert(GA % WAVES == 0 && GB % WAVES == 0, "every wave copies the same number of groups of each operand");
     static_assert(TY == BF16 || (!TA && !TB), "8-bit operands have k along their rows");
-    static __host__ __device__ __forceinline__ int steps(const JvMm& a) { return (a.kph >> 1) * a.segs; }
+    static __host__ __device__ __forceinline__ int steps(const JvMm& a) { return a.kph >> 1; }
 
     template <int PIECES>   // 16-B pieces of a row
     static __device__ __forceinline__ int swirl(int k) {
@@ -91,7 +87,7 @@ struct Tile {
 
     // C tile at (m0, n0), steps [k0, k1).  Rows behind the operands' last are read as their last.
     static __device__ __forceinline__ void run(const JvMm& a, int m0, int n0, int k0, int k1, unsigned char* smem, f32x16 (&acc)[MT][NT]) {
-        const int nk = a.kph >> 1;   // steps of a segment
+        const int nk = a.kph >> 1;   // scales of a row
         const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
         const int lr = lane >> 3, lp = (lane & 7) ^ lr;
         const char* src[PER];   // k along rows: the row's piece; k across: the column's piece of row 0
@@ -135,18 +131,17 @@ struct Tile {
 #pragma unroll
                 for (int e = 0; e < 16; e++) acc[m][n][e] = 0.0f;
 
-        int seg = k0 / nk, kin = k0 - seg * nk;   // of the next step to be staged
+        int kin = k0;   // the next step to be staged
         auto stage = [&](int buf) {
-            int64_t offa = TA ? 0 : (int64_t)kin * 128, offb = TB ? 0 : (int64_t)kin * 128;
-            if (a.segs > 1) offa += plane_a(seg) * a.plane_a, offb += plane_b(seg) * a.plane_b;
+            const int64_t off = (int64_t)kin * 128;
             unsigned char* dst = smem + buf * BUF;
 #pragma unroll
             for (int i = 0; i < CA; i++)
-                glds16(src[i] + offa + (TA ? (int64_t)min(kin * 64 + krow[i], a.ka - 1) * a.lda : 0), dst + (i * WAVES + w) * (TA ? 1024 : GROUP));
+                glds16(src[i] + (TA ? (int64_t)min(kin * 64 + krow[i], a.ka - 1) * a.lda : off), dst + (i * WAVES + w) * (TA ? 1024 : GROUP));
 #pragma unroll
             for (int i = 0; i < CB; i++)
-                glds16(src[CA + i] + (TB ? offb + (int64_t)min(kin * 64 + krow[CA + i], a.kb - 1) * a.ldb : min(offb, (int64_t)(a.end_b - 16 - lp * 16))), dst + GA * GROUP + (i * WAVES + w) * (TB ? 1024 : GROUP));
-            if (++kin == nk) kin = 0, seg++;
+                glds16(src[CA + i] + (TB ? (int64_t)min(kin * 64 + krow[CA + i], a.kb - 1) * a.ldb : min(off, (int64_t)(a.end_b - 16 - lp * 16))), dst + GA * GROUP + (i * WAVES + w) * (TB ? 1024 : GROUP));
+            kin++;
         };
 #pragma unroll
         for (int i = 0; i < NS - 1; i++)

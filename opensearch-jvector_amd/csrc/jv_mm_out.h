@@ -38,7 +38,7 @@ __global__ __launch_bounds__(512) void jvm_out_pipe_kernel(const JvMmOut a) {
     const int tm = (a.mm.M + P::TM - 1) / P::TM, tn = (a.mm.N + P::TN - 1) / P::TN, tiles = tm * tn;
     const Share share(tiles * a.splits);
     if (!share.mine()) return;
-    const int phases = a.mm.kph * a.mm.segs;
+    const int phases = a.mm.kph;
     auto work = [&](int i, Work& w) {
         int L;
         if (!share.at(i, L)) return false;
@@ -64,7 +64,7 @@ static hipError_t mm_out_pipe(const JvMmOut& a, hipStream_t s) {
     using P = Pipe<TY, TA, TB>;
     if (a.mm.M <= 0 || a.mm.N <= 0) return hipSuccess;
     const int64_t all = (int64_t)((a.mm.M + P::TM - 1) / P::TM) * ((a.mm.N + P::TN - 1) / P::TN) * a.splits;
-    if (all > 0x7fffffffll || a.splits < 1 || a.splits > a.mm.kph * a.mm.segs) return hipErrorInvalidValue;
+    if (all > 0x7fffffffll || a.splits < 1 || a.splits > a.mm.kph) return hipErrorInvalidValue;
     hipError_t e = lds_of(jvm_out_pipe_kernel<TY, TA, TB>, P::LDS);
     if (e != hipSuccess) return e;
     jvm_out_pipe_kernel<TY, TA, TB><<<(unsigned)(all < 256 ? (all + 7) / 8 * 8 : 256), P::THREADS, P::LDS, s>>>(a);
@@ -129,7 +129,7 @@ __device__ __forceinline__ void out_tile(const JvMmOut& a, int i, unsigned char*
 }
 
 template <class T>
-__global__ __launch_bounds__(T::THREADS) void jvm_out_tile_kernel(const JvMmOut a) {
+__global__ __launch_bounds__(T::THREADS, T::RESIDENT) void jvm_out_tile_kernel(const JvMmOut a) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     out_tile<T>(a, blockIdx.x, smem);
 }

@@ -5,17 +5,15 @@
 
 // One matrix product C[M][N].  An operand lies with k along its rows (lda / ldb bytes apart, M / N of them), or with k across them
 // (ka / kb rows, of ca / cb bf16 columns; what lies behind the last row reads as the last row again, so the OTHER operand holds zeros there).
-// k is whole phases of 64 B a row (32 bf16, 64 e4m3; an even number, zeros behind the data) and everything is 16-B aligned.
-// A float32 operand is three bf16 planes side by side in its row (x = h + m + l, 24 bits); its product is the six plane pairs that reach
-// 2^-24, walked as six segments of the same k range, the smallest first.
+// 8-bit and bf16 operands: k is whole phases of 64 B a row (32 bf16, 64 e4m3; an even number, zeros behind the data), everything is 4-B aligned
+// and columns come in eights.  float32 operands: jv_tile32.h, jv_tile3.h.
 struct JvMm {
     const char *a, *b;
     int64_t lda, ldb;
     int32_t M, N;
-    int32_t k;               // components (float32 as it lies, jv_tile32.h: nothing is padded there, and planes and segments do not count)
-    int32_t kph;             // phases of one segment
-    int32_t segs;            // 1 (bf16, e4m3) or 6 (float32)
-    int64_t plane_a, plane_b;  // bytes from plane to plane
+    int32_t k;               // components (float32)
+    int32_t kph;             // phases (bf16, e4m3)
+    int64_t plane_a;         // float32 as bf16 planes: bytes from plane to plane
     int32_t ka, kb, ca, cb;  // operands with k across their rows
     int32_t end_b;           // bytes of k that a row of B has, a multiple of 16 (k along its rows): what lies behind reads as the last 16, A holds zeros there
     const uint8_t *sa, *sb;  // e4m3: scale bytes [M][kph / 2] / [N][kph / 2]
@@ -51,8 +49,8 @@ struct JvSxQuery {
     int32_t target;        // row, -1 = none
     int32_t pad;
 };
-// one piece of the gradient's weights G = w (p - [j = target]): bf16 planes [up(M, 64)][planes][kv], or float32 [up(M, 64)][kv] (JV_SX_RAW), zeros
-// behind M and N; `segs` says float32's three planes (6) from bf16's one (1)
+// One piece of the gradient's weights G = w (p - [j = target]), zeros behind M and N: bf16 [up(M, 64)][kv]; float32 as three planes
+// [up(M, 32)][3][kv] (JV_SX_PLANES) or as it is [up(M, 32)][kv] (JV_SX_RAW).
 struct JvSxWeights {
     JvMm mm;               // A = queries, B = vectors of this piece
     float c;
@@ -62,7 +60,7 @@ struct JvSxWeights {
     const int32_t* targets;
     int64_t n;             // rows in all
     int32_t path;          // JvSxPath
-    void* g;               // one plane of bf16 (JV_SX_RAW: float32, or three planes)
+    void* g;
     int32_t kv;            // N padded to 64
     float* rest;           // [M] bf16: what G's entry at the target lacks of its float32 value
 };
@@ -96,12 +94,12 @@ hipError_t jvk_f8_score(const JvMmOut* a, hipStream_t s);
 hipError_t jvk_sx_prepare(const JvSxPrepare* a, hipStream_t s);
 // How the products of a shape are computed.
 enum JvSxPath {
-    JV_SX_LARGE,    // 256 x 256 tiles (jv_pipe.h); float32 as planes
+    JV_SX_LARGE,    // bf16, 256 x 256 tiles (jv_pipe.h)
     JV_SX_TILES,    // bf16 on smaller tiles (jv_mm.h)
     JV_SX_PLANES,   // float32: queries and g as planes, vectors as they lie (jv_tile3.h)
     JV_SX_RAW       // float32, few tiles: everything as it lies (jv_tile32.h)
 };
-int jvk_sx_path(int nq, int64_t rows, int d, int f32);
+int jvk_sx_path(int nq, int64_t rows, int f32);
 int jvk_sx_loss_splits(int path, int nq, int64_t rows);   // workgroups that share a panel of queries
 hipError_t jvk_sx_loss(const JvSxLoss* a, hipStream_t s);
 hipError_t jvk_sx_join(const float2* part, int splits, int nq, const float* hit, const int32_t* targets, int64_t n, float* loss, float* lse, hipStream_t s);

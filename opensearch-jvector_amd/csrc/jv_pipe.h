@@ -22,7 +22,7 @@ namespace jvmm {
 
 struct Work {
     int m0, n0;      // first row and column of the tile
-    int k0, k1;      // phases of the segs * kph in all
+    int k0, k1;      // phases of the kph in all
     int part;        // which k range
 };
 
@@ -65,7 +65,7 @@ struct Pipe {
         // ---- copies: two of A and two of B for each wave and phase ----
         Work sw;
         work(0, sw);
-        int si = 0, sk = sw.k0, sseg = sw.k0 / a.kph, skin = sw.k0 - sseg * a.kph, sreg = 0;
+        int si = 0, sk = sw.k0, sreg = 0;
         const char *pa[2], *pb[2];   // k along rows: the row's piece; k across: the column's piece of row 0
         auto rows = [&]() {
 #pragma unroll
@@ -80,20 +80,18 @@ struct Pipe {
         rows();
         const int64_t end_b = a.end_b - 16 - ((lane & 3) ^ ((lane >> 4) & 3)) * 16;
         auto stage = [&]() {
-            int64_t offa = TA ? 0 : (int64_t)skin * 64, offb = TB ? 0 : (int64_t)skin * 64;
-            if (a.segs > 1) offa += plane_a(sseg) * a.plane_a, offb += plane_b(sseg) * a.plane_b;
+            const int64_t off = (int64_t)sk * 64;
             unsigned char* dst = smem + sreg * REGION + w * 1024;
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const int k = skin * 32 + 16 * i + 2 * w + (lane >> 5);
-                glds16(pa[i] + offa + (TA ? (int64_t)min(k, a.ka - 1) * a.lda : 0), dst + i * 8192);
-                glds16(pb[i] + (TB ? offb + (int64_t)min(k, a.kb - 1) * a.ldb : min(offb, end_b)), dst + 16384 + i * 8192);
+                const int k = sk * 32 + 16 * i + 2 * w + (lane >> 5);
+                glds16(pa[i] + (TA ? (int64_t)min(k, a.ka - 1) * a.lda : off), dst + i * 8192);
+                glds16(pb[i] + (TB ? (int64_t)min(k, a.kb - 1) * a.ldb : min(off, end_b)), dst + 16384 + i * 8192);
             }
             sreg = (sreg + 1) & 3;
-            if (++skin == a.kph) skin = 0, sseg++;
             if (++sk == sw.k1) {   // on to the next tile (behind the last: the same one again, never read)
                 if (work(si + 1, sw)) si++;
-                sk = sw.k0, sseg = sw.k0 / a.kph, skin = sw.k0 - sseg * a.kph;
+                sk = sw.k0;
                 rows();
             }
         };

@@ -15,6 +15,7 @@ namespace jvmm {
 
 template <int MT_, bool TA, bool TB>
 struct Tile3 {
+    static constexpr int RESIDENT = 2;   // workgroups a CU
     static constexpr int MT = MT_, NT = 1, WAVES = 4, THREADS = 256, TM = 32 * MT, TN = 128;
     static constexpr int KA = 6 * MT, PA = (KA + 3) / 4, PB = 4, PER = PA + PB;   // KB of A in a step; copies of one wave (the last of A twice, if need be)
     static constexpr int BUF = (KA + 16) * 1024, LDS = 2 * BUF;
@@ -66,7 +67,7 @@ struct Tile3 {
                 for (int p = 0; p < 3; p++) va[t][p] = part_a(base, t, p, kk);
 #pragma unroll
             for (int g = 0; g < 6; g++) {
-                const int pa = (0x052 >> (2 * g)) & 3, pb = (0x118 >> (2 * g)) & 3;
+                const int pa = part_of_a(g), pb = part_of_b(g);
 #pragma unroll
                 for (int m = 0; m < MT; m++) acc[m][0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vb[pb], va[m][pa], acc[m][0], 0, 0, 0);
             }

@@ -13,9 +13,13 @@
 
 namespace jvmm {
 
+// the six pairs of parts (2,0) (0,2) (1,1) (1,0) (0,1) (0,0), the smallest products first
+__device__ __forceinline__ constexpr int part_of_a(int g) { return (0x052 >> (2 * g)) & 3; }
+__device__ __forceinline__ constexpr int part_of_b(int g) { return (0x118 >> (2 * g)) & 3; }
+
 template <int MT_, int NT_, int WM, int WN, int NS, bool TA, bool TB>
 struct Tile32 {
-    static constexpr int MT = MT_, NT = NT_;
+    static constexpr int MT = MT_, NT = NT_, RESIDENT = 1;
     static constexpr int TM = 32 * MT * WM, TN = 32 * NT * WN, WAVES = WM * WN, THREADS = 64 * WAVES;
     static constexpr int GA = TM / 8, GB = TN / 8;                       // KB of a step
     static constexpr int PER = (GA + GB) / WAVES;                        // copies of one wave a step
@@ -120,7 +124,7 @@ struct Tile32 {
             for (int t = 0; t < NT; t++) Side<TB, GB>::template read<LAST>(base + GA * GROUP, rb[t], kk, valid, a.k, vb[t]);
 #pragma unroll
             for (int g = 0; g < 6; g++) {
-                const int pa = (0x052 >> (2 * g)) & 3, pb = (0x118 >> (2 * g)) & 3;
+                const int pa = part_of_a(g), pb = part_of_b(g);
 #pragma unroll
                 for (int m = 0; m < MT; m++)
 #pragma unroll
