@@ -115,7 +115,7 @@ Plan make_plan(int dtype, int nq, int64_t n, int d, uint32_t what) {
     p.off_q4 = take((int64_t)(d < 4 ? nq : 0) * 16);   // (float32 rows of fewer than four components, as they lie but with four)
     if (what & JV_SOFTMAX_LOSS) {
         p.path_f = jvk_sx_path(nq, n, dtype == JV_DTYPE_F32);
-        p.splits_f = jvk_sx_loss_splits(p.path_f, nq, n);
+        p.splits_f = jvk_sx_loss_splits(p.path_f, nq, n, d);
         p.off_part = take((int64_t)p.splits_f * nq * 8);
         p.off_hit = take((int64_t)nq * 4);
         p.off_v = take(std::min<int64_t>(p.rows_f, n) * row);

@@ -147,18 +147,18 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
 // scaled difference (c <= 0: the smallest product is the largest logit), the exponential, the sum.
 // `m0`, `n0`: where the tile lies; the target's own logit is taken from the same product, so that a loss near 0 keeps its digits.
 template <class Core, int MT, int NT>
-__device__ __forceinline__ void add_tile(const JvSxLoss& a, f32x16 (&acc)[MT][NT], int m0, int n0, const int (&want)[MT], float (&top)[MT], float (&sum)[MT]) {
+__device__ __forceinline__ void add_tile(const JvSxLoss& a, typename Core::acc_t (&acc)[MT][NT], int m0, int n0, const int (&want)[MT], float (&top)[MT], float (&sum)[MT]) {
     const float c = a.c;
     const int rows = a.mm.N - n0;
-    const int first = Core::col(0, 0) & ~31;   // this wave's columns
+    const int first = Core::col(0, 0) & ~(Core::WIDE < 32 ? 7 : 31);   // this wave's columns
 #pragma unroll
     for (int m = 0; m < MT; m++) {
         const int at = want[m] - n0;
-        if (__any(at >= first && at < first + 32 * NT)) {
+        if (__any(at >= first && at < first + Core::WIDE)) {
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
-                for (int e = 0; e < 16; e++)
+                for (int e = 0; e < Core::E; e++)
                     if (Core::col(n, e) == at) a.hit[m0 + Core::row(m)] = acc[m][n][e] * c;
         }
     }
@@ -169,7 +169,7 @@ __device__ __forceinline__ void add_tile(const JvSxLoss& a, f32x16 (&acc)[MT][NT
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
-                for (int e = 0; e < 16; e++) acc[m][n][e] = Core::col(n, e) < rows ? acc[m][n][e] : none;
+                for (int e = 0; e < Core::E; e++) acc[m][n][e] = Core::col(n, e) < rows ? acc[m][n][e] : none;
     }
     float best[MT];
     if (c < 0.0f) {
@@ -179,7 +179,7 @@ __device__ __forceinline__ void add_tile(const JvSxLoss& a, f32x16 (&acc)[MT][NT
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
-                for (int e = 0; e < 16; e++) best[m] = fminf(best[m], acc[m][n][e]);
+                for (int e = 0; e < Core::E; e++) best[m] = fminf(best[m], acc[m][n][e]);
         }
     } else {
 #pragma unroll
@@ -188,7 +188,7 @@ __device__ __forceinline__ void add_tile(const JvSxLoss& a, f32x16 (&acc)[MT][NT
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
-                for (int e = 0; e < 16; e++) best[m] = fmaxf(best[m], acc[m][n][e]);
+                for (int e = 0; e < Core::E; e++) best[m] = fmaxf(best[m], acc[m][n][e]);
         }
     }
 #pragma unroll
@@ -200,12 +200,12 @@ __device__ __forceinline__ void add_tile(const JvSxLoss& a, f32x16 (&acc)[MT][NT
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
-                for (int e = 0; e < 16; e++) s += acc[m][n][e] == none ? 0.0f : exp2_(acc[m][n][e] * 0.0f);
+                for (int e = 0; e < Core::E; e++) s += acc[m][n][e] == none ? 0.0f : exp2_(acc[m][n][e] * 0.0f);
         } else {
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
-                for (int e = 0; e < 16; e++) s += exp2_(fmaf(acc[m][n][e], c, -ref));
+                for (int e = 0; e < Core::E; e++) s += exp2_(fmaf(acc[m][n][e], c, -ref));
         }
         top[m] = now;
         sum[m] = s;
@@ -286,7 +286,7 @@ __global__ __launch_bounds__(T::THREADS, T::RESIDENT) void jvs_loss_tile_kernel(
 #pragma unroll
     for (int m = 0; m < MT; m++) top[m] = -__builtin_inff(), sum[m] = 0.0f, want[m] = wanted(a, m0 + T::row(m));
     for (int t = split; t < tiles; t += a.splits) {
-        f32x16 acc[MT][NT];
+        typename T::acc_t acc[MT][NT];
         T::run(a.mm, m0, t * T::TN, 0, T::steps(a.mm), smem, acc);
         add_tile<T>(a, acc, m0, t * T::TN, want, top, sum);
     }
@@ -303,13 +303,16 @@ extern "C" int jvk_sx_path(int nq, int64_t rows, int f32) {
 
 // Queries and rows of the smaller tiles: 32 x 128 and 64 x 128 (float32 also 96 x 128) for up to so many queries, the rows being streamed and as
 // little as possible multiplied for nothing; 128 x 128 otherwise; but where that is no more than one tile a CU 64 x 64, with four steps of k
-// under way: the way to memory and the multiplications of one tile's steps are what counts then (float32, 118 x 18 x 843: 66 -> 36 us)
+// under way: the way to memory and the multiplications of one tile's steps are what counts then (float32, 118 x 18 x 843: 66 -> 36 us).
+// float32 with no more than a tile of 32 x 32 a CU and at least eight steps of k: those, four waves sharing a tile's steps (a step of 28 x 46 x 1167:
+// 90 -> 43 us, of 100 x 2000 x 768: 80 -> 49; bf16, a fifth of the instructions a step: 54 and 54).
 struct Shape {
     int m, n;
     bool few;
 };
-static Shape shape_of(int path, int nq, int64_t rows) {
+static Shape shape_of(int path, int nq, int64_t rows, int d) {
     if (path == JV_SX_LARGE) return {256, 256, false};
+    if (path == JV_SX_RAW && d > 7 * 32 && (int64_t)((nq + 31) / 32) * ((rows + 31) / 32) <= 256) return {32, 32, true};
     const bool few = (int64_t)((nq + 127) / 128) * ((rows + 127) / 128) <= 256;
     if (path == JV_SX_PLANES) return {nq > 96 ? 128 : (nq + 31) / 32 * 32, 128, false};
     if (nq <= 32) return {32, 128, few};
@@ -318,9 +321,9 @@ static Shape shape_of(int path, int nq, int64_t rows) {
 }
 
 // one for each CU with the large tiles, two or three with the small ones
-extern "C" int jvk_sx_loss_splits(int path, int nq, int64_t rows) {
-    const Shape t = shape_of(path, nq, rows);
-    const int full = t.m == 256 ? 256 : t.m == 128 || t.n == 64 || path == JV_SX_PLANES ? 512 : 768;
+extern "C" int jvk_sx_loss_splits(int path, int nq, int64_t rows, int d) {
+    const Shape t = shape_of(path, nq, rows, d);
+    const int full = t.m == 256 || t.n == 32 ? 256 : t.m == 128 || t.n == 64 || path == JV_SX_PLANES ? 512 : 768;
     const int64_t panels = std::max((nq + t.m - 1) / t.m, 1), tiles = std::max<int64_t>((rows + t.n - 1) / t.n, 1);
     return (int)std::min(std::max<int64_t>(full / panels, 1), tiles);
 }
@@ -338,7 +341,8 @@ extern "C" hipError_t jvk_sx_loss(const JvSxLoss* a, hipStream_t s) {
     using P = Pipe<BF16>;
     if (a->mm.N <= 0 || a->mm.M <= 0) return hipSuccess;
     if (a->splits < 1) return hipErrorInvalidValue;
-    const Shape t = shape_of(a->path, a->mm.M, a->mm.N);
+    const Shape t = shape_of(a->path, a->mm.M, a->mm.N, a->mm.k);
+    if (t.n == 32) return loss_tile<KSplit<Tile32<1, 1, 1, 1, 4, false, false, true>>, 1, 4>(*a, s);
     if (a->path == JV_SX_RAW) return t.m == 32 ? loss_tile<Tile32<1, 1, 1, 4, 4, false, false>, 1, 4>(*a, s) : loss_tile<Tile32<1, 1, 2, 2, 4, false, false>, 2, 2>(*a, s);
     if (a->path == JV_SX_PLANES) {
         if (t.m == 32) return loss_tile<Tile3<1, false, false>, 1, 4>(*a, s);
@@ -389,17 +393,17 @@ extern "C" hipError_t jvk_sx_join(const float2* part, int splits, int nq, const 
 // g of a lane's columns of one query, in place of the logits; `cols`: how many of the tile's columns are rows of the piece; `hit`: the target's
 // column.  Three instructions a value; the target, which few tiles hold, and the last tile's end are seen to apart.
 template <class Core, int NT>
-__device__ __forceinline__ void weigh(f32x16 (&acc)[NT], const JvSxQuery& q, float c, int cols, int hit, bool lossy, float* rest) {
+__device__ __forceinline__ void weigh(typename Core::acc_t (&acc)[NT], const JvSxQuery& q, float c, int cols, int hit, bool lossy, float* rest) {
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
-        for (int e = 0; e < 16; e++) acc[n][e] = exp2_(fmaf(acc[n][e], c, -q.lse2)) * q.w;
-    const int first = Core::col(0, 0) & ~31;   // this wave's columns
-    if (__any(hit >= first && hit < first + 32 * NT)) {
+        for (int e = 0; e < Core::E; e++) acc[n][e] = exp2_(fmaf(acc[n][e], c, -q.lse2)) * q.w;
+    const int first = Core::col(0, 0) & ~(Core::WIDE < 32 ? 7 : 31);   // this wave's columns
+    if (__any(hit >= first && hit < first + Core::WIDE)) {
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int e = 0; e < 16; e++)
+            for (int e = 0; e < Core::E; e++)
                 if (Core::col(n, e) == hit) {
                     acc[n][e] -= q.w;
                     if (lossy) *rest = acc[n][e] - (float)(__bf16)acc[n][e];   // (one lane holds it; three planes lack nothing)
@@ -409,7 +413,7 @@ __device__ __forceinline__ void weigh(f32x16 (&acc)[NT], const JvSxQuery& q, flo
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int e = 0; e < 16; e++) acc[n][e] = Core::col(n, e) < cols ? acc[n][e] : 0.0f;
+            for (int e = 0; e < Core::E; e++) acc[n][e] = Core::col(n, e) < cols ? acc[n][e] : 0.0f;
     }
 }
 
@@ -454,9 +458,9 @@ __global__ __launch_bounds__(T::THREADS, T::RESIDENT) void jvs_weights_tile_kern
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int padded = padded_queries(a);
     int m0, n0;
-    band_order(xcd_order(blockIdx.x, gridDim.x), (padded + T::TM - 1) / T::TM, (a.mm.N + T::TN - 1) / T::TN, m0, n0);
+    band_order(xcd_order(blockIdx.x, gridDim.x), (padded + T::TM - 1) / T::TM, (a.kv + T::TN - 1) / T::TN, m0, n0);
     m0 *= T::TM, n0 *= T::TN;
-    f32x16 acc[MT][NT];
+    typename T::acc_t acc[MT][NT];
     T::run(a.mm, m0, n0, 0, T::steps(a.mm), smem, acc);
 #pragma unroll
     for (int m = 0; m < MT; m++) {
@@ -469,7 +473,7 @@ __global__ __launch_bounds__(T::THREADS, T::RESIDENT) void jvs_weights_tile_kern
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
-                for (int g = 0; g < 4; g++) {
+                for (int g = 0; g < T::E / 4; g++) {
                     const int col = n0 + T::col(n, 4 * g);
                     if (r < padded && col < a.kv)
                         *(f32x4*)((float*)a.g + (int64_t)r * a.kv + col) = (f32x4){acc[m][n][4 * g], acc[m][n][4 * g + 1], acc[m][n][4 * g + 2], acc[m][n][4 * g + 3]};
@@ -481,7 +485,7 @@ __global__ __launch_bounds__(T::THREADS, T::RESIDENT) void jvs_weights_tile_kern
 #pragma unroll
                 for (int n = 0; n < NT; n++)
 #pragma unroll
-                    for (int g = 0; g < 4; g++) {
+                    for (int g = 0; g < T::E / 4; g++) {
                         const int col = n0 + T::col(n, 4 * g);
                         bf16x4 v;
 #pragma unroll
@@ -498,7 +502,7 @@ __global__ __launch_bounds__(T::THREADS, T::RESIDENT) void jvs_weights_tile_kern
 
 template <class T>
 static hipError_t weights_tile(const JvSxWeights& a, hipStream_t s) {
-    const int64_t all = (int64_t)((padded_queries(a) + T::TM - 1) / T::TM) * ((a.mm.N + T::TN - 1) / T::TN);
+    const int64_t all = (int64_t)((padded_queries(a) + T::TM - 1) / T::TM) * ((a.kv + T::TN - 1) / T::TN);
     if (all > 0x7fffffffll) return hipErrorInvalidValue;
     hipError_t e = lds_of(jvs_weights_tile_kernel<T>, T::LDS);
     if (e != hipSuccess) return e;
@@ -509,7 +513,8 @@ static hipError_t weights_tile(const JvSxWeights& a, hipStream_t s) {
 extern "C" hipError_t jvk_sx_weights(const JvSxWeights* a, hipStream_t s) {
     using P = Pipe<BF16>;
     if (a->mm.M <= 0 || a->mm.N <= 0) return hipSuccess;
-    const Shape t = shape_of(a->path, a->mm.M, a->mm.N);
+    const Shape t = shape_of(a->path, a->mm.M, a->mm.N, a->mm.k);
+    if (t.n == 32) return weights_tile<KSplit<Tile32<1, 1, 1, 1, 4, false, false, true>>>(*a, s);
     if (a->path == JV_SX_RAW) return weights_tile<Tile32<1, 1, 2, 2, 4, false, false>>(*a, s);
     if (a->path == JV_SX_PLANES) {
         if (t.m == 32) return weights_tile<Tile3<1, false, false>>(*a, s);
@@ -554,7 +559,7 @@ static int grads_path(int path, int d) { return path == JV_SX_LARGE && d <= 128 
 // joined costs a launch more)
 extern "C" int jvk_sx_grad_splits(int path, int nq, int d, int64_t rows) {
     path = grads_path(path, d);
-    const int tm = path == JV_SX_LARGE ? 256 : path == JV_SX_PLANES ? shape_of(path, nq, rows).m : 128, tn = path == JV_SX_LARGE ? 256 : 128;
+    const int tm = path == JV_SX_LARGE ? 256 : path == JV_SX_PLANES ? shape_of(path, nq, rows, 0).m : 128, tn = path == JV_SX_LARGE ? 256 : 128;
     const int64_t tiles = std::max<int64_t>((nq + tm - 1) / tm, 1) * ((d + tn - 1) / tn);
     const int64_t steps = path == JV_SX_RAW || path == JV_SX_PLANES ? (rows + 31) / 32 : (rows + 63) / 64;
     return (int)std::max<int64_t>(std::min<int64_t>((path == JV_SX_LARGE ? 256 : 512) / tiles, steps / (path == JV_SX_LARGE ? 4 : 8)), 1);
@@ -569,7 +574,7 @@ extern "C" hipError_t jvk_sx_grads(const JvMmOut* q, const JvMmOut* v, int path,
     }
     if (path == JV_SX_PLANES) {
         if (q) {
-            const int m = shape_of(path, q->mm.M, 0).m;
+            const int m = shape_of(path, q->mm.M, 0, 0).m;
             e = m == 32 ? mm_out_tile<Tile3<1, false, true>>(*q, s) : m == 64 ? mm_out_tile<Tile3<2, false, true>>(*q, s) : m == 96 ? mm_out_tile<Tile3<3, false, true>>(*q, s) : mm_out_tile<Tile3<4, false, true>>(*q, s);
         }
         if (v && e == hipSuccess) e = mm_out_tile<Tile3<4, true, true>>(*v, s);

@@ -47,15 +47,22 @@ __device__ __forceinline__ s16x4 read_across(const unsigned char* p) {   // 16 l
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
 }
 
-// This wave's copies of a step have landed and everybody's have, `left` steps (PER copies each, NS - 1 at most) being under way behind it.
-template <int NS, int PER>
+// This wave's copies of a step have landed and everybody's have (SOLO: a wave with LDS of its own), `left` steps (PER copies each, NS - 1 at most) being under way behind it.
+template <int NS, int PER, bool SOLO = false>
 __device__ __forceinline__ void wait_step(int left) {
     static_assert(NS >= 2 && NS <= 4);
     constexpr int most = 63;   // (what the counter holds)
-    if (left >= NS - 1) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((NS - 1) * PER < most ? (NS - 1) * PER : most) : "memory");
-    else if (NS > 3 && left == 2) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * PER < most ? 2 * PER : most) : "memory");
-    else if (NS > 2 && left == 1) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(PER < most ? PER : most) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    if (left >= NS - 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 1) * PER < most ? (NS - 1) * PER : most) : "memory");
+    else if (NS > 3 && left == 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PER < most ? 2 * PER : most) : "memory");
+    else if (NS > 2 && left == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PER < most ? PER : most) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if constexpr (!SOLO) asm volatile("s_barrier" ::: "memory");
+}
+// Every fragment read of a buffer has returned before any wave stages into it again.
+template <bool SOLO>
+__device__ __forceinline__ void release_step() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if constexpr (!SOLO) asm volatile("s_barrier" ::: "memory");
 }
 
 // The product for small shapes: MT x NT accumulators of 32 x 32 for each of WM x WN waves, NS steps of k in LDS: two and
@@ -64,7 +71,8 @@ __device__ __forceinline__ void wait_step(int left) {
 // lies at p ^ (swirl << 2) so that they are the four quarters of a 256-B bank row.
 template <int TY, int MT_, int NT_, int WM, int WN, int NS, bool TA = false, bool TB = false>
 struct Tile {
-    static constexpr int MT = MT_, NT = NT_, RESIDENT = 1;
+    using acc_t = f32x16;
+    static constexpr int MT = MT_, NT = NT_, RESIDENT = 1, E = 16, WIDE = 32 * NT;   // values of an accumulator; columns of a wave
     static constexpr int TM = 32 * MT * WM, TN = 32 * NT * WN, WAVES = WM * WN, THREADS = 64 * WAVES;
     static constexpr int GA = TM / 8, GB = TN / 8;                               // 8-row groups
     static constexpr int CA = GA / WAVES, CB = GB / WAVES, PER = CA + CB;        // copies of one wave a step
@@ -146,8 +154,8 @@ struct Tile {
 #pragma unroll
         for (int i = 0; i < NS - 1; i++)
             if (k0 + i < k1) stage(i);
+        int buf = 0;
         for (int s = k0; s < k1; s++) {
-            const int buf = (s - k0) % NS;
             int fa[MT], fb[NT];
             if constexpr (TY != BF16) {
 #pragma unroll
@@ -155,7 +163,7 @@ struct Tile {
 #pragma unroll
                 for (int t = 0; t < NT; t++) fb[t] = pb[t][s];
             }
-            if (s + NS - 1 < k1) stage((s - k0 + NS - 1) % NS);
+            if (s + NS - 1 < k1) stage(buf == 0 ? NS - 1 : buf - 1);
             wait_step<NS, PER>(k1 - 1 - s);
             const unsigned char* base = smem + buf * BUF;
             if constexpr (TY == BF16) {
@@ -220,8 +228,8 @@ struct Tile {
                             acc[m][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(vb[n], va[m], acc[m][n], 0, 0, 0, fb[n], 0, fa[m]);
                 }
             }
-            // every fragment read of this buffer has returned before any wave stages into it again
-            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            release_step<false>();
+            buf = buf + 1 == NS ? 0 : buf + 1;
         }
     }
     // acc[m][n][e] is C[row(m)][col(n, e)] of the tile, four consecutive e are four consecutive columns

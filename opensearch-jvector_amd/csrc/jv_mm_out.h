@@ -87,7 +87,7 @@ __device__ __forceinline__ void out_tile(const JvMmOut& a, int i, unsigned char*
     band_order(L, tm, tn, m0, n0);
     m0 *= T::TM, n0 *= T::TN;
     const int steps = T::steps(a.mm);
-    f32x16 acc[MT][NT];
+    typename T::acc_t acc[MT][NT];
     T::run(a.mm, m0, n0, (int)((int64_t)steps * part / a.splits), (int)((int64_t)steps * (part + 1) / a.splits), smem, acc);
     const float mul = a.norm ? a.mul * *a.norm : a.mul;
     const bool wide = (uintptr_t)a.out % 16 == 0 && a.ldo % (a.dtype == 0 ? 4 : 8) == 0;

@@ -100,7 +100,7 @@ enum JvSxPath {
     JV_SX_RAW       // float32, few tiles: everything as it lies (jv_tile32.h)
 };
 int jvk_sx_path(int nq, int64_t rows, int f32);
-int jvk_sx_loss_splits(int path, int nq, int64_t rows);   // workgroups that share a panel of queries
+int jvk_sx_loss_splits(int path, int nq, int64_t rows, int d);   // workgroups that share a panel of queries
 hipError_t jvk_sx_loss(const JvSxLoss* a, hipStream_t s);
 hipError_t jvk_sx_join(const float2* part, int splits, int nq, const float* hit, const int32_t* targets, int64_t n, float* loss, float* lse, hipStream_t s);
 hipError_t jvk_sx_weights(const JvSxWeights* a, hipStream_t s);

@@ -28,6 +28,8 @@ struct Work {
 
 template <int TY, bool TA = false, bool TB = false>
 struct Pipe {
+    using acc_t = f32x16;
+    static constexpr int E = 16, WIDE = 64;
     static constexpr int MT = 4, NT = 2, TM = 256, TN = 256, THREADS = 512;   // waves: 2 along M, 4 along N
     static constexpr int REGION = 32768, SCALES = 4 * REGION, SCRATCH = SCALES + (TY == BF16 ? 0 : 2 * 8192);
     static constexpr int LDS = SCRATCH + 4 * 4096;   // 4 KB for waves w and w + 4: they are never in their epilogue at the same time

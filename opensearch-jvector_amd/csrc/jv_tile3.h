@@ -15,7 +15,9 @@ namespace jvmm {
 
 template <int MT_, bool TA, bool TB>
 struct Tile3 {
+    using acc_t = f32x16;
     static constexpr int RESIDENT = 2;   // workgroups a CU
+    static constexpr int E = 16, WIDE = 32;
     static constexpr int MT = MT_, NT = 1, WAVES = 4, THREADS = 256, TM = 32 * MT, TN = 128;
     static constexpr int KA = 6 * MT, PA = (KA + 3) / 4, PB = 4, PER = PA + PB;   // KB of A in a step; copies of one wave (the last of A twice, if need be)
     static constexpr int BUF = (KA + 16) * 1024, LDS = 2 * BUF;
@@ -128,8 +130,7 @@ struct Tile3 {
             const unsigned char* base = smem + ((s - k0) & 1) * BUF;
             if (TB || (s + 1) * 32 <= a.k) multiply<false>(a, base, rb, 32, acc);
             else multiply<true>(a, base, rb, a.k - s * 32, acc);
-            // every fragment read of this buffer has returned before any wave stages into it again
-            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            release_step<false>();
         }
     }
     // acc[m][0][e] is C[row(m)][col(0, e)] of the tile, four consecutive e are four consecutive columns

@@ -17,9 +17,11 @@ namespace jvmm {
 __device__ __forceinline__ constexpr int part_of_a(int g) { return (0x052 >> (2 * g)) & 3; }
 __device__ __forceinline__ constexpr int part_of_b(int g) { return (0x118 >> (2 * g)) & 3; }
 
-template <int MT_, int NT_, int WM, int WN, int NS, bool TA, bool TB>
+// SOLO: one wave (WM = WN = 1) of a workgroup works by itself, in LDS of its own, on every `stride`-th step (KSplit).
+template <int MT_, int NT_, int WM, int WN, int NS, bool TA, bool TB, bool SOLO = false>
 struct Tile32 {
-    static constexpr int MT = MT_, NT = NT_, RESIDENT = 1;
+    using acc_t = f32x16;
+    static constexpr int MT = MT_, NT = NT_, RESIDENT = 1, E = 16, WIDE = 32 * NT;
     static constexpr int TM = 32 * MT * WM, TN = 32 * NT * WN, WAVES = WM * WN, THREADS = 64 * WAVES;
     static constexpr int GA = TM / 8, GB = TN / 8;                       // KB of a step
     static constexpr int PER = (GA + GB) / WAVES;                        // copies of one wave a step
@@ -59,7 +61,7 @@ struct Tile32 {
 
         // copy i of this wave is KB number i * WAVES + w: eight rows of 128 B (k along), or rows of GROUPS * 32 B (k across)
         __device__ __forceinline__ void init(const char* base, int64_t ld, int first, int rows, int cols) {
-            const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+            const int lane = threadIdx.x & 63, w = SOLO ? 0 : threadIdx.x >> 6;
 #pragma unroll
             for (int i = 0; i < COPIES; i++) {
                 const int c = i * WAVES + w;
@@ -73,7 +75,7 @@ struct Tile32 {
             }
         }
         __device__ __forceinline__ void copy(int64_t ld, int step, int k, unsigned char* dst) {
-            const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+            const int lane = threadIdx.x & 63, w = SOLO ? 0 : threadIdx.x >> 6;
 #pragma unroll
             for (int i = 0; i < COPIES; i++) {
                 const int c = i * WAVES + w;
@@ -133,8 +135,8 @@ struct Tile32 {
         }
     }
     // C tile at (m0, n0), steps [k0, k1) of ceil(k / 32)
-    static __device__ __forceinline__ void run(const JvMm& a, int m0, int n0, int k0, int k1, unsigned char* smem, f32x16 (&acc)[MT][NT]) {
-        const int w = threadIdx.x >> 6, r31 = threadIdx.x & 31, wm = w % WM, wn = w / WM;
+    static __device__ __forceinline__ void run(const JvMm& a, int m0, int n0, int k0, int k1, unsigned char* smem, f32x16 (&acc)[MT][NT], int stride = 1) {
+        const int w = SOLO ? 0 : threadIdx.x >> 6, r31 = threadIdx.x & 31, wm = w % WM, wn = w / WM;
         Side<TA, GA> sa;
         Side<TB, GB> sb;
         sa.init(a.a, a.lda, m0, a.M, a.ca);
@@ -150,22 +152,23 @@ struct Tile32 {
         for (int t = 0; t < MT; t++) ra[t] = (wm * MT + t) * 32 + r31, ra[t] = TA ? sa.place(ra[t], m0, a.ca) : ra[t];
 #pragma unroll
         for (int t = 0; t < NT; t++) rb[t] = (wn * NT + t) * 32 + r31, rb[t] = TB ? sb.place(rb[t], n0, a.cb) : rb[t];
-        auto stage = [&](int s) {
-            unsigned char* dst = smem + (s - k0) % NS * BUF;
+        auto stage = [&](int s, int to) {
+            unsigned char* dst = smem + to * BUF;
             sa.copy(a.lda, s, TA ? a.ka : a.k, dst);
             sb.copy(a.ldb, s, TB ? a.kb : a.k, dst + GA * GROUP);
         };
 #pragma unroll
         for (int i = 0; i < NS - 1; i++)
-            if (k0 + i < k1) stage(k0 + i);
-        for (int s = k0; s < k1; s++) {
-            if (s + NS - 1 < k1) stage(s + NS - 1);
-            wait_step<NS, PER>(k1 - 1 - s);
-            const unsigned char* base = smem + (s - k0) % NS * BUF;
+            if (k0 + i * stride < k1) stage(k0 + i * stride, i);
+        int buf = 0;
+        for (int s = k0; s < k1; s += stride) {
+            if (s + (NS - 1) * stride < k1) stage(s + (NS - 1) * stride, buf == 0 ? NS - 1 : buf - 1);
+            wait_step<NS, PER, SOLO>(SOLO ? (k1 - 1 - s) / stride : k1 - 1 - s);
+            const unsigned char* base = smem + buf * BUF;
             if ((s + 1) * 32 <= a.k) multiply<false>(a, base, ra, rb, 32, acc);
             else multiply<true>(a, base, ra, rb, a.k - s * 32, acc);   // (apart: the masks would cost every step a third more)
-            // every fragment read of this buffer has returned before any wave stages into it again
-            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            release_step<SOLO>();
+            buf = buf + 1 == NS ? 0 : buf + 1;
         }
     }
     // acc[m][n][e] is C[row(m)][col(n, e)] of the tile, four consecutive e are four consecutive columns
@@ -173,6 +176,29 @@ struct Tile32 {
     static __device__ __forceinline__ int col(int n, int e) {
         return (((threadIdx.x >> 6) / WM) * NT + n) * 32 + (e & 3) + 8 * (e >> 2) + 4 * ((threadIdx.x >> 5) & 1);
     }
+};
+
+// A 32 x 32 tile whose k steps four waves share, each with its own LDS and no barrier between steps; wave w ends up with 8 of the 32 columns.
+// For few tiles with a long k, where the way through one tile's steps is what counts.
+template <class Solo>
+struct KSplit {
+    using acc_t = f32x4;
+    static constexpr int MT = 1, NT = 1, RESIDENT = 1, E = 4, WIDE = 8, TM = 32, TN = 32, THREADS = 256, LDS = 4 * Solo::LDS;
+    static __host__ __device__ __forceinline__ int steps(const JvMm& a) { return Solo::steps(a); }
+    static __device__ __forceinline__ void run(const JvMm& a, int m0, int n0, int k0, int k1, unsigned char* smem, f32x4 (&acc)[1][1]) {
+        const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+        f32x16 mine[1][1];
+        Solo::run(a, m0, n0, k0 + w, k1, smem + w * Solo::LDS, mine, 4);
+        __syncthreads();
+        f32x4* sh = (f32x4*)smem;   // [wave][four values][lane]
+#pragma unroll
+        for (int g = 0; g < 4; g++) sh[(w * 4 + g) * 64 + lane] = (f32x4){mine[0][0][4 * g], mine[0][0][4 * g + 1], mine[0][0][4 * g + 2], mine[0][0][4 * g + 3]};
+        __syncthreads();
+        acc[0][0] = (sh[w * 64 + lane] + sh[(4 + w) * 64 + lane]) + (sh[(8 + w) * 64 + lane] + sh[(12 + w) * 64 + lane]);
+        __syncthreads();
+    }
+    static __device__ __forceinline__ int row(int) { return threadIdx.x & 31; }
+    static __device__ __forceinline__ int col(int, int e) { return (threadIdx.x >> 6) * 8 + 4 * ((threadIdx.x >> 5) & 1) + e; }
 };
 
 }  // namespace jvmm

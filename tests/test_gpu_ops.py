@@ -137,7 +137,8 @@ def test_scores_do_not_touch_what_lies_between_rows(torch, ops, pkg):
 LOSS = [(1, 1, 1, 0, 0, 1.0), (1, 5, 3, 0, 0, 2.0), (3, 129, 64, 0, 0, 20.0), (2, 300, 17, 5, 1, 5.0), (129, 127, 65, 1, 3, 20.0), (64, 640, 128, 8, 0, 30.0),
         (130, 3000, 100, 0, 0, 10.0), (257, 1025, 384, 64, 8, 20.0), (31, 2000, 768, 0, 0, 20.0), (512, 260, 200, 0, 0, -3.0), (7, 1000, 1536, 0, 0, 50.0),
         (40, 130, 2, 1, 1, 3.0), (5, 70, 4, 0, 1, 3.0), (35, 77, 31, 0, 2, 9.0), (90, 261, 33, 6, 5, 9.0), (70, 300, 62, 3, 7, 9.0), (118, 18, 843, 24, 0, 10.0),
-        (66, 520, 134, 2, 2, 12.0), (30, 1000, 72, 2, 2, 12.0), (100, 900, 8, 0, 0, 3.0), (61, 40, 200, 8, 6, 12.0)]
+        (66, 520, 134, 2, 2, 12.0), (30, 1000, 72, 2, 2, 12.0), (100, 900, 8, 0, 0, 3.0), (61, 40, 200, 8, 6, 12.0), (28, 46, 1167, 0, 0, 12.0),
+        (2, 3258, 1084, 0, 0, 12.0), (1, 1, 700, 3, 1, 1.0), (100, 2100, 519, 1, 1, -6.0), (33, 65, 2100, 8, 0, 20.0)]
 
 
 def loss_case(torch, nq, n, d, dtype, pad=0, shift=0, seed=0):
