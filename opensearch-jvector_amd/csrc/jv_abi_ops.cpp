@@ -77,7 +77,7 @@ int check_shape(int64_t n, int d, const char* what) {
 
 // ---- the softmax loss: what a call needs, from its shape alone ----
 struct Plan {
-    int P, dp, kq;                    // planes; d and nq padded to 64
+    int P, dp, kq, gq;                // planes; d and nq padded to 64; rows of g (the large tiles write whole steps, the small ones one row behind the queries)
     int64_t rows_f, rows_b;           // rows of one piece, forward (where the vectors have to be laid out) / backward
     int path_f, path_b, splits_f, splits_q;   // forward, backward
     int64_t off_q, off_q4, off_v, off_part, off_hit, off_query, off_norm, off_rest, off_g, off_slab, bytes;
@@ -101,10 +101,11 @@ Plan make_plan(int dtype, int nq, int64_t n, int d, uint32_t what) {
     p.P = dtype == JV_DTYPE_F32 ? 3 : 1;
     p.dp = (int)up(d, 64);
     p.kq = (int)up(std::max(nq, 1), 64);
+    p.gq = nq > 128 ? p.kq : nq + 1;
     const int64_t panels = std::max((nq + 255) / 256, 1), row = (int64_t)p.P * p.dp * 2;
     const int64_t fill = 256 * ((1024 + panels - 1) / panels);   // rows whose tiles fill the chip four times
     p.rows_f = piece(n, std::max<int64_t>((128ll << 20) / row, fill));
-    p.rows_b = piece(n, std::max<int64_t>((kWeights << 20) / ((int64_t)p.P * 2 * p.kq), fill));
+    p.rows_b = piece(n, std::max<int64_t>((kWeights << 20) / ((int64_t)p.P * 2 * p.gq), fill));
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
         const int64_t o = at;
@@ -126,7 +127,7 @@ Plan make_plan(int dtype, int nq, int64_t n, int d, uint32_t what) {
         p.off_query = take((int64_t)nq * sizeof(JvSxQuery));
         p.off_norm = take(4);
         p.off_rest = take((int64_t)nq * 4);
-        p.off_g = take((int64_t)p.kq * p.P * p.rows_b * 2);
+        p.off_g = take((int64_t)p.gq * p.P * p.rows_b * 2);
         if (what & JV_SOFTMAX_QUERY_GRAD) {
             p.splits_q = jvk_sx_grad_splits(p.path_b, nq, d, std::min<int64_t>(p.rows_b, n));
             p.off_slab = take((int64_t)p.splits_q * nq * p.dp * 4);
@@ -359,7 +360,7 @@ int jv_softmax_grad_device(const jv_softmax_params* p, const float* d_lse, const
             q = o;
         }
         if (d_out_vector_grad) {   // G across times the queries: k = the queries
-            o.mm.M = rows, o.mm.k = (int)up(p->nq, 32), o.mm.kph = plan.kq / 32, o.mm.ka = f32 ? o.mm.k : plan.kq, o.mm.ca = w.kv;
+            o.mm.M = rows, o.mm.k = (int)up(p->nq, 32), o.mm.kph = plan.kq / 32, o.mm.ka = p->nq % (f32 ? 32 : 64) ? p->nq + 1 : p->nq, o.mm.ca = w.kv;
             o.mm.b = q_rows, o.mm.ldb = q_ld, o.mm.kb = p->nq, o.mm.cb = rb.ready || rb.kp == 4 ? p->d : plan.dp;
             o.mul = p->scale, o.norm = norm, o.dtype = p->dtype, o.splits = 1, o.add = 0;
             o.out = (char*)d_out_vector_grad + at * vector_grad_stride * size_of(p->dtype), o.ldo = vector_grad_stride;

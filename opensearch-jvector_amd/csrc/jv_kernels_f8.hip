@@ -140,12 +140,12 @@ extern "C" hipError_t jvk_f8_decode(const uint8_t* codes, const uint8_t* scales,
 }
 
 // bf16 scores keep 8 bits: the 8-bit unit's sums are enough.  float32 scores take the bf16 unit (jv_mm.h).  Tiles: 256 x 256 where they fill the
-// chip and more than half of one is queries; 32 x 128 and 64 x 128 for up to 32 and 64 queries (the rows are streamed); 128 x 128 otherwise, but 64 x 64 where that is no more than
+// chip, more than half of one is queries and the output's rows are 16-B aligned; 32 x 128 and 64 x 128 for up to 32 and 64 queries (the rows are streamed); 128 x 128 otherwise, but 64 x 64 where that is no more than
 // one tile a CU.
 template <int TY>
 static hipError_t score(const JvMmOut& a, hipStream_t s) {
     const int64_t M = a.mm.M, N = a.mm.N, tiles = (M + 127) / 128 * ((N + 127) / 128);
-    if (M > 128 && (M + 255) / 256 * ((N + 255) / 256) >= 192 && N >= 16) return mm_out_pipe<TY>(a, s);
+    if (M > 128 && (M + 255) / 256 * ((N + 255) / 256) >= 192 && N >= 16 && aligned_rows(a)) return mm_out_pipe<TY>(a, s);
     if (M <= 32) return tiles <= 256 ? mm_out_tile<Tile<TY, 1, 1, 1, 4, 4>>(a, s) : mm_out_tile<Tile<TY, 1, 1, 1, 4, 2>>(a, s);
     if (tiles <= 256) return mm_out_tile<Tile<TY, 1, 1, 2, 2, 4>>(a, s);
     return M <= 64 ? mm_out_tile<Tile<TY, 2, 1, 1, 4, 2>>(a, s) : mm_out_tile<Tile<TY, 2, 2, 2, 2, 2>>(a, s);

@@ -441,14 +441,15 @@ __global__ __launch_bounds__(512) void jvs_weights_kernel(const JvSxWeights a) {
                 if (r < a.mm.M) q = a.query[r];
                 weigh<P>(acc[m], q, a.c, a.mm.N - w.n0, q.target >= 0 ? (int)(q.target - a.row0) - w.n0 : -1, true, a.rest + r);
             }
-            return P::write_bf16(smem, (uint16_t*)a.g, a.kv, true, w, padded, a.kv, [&](int m, int n, int e) { return acc[m][n][e]; });
+            return P::write_bf16(smem, (uint16_t*)a.g, a.kv, w, padded, a.kv, [&](int m, int n, int e) { return acc[m][n][e]; });
         });
 }
 
-// rows of G: whole steps of the product that has the queries for k
+// Rows of G: the queries and, where they are no whole steps of the product that has them for k, a row of zeros, which that product reads as
+// all the rows behind it.
 static __host__ __device__ __forceinline__ int padded_queries(const JvSxWeights& a) {
     const int step = a.path == JV_SX_RAW || a.path == JV_SX_PLANES ? 32 : 64;
-    return (a.mm.M + step - 1) / step * step;
+    return a.mm.M % step ? a.mm.M + 1 : a.mm.M;
 }
 
 // the same on small tiles, one a workgroup
@@ -469,32 +470,30 @@ __global__ __launch_bounds__(T::THREADS, T::RESIDENT) void jvs_weights_tile_kern
         if (r < a.mm.M) q = a.query ? a.query[r] : query_of(a.lse, a.w, a.targets, a.n, r);
         weigh<T>(acc[m], q, a.c, a.mm.N - n0, q.target >= 0 ? (int)(q.target - a.row0) - n0 : -1, a.path == JV_SX_TILES, a.rest + r);
         // (kv is a multiple of 64: four columns are in or out together)
-        if (a.path == JV_SX_RAW) {
-#pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-                for (int g = 0; g < T::E / 4; g++) {
-                    const int col = n0 + T::col(n, 4 * g);
-                    if (r < padded && col < a.kv)
-                        *(f32x4*)((float*)a.g + (int64_t)r * a.kv + col) = (f32x4){acc[m][n][4 * g], acc[m][n][4 * g + 1], acc[m][n][4 * g + 2], acc[m][n][4 * g + 3]};
-                }
-        } else {
+        auto put = [&](int r, int c, f32x4 v) {
+            if (r >= padded || c >= a.kv) return;
+            if (a.path == JV_SX_RAW) {
+                *(f32x4*)((float*)a.g + (int64_t)r * a.kv + c) = v;
+                return;
+            }
             const int planes = a.path == JV_SX_PLANES ? 3 : 1;
-            for (int k = 0; k < planes; k++) {
-                uint16_t* row = (uint16_t*)a.g + ((int64_t)r * planes + k) * a.kv;
+            uint16_t* p = (uint16_t*)a.g + (int64_t)r * planes * a.kv + c;
+            for (int k = 0; k < planes; k++, p += a.kv) {
+                const bf16x4 b = {(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+                *(bf16x4*)p = b;
 #pragma unroll
-                for (int n = 0; n < NT; n++)
+                for (int e = 0; e < 4; e++) v[e] -= (float)b[e];
+            }
+        };
+        if constexpr (T::E == 4) {
+            put(r, n0 + T::col(0, 0), acc[m][0]);
+        } else {
+            const Turn<T> turn(smem, m, acc[m]);
 #pragma unroll
-                    for (int g = 0; g < T::E / 4; g++) {
-                        const int col = n0 + T::col(n, 4 * g);
-                        bf16x4 v;
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            v[e] = (__bf16)acc[m][n][4 * g + e];
-                            acc[m][n][4 * g + e] -= (float)v[e];
-                        }
-                        if (r < padded && col < a.kv) *(bf16x4*)(row + col) = v;
-                    }
+            for (int i = 0; i < Turn<T>::WIDE_STORES; i++) {
+                int tr, tc;
+                const f32x4 v = turn.four(i, tr, tc);
+                put(m0 + tr, n0 + tc, v);
             }
         }
     }
@@ -569,7 +568,7 @@ extern "C" hipError_t jvk_sx_grads(const JvMmOut* q, const JvMmOut* v, int path,
     hipError_t e = hipSuccess;
     if (path == JV_SX_LARGE) {
         if (q) e = mm_out_pipe<BF16, false, true>(*q, s);
-        if (v && e == hipSuccess) e = mm_out_pipe<BF16, true, true>(*v, s);
+        if (v && e == hipSuccess) e = aligned_rows(*v) ? mm_out_pipe<BF16, true, true>(*v, s) : mm_out_tile<Tile<BF16, 2, 2, 2, 2, 2, true, true>>(*v, s);
         return e;
     }
     if (path == JV_SX_PLANES) {
@@ -592,27 +591,38 @@ extern "C" hipError_t jvk_sx_grads(const JvMmOut* q, const JvMmOut* v, int path,
     return grads_tile<Tile<BF16, 2, 2, 2, 2, 2, false, true>, Tile<BF16, 2, 2, 2, 2, 2, true, true>>(q, v, s);
 }
 
-// partial sums -> the queries' gradient, and what G lacked at the target: one wave a row, four columns a lane
-template <typename T>
+// partial sums -> the queries' gradient, and what G lacked at the target.  A row's columns, four a lane, are shared by 256 / G lanes, its partial
+// sums by G lanes, which are joined in a fixed order: with few columns and hundreds of partial sums the way through one lane's sums is
+// what counts (64 x 32 of 512 partial sums: 31 us with G = 1, 4 with 16).
+template <typename T, int G>
 __global__ __launch_bounds__(256) void jvs_finish_kernel(const float* __restrict__ slab, int splits, int64_t rows, int d, int64_t lds, const float* __restrict__ rest,
                                                          const JvSxQuery* __restrict__ query, const T* __restrict__ v, int64_t v_stride, float mul,
                                                          const float* __restrict__ norm, T* __restrict__ out, int64_t ldo) {
-    const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (r >= rows) return;
+    constexpr int L = 256 / G;
+    __shared__ f32x4 part[G > 1 ? 256 : 1];
+    const int64_t r = blockIdx.x;
+    const int g = threadIdx.x / L, c = ((int)threadIdx.x % L + (int)blockIdx.y * L) * 4;   // (lds is a multiple of 64)
+    f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (c < d) {
+        const float* p = slab + r * lds + c;
+#pragma unroll 8
+        for (int k = g; k < splits; k += G) x += *(const f32x4*)(p + k * rows * lds);
+    }
+    if constexpr (G > 1) {
+        part[threadIdx.x] = x;
+        __syncthreads();
+        if (g > 0) return;
+#pragma unroll
+        for (int k = 1; k < G; k++) x += part[k * L + threadIdx.x];
+    }
     const float by = norm ? mul * *norm : mul, lack = rest ? rest[r] : 0.0f;
     const int64_t target = lack != 0.0f ? query[r].target : 0;
-    for (int c = (threadIdx.x & 63) * 4 + blockIdx.y * 256; c < d; c += gridDim.y * 256) {   // (lds is a multiple of 64)
-        const float* p = slab + r * lds + c;
-        f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 8
-        for (int k = 0; k < splits; k++) x += *(const f32x4*)(p + k * rows * lds);
 #pragma unroll
-        for (int e = 0; e < 4; e++)
-            if (c + e < d) {
-                const float y = lack != 0.0f ? fmaf(lack, (float)v[target * v_stride + c + e], x[e]) : x[e];
-                out[r * ldo + c + e] = (T)(y * by);
-            }
-    }
+    for (int e = 0; e < 4; e++)
+        if (c + e < d) {
+            const float y = lack != 0.0f ? fmaf(lack, (float)v[target * v_stride + c + e], x[e]) : x[e];
+            out[r * ldo + c + e] = (T)(y * by);
+        }
 }
 template <typename T>
 __global__ __launch_bounds__(256) void jvs_fill_kernel(T* __restrict__ out, int64_t stride, int64_t rows, int d, float value) {
@@ -628,11 +638,14 @@ static unsigned grid_for(int64_t items) {
 extern "C" hipError_t jvk_sx_finish(const float* slab, int splits, int64_t rows, int d, int64_t lds, const float* rest, const JvSxQuery* query, const void* v,
                                     int64_t v_stride, float mul, const float* norm, void* out, int dtype, int64_t ldo, hipStream_t s) {
     if (rows <= 0 || d <= 0) return hipSuccess;
-    const dim3 grid((unsigned)((rows + 3) / 4), (unsigned)std::min((d + 255) / 256, 16));
-    if (dtype == 0)
-        jvs_finish_kernel<float><<<grid, 256, 0, s>>>(slab, splits, rows, d, lds, rest, query, (const float*)v, v_stride, mul, norm, (float*)out, ldo);
-    else
-        jvs_finish_kernel<__bf16><<<grid, 256, 0, s>>>(slab, splits, rows, d, lds, rest, query, (const __bf16*)v, v_stride, mul, norm, (__bf16*)out, ldo);
+    const int groups = splits >= 32 ? 16 : splits >= 4 ? 4 : 1, lanes = 256 / groups;
+    const dim3 grid((unsigned)rows, (unsigned)((d + 4 * lanes - 1) / (4 * lanes)));
+    auto run = [&](auto kernel, auto type) {
+        using T = decltype(type);
+        kernel<<<grid, 256, 0, s>>>(slab, splits, rows, d, lds, rest, query, (const T*)v, v_stride, mul, norm, (T*)out, ldo);
+    };
+    if (dtype == 0) run(groups == 16 ? jvs_finish_kernel<float, 16> : groups == 4 ? jvs_finish_kernel<float, 4> : jvs_finish_kernel<float, 1>, 0.0f);
+    else run(groups == 16 ? jvs_finish_kernel<__bf16, 16> : groups == 4 ? jvs_finish_kernel<__bf16, 4> : jvs_finish_kernel<__bf16, 1>, (__bf16)0.0f);
     return hipGetLastError();
 }
 extern "C" hipError_t jvk_sx_fill(void* out, int dtype, int64_t stride, int64_t rows, int d, float value, hipStream_t s) {

@@ -9,6 +9,9 @@
 
 namespace jvmm {
 
+// the output's rows are 16-B aligned
+__host__ __device__ __forceinline__ bool aligned_rows(const JvMmOut& a) { return (uintptr_t)a.out % 16 == 0 && a.ldo % (a.dtype == 0 ? 4 : 8) == 0; }
+
 // Tile L of tm x tn in bands of 8 tiles of A: the 32 workgroups that an XCD runs at a time share 8 tiles of A and 4 of B.
 __device__ __forceinline__ void band_order(int L, int tm, int tn, int& m, int& n) {
     const int band = L / (8 * tn), in = L - band * 8 * tn, high = min(8, tm - band * 8);
@@ -51,11 +54,10 @@ __global__ __launch_bounds__(512) void jvm_out_pipe_kernel(const JvMmOut a) {
         return true;
     };
     const float mul = a.norm ? a.mul * *a.norm : a.mul;
-    const bool wide = (uintptr_t)a.out % 16 == 0 && a.ldo % (a.dtype == 0 ? 4 : 8) == 0;
     P::run(a.mm, smem, work, [&](const Work& w, f32x16 (&acc)[4][2]) -> int {
         auto value = [&](int m, int n, int e) { return acc[m][n][e] * mul; };
-        if (a.dtype != 0) return P::write_bf16(smem, (uint16_t*)a.out, a.ldo, wide, w, a.mm.M, a.mm.N, value);
-        return P::write_f32(smem, (float*)a.out + (int64_t)w.part * a.mm.M * a.ldo, a.ldo, wide, a.add, w, a.mm.M, a.mm.N, value);
+        if (a.dtype != 0) return P::write_bf16(smem, (uint16_t*)a.out, a.ldo, w, a.mm.M, a.mm.N, value);
+        return P::write_f32(smem, (float*)a.out + (int64_t)w.part * a.mm.M * a.ldo, a.ldo, a.add, w, a.mm.M, a.mm.N, value);
     });
 }
 
@@ -64,7 +66,7 @@ static hipError_t mm_out_pipe(const JvMmOut& a, hipStream_t s) {
     using P = Pipe<TY, TA, TB>;
     if (a.mm.M <= 0 || a.mm.N <= 0) return hipSuccess;
     const int64_t all = (int64_t)((a.mm.M + P::TM - 1) / P::TM) * ((a.mm.N + P::TN - 1) / P::TN) * a.splits;
-    if (all > 0x7fffffffll || a.splits < 1 || a.splits > a.mm.kph) return hipErrorInvalidValue;
+    if (all > 0x7fffffffll || a.splits < 1 || a.splits > a.mm.kph || !aligned_rows(a)) return hipErrorInvalidValue;
     hipError_t e = lds_of(jvm_out_pipe_kernel<TY, TA, TB>, P::LDS);
     if (e != hipSuccess) return e;
     jvm_out_pipe_kernel<TY, TA, TB><<<(unsigned)(all < 256 ? (all + 7) / 8 * 8 : 256), P::THREADS, P::LDS, s>>>(a);
@@ -77,6 +79,43 @@ __device__ __forceinline__ int xcd_order(int i, int n) {
     return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + slot;
 }
 
+// A wave's accumulators of 32 rows, turned by way of its own part of LDS (free after T::run), so that a store writes a row's 32 * NT columns one
+// behind another: as the lanes hold them, each store would touch 32 rows (dv of 20 x 265 213 x 335, rows not aligned: 285 -> 151 us).
+// Piece p (16 B) of row r lies at p ^ (r & 7).
+template <class T>
+struct Turn {
+    static constexpr int COLS = 32 * T::NT, WIDE_STORES = COLS / 8, NARROW_STORES = COLS / 2;
+    static_assert(T::THREADS / 64 * COLS * 128 <= T::LDS);
+    const unsigned char* at;
+    int r0, c0;   // the tile's row and column of the first element
+    __device__ __forceinline__ Turn(unsigned char* smem, int m, const f32x16 (&acc)[T::NT]) {
+        const int r31 = threadIdx.x & 31, h = (threadIdx.x >> 5) & 1;
+        unsigned char* to = smem + (threadIdx.x >> 6) * (COLS * 128);
+        at = to, r0 = T::row(m) - r31, c0 = T::col(0, 0) - 4 * h;
+        asm volatile("" ::: "memory");   // (a wave's LDS accesses are carried out in order: the last rows have been read)
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int n = 0; n < T::NT; n++)
+#pragma unroll
+            for (int g = 0; g < 4; g++)
+                *(f32x4*)(to + (r31 * (COLS / 4) + ((8 * n + 2 * g + h) ^ (r31 & 7))) * 16) = (f32x4){acc[n][4 * g], acc[n][4 * g + 1], acc[n][4 * g + 2], acc[n][4 * g + 3]};
+        __builtin_amdgcn_wave_barrier();
+        asm volatile("" ::: "memory");
+    }
+    // four columns of the i-th of WIDE_STORES; `r`, `c`: their place in the tile
+    __device__ __forceinline__ f32x4 four(int i, int& r, int& c) const {
+        const int k = i * 64 + (threadIdx.x & 63), row = k / (COLS / 4), piece = k % (COLS / 4);
+        r = r0 + row, c = c0 + piece * 4;
+        return *(const f32x4*)(at + (row * (COLS / 4) + (piece ^ (row & 7))) * 16);
+    }
+    // one column of the i-th of NARROW_STORES
+    __device__ __forceinline__ float one(int i, int& r, int& c) const {
+        const int k = i * 64 + (threadIdx.x & 63), row = k / COLS, col = k % COLS;
+        r = r0 + row, c = c0 + col;
+        return *(const float*)(at + (row * (COLS / 4) + ((col >> 2) ^ (row & 7))) * 16 + (col & 3) * 4);
+    }
+};
+
 // workgroup `i` of tiles * splits: one tile over one k range
 template <class T>
 __device__ __forceinline__ void out_tile(const JvMmOut& a, int i, unsigned char* smem) {
@@ -87,44 +126,51 @@ __device__ __forceinline__ void out_tile(const JvMmOut& a, int i, unsigned char*
     band_order(L, tm, tn, m0, n0);
     m0 *= T::TM, n0 *= T::TN;
     const int steps = T::steps(a.mm);
-    typename T::acc_t acc[MT][NT];
+    f32x16 acc[MT][NT];
     T::run(a.mm, m0, n0, (int)((int64_t)steps * part / a.splits), (int)((int64_t)steps * (part + 1) / a.splits), smem, acc);
     const float mul = a.norm ? a.mul * *a.norm : a.mul;
-    const bool wide = (uintptr_t)a.out % 16 == 0 && a.ldo % (a.dtype == 0 ? 4 : 8) == 0;
+    const bool wide = aligned_rows(a);
     const int64_t slab = (int64_t)part * a.mm.M * a.ldo;
 #pragma unroll
     for (int m = 0; m < MT; m++) {
-        const int row = m0 + T::row(m);
-        if (row >= a.mm.M) continue;
+        const Turn<T> turn(smem, m, acc[m]);
+        int r, c;
+        if (wide) {   // (four columns: all of them, or the row ends inside)
 #pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int g = 0; g < 4; g++) {
-                const int col = n0 + T::col(n, 4 * g);
-                f32x4 v;
-#pragma unroll
-                for (int e = 0; e < 4; e++) v[e] = acc[m][n][4 * g + e] * mul;
+            for (int i = 0; i < Turn<T>::WIDE_STORES; i++) {
+                f32x4 v = turn.four(i, r, c) * mul;
+                r += m0, c += n0;
+                if (r >= a.mm.M || c >= a.mm.N) continue;
                 if (a.dtype == 0) {
-                    float* p = (float*)a.out + slab + (int64_t)row * a.ldo + col;
-                    if (wide && col + 4 <= a.mm.N) {
+                    float* p = (float*)a.out + slab + (int64_t)r * a.ldo + c;
+                    if (c + 4 <= a.mm.N) {
                         if (a.add) v += *(const f32x4*)p;
                         *(f32x4*)p = v;
                     } else {
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            if (col + e < a.mm.N) p[e] = a.add ? p[e] + v[e] : v[e];
+                        for (int e = 0; c + e < a.mm.N; e++) p[e] = a.add ? p[e] + v[e] : v[e];
                     }
                 } else {
-                    __bf16* p = (__bf16*)a.out + (int64_t)row * a.ldo + col;
-                    if (wide && col + 4 <= a.mm.N) {
-                        *(bf16x4*)p = (bf16x4){(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            if (col + e < a.mm.N) p[e] = (__bf16)v[e];
-                    }
+                    __bf16* p = (__bf16*)a.out + (int64_t)r * a.ldo + c;
+                    const bf16x4 b = {(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+                    if (c + 4 <= a.mm.N) *(bf16x4*)p = b;
+                    else
+                        for (int e = 0; c + e < a.mm.N; e++) p[e] = b[e];
                 }
             }
+        } else {
+#pragma unroll 8
+            for (int i = 0; i < Turn<T>::NARROW_STORES; i++) {
+                const float v = turn.one(i, r, c) * mul;
+                r += m0, c += n0;
+                if (r >= a.mm.M || c >= a.mm.N) continue;
+                if (a.dtype == 0) {
+                    float* p = (float*)a.out + slab + (int64_t)r * a.ldo + c;
+                    *p = a.add ? *p + v : v;
+                } else {
+                    ((__bf16*)a.out)[(int64_t)r * a.ldo + c] = (__bf16)v;
+                }
+            }
+        }
     }
 }
 

@@ -253,27 +253,22 @@ struct Pipe {
         __syncthreads();
     }
 
-    // Writes a tile whose elements are value(m, n, e) as rows of float32 or bf16, `ldo` elements apart, rows < M and columns < N.  Rows that are
-    // 16-B aligned (`wide`) go through LDS, so that a store writes whole 128-B lines: 32 rows of 128 B at a time, piece p of row r at
-    // p ^ ((r >> 1) & 7).  Returns the stores that every wave has issued.
+    // threadIdx.x, computed anew: an epilogue's addresses would otherwise be kept through the whole product, whose registers are all taken
+    // (scores of 256 x 500 000 x 128: 155 and 133 us).
+    static __device__ __forceinline__ int own_thread() {
+        int t = threadIdx.x;
+        asm volatile("" : "+v"(t));
+        return t;
+    }
+
+    // Writes a tile whose elements are value(m, n, e) as rows of float32 or bf16, `ldo` elements apart, rows < M and columns < N; the rows
+    // are 16-B aligned.  They go through LDS, so that a store writes whole 128-B lines: 32 rows of 128 B at a time, piece p of row r at
+    // p ^ ((r >> 1) & 7).  (Other rows go to the small tiles: element by element from here, scores of 256 x 500 001 x 768 took 496 us, there 343.)  Returns the stores that every wave has issued.
     template <class V>
-    static __device__ __forceinline__ int write_bf16(unsigned char* smem, uint16_t* out, int64_t ldo, bool wide, const Work& at, int M, int N, V&& value) {
-        const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, h = lane >> 5, r31 = lane & 31;
+    static __device__ __forceinline__ int write_bf16(unsigned char* smem, uint16_t* out, int64_t ldo, const Work& at, int M, int N, V&& value) {
+        const int tid = own_thread(), lane = tid & 63, w = tid >> 6, h = lane >> 5, r31 = lane & 31;
         const int m0 = at.m0 + (w & 1) * 128, n0 = at.n0 + (w >> 1) * 64;
         unsigned char* sc = smem + SCRATCH + (w & 3) * 4096;
-        if (!wide) {
-#pragma unroll
-            for (int m = 0; m < MT; m++)
-#pragma unroll
-                for (int n = 0; n < NT; n++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        const __bf16 b = (__bf16)value(m, n, e);
-                        const int r = at.m0 + row(m), c = at.n0 + col(n, e);
-                        if (r < M && c < N) out[(int64_t)r * ldo + c] = __builtin_bit_cast(uint16_t, b);
-                    }
-            return 0;
-        }
         const bool full = at.m0 + TM <= M && at.n0 + TN <= N;
 #pragma unroll
         for (int m = 0; m < MT; m++) {
@@ -308,25 +303,10 @@ struct Pipe {
         return full ? 16 : 0;
     }
     template <class V>
-    static __device__ __forceinline__ int write_f32(unsigned char* smem, float* out, int64_t ldo, bool wide, bool add, const Work& at, int M, int N, V&& value) {
-        const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, h = lane >> 5, r31 = lane & 31;
+    static __device__ __forceinline__ int write_f32(unsigned char* smem, float* out, int64_t ldo, bool add, const Work& at, int M, int N, V&& value) {
+        const int tid = own_thread(), lane = tid & 63, w = tid >> 6, h = lane >> 5, r31 = lane & 31;
         const int m0 = at.m0 + (w & 1) * 128, n0 = at.n0 + (w >> 1) * 64;
         unsigned char* sc = smem + SCRATCH + (w & 3) * 4096;
-        if (!wide) {
-#pragma unroll
-            for (int m = 0; m < MT; m++)
-#pragma unroll
-                for (int n = 0; n < NT; n++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        const int r = at.m0 + row(m), c = at.n0 + col(n, e);
-                        if (r < M && c < N) {
-                            float* p = out + (int64_t)r * ldo + c;
-                            *p = add ? *p + value(m, n, e) : value(m, n, e);
-                        }
-                    }
-            return 0;
-        }
         const bool full = at.m0 + TM <= M && at.n0 + TN <= N;
 #pragma unroll
         for (int m = 0; m < MT; m++)
