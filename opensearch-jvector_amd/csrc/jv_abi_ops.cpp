@@ -79,8 +79,8 @@ int check_shape(int64_t n, int d, const char* what) {
 struct Plan {
     int P, dp, kq, gq;                // planes; d and nq padded to 64; rows of g (the large tiles write whole steps, the small ones one row behind the queries)
     int64_t rows_f, rows_b;           // rows of one piece, forward (where the vectors have to be laid out) / backward
-    int path_f, path_b, splits_f, splits_q;   // forward, backward
-    int64_t off_q, off_q4, off_v, off_part, off_hit, off_query, off_norm, off_rest, off_g, off_slab, bytes;
+    int path_f, path_b, splits_f, splits_q, splits_v;   // forward, backward
+    int64_t off_q, off_q4, off_v, off_part, off_hit, off_query, off_norm, off_rest, off_g, off_slab, off_slab_v, bytes;
 };
 
 // MB of one piece's weights g: few large pieces, for every piece writes and reads dq's partial sums again and starts its tiles anew (step
@@ -129,8 +129,13 @@ Plan make_plan(int dtype, int nq, int64_t n, int d, uint32_t what) {
         p.off_rest = take((int64_t)nq * 4);
         p.off_g = take((int64_t)p.gq * p.P * p.rows_b * 2);
         if (what & JV_SOFTMAX_QUERY_GRAD) {
-            p.splits_q = jvk_sx_grad_splits(p.path_b, nq, d, std::min<int64_t>(p.rows_b, n));
+            p.splits_q = jvk_sx_grad_splits(p.path_b, nq, d, std::min<int64_t>(p.rows_b, n), 0);
             p.off_slab = take((int64_t)p.splits_q * nq * p.dp * 4);
+        }
+        if (what & JV_SOFTMAX_VECTOR_GRAD) {
+            const int64_t rows = std::min<int64_t>(p.rows_b, n);
+            p.splits_v = jvk_sx_grad_splits(p.path_b, rows, d, nq, 1);
+            p.off_slab_v = take(p.splits_v > 1 ? p.splits_v * rows * p.dp * 4 : 0);
         }
     }
     p.bytes = at;
@@ -341,6 +346,12 @@ int jv_softmax_grad_device(const jv_softmax_params* p, const float* d_lse, const
     } else {
         q_rows = w.mm.a, q_ld = w.mm.lda;
     }
+    JvSxFinish fq{}, fv{};
+    if (d_out_query_grad) {
+        fq.slab = (const float*)(ws + plan.off_slab), fq.splits = std::min(plan.splits_q, splits_of(plan, std::min<int64_t>(plan.rows_b, p->n)));
+        fq.rows = p->nq, fq.out = d_out_query_grad, fq.ldo = query_grad_stride;
+        fq.rest = w.rest, fq.query = query, fq.vectors = p->vectors, fq.v_stride = p->vector_stride;
+    }
     for (int64_t at = 0; at < p->n; at += plan.rows_b) {
         const int rows = (int)std::min<int64_t>(plan.rows_b, p->n - at);
         w.mm.N = rows, w.row0 = at, w.kv = (int)up(rows, 64);
@@ -362,15 +373,18 @@ int jv_softmax_grad_device(const jv_softmax_params* p, const float* d_lse, const
         if (d_out_vector_grad) {   // G across times the queries: k = the queries
             o.mm.M = rows, o.mm.k = (int)up(p->nq, 32), o.mm.kph = plan.kq / 32, o.mm.ka = p->nq % (f32 ? 32 : 64) ? p->nq + 1 : p->nq, o.mm.ca = w.kv;
             o.mm.b = q_rows, o.mm.ldb = q_ld, o.mm.kb = p->nq, o.mm.cb = rb.ready || rb.kp == 4 ? p->d : plan.dp;
-            o.mul = p->scale, o.norm = norm, o.dtype = p->dtype, o.splits = 1, o.add = 0;
-            o.out = (char*)d_out_vector_grad + at * vector_grad_stride * size_of(p->dtype), o.ldo = vector_grad_stride;
+            o.splits = plan.splits_v, o.add = 0;
+            fv.out = (char*)d_out_vector_grad + at * vector_grad_stride * size_of(p->dtype), fv.ldo = vector_grad_stride;
+            if (plan.splits_v > 1) {
+                o.mul = 1.0f, o.out = ws + plan.off_slab_v, o.ldo = plan.dp;
+                fv.slab = (const float*)o.out, fv.splits = o.splits, fv.rows = rows;
+            } else {
+                o.mul = p->scale, o.norm = norm, o.dtype = p->dtype, o.out = fv.out, o.ldo = fv.ldo;
+            }
         }
         CHK(jvk_sx_grads(d_out_query_grad ? &q : nullptr, d_out_vector_grad ? &o : nullptr, plan.path_b, s));
-    }
-    if (d_out_query_grad && !direct) {
-        const int splits = std::min(plan.splits_q, splits_of(plan, std::min<int64_t>(plan.rows_b, p->n)));
-        CHK(jvk_sx_finish((const float*)(ws + plan.off_slab), splits, p->nq, p->d, plan.dp, w.rest, query, p->vectors, p->vector_stride, p->scale, norm, d_out_query_grad,
-                          p->dtype, query_grad_stride, s));
+        const bool join_q = d_out_query_grad && !direct && at + plan.rows_b >= p->n, join_v = fv.slab;
+        if (join_q || join_v) CHK(jvk_sx_finish(join_q ? &fq : nullptr, join_v ? &fv : nullptr, p->d, plan.dp, p->scale, norm, p->dtype, s));
     }
     return done(hip_stream);
 }

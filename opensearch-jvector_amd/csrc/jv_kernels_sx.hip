@@ -89,43 +89,48 @@ __device__ __forceinline__ JvSxQuery query_of(const float* lse, const float* w, 
 }
 
 // The weights are divided by the largest of them (`norm`, multiplied back in float32 at the end): an entry of g at a target is then just
-// below 1 for the largest weight, where bf16's step is finest in relation.
-__device__ __forceinline__ void queries(const JvSxPrepare& a) {
-    __shared__ float part[4];
+// below 1 for the largest weight, where bf16's step is finest in relation.  Every workgroup finds the largest anew and sees to 256 queries.
+__device__ __forceinline__ void queries(const JvSxPrepare& a, int part) {
+    __shared__ float tops[4];
     float top = 0.0f;
-    if (a.w)
-        for (int i = threadIdx.x; i < a.nq; i += 256)
-            if (a.targets[i] >= 0 && a.targets[i] < a.n) top = fmaxf(top, fabsf(a.w[i]));
+    if (a.w) {
+#pragma unroll 8
+        for (int i = threadIdx.x; i < a.nq; i += 256) {
+            const int t = a.targets[i];
+            const float w = a.w[i];
+            if (t >= 0 && t < a.n) top = fmaxf(top, fabsf(w));
+        }
+    }
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
+    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
     __syncthreads();
-    top = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
     // (no weights, none but zeros, or one that is not finite: 1, so that what is not finite shows in the gradient)
     const float unit = a.w && top > 0.0f && top < __builtin_inff() ? top : 1.0f;
-    if (threadIdx.x == 0) *a.norm = unit;
-    for (int i = threadIdx.x; i < a.nq; i += 256) {
-        JvSxQuery q = query_of(a.lse, a.w, a.targets, a.n, i);
-        q.w /= unit;
-        a.query[i] = q;
-        a.rest[i] = 0.0f;
-    }
+    const int i = part * 256 + threadIdx.x;
+    if (i == 0) *a.norm = unit;
+    if (i >= a.nq) return;
+    JvSxQuery q = query_of(a.lse, a.w, a.targets, a.n, i);
+    q.w /= unit;
+    a.query[i] = q;
+    a.rest[i] = 0.0f;
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void jvs_prepare_kernel(const JvSxPrepare a, int g0, int g1, int g2) {   // workgroups for the matrices, one more for the queries
+__global__ __launch_bounds__(256) void jvs_prepare_kernel(const JvSxPrepare a, int g0, int g1, int g2) {   // workgroups for the matrices, the rest for the queries
     int i = blockIdx.x;
     if (i < g0) return pack<T>(a.m[0], a.d, (int64_t)i * 256 + threadIdx.x, (int64_t)g0 * 256);
     i -= g0;
     if (i < g1) return pack<T>(a.m[1], a.d, (int64_t)i * 256 + threadIdx.x, (int64_t)g1 * 256);
     i -= g1;
     if (i < g2) return pack<T>(a.m[2], a.d, (int64_t)i * 256 + threadIdx.x, (int64_t)g2 * 256);
-    queries(a);
+    queries(a, i - g2);
 }
 extern "C" hipError_t jvk_sx_prepare(const JvSxPrepare* a, hipStream_t s) {
     int g[3];
     for (int k = 0; k < 3; k++) g[k] = (int)std::min<int64_t>((a->m[k].rows * std::max(a->m[k].kp / 8, 1) + 255) / 256, 32768);
-    const unsigned grid = (unsigned)(g[0] + g[1] + g[2] + (a->query ? 1 : 0));
+    const unsigned grid = (unsigned)(g[0] + g[1] + g[2] + (a->query ? (a->nq + 255) / 256 : 0));
     if (grid == 0) return hipSuccess;
     if (a->dtype == 0) jvs_prepare_kernel<float><<<grid, 256, 0, s>>>(*a, g[0], g[1], g[2]);
     else jvs_prepare_kernel<__bf16><<<grid, 256, 0, s>>>(*a, g[0], g[1], g[2]);
@@ -554,14 +559,16 @@ static hipError_t grads_tile(const JvMmOut* q, const JvMmOut* v, hipStream_t s) 
 // The gradients' products have d columns: with up to 128 half a large tile would be multiplied for nothing.
 static int grads_path(int path, int d) { return path == JV_SX_LARGE && d <= 128 ? JV_SX_TILES : path; }
 
-// k ranges of dq: once around the CUs with the large tiles, twice with the small ones; at least four and eight steps in each (a range that is
-// joined costs a launch more)
-extern "C" int jvk_sx_grad_splits(int path, int nq, int d, int64_t rows) {
+// k ranges of a gradient of `rows` rows: once around the CUs with the large tiles, twice with the small ones; at least four and eight steps in
+// each.  dv (`across`) is written as it is if it has one range, joining more costs a launch: twice as many steps (step 4096 x 4096 x 768, bf16:
+// dv 104 us of one range, 40 of five).
+extern "C" int jvk_sx_grad_splits(int path, int64_t rows, int d, int64_t k, int across) {
     path = grads_path(path, d);
-    const int tm = path == JV_SX_LARGE ? 256 : path == JV_SX_PLANES ? shape_of(path, nq, rows, 0).m : 128, tn = path == JV_SX_LARGE ? 256 : 128;
-    const int64_t tiles = std::max<int64_t>((nq + tm - 1) / tm, 1) * ((d + tn - 1) / tn);
-    const int64_t steps = path == JV_SX_RAW || path == JV_SX_PLANES ? (rows + 31) / 32 : (rows + 63) / 64;
-    return (int)std::max<int64_t>(std::min<int64_t>((path == JV_SX_LARGE ? 256 : 512) / tiles, steps / (path == JV_SX_LARGE ? 4 : 8)), 1);
+    const bool large = path == JV_SX_LARGE;
+    const int tm = large ? 256 : path == JV_SX_PLANES && !across ? shape_of(path, (int)rows, k, 0).m : 128, tn = large ? 256 : 128;
+    const int64_t tiles = std::max<int64_t>((rows + tm - 1) / tm, 1) * ((d + tn - 1) / tn);
+    const int64_t steps = path == JV_SX_RAW || path == JV_SX_PLANES ? (k + 31) / 32 : (k + 63) / 64;
+    return (int)std::max<int64_t>(std::min<int64_t>((large ? 256 : 512) / tiles, steps / ((large ? 4 : 8) * (across ? 2 : 1))), 1);
 }
 extern "C" hipError_t jvk_sx_grads(const JvMmOut* q, const JvMmOut* v, int path, hipStream_t s) {
     path = grads_path(path, q ? q->mm.N : v->mm.N);
@@ -595,18 +602,18 @@ extern "C" hipError_t jvk_sx_grads(const JvMmOut* q, const JvMmOut* v, int path,
 // sums by G lanes, which are joined in a fixed order: with few columns and hundreds of partial sums the way through one lane's sums is
 // what counts (64 x 32 of 512 partial sums: 31 us with G = 1, 4 with 16).
 template <typename T, int G>
-__global__ __launch_bounds__(256) void jvs_finish_kernel(const float* __restrict__ slab, int splits, int64_t rows, int d, int64_t lds, const float* __restrict__ rest,
-                                                         const JvSxQuery* __restrict__ query, const T* __restrict__ v, int64_t v_stride, float mul,
-                                                         const float* __restrict__ norm, T* __restrict__ out, int64_t ldo) {
+__global__ __launch_bounds__(256) void jvs_finish_kernel(const JvSxFinish q, const JvSxFinish v, int d, int64_t lds, float mul, const float* __restrict__ norm) {
     constexpr int L = 256 / G;
     __shared__ f32x4 part[G > 1 ? 256 : 1];
-    const int64_t r = blockIdx.x;
+    const bool second = blockIdx.x >= q.rows;
+    const JvSxFinish& a = second ? v : q;
+    const int64_t r = second ? blockIdx.x - q.rows : blockIdx.x;
     const int g = threadIdx.x / L, c = ((int)threadIdx.x % L + (int)blockIdx.y * L) * 4;   // (lds is a multiple of 64)
     f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
     if (c < d) {
-        const float* p = slab + r * lds + c;
+        const float* p = a.slab + r * lds + c;
 #pragma unroll 8
-        for (int k = g; k < splits; k += G) x += *(const f32x4*)(p + k * rows * lds);
+        for (int k = g; k < a.splits; k += G) x += *(const f32x4*)(p + k * a.rows * lds);
     }
     if constexpr (G > 1) {
         part[threadIdx.x] = x;
@@ -615,14 +622,12 @@ __global__ __launch_bounds__(256) void jvs_finish_kernel(const float* __restrict
 #pragma unroll
         for (int k = 1; k < G; k++) x += part[k * L + threadIdx.x];
     }
-    const float by = norm ? mul * *norm : mul, lack = rest ? rest[r] : 0.0f;
-    const int64_t target = lack != 0.0f ? query[r].target : 0;
+    const float by = norm ? mul * *norm : mul, lack = a.rest ? a.rest[r] : 0.0f;
+    const T* target = lack != 0.0f ? (const T*)a.vectors + a.query[r].target * a.v_stride : nullptr;
+    T* out = (T*)a.out + r * a.ldo;
 #pragma unroll
     for (int e = 0; e < 4; e++)
-        if (c + e < d) {
-            const float y = lack != 0.0f ? fmaf(lack, (float)v[target * v_stride + c + e], x[e]) : x[e];
-            out[r * ldo + c + e] = (T)(y * by);
-        }
+        if (c + e < d) out[c + e] = (T)((lack != 0.0f ? fmaf(lack, (float)target[c + e], x[e]) : x[e]) * by);
 }
 template <typename T>
 __global__ __launch_bounds__(256) void jvs_fill_kernel(T* __restrict__ out, int64_t stride, int64_t rows, int d, float value) {
@@ -635,17 +640,15 @@ static unsigned grid_for(int64_t items) {
     const int64_t want = (items + 255) / 256;
     return (unsigned)(want < 16384 ? want : 16384);
 }
-extern "C" hipError_t jvk_sx_finish(const float* slab, int splits, int64_t rows, int d, int64_t lds, const float* rest, const JvSxQuery* query, const void* v,
-                                    int64_t v_stride, float mul, const float* norm, void* out, int dtype, int64_t ldo, hipStream_t s) {
+extern "C" hipError_t jvk_sx_finish(const JvSxFinish* q, const JvSxFinish* v, int d, int64_t lds, float mul, const float* norm, int dtype, hipStream_t s) {
+    const int64_t rows = (q ? q->rows : 0) + (v ? v->rows : 0);
     if (rows <= 0 || d <= 0) return hipSuccess;
-    const int groups = splits >= 32 ? 16 : splits >= 4 ? 4 : 1, lanes = 256 / groups;
+    if (rows > 0x7fffffffll) return hipErrorInvalidValue;
+    const int splits = std::max(q ? q->splits : 1, v ? v->splits : 1), groups = splits >= 32 ? 16 : splits >= 4 ? 4 : 1, lanes = 256 / groups;
     const dim3 grid((unsigned)rows, (unsigned)((d + 4 * lanes - 1) / (4 * lanes)));
-    auto run = [&](auto kernel, auto type) {
-        using T = decltype(type);
-        kernel<<<grid, 256, 0, s>>>(slab, splits, rows, d, lds, rest, query, (const T*)v, v_stride, mul, norm, (T*)out, ldo);
-    };
-    if (dtype == 0) run(groups == 16 ? jvs_finish_kernel<float, 16> : groups == 4 ? jvs_finish_kernel<float, 4> : jvs_finish_kernel<float, 1>, 0.0f);
-    else run(groups == 16 ? jvs_finish_kernel<__bf16, 16> : groups == 4 ? jvs_finish_kernel<__bf16, 4> : jvs_finish_kernel<__bf16, 1>, (__bf16)0.0f);
+    auto run = [&](auto kernel) { kernel<<<grid, 256, 0, s>>>(q ? *q : JvSxFinish{}, v ? *v : JvSxFinish{}, d, lds, mul, norm); };
+    if (dtype == 0) run(groups == 16 ? jvs_finish_kernel<float, 16> : groups == 4 ? jvs_finish_kernel<float, 4> : jvs_finish_kernel<float, 1>);
+    else run(groups == 16 ? jvs_finish_kernel<__bf16, 16> : groups == 4 ? jvs_finish_kernel<__bf16, 4> : jvs_finish_kernel<__bf16, 1>);
     return hipGetLastError();
 }
 extern "C" hipError_t jvk_sx_fill(void* out, int dtype, int64_t stride, int64_t rows, int d, float value, hipStream_t s) {

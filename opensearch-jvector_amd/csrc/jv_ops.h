@@ -49,6 +49,18 @@ struct JvSxQuery {
     int32_t target;        // row, -1 = none
     int32_t pad;
 };
+// partial sums of a gradient, [splits][rows][lds], to be joined
+struct JvSxFinish {
+    const float* slab;
+    int32_t splits;
+    int64_t rows;
+    void* out;             // [rows][ldo]
+    int64_t ldo;
+    const float* rest;     // per row, times the row's target: added; nullptr = none
+    const JvSxQuery* query;
+    const void* vectors;
+    int64_t v_stride;
+};
 // One piece of the gradient's weights G = w (p - [j = target]), zeros behind M and N: bf16 [up(M, 64)][kv]; float32 as three planes
 // [up(M, 32)][3][kv] (JV_SX_PLANES) or as it is [up(M, 32)][kv] (JV_SX_RAW).
 struct JvSxWeights {
@@ -105,9 +117,8 @@ hipError_t jvk_sx_loss(const JvSxLoss* a, hipStream_t s);
 hipError_t jvk_sx_join(const float2* part, int splits, int nq, const float* hit, const int32_t* targets, int64_t n, float* loss, float* lse, hipStream_t s);
 hipError_t jvk_sx_weights(const JvSxWeights* a, hipStream_t s);
 // dq = G V and dv = G^T Q (nullptr: not asked for)
-int jvk_sx_grad_splits(int path, int nq, int d, int64_t rows);
+int jvk_sx_grad_splits(int path, int64_t rows, int d, int64_t k, int across);
 hipError_t jvk_sx_grads(const JvMmOut* q, const JvMmOut* v, int path, hipStream_t s);
-hipError_t jvk_sx_finish(const float* slab, int splits, int64_t rows, int d, int64_t lds, const float* rest, const JvSxQuery* query, const void* v, int64_t v_stride,
-                         float mul, const float* norm, void* out, int dtype, int64_t ldo, hipStream_t s);
+hipError_t jvk_sx_finish(const JvSxFinish* q, const JvSxFinish* v, int d, int64_t lds, float mul, const float* norm, int dtype, hipStream_t s);
 hipError_t jvk_sx_fill(void* out, int dtype, int64_t stride, int64_t rows, int d, float value, hipStream_t s);
 }
