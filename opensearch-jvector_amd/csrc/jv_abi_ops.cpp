@@ -80,7 +80,7 @@ struct Plan {
     int P, dp, kq, gq;                // planes; d and nq padded to 64; rows of g (the large tiles write whole steps, the small ones one row behind the queries)
     int64_t rows_f, rows_b;           // rows of one piece, forward (where the vectors have to be laid out) / backward
     int path_f, path_b, splits_f, splits_q, splits_v;   // forward, backward
-    int64_t off_q, off_q4, off_v, off_part, off_hit, off_query, off_norm, off_rest, off_g, off_slab, off_slab_v, bytes;
+    int64_t off_q, off_clean, off_v, off_part, off_hit, off_query, off_norm, off_rest, off_g, off_slab, off_slab_v, bytes;
 };
 
 // MB of one piece's weights g: few large pieces, for every piece writes and reads dq's partial sums again and starts its tiles anew (step
@@ -113,7 +113,6 @@ Plan make_plan(int dtype, int nq, int64_t n, int d, uint32_t what) {
         return o;
     };
     p.off_q = take((int64_t)nq * row);
-    p.off_q4 = take((int64_t)(d < 4 ? nq : 0) * 16);   // (float32 rows of fewer than four components, as they lie but with four)
     if (what & JV_SOFTMAX_LOSS) {
         p.path_f = jvk_sx_path(nq, n, dtype == JV_DTYPE_F32);
         p.splits_f = jvk_sx_loss_splits(p.path_f, nq, n, d);
@@ -135,6 +134,7 @@ Plan make_plan(int dtype, int nq, int64_t n, int d, uint32_t what) {
         if (what & JV_SOFTMAX_VECTOR_GRAD) {
             const int64_t rows = std::min<int64_t>(p.rows_b, n);
             p.splits_v = jvk_sx_grad_splits(p.path_b, rows, d, nq, 1);
+            if (dtype == JV_DTYPE_F32) p.off_clean = take((int64_t)nq * std::max(d, 4) * 4);
             p.off_slab_v = take(p.splits_v > 1 ? p.splits_v * rows * p.dp * 4 : 0);
         }
     }
@@ -150,11 +150,13 @@ struct Rows {
     int64_t stride;   // bytes
     bool ready;
     int kp;           // components of a row that is laid out instead
+    bool raw;         // as float32, not as planes
+    int cols(int d) const { return ready || raw ? d : kp; }
 };
 Rows rows_of(const void* p, int64_t stride, const jv_softmax_params* q, const Plan& plan, int path, bool vectors) {
-    Rows r{(const char*)p, stride * size_of(q->dtype), false, plan.dp};
+    Rows r{(const char*)p, stride * size_of(q->dtype), false, plan.dp, false};
     if (q->dtype == JV_DTYPE_BF16) r.ready = (uintptr_t)p % 4 == 0 && stride % 2 == 0 && q->d % (vectors ? 8 : 64) == 0;
-    else if (path == JV_SX_RAW || (path == JV_SX_PLANES && vectors)) r.ready = q->d >= 4, r.kp = 4;
+    else if (path == JV_SX_RAW || (path == JV_SX_PLANES && vectors)) r.ready = q->d >= 4, r.kp = 4, r.raw = true;
     return r;
 }
 
@@ -200,9 +202,9 @@ void take_rows(const Rows& r, int dtype, int64_t at, int64_t rows, const Plan& p
         m->rows = 0;
         return;
     }
-    m->x = r.p + at * r.stride, m->stride = r.stride / size_of(dtype), m->rows = rows, m->out = to, m->kp = r.kp;
+    m->x = r.p + at * r.stride, m->stride = r.stride / size_of(dtype), m->rows = rows, m->out = to, m->kp = r.kp, m->raw = r.raw;
     *out = to;
-    *ld = r.kp == 4 ? 16 : (int64_t)plan.P * plan.dp * 2;
+    *ld = r.raw ? (int64_t)r.kp * 4 : (int64_t)plan.P * plan.dp * 2;
 }
 
 }  // namespace
@@ -318,7 +320,8 @@ int jv_softmax_grad_device(const jv_softmax_params* p, const float* d_lse, const
         return done(hip_stream);
     }
     char* ws = (char*)p->workspace;
-    const Rows rq = rows_of(p->queries, p->query_stride, p, plan, plan.path_b, false), rv = rows_of(p->vectors, p->vector_stride, p, plan, plan.path_b, true);
+    Rows rq = rows_of(p->queries, p->query_stride, p, plan, plan.path_b, false);
+    const Rows rv = rows_of(p->vectors, p->vector_stride, p, plan, plan.path_b, true);
     const bool f32 = p->dtype == JV_DTYPE_F32, raw = plan.path_b == JV_SX_RAW;
     JvSxWeights w{};
     w.mm = logits(plan, p->nq, p->d);
@@ -334,17 +337,26 @@ int jv_softmax_grad_device(const jv_softmax_params* p, const float* d_lse, const
         w.lse = d_lse, w.w = d_loss_grad, w.targets = p->targets, w.n = p->n;
     } else {
         w.query = query = (JvSxQuery*)(ws + plan.off_query), w.rest = (float*)(ws + plan.off_rest), norm = (float*)(ws + plan.off_norm);
-        pre.lse = d_lse, pre.w = d_loss_grad, pre.targets = p->targets, pre.nq = p->nq, pre.n = p->n, pre.query = query, pre.norm = norm, pre.rest = w.rest;
+        pre.lse = d_lse, pre.w = d_loss_grad, pre.nq = p->nq, pre.query = query, pre.norm = norm, pre.rest = w.rest;
     }
     const bool direct = raw && plan.splits_q == 1 && plan.rows_b >= p->n;   // dq is complete at once
-    const char* q_rows;   // the queries as dv's product reads them: the same but for planes, which it splits itself
-    int64_t q_ld;
+    // Queries without a target are laid out as zeros.  dv's product reads them so: bf16 as they are laid out, float32 as a copy.
+    const char* q_rows = ws + plan.off_clean;
+    int64_t q_ld = (int64_t)p->d * 4;
+    pre.targets = p->targets, pre.n = p->n;
+    if (!f32) rq.ready = false;
+    Rows rb = rq;
     take_rows(rq, p->dtype, 0, p->nq, plan, ws + plan.off_q, &pre.m[0], &w.mm.a, &w.mm.lda);
-    const Rows rb = plan.path_b == JV_SX_PLANES ? rows_of(p->queries, p->query_stride, p, plan, JV_SX_RAW, false) : rq;
-    if (plan.path_b == JV_SX_PLANES) {
-        take_rows(rb, p->dtype, 0, p->nq, plan, ws + plan.off_q4, &pre.m[2], &q_rows, &q_ld);
-    } else {
+    pre.m[0].clean = !rq.ready;
+    if (!rq.ready && (!f32 || rq.raw)) {
         q_rows = w.mm.a, q_ld = w.mm.lda;
+    } else if (d_out_vector_grad && plan.path_b == JV_SX_PLANES) {
+        rb = rows_of(p->queries, p->query_stride, p, plan, JV_SX_RAW, false);
+        rb.ready = false, rb.kp = std::max(p->d, 4);
+        take_rows(rb, p->dtype, 0, p->nq, plan, ws + plan.off_clean, &pre.m[2], &q_rows, &q_ld);
+        pre.m[2].clean = 1;
+    } else if (d_out_vector_grad) {
+        w.clean = (float*)(ws + plan.off_clean);
     }
     JvSxFinish fq{}, fv{};
     if (d_out_query_grad) {
@@ -364,7 +376,7 @@ int jv_softmax_grad_device(const jv_softmax_params* p, const float* d_lse, const
         o.mm.N = p->d, o.mm.end_b = kNoEnd;
         if (d_out_query_grad) {   // G times the piece's vectors: k = its rows
             o.mm.M = p->nq, o.mm.k = w.kv, o.mm.kph = w.kv / 32;
-            o.mm.b = w.mm.b, o.mm.ldb = w.mm.ldb, o.mm.kb = rows, o.mm.cb = rv.ready || rv.kp == 4 ? p->d : plan.dp;
+            o.mm.b = w.mm.b, o.mm.ldb = w.mm.ldb, o.mm.kb = rows, o.mm.cb = rv.cols(p->d);
             o.mul = 1.0f, o.out = ws + plan.off_slab, o.ldo = plan.dp, o.add = at > 0;
             o.splits = std::min(plan.splits_q, splits_of(plan, rows));   // (only the last piece can be that short: it adds to the first ranges)
             if (direct) o.mul = p->scale, o.out = d_out_query_grad, o.ldo = query_grad_stride;
@@ -372,7 +384,7 @@ int jv_softmax_grad_device(const jv_softmax_params* p, const float* d_lse, const
         }
         if (d_out_vector_grad) {   // G across times the queries: k = the queries
             o.mm.M = rows, o.mm.k = (int)up(p->nq, 32), o.mm.kph = plan.kq / 32, o.mm.ka = p->nq % (f32 ? 32 : 64) ? p->nq + 1 : p->nq, o.mm.ca = w.kv;
-            o.mm.b = q_rows, o.mm.ldb = q_ld, o.mm.kb = p->nq, o.mm.cb = rb.ready || rb.kp == 4 ? p->d : plan.dp;
+            o.mm.b = q_rows, o.mm.ldb = q_ld, o.mm.kb = p->nq, o.mm.cb = rb.cols(p->d);
             o.splits = plan.splits_v, o.add = 0;
             fv.out = (char*)d_out_vector_grad + at * vector_grad_stride * size_of(p->dtype), fv.ldo = vector_grad_stride;
             if (plan.splits_v > 1) {

@@ -41,12 +41,21 @@ __device__ __forceinline__ void planes3(float x, uint16_t (&p)[3]) {
 // ---------------------------------------------------------------------------------------------
 // what has to be laid out: rows as padded bf16 planes [rows][planes][kp], and what the gradient needs of each query
 // ---------------------------------------------------------------------------------------------
+// A query without a target takes no part in the gradients, whatever it holds (a batch's padding may be NaN): its row of g is zeros, and so is
+// its row among dv's operands.
+__device__ __forceinline__ bool known(int target, int64_t n) { return target >= 0 && target < n; }
+
 template <typename T>
-__device__ __forceinline__ void pack(const JvSxPrepare::Matrix& m, int d, int64_t first, int64_t step) {   // eight components a thread
+__device__ __forceinline__ void pack(const JvSxPrepare& a, const JvSxPrepare::Matrix& m, int64_t first, int64_t step) {   // eight components a thread
     constexpr int P = sizeof(T) == 4 ? 3 : 1;
-    const int kp = m.kp, per = kp / 8;
-    if (kp == 4) {
-        for (int64_t i = first; i < m.rows * 4; i += step) ((float*)m.out)[i] = (i & 3) < d ? (float)((const T*)m.x)[(i >> 2) * m.stride + (i & 3)] : 0.0f;
+    const int d = a.d, kp = m.kp, per = kp / 8;
+    auto dead = [&](int64_t r) { return m.clean && !known(a.targets[r], a.n); };
+    if (m.raw) {
+        for (int64_t i = first; i < m.rows * kp; i += step) {
+            const int64_t r = i / kp;
+            const int c = (int)(i - r * kp);
+            ((float*)m.out)[i] = c < d && !dead(r) ? (float)((const T*)m.x)[r * m.stride + c] : 0.0f;
+        }
         return;
     }
     for (int64_t i = first; i < m.rows * per; i += step) {
@@ -54,7 +63,10 @@ __device__ __forceinline__ void pack(const JvSxPrepare::Matrix& m, int d, int64_
         const int at = (int)(i - r * per) * 8;
         const T* row = (const T*)m.x + r * m.stride;
         T x[8];
-        if (at + 8 <= d) {
+        if (dead(r)) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = (T)0.0f;
+        } else if (at + 8 <= d) {
             __builtin_memcpy(x, row + at, sizeof(x));   // (no alignment is asked for)
         } else {
 #pragma unroll
@@ -84,8 +96,8 @@ __device__ __forceinline__ void pack(const JvSxPrepare::Matrix& m, int d, int64_
 
 __device__ __forceinline__ JvSxQuery query_of(const float* lse, const float* w, const int32_t* targets, int64_t n, int i) {
     const int t = targets[i];
-    const bool known = t >= 0 && t < n;
-    return {known ? lse[i] * 1.44269504088896341f : __builtin_inff(), known ? (w ? w[i] : 1.0f) : 0.0f, known ? t : -1, 0};   // (no target: 2^-inf * 0)
+    const bool has = known(t, n);
+    return {has ? lse[i] * 1.44269504088896341f : __builtin_inff(), has ? (w ? w[i] : 1.0f) : 0.0f, has ? t : -1, 0};
 }
 
 // The weights are divided by the largest of them (`norm`, multiplied back in float32 at the end): an entry of g at a target is then just
@@ -98,7 +110,7 @@ __device__ __forceinline__ void queries(const JvSxPrepare& a, int part) {
         for (int i = threadIdx.x; i < a.nq; i += 256) {
             const int t = a.targets[i];
             const float w = a.w[i];
-            if (t >= 0 && t < a.n) top = fmaxf(top, fabsf(w));
+            if (known(t, a.n)) top = fmaxf(top, fabsf(w));
         }
     }
 #pragma unroll
@@ -120,11 +132,11 @@ __device__ __forceinline__ void queries(const JvSxPrepare& a, int part) {
 template <typename T>
 __global__ __launch_bounds__(256) void jvs_prepare_kernel(const JvSxPrepare a, int g0, int g1, int g2) {   // workgroups for the matrices, the rest for the queries
     int i = blockIdx.x;
-    if (i < g0) return pack<T>(a.m[0], a.d, (int64_t)i * 256 + threadIdx.x, (int64_t)g0 * 256);
+    if (i < g0) return pack<T>(a, a.m[0], (int64_t)i * 256 + threadIdx.x, (int64_t)g0 * 256);
     i -= g0;
-    if (i < g1) return pack<T>(a.m[1], a.d, (int64_t)i * 256 + threadIdx.x, (int64_t)g1 * 256);
+    if (i < g1) return pack<T>(a, a.m[1], (int64_t)i * 256 + threadIdx.x, (int64_t)g1 * 256);
     i -= g1;
-    if (i < g2) return pack<T>(a.m[2], a.d, (int64_t)i * 256 + threadIdx.x, (int64_t)g2 * 256);
+    if (i < g2) return pack<T>(a, a.m[2], (int64_t)i * 256 + threadIdx.x, (int64_t)g2 * 256);
     queries(a, i - g2);
 }
 extern "C" hipError_t jvk_sx_prepare(const JvSxPrepare* a, hipStream_t s) {
@@ -414,11 +426,11 @@ __device__ __forceinline__ void weigh(typename Core::acc_t (&acc)[NT], const JvS
                     if (lossy) *rest = acc[n][e] - (float)(__bf16)acc[n][e];   // (one lane holds it; three planes lack nothing)
                 }
     }
-    if (cols < Core::TN) {
+    if (cols < Core::TN || (Core::RAW && __any(q.target < 0))) {   // (laid out, a query without a target is zeros)
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int e = 0; e < Core::E; e++) acc[n][e] = Core::col(n, e) < cols ? acc[n][e] : 0.0f;
+            for (int e = 0; e < Core::E; e++) acc[n][e] = (!Core::RAW || q.target >= 0) && Core::col(n, e) < cols ? acc[n][e] : 0.0f;
     }
 }
 
@@ -457,14 +469,28 @@ static __host__ __device__ __forceinline__ int padded_queries(const JvSxWeights&
     return a.mm.M % step ? a.mm.M + 1 : a.mm.M;
 }
 
+constexpr int CLEANED = 2048;   // values that a workgroup copies
+
 // the same on small tiles, one a workgroup
 template <class T>
 __global__ __launch_bounds__(T::THREADS, T::RESIDENT) void jvs_weights_tile_kernel(const JvSxWeights a) {
     constexpr int MT = T::MT, NT = T::NT;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    const int padded = padded_queries(a);
+    const int padded = padded_queries(a), tm = (padded + T::TM - 1) / T::TM, tn = (a.kv + T::TN - 1) / T::TN;
+    const int copies = gridDim.x - tm * tn;   // workgroups that copy the queries for dv, the first ones: short beside a tile's
+    if constexpr (T::RAW) {
+        if ((int)blockIdx.x < copies) {
+            const uint32_t d = a.mm.k, all = (uint32_t)a.mm.M * d;
+#pragma unroll
+            for (int k = 0; k < CLEANED / 256; k++) {
+                const uint32_t i = blockIdx.x * CLEANED + k * 256 + threadIdx.x, r = i / d;
+                if (i < all) a.clean[i] = known(a.targets[r], a.n) ? *((const float*)(a.mm.a + r * a.mm.lda) + (i - r * d)) : 0.0f;
+            }
+            return;
+        }
+    }
     int m0, n0;
-    band_order(xcd_order(blockIdx.x, gridDim.x), (padded + T::TM - 1) / T::TM, (a.kv + T::TN - 1) / T::TN, m0, n0);
+    band_order(xcd_order(blockIdx.x - copies, tm * tn), tm, tn, m0, n0);
     m0 *= T::TM, n0 *= T::TN;
     typename T::acc_t acc[MT][NT];
     T::run(a.mm, m0, n0, 0, T::steps(a.mm), smem, acc);
@@ -507,10 +533,11 @@ __global__ __launch_bounds__(T::THREADS, T::RESIDENT) void jvs_weights_tile_kern
 template <class T>
 static hipError_t weights_tile(const JvSxWeights& a, hipStream_t s) {
     const int64_t all = (int64_t)((padded_queries(a) + T::TM - 1) / T::TM) * ((a.kv + T::TN - 1) / T::TN);
-    if (all > 0x7fffffffll) return hipErrorInvalidValue;
+    const int64_t extra = a.clean ? ((int64_t)a.mm.M * a.mm.k + CLEANED - 1) / CLEANED : 0;
+    if (all + extra > 0x7fffffffll || extra * CLEANED > 0x7fffffffll) return hipErrorInvalidValue;
     hipError_t e = lds_of(jvs_weights_tile_kernel<T>, T::LDS);
     if (e != hipSuccess) return e;
-    jvs_weights_tile_kernel<T><<<(unsigned)all, T::THREADS, T::LDS, s>>>(a);
+    jvs_weights_tile_kernel<T><<<(unsigned)(all + extra), T::THREADS, T::LDS, s>>>(a);
     return hipGetLastError();
 }
 

@@ -72,6 +72,7 @@ __device__ __forceinline__ void release_step() {
 template <int TY, int MT_, int NT_, int WM, int WN, int NS, bool TA = false, bool TB = false>
 struct Tile {
     using acc_t = f32x16;
+    static constexpr bool RAW = false;
     static constexpr int MT = MT_, NT = NT_, RESIDENT = 1, E = 16, WIDE = 32 * NT;   // values of an accumulator; columns of a wave
     static constexpr int TM = 32 * MT * WM, TN = 32 * NT * WN, WAVES = WM * WN, THREADS = 64 * WAVES;
     static constexpr int GA = TM / 8, GB = TN / 8;                               // 8-row groups

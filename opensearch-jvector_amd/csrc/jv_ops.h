@@ -15,7 +15,7 @@ struct JvMm {
     int32_t kph;             // phases (bf16, e4m3)
     int64_t plane_a;         // float32 as bf16 planes: bytes from plane to plane
     int32_t ka, kb, ca, cb;  // operands with k across their rows
-    int32_t end_b;           // bytes of k that a row of B has, a multiple of 16 (k along its rows): what lies behind reads as the last 16, A holds zeros there
+    int32_t end_b;           // bytes of k that a row of B has, a multiple of 16 (bf16, k along its rows): what lies behind reads as the last 16, A holds zeros there
     const uint8_t *sa, *sb;  // e4m3: scale bytes [M][kph / 2] / [N][kph / 2]
 };
 
@@ -61,8 +61,8 @@ struct JvSxFinish {
     const void* vectors;
     int64_t v_stride;
 };
-// One piece of the gradient's weights G = w (p - [j = target]), zeros behind M and N: bf16 [up(M, 64)][kv]; float32 as three planes
-// [up(M, 32)][3][kv] (JV_SX_PLANES) or as it is [up(M, 32)][kv] (JV_SX_RAW).
+// One piece of the gradient's weights G = w (p - [j = target]), zeros where a query has no target: bf16 [M][kv]; float32 as three
+// planes [M][3][kv] (JV_SX_PLANES) or as it is [M][kv] (JV_SX_RAW).  Behind the last query: zeros, one row of them or up to a multiple of 64.
 struct JvSxWeights {
     JvMm mm;               // A = queries, B = vectors of this piece
     float c;
@@ -75,6 +75,7 @@ struct JvSxWeights {
     void* g;
     int32_t kv;            // N padded to 64
     float* rest;           // [M] bf16: what G's entry at the target lacks of its float32 value
+    float* clean;          // JV_SX_RAW: the queries [M][d], those without a target as zeros, written beside; nullptr = none
 };
 
 // what has to be laid out before a product: up to three matrices (rows -> bf16 planes [rows][planes][kp]) and the queries' constants, one launch
@@ -83,14 +84,16 @@ struct JvSxPrepare {
         const void* x;
         int64_t stride, rows;   // rows = 0: none
         void* out;
-        int32_t kp;             // 4: float32 rows of fewer than four components, as rows of four
+        int32_t kp;
+        int32_t raw;            // float32 rows [rows][kp] as they are
+        int32_t clean;          // rows without a target become zeros
     } m[3];
     int32_t dtype, d;
+    const int32_t* targets;     // of the queries, for n rows
+    int64_t n;
     // the gradient's queries (query == nullptr: none)
     const float *lse, *w;
-    const int32_t* targets;
     int32_t nq;
-    int64_t n;
     JvSxQuery* query;
     float *norm, *rest;
 };

@@ -29,6 +29,7 @@ struct Work {
 template <int TY, bool TA = false, bool TB = false>
 struct Pipe {
     using acc_t = f32x16;
+    static constexpr bool RAW = false;
     static constexpr int E = 16, WIDE = 64;
     static constexpr int MT = 4, NT = 2, TM = 256, TN = 256, THREADS = 512;   // waves: 2 along M, 4 along N
     static constexpr int REGION = 32768, SCALES = 4 * REGION, SCRATCH = SCALES + (TY == BF16 ? 0 : 2 * 8192);

@@ -16,6 +16,7 @@ namespace jvmm {
 template <int MT_, bool TA, bool TB>
 struct Tile3 {
     using acc_t = f32x16;
+    static constexpr bool RAW = false;
     static constexpr int RESIDENT = 2;   // workgroups a CU
     static constexpr int E = 16, WIDE = 32;
     static constexpr int MT = MT_, NT = 1, WAVES = 4, THREADS = 256, TM = 32 * MT, TN = 128;

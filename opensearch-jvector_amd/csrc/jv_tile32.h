@@ -21,6 +21,7 @@ __device__ __forceinline__ constexpr int part_of_b(int g) { return (0x118 >> (2 
 template <int MT_, int NT_, int WM, int WN, int NS, bool TA, bool TB, bool SOLO = false>
 struct Tile32 {
     using acc_t = f32x16;
+    static constexpr bool RAW = true;   // float32 operands as they lie
     static constexpr int MT = MT_, NT = NT_, RESIDENT = 1, E = 16, WIDE = 32 * NT;
     static constexpr int TM = 32 * MT * WM, TN = 32 * NT * WN, WAVES = WM * WN, THREADS = 64 * WAVES;
     static constexpr int GA = TM / 8, GB = TN / 8;                       // KB of a step
@@ -183,6 +184,7 @@ struct Tile32 {
 template <class Solo>
 struct KSplit {
     using acc_t = f32x4;
+    static constexpr bool RAW = true;   // float32 operands as they lie
     static constexpr int MT = 1, NT = 1, RESIDENT = 1, E = 4, WIDE = 8, TM = 32, TN = 32, THREADS = 256, LDS = 4 * Solo::LDS;
     static __host__ __device__ __forceinline__ int steps(const JvMm& a) { return Solo::steps(a); }
     static __device__ __forceinline__ void run(const JvMm& a, int m0, int n0, int k0, int k1, unsigned char* smem, f32x4 (&acc)[1][1]) {

@@ -286,6 +286,27 @@ def test_a_row_that_is_not_finite_shows(torch, ops):
     assert torch.isnan(lse[2]) and torch.isfinite(lse[torch.arange(20) != 2]).all()
 
 
+@pytest.mark.parametrize("dtype,nq,n,d", [("f32", 40, 300, 700), ("f32", 100, 2000, 50), ("f32", 70, 40000, 96), ("f32", 150, 24000, 33), ("f32", 9, 70, 3), ("f32", 20, 300000, 2),
+                                          ("bf16", 70, 500, 128), ("bf16", 70, 500, 100), ("bf16", 300, 30000, 192), ("bf16", 520, 17000, 72)])
+def test_a_batch_padded_with_anything(torch, ops, dtype, nq, n, d):
+    """Queries without a target take no part, whatever they, their lse and their weight hold: the same bits as with zeros."""
+    q, v, t, w, *_ = loss_case(torch, nq, n, d, dtype)
+    t[5::7] = -1
+    t[nq - 2:] = torch.tensor([n, -7], dtype=torch.int32)
+    dead = (t < 0) | (t >= n)
+    q[dead] = 0
+    want, lse = ops.softmax_loss(q, v, t, 9.0)
+    grads = ops.softmax_loss_grad(q, v, t, 9.0, lse, w)
+    garbage = torch.tensor([float("nan"), float("inf"), -float("inf"), 3e38], device="cuda").to(q.dtype)
+    q[dead] = garbage[torch.arange(int(dead.sum()), device="cuda") % 4][:, None].expand(-1, d).clone()
+    got, lse2 = ops.softmax_loss(q, v, t, 9.0)
+    assert torch.equal(got, want) and torch.equal(lse2[~dead], lse[~dead])
+    lse2[dead], w[dead] = float("nan"), float("inf")
+    dq, dv = ops.softmax_loss_grad(q, v, t, 9.0, lse2, w)
+    assert torch.equal(dq, grads[0]) and torch.equal(dv, grads[1])
+    assert (dq[dead] == 0).all() and torch.isfinite(dv.float()).all() and not (dv == 0).all()
+
+
 def test_gradients_into_rows_that_lie_apart(torch, ops, pkg):
     b = pkg.binding
     q, v, t, w, *_ = loss_case(torch, 70, 333, 96, "bf16")
