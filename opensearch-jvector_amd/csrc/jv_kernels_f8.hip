@@ -140,8 +140,13 @@ extern "C" hipError_t jvk_f8_decode(const uint8_t* codes, const uint8_t* scales,
 }
 
 // bf16 scores keep 8 bits: the 8-bit unit's sums are enough.  float32 scores take the bf16 unit (jv_mm.h).  Tiles: 256 x 256 where they fill the
-// chip, more than half of one is queries and the output's rows are 16-B aligned; 32 x 128 and 64 x 128 for up to 32 and 64 queries (the rows are streamed); 128 x 128 otherwise, but 64 x 64 where that is no more than
-// one tile a CU.
+// chip, more than half of one is queries and the output's rows are 16-B aligned (jv_pipe.h); 32 x 128 and 64 x 128 for up to 32 and 64 queries (the
+// rows are streamed); 128 x 128 otherwise, but 64 x 64 where that is no more than one tile a CU.
+//   1 x 100 000 x 768: 22 us, the launches of the two calls (the query's encoding and this) and 77 MB of codes.
+//   256 x 500 000 x 768, float32: 265 us, 3.4 TB/s, more than half of it the scores; the stores of one tile and the products of the next
+//     share a wave's order of memory operations, so they overlap by two phases only.  d = 128: 133 us, 4.3 TB/s (large copy: 4.7).
+//   4096 x 65 536 x 1536, bf16: 465 us, 1770 TFLOP/s (a large library product of 8-bit floats: 2785); 8-bit products draw the most power and the
+//     clock gives way.  256 x 256 against 128 x 128 tiles: 1024 x 100 000 x 768, bf16: 128 and 178 us.
 template <int TY>
 static hipError_t score(const JvMmOut& a, hipStream_t s) {
     const int64_t M = a.mm.M, N = a.mm.N, tiles = (M + 127) / 128 * ((N + 127) / 128);

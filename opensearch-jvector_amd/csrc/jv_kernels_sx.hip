@@ -3,14 +3,22 @@
 //   z_ij = scale q_i . v_j     lse_i = log sum_j exp z_ij     loss_i = lse_i - z_i,t(i)
 //   g_ij = w_i scale (exp(z_ij - lse_i) - [j = t(i)])         dq_i = sum_j g_ij v_j         dv_j = sum_i g_ij q_i
 //
-// Everything is a product of rows with rows (jv_mm.h).  Forward: a workgroup walks tiles of rows for one panel of queries, and every
-// lane keeps the running maximum and sum of ITS rows (one column of the accumulators is one query: no exchange until the end).
-// Backward: the logits are computed again, a piece of the rows at a time, and g is written twice, by query and by row, so that both
-// gradients are products of rows with rows too.  Logarithms and exponentials are base 2 inside (c = scale log2 e).
+// Forward: a workgroup walks tiles of rows for one panel of queries, and every lane keeps the running maximum and sum of ITS rows (one column of
+// the accumulators is one query: no exchange until the end); the workgroups' partials are joined by a second kernel.  Backward: the logits
+// are computed again, a piece of the rows at a time, and written once as g [query][row]; dq reads g with k along its rows, dv with k across
+// them (the transposing LDS read), so nothing is transposed in memory.  Logarithms and exponentials are base 2 inside (c = scale log2 e).
 //
-// bf16 operands are multiplied as they are (products exact in float32, float32 sums); g is rounded to bf16 once: 2^-9 relative for each
-// term of a sum over rows or queries, the size of the gradient's own final rounding.  float32 operands and g are three bf16 planes (24 bits)
-// and a product is the six plane pairs that reach 2^-24: float32's accuracy at 2.7 times the rate of its own matrix instruction.
+// bf16 operands are multiplied as they are (products exact in float32, float32 sums); g is rounded to bf16 once: half a step, 2^-8 relative, for
+// each term of a sum over rows or queries, the size of the gradient's own final rounding.  The entry at a query's target is the one term that
+// stands alone: what it lacks (`rest`) is added to dq in float32.  float32 operands and g are three bf16 parts (24 bits) and a product is the six
+// pairs of them that reach 2^-24: float32's accuracy at 1.5 times the rate of its own matrix instruction (1423 / 6 against 154 TFLOP/s).
+//
+// What bounds it (MI355X; a large copy moves 4.7 TB/s, a large bf16 product runs at 1423 TFLOP/s):
+//   few queries (bf16 300, float32 100: as many operations as a byte of rows pays for): the rows' bytes.  Loss 256 x 1 000 000 x 768 bf16: 445 us,
+//     3.5 TB/s and 880 TFLOP/s, near both; loss 11 x 257 776 x 1272 float32: 268 us, 4.9 TB/s.
+//   many queries: the matrix unit, and behind each tile the exponentials (a quarter of the rate of other instructions), which no product runs
+//     beside.  Step 4096 x 131 072 x 1024 bf16: 4.15 ms, 1060 TFLOP/s over its four products; float32 777 x 30 011 x 381: 550 us, 775 TFLOP/s.
+//   little of everything: the launches.  Step 32 x 1000 x 64 float32: 42 us for four.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -229,10 +237,10 @@ __device__ __forceinline__ void add_tile(const JvSxLoss& a, typename Core::acc_t
     }
 }
 
-// the piece's row that is query `q`'s target, far away if there is none
+// the piece's row that is query `q`'s target, -1 if there is none
 __device__ __forceinline__ int wanted(const JvSxLoss& a, int q) {
     const int64_t at = q < a.mm.M && a.targets ? a.targets[q] - a.row0 : -1;
-    return at >= 0 && at < a.mm.N ? (int)at : -0x40000000;
+    return at >= 0 && at < a.mm.N ? (int)at : -1;
 }
 
 // joins what the lanes and waves of a workgroup hold of the same queries and writes one partial for each of the panel's queries
@@ -347,7 +355,7 @@ extern "C" int jvk_sx_loss_splits(int path, int nq, int64_t rows, int d) {
 
 template <class T, int WM, int WN>
 static hipError_t loss_tile(const JvSxLoss& a, hipStream_t s) {
-    hipError_t e = lds_of(jvs_loss_tile_kernel<T, WM, WN>, T::LDS);
+    hipError_t e = lds_of<jvs_loss_tile_kernel<T, WM, WN>>(T::LDS);
     if (e != hipSuccess) return e;
     const int64_t all = (int64_t)((a.mm.M + T::TM - 1) / T::TM) * a.splits;
     if (all > 0x7ffffff0ll) return hipErrorInvalidValue;
@@ -372,7 +380,7 @@ extern "C" hipError_t jvk_sx_loss(const JvSxLoss* a, hipStream_t s) {
         if (t.m == 64) return loss_tile<Tile<BF16, 2, 1, 1, 4, 2>, 1, 4>(*a, s);
         return t.few ? loss_tile<Tile<BF16, 1, 1, 1, 4, 4>, 1, 4>(*a, s) : loss_tile<Tile<BF16, 1, 1, 1, 4, 2>, 1, 4>(*a, s);
     }
-    hipError_t e = lds_of(jvs_loss_pipe_kernel, P::LDS);
+    hipError_t e = lds_of<jvs_loss_pipe_kernel>(P::LDS);
     if (e != hipSuccess) return e;
     const int64_t all = (int64_t)((a->mm.M + P::TM - 1) / P::TM) * a->splits;
     if (all > 0x7ffffff0ll) return hipErrorInvalidValue;
@@ -535,7 +543,7 @@ static hipError_t weights_tile(const JvSxWeights& a, hipStream_t s) {
     const int64_t all = (int64_t)((padded_queries(a) + T::TM - 1) / T::TM) * ((a.kv + T::TN - 1) / T::TN);
     const int64_t extra = a.clean ? ((int64_t)a.mm.M * a.mm.k + CLEANED - 1) / CLEANED : 0;
     if (all + extra > 0x7fffffffll || extra * CLEANED > 0x7fffffffll) return hipErrorInvalidValue;
-    hipError_t e = lds_of(jvs_weights_tile_kernel<T>, T::LDS);
+    hipError_t e = lds_of<jvs_weights_tile_kernel<T>>(T::LDS);
     if (e != hipSuccess) return e;
     jvs_weights_tile_kernel<T><<<(unsigned)(all + extra), T::THREADS, T::LDS, s>>>(a);
     return hipGetLastError();
@@ -558,7 +566,7 @@ extern "C" hipError_t jvk_sx_weights(const JvSxWeights* a, hipStream_t s) {
     }
     const int64_t all = (int64_t)((a->mm.M + P::TM - 1) / P::TM) * ((a->mm.N + P::TN - 1) / P::TN);
     if (all > 0x7fffffffll) return hipErrorInvalidValue;
-    hipError_t e = lds_of(jvs_weights_kernel, P::LDS);
+    hipError_t e = lds_of<jvs_weights_kernel>(P::LDS);
     if (e != hipSuccess) return e;
     jvs_weights_kernel<<<(unsigned)(all < 256 ? (all + 7) / 8 * 8 : 256), P::THREADS, P::LDS, s>>>(*a);
     return hipGetLastError();
@@ -577,7 +585,7 @@ static hipError_t grads_tile(const JvMmOut* q, const JvMmOut* v, hipStream_t s) 
     const int64_t nq = q ? tile_count(*q, TQ::TM, TQ::TN, TQ::steps(q->mm)) : 0, nv = v ? tile_count(*v, TV::TM, TV::TN, TV::steps(v->mm)) : 0;
     if (nq < 0 || nv < 0 || nq + nv > 0x7fffffffll) return hipErrorInvalidValue;
     if (nq + nv == 0) return hipSuccess;
-    hipError_t e = lds_of(jvs_grads_tile_kernel<TQ, TV>, TQ::LDS);
+    hipError_t e = lds_of<jvs_grads_tile_kernel<TQ, TV>>(TQ::LDS);
     if (e != hipSuccess) return e;
     jvs_grads_tile_kernel<TQ, TV><<<(unsigned)(nq + nv), 256, TQ::LDS, s>>>(q ? *q : JvMmOut{}, v ? *v : JvMmOut{}, (int)nq);
     return hipGetLastError();

@@ -1,8 +1,6 @@
 // jv_mm_out.h — matrix products written as they are, on the tiles of jv_mm.h (small) and jv_pipe.h (large).
 #pragma once
-#include <mutex>
-#include <set>
-#include <utility>
+#include <atomic>
 
 #include "jv_pipe.h"
 #include "jv_tile3.h"
@@ -20,17 +18,15 @@ __device__ __forceinline__ void band_order(int L, int tm, int tn, int& m, int& n
 }
 
 // Lets a kernel have that much LDS, once for each device (a second thread that gets here meanwhile does the same again).
-template <class... Args>
-static hipError_t lds_of(void (*kernel)(Args...), int bytes) {
-    static std::mutex lock;
-    static std::set<std::pair<const void*, int>> known;
+template <auto KERNEL>
+static hipError_t lds_of(int bytes) {
+    static std::atomic<uint64_t> done[4];   // a bit for each device
     int device = 0;
     hipError_t e = hipGetDevice(&device);
     if (e != hipSuccess) return e;
-    std::lock_guard<std::mutex> hold(lock);
-    if (known.count({(const void*)kernel, device})) return hipSuccess;
-    e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e == hipSuccess) known.insert({(const void*)kernel, device});
+    if (device < 256 && (done[device >> 6].load(std::memory_order_relaxed) >> (device & 63) & 1)) return hipSuccess;
+    e = hipFuncSetAttribute((const void*)KERNEL, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == hipSuccess && device < 256) done[device >> 6].fetch_or(1ull << (device & 63), std::memory_order_relaxed);
     return e;
 }
 
@@ -67,7 +63,7 @@ static hipError_t mm_out_pipe(const JvMmOut& a, hipStream_t s) {
     if (a.mm.M <= 0 || a.mm.N <= 0) return hipSuccess;
     const int64_t all = (int64_t)((a.mm.M + P::TM - 1) / P::TM) * ((a.mm.N + P::TN - 1) / P::TN) * a.splits;
     if (all > 0x7fffffffll || a.splits < 1 || a.splits > a.mm.kph || !aligned_rows(a)) return hipErrorInvalidValue;
-    hipError_t e = lds_of(jvm_out_pipe_kernel<TY, TA, TB>, P::LDS);
+    hipError_t e = lds_of<jvm_out_pipe_kernel<TY, TA, TB>>(P::LDS);
     if (e != hipSuccess) return e;
     jvm_out_pipe_kernel<TY, TA, TB><<<(unsigned)(all < 256 ? (all + 7) / 8 * 8 : 256), P::THREADS, P::LDS, s>>>(a);
     return hipGetLastError();
@@ -192,7 +188,7 @@ template <class T>
 static hipError_t mm_out_tile(const JvMmOut& a, hipStream_t s) {
     const int64_t all = tile_count(a, T::TM, T::TN, T::steps(a.mm));
     if (all <= 0) return all ? hipErrorInvalidValue : hipSuccess;
-    hipError_t e = lds_of(jvm_out_tile_kernel<T>, T::LDS);
+    hipError_t e = lds_of<jvm_out_tile_kernel<T>>(T::LDS);
     if (e != hipSuccess) return e;
     jvm_out_tile_kernel<T><<<(unsigned)all, T::THREADS, T::LDS, s>>>(a);
     return hipGetLastError();
