@@ -452,3 +452,56 @@ def test_softmax_on_the_large_tiles(torch, ops, dtype, nq, n, d, pad):
     for got, a, of, b, k in ((dq, g, p, v.double(), n), (dv, g.t(), p.t(), q.double(), nq)):
         want, reach = a @ b, a.abs() @ b.abs()
         assert ((got.double() - want).abs() <= (r + 6 * k * 2.0 ** -23) * reach + 4 * de * (of @ b.abs()) + 2 * ref.half_step(dtype) * want.abs() + 1e-30).all()
+
+
+# ------------------------------------------------------------------------------------------------ offsets that pass 32 bits
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_rows_that_lie_far_apart(torch, ops, dtype):
+    """70 000 components from row to row, 4.9 G in all: the same bits as with the rows side by side."""
+    q, v, t, w, *_ = loss_case(torch, 33, 70001, 24, dtype)
+    wide = torch.empty(70001 * 70000, dtype=v.dtype, device="cuda")
+    far = wide.view(70001, 70000)[:, 69976:]
+    far.copy_(v)
+    want, got = step(torch, ops, q, v, t, w), step(torch, ops, q, far, t, w)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_a_gradient_of_more_than_4_gib(torch, ops):
+    n, d = 1200001, 1000
+    g = torch.Generator(device="cuda").manual_seed(5)
+    v = torch.randn((n, d), generator=g, device="cuda") / 32
+    q, t = v[[3, n - 2, n // 2]] * 1.0, torch.tensor([3, n - 2, 9], dtype=torch.int32, device="cuda")
+    loss, lse = ops.softmax_loss(q, v, t, 10.0)
+    _, dv = ops.softmax_loss_grad(q, v, t, 10.0, lse, queries_grad=False)
+    total = torch.zeros(3, dtype=torch.float64, device="cuda")
+    for at in range(0, n, 100000):
+        total += torch.exp(10.0 * (q.double() @ v[at:at + 100000].double().t())).sum(1)   # (|z| stays below 20)
+    de = (6 * d + 2) * 2.0 ** -23 * 12 + n * 2.0 ** -24   # a logit's sum (its reach: below 12), the sum of n exponentials
+    assert (lse - total.log()).abs().max().item() <= de
+    for rows in (slice(0, 1000), slice(n // 2 - 500, n // 2 + 500), slice(n - 1000, n)):
+        p = torch.exp(10.0 * (q.double() @ v[rows].double().t()) - total.log()[:, None])
+        part = p.clone()
+        for i in range(3):
+            if rows.start <= int(t[i]) < rows.stop:
+                part[i, int(t[i]) - rows.start] -= 1
+        want = 10.0 * part.t() @ q.double()
+        off = 10.0 * (4 * de * p.t() + 2.0 ** -20 * part.abs().t()) @ q.double().abs() + 2.0 ** -23 * want.abs()
+        assert ((dv[rows].double() - want).abs() <= off + 1e-30).all()
+
+
+def test_codes_and_scores_of_more_than_4_gib(torch, ops):
+    n, d = 4500001, 1000
+    g = torch.Generator(device="cuda").manual_seed(6)
+    v = torch.empty((n, d), dtype=torch.bfloat16, device="cuda")
+    for at in range(0, n, 500000):
+        v[at:at + 500000] = torch.randn((min(500000, n - at), d), generator=g, device="cuda")
+    codes, scales = ops.encode_blocks(v)
+    tail = slice(n - 1000, n)
+    some, some_scales = ops.encode_blocks(v[tail].clone())
+    assert torch.equal(codes[tail], some) and torch.equal(scales[tail], some_scales)
+    assert torch.equal(ops.decode_blocks(codes, scales, d, torch.bfloat16)[tail], ops.decode_blocks(some, some_scales, d, torch.bfloat16))
+    del v
+    nq = 600   # 2.7 G scores
+    got = ops.score_blocks(codes[:nq].contiguous(), scales[:nq].contiguous(), codes, scales, d)
+    a, b = ops.decode_blocks(codes[:nq].contiguous(), scales[:nq].contiguous(), d).double(), ops.decode_blocks(some, some_scales, d).double()
+    assert ((got[:, tail].double() - a @ b.t()).abs() <= (d + 2) * 2.0 ** -23 * (a.abs() @ b.abs().t())).all()
