@@ -345,10 +345,23 @@ static Shape shape_of(int path, int nq, int64_t rows, int d) {
     return {nq <= 64 ? 64 : 128, 128, false};
 }
 
-// one for each CU with the large tiles, two or three with the small ones
+// Workgroups that share a panel of 256 queries: as many as make up whole rounds of the 256 CUs, each of them walking as many of the tiles and
+// costing about one more to begin.
+static int large_splits(int nq, int64_t rows) {
+    const int64_t panels = std::max((nq + 255) / 256, 1), tiles = std::max<int64_t>((rows + 255) / 256, 1);
+    int64_t best = 1, least = INT64_MAX;
+    for (int rounds = 1; rounds <= 8; rounds++) {
+        const int64_t s = std::min(std::max<int64_t>(256 * rounds / panels, 1), tiles), cost = (panels * s + 255) / 256 * ((tiles + s - 1) / s + 1);
+        if (cost < least) best = s, least = cost;
+    }
+    return (int)best;
+}
+
+// (two or three workgroups a CU with the small tiles)
 extern "C" int jvk_sx_loss_splits(int path, int nq, int64_t rows, int d) {
     const Shape t = shape_of(path, nq, rows, d);
-    const int full = t.m == 256 || t.n == 32 ? 256 : t.m == 128 || t.n == 64 || path == JV_SX_PLANES ? 512 : 768;
+    if (path == JV_SX_LARGE) return large_splits(nq, rows);
+    const int full = t.n == 32 ? 256 : t.m == 128 || t.n == 64 || path == JV_SX_PLANES ? 512 : 768;
     const int64_t panels = std::max((nq + t.m - 1) / t.m, 1), tiles = std::max<int64_t>((rows + t.n - 1) / t.n, 1);
     return (int)std::min(std::max<int64_t>(full / panels, 1), tiles);
 }
@@ -442,30 +455,39 @@ __device__ __forceinline__ void weigh(typename Core::acc_t (&acc)[NT], const JvS
     }
 }
 
-__global__ __launch_bounds__(512) void jvs_weights_kernel(const JvSxWeights a) {
+// One panel of queries and every `splits`-th tile of rows a workgroup, as in the forward pass: what it needs of its queries stays in registers
+// (loaded behind each tile, it would wait for the copies under way: adapter 256 x 400 000 x 128, 231 -> 215 us; step 4096 x 131 072 x 1024, 4.22 -> 4.14 ms).
+__global__ __launch_bounds__(512) void jvs_weights_kernel(const JvSxWeights a, int splits) {
     using P = Pipe<BF16>;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    const int tm = (a.mm.M + P::TM - 1) / P::TM, tn = (a.mm.N + P::TN - 1) / P::TN;
-    const Share share(tm * tn);
-    if (!share.mine()) return;
+    const int panels = (a.mm.M + P::TM - 1) / P::TM, tiles = (a.mm.N + P::TN - 1) / P::TN;
+    const Share share(panels * splits);
+    int L;
+    if (!share.at(0, L)) return;
+    const int split = L / panels, m0 = (L - split * panels) * P::TM;
     const int padded = (a.mm.M + 63) / 64 * 64;
+    JvSxQuery q[4];
+    int at[4];
+#pragma unroll
+    for (int m = 0; m < 4; m++) {
+        const int r = m0 + P::row(m);
+        q[m] = {__builtin_inff(), 0.0f, -1, 0};
+        if (r < a.mm.M) q[m] = a.query[r];
+        const int64_t t = q[m].target - a.row0;
+        at[m] = q[m].target >= 0 && t >= 0 && t < a.mm.N ? (int)t : -1;
+    }
+    if (split >= tiles) return;
     P::run(
         a.mm, smem,
         [&](int i, Work& w) {
-            int L, m, n;
-            if (!share.at(i, L)) return false;
-            band_order(L, tm, tn, m, n);
-            w.m0 = m * P::TM, w.n0 = n * P::TN, w.k0 = 0, w.k1 = a.mm.kph;
+            const int t = split + i * splits;
+            if (t >= tiles) return false;
+            w.m0 = m0, w.n0 = t * P::TN, w.k0 = 0, w.k1 = a.mm.kph;
             return true;
         },
         [&](const Work& w, f32x16 (&acc)[4][2]) -> int {
 #pragma unroll
-            for (int m = 0; m < 4; m++) {
-                const int r = w.m0 + P::row(m);
-                JvSxQuery q = {__builtin_inff(), 0.0f, -1, 0};
-                if (r < a.mm.M) q = a.query[r];
-                weigh<P>(acc[m], q, a.c, a.mm.N - w.n0, q.target >= 0 ? (int)(q.target - a.row0) - w.n0 : -1, true, a.rest + r);
-            }
+            for (int m = 0; m < 4; m++) weigh<P>(acc[m], q[m], a.c, a.mm.N - w.n0, at[m] - w.n0, true, a.rest + w.m0 + P::row(m));
             return P::write_bf16(smem, (uint16_t*)a.g, a.kv, w, padded, a.kv, [&](int m, int n, int e) { return acc[m][n][e]; });
         });
 }
@@ -564,11 +586,12 @@ extern "C" hipError_t jvk_sx_weights(const JvSxWeights* a, hipStream_t s) {
         if (t.few) return weights_tile<Tile<BF16, 1, 1, 2, 2, 4>>(*a, s);
         return t.m == 128 ? weights_tile<Tile<BF16, 2, 2, 2, 2, 2>>(*a, s) : weights_tile<Tile<BF16, 2, 1, 1, 4, 2>>(*a, s);
     }
-    const int64_t all = (int64_t)((a->mm.M + P::TM - 1) / P::TM) * ((a->mm.N + P::TN - 1) / P::TN);
-    if (all > 0x7fffffffll) return hipErrorInvalidValue;
+    const int splits = large_splits(a->mm.M, a->mm.N);
+    const int64_t all = (int64_t)((a->mm.M + P::TM - 1) / P::TM) * splits;
+    if (all > 0x7ffffff0ll) return hipErrorInvalidValue;
     hipError_t e = lds_of<jvs_weights_kernel>(P::LDS);
     if (e != hipSuccess) return e;
-    jvs_weights_kernel<<<(unsigned)(all < 256 ? (all + 7) / 8 * 8 : 256), P::THREADS, P::LDS, s>>>(*a);
+    jvs_weights_kernel<<<(unsigned)((all + 7) / 8 * 8), P::THREADS, P::LDS, s>>>(*a, splits);
     return hipGetLastError();
 }
 
