@@ -329,15 +329,18 @@ extern "C" int jvk_sx_path(int nq, int64_t rows, int f32) {
 // Queries and rows of the smaller tiles: 32 x 128 and 64 x 128 (float32 also 96 x 128) for up to so many queries, the rows being streamed and as
 // little as possible multiplied for nothing; 128 x 128 otherwise; but where that is no more than one tile a CU 64 x 64, with four steps of k
 // under way: the way to memory and the multiplications of one tile's steps are what counts then (float32, 118 x 18 x 843: 66 -> 36 us).
-// float32 with no more than a tile of 32 x 32 a CU and at least eight steps of k: those, four waves sharing a tile's steps (a step of 28 x 46 x 1167:
-// 90 -> 43 us, of 100 x 2000 x 768: 80 -> 49; bf16, a fifth of the instructions a step: 54 and 54).
+// float32 with no more than four tiles of 32 x 32 a CU and at least eight steps of k: those, four waves sharing a tile's steps, two steps of
+// each wave under way where there is more than one tile a CU and four otherwise (a step of 28 x 46 x 1167: 90 -> 43 us, of 100 x 2000 x 768: 80 -> 49;
+// a loss of 256 x 2000 x 768: 32 -> 20, of 16 x 30 000 x 768: 34 -> 29; of 512 x 4000 x 768, eight tiles a CU: 43 and 47; bf16, a fifth of the
+// instructions a step: 54 and 54).
 struct Shape {
     int m, n;
     bool few;
 };
+static int64_t tiles32(int nq, int64_t rows) { return (int64_t)((nq + 31) / 32) * ((rows + 31) / 32); }
 static Shape shape_of(int path, int nq, int64_t rows, int d) {
     if (path == JV_SX_LARGE) return {256, 256, false};
-    if (path == JV_SX_RAW && d > 7 * 32 && (int64_t)((nq + 31) / 32) * ((rows + 31) / 32) <= 256) return {32, 32, true};
+    if (path == JV_SX_RAW && d > 7 * 32 && tiles32(nq, rows) <= 1024) return {32, 32, true};
     const bool few = (int64_t)((nq + 127) / 128) * ((rows + 127) / 128) <= 256;
     if (path == JV_SX_PLANES) return {nq > 96 ? 128 : (nq + 31) / 32 * 32, 128, false};
     if (nq <= 32) return {32, 128, few};
@@ -361,7 +364,7 @@ static int large_splits(int nq, int64_t rows) {
 extern "C" int jvk_sx_loss_splits(int path, int nq, int64_t rows, int d) {
     const Shape t = shape_of(path, nq, rows, d);
     if (path == JV_SX_LARGE) return large_splits(nq, rows);
-    const int full = t.n == 32 ? 256 : t.m == 128 || t.n == 64 || path == JV_SX_PLANES ? 512 : 768;
+    const int full = t.n == 32 ? 512 : t.m == 128 || t.n == 64 || path == JV_SX_PLANES ? 512 : 768;
     const int64_t panels = std::max((nq + t.m - 1) / t.m, 1), tiles = std::max<int64_t>((rows + t.n - 1) / t.n, 1);
     return (int)std::min(std::max<int64_t>(full / panels, 1), tiles);
 }
@@ -380,7 +383,7 @@ extern "C" hipError_t jvk_sx_loss(const JvSxLoss* a, hipStream_t s) {
     if (a->mm.N <= 0 || a->mm.M <= 0) return hipSuccess;
     if (a->splits < 1) return hipErrorInvalidValue;
     const Shape t = shape_of(a->path, a->mm.M, a->mm.N, a->mm.k);
-    if (t.n == 32) return loss_tile<KSplit<Tile32<1, 1, 1, 1, 4, false, false, true>>, 1, 4>(*a, s);
+    if (t.n == 32) return tiles32(a->mm.M, a->mm.N) <= 256 ? loss_tile<KSplit<Tile32<1, 1, 1, 1, 4, false, false, true>>, 1, 4>(*a, s) : loss_tile<KSplit<Tile32<1, 1, 1, 1, 2, false, false, true>>, 1, 4>(*a, s);
     if (a->path == JV_SX_RAW) return t.m == 32 ? loss_tile<Tile32<1, 1, 1, 4, 4, false, false>, 1, 4>(*a, s) : loss_tile<Tile32<1, 1, 2, 2, 4, false, false>, 2, 2>(*a, s);
     if (a->path == JV_SX_PLANES) {
         if (t.m == 32) return loss_tile<Tile3<1, false, false>, 1, 4>(*a, s);
@@ -551,9 +554,9 @@ __global__ __launch_bounds__(T::THREADS, T::RESIDENT) void jvs_weights_tile_kern
         } else {
             const Turn<T> turn(smem, m, acc[m]);
 #pragma unroll
-            for (int i = 0; i < Turn<T>::WIDE_STORES; i++) {
+            for (int i = 0; i < Turn<T>::COLS / 8; i++) {
                 int tr, tc;
-                const f32x4 v = turn.four(i, tr, tc);
+                const f32x4 v = turn.template get<f32x4>(i, tr, tc);
                 put(m0 + tr, n0 + tc, v);
             }
         }
@@ -575,7 +578,7 @@ extern "C" hipError_t jvk_sx_weights(const JvSxWeights* a, hipStream_t s) {
     using P = Pipe<BF16>;
     if (a->mm.M <= 0 || a->mm.N <= 0) return hipSuccess;
     const Shape t = shape_of(a->path, a->mm.M, a->mm.N, a->mm.k);
-    if (t.n == 32) return weights_tile<KSplit<Tile32<1, 1, 1, 1, 4, false, false, true>>>(*a, s);
+    if (t.n == 32) return tiles32(a->mm.M, a->mm.N) <= 256 ? weights_tile<KSplit<Tile32<1, 1, 1, 1, 4, false, false, true>>>(*a, s) : weights_tile<KSplit<Tile32<1, 1, 1, 1, 2, false, false, true>>>(*a, s);
     if (a->path == JV_SX_RAW) return weights_tile<Tile32<1, 1, 2, 2, 4, false, false>>(*a, s);
     if (a->path == JV_SX_PLANES) {
         if (t.m == 32) return weights_tile<Tile3<1, false, false>>(*a, s);
