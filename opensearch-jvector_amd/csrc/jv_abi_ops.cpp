@@ -80,7 +80,7 @@ struct Plan {
     int P, dp, kq, gq;                // planes; d and nq padded to 64; rows of g (the large tiles write whole steps, the small ones one row behind the queries)
     int64_t rows_f, rows_b;           // rows of one piece, forward (where the vectors have to be laid out) / backward
     int path_f, path_b, splits_f, splits_q, splits_v;   // forward, backward
-    int64_t off_q, off_clean, off_v, off_part, off_hit, off_query, off_norm, off_rest, off_g, off_slab, off_slab_v, bytes;
+    int64_t off_q, off_clean, off_v, off_part, off_hit, off_query, off_norm, off_tail, off_rest, off_g, off_slab, off_slab_v, bytes;
 };
 
 // MB of one piece's weights g: few large pieces, for every piece writes and reads dq's partial sums again and starts its tiles anew (step
@@ -125,6 +125,7 @@ Plan make_plan(int dtype, int nq, int64_t n, int d, uint32_t what) {
         p.off_v = take(std::min<int64_t>(p.rows_b, n) * row);
         p.off_query = take((int64_t)nq * sizeof(JvSxQuery));
         p.off_norm = take(4);
+        p.off_tail = take(16);
         p.off_rest = take((int64_t)nq * 4);
         p.off_g = take((int64_t)p.gq * p.P * p.rows_b * 2);
         if (what & JV_SOFTMAX_QUERY_GRAD) {
@@ -134,7 +135,7 @@ Plan make_plan(int dtype, int nq, int64_t n, int d, uint32_t what) {
         if (what & JV_SOFTMAX_VECTOR_GRAD) {
             const int64_t rows = std::min<int64_t>(p.rows_b, n);
             p.splits_v = jvk_sx_grad_splits(p.path_b, rows, d, nq, 1);
-            if (dtype == JV_DTYPE_F32) p.off_clean = take((int64_t)nq * std::max(d, 4) * 4);
+            p.off_clean = take(dtype == JV_DTYPE_F32 ? (int64_t)nq * std::max(d, 4) * 4 : d % 8 ? (int64_t)nq * p.dp * 2 : 0);
             p.off_slab_v = take(p.splits_v > 1 ? p.splits_v * rows * p.dp * 4 : 0);
         }
     }
@@ -143,7 +144,8 @@ Plan make_plan(int dtype, int nq, int64_t n, int d, uint32_t what) {
 }
 
 // Rows as a product takes them: the caller's own where they are
-//   bf16, 4-B aligned, with whole 16 B of components (the queries, whose padding stands for zeros behind the vectors', with whole steps of 64), or
+//   bf16, 4-B aligned, with an even number of components, eight at least (the queries, whose padding stands for zeros behind the vectors', with
+//   whole steps of 64), or
 //   float32 with at least four components, and the path takes them as they lie (JV_SX_RAW all of them, JV_SX_PLANES the vectors).
 struct Rows {
     const char* p;
@@ -151,11 +153,11 @@ struct Rows {
     bool ready;
     int kp;           // components of a row that is laid out instead
     bool raw;         // as float32, not as planes
-    int cols(int d) const { return ready || raw ? d : kp; }
+    int cols(int d) const { return raw ? d : ready ? (int)up(d, 8) : kp; }
 };
 Rows rows_of(const void* p, int64_t stride, const jv_softmax_params* q, const Plan& plan, int path, bool vectors) {
     Rows r{(const char*)p, stride * size_of(q->dtype), false, plan.dp, false};
-    if (q->dtype == JV_DTYPE_BF16) r.ready = (uintptr_t)p % 4 == 0 && stride % 2 == 0 && q->d % (vectors ? 8 : 64) == 0;
+    if (q->dtype == JV_DTYPE_BF16) r.ready = (uintptr_t)p % 4 == 0 && stride % 2 == 0 && (vectors ? q->d % 2 == 0 && q->d >= 8 : q->d % 64 == 0);
     else if (path == JV_SX_RAW || (path == JV_SX_PLANES && vectors)) r.ready = q->d >= 4, r.kp = 4, r.raw = true;
     return r;
 }
@@ -283,11 +285,13 @@ int jv_softmax_loss_device(const jv_softmax_params* p, float* d_out_loss, float*
         a.mm = logits(plan, p->nq, p->d);
         a.c = p->scale * 1.44269504088896341f;
         a.targets = p->targets, a.hit = (float*)(ws + plan.off_hit);
+        const bool shift = rv.ready && p->dtype == JV_DTYPE_BF16 && p->d % 8;   // (JvMm.end_b)
         if (rv.ready && p->dtype == JV_DTYPE_BF16) a.mm.end_b = p->d * 2;
         a.path = plan.path_f, a.splits = p->n > 0 ? plan.splits_f : 0, a.part = (float2*)(ws + plan.off_part);
         JvSxPrepare pre{};
         pre.dtype = p->dtype, pre.d = p->d;
         take_rows(rq, p->dtype, 0, p->nq, plan, ws + plan.off_q, &pre.m[0], &a.mm.a, &a.mm.lda);
+        pre.m[0].shift = shift;
         for (int64_t at = 0; at < p->n; at += step) {
             a.mm.N = (int)std::min<int64_t>(step, p->n - at);
             a.first = at == 0, a.row0 = at;
@@ -340,7 +344,8 @@ int jv_softmax_grad_device(const jv_softmax_params* p, const float* d_lse, const
         pre.lse = d_lse, pre.w = d_loss_grad, pre.nq = p->nq, pre.query = query, pre.norm = norm, pre.rest = w.rest;
     }
     const bool direct = raw && plan.splits_q == 1 && plan.rows_b >= p->n;   // dq is complete at once
-    // Queries without a target are laid out as zeros.  dv's product reads them so: bf16 as they are laid out, float32 as a copy.
+    // Queries without a target are laid out as zeros.  dv's product reads them so: bf16 as they are laid out (again if the end is shifted),
+    // float32 as a copy.
     const char* q_rows = ws + plan.off_clean;
     int64_t q_ld = (int64_t)p->d * 4;
     pre.targets = p->targets, pre.n = p->n;
@@ -348,7 +353,15 @@ int jv_softmax_grad_device(const jv_softmax_params* p, const float* d_lse, const
     Rows rb = rq;
     take_rows(rq, p->dtype, 0, p->nq, plan, ws + plan.off_q, &pre.m[0], &w.mm.a, &w.mm.lda);
     pre.m[0].clean = !rq.ready;
-    if (!rq.ready && (!f32 || rq.raw)) {
+    const bool shift = rv.ready && !f32 && p->d % 8;   // (JvMm.end_b)
+    if (shift) {
+        pre.m[0].shift = 1;
+        if (d_out_query_grad) pre.last = (const char*)p->vectors + (int64_t)(p->n - 1) * p->vector_stride * 2, pre.tail = ws + plan.off_tail;
+    }
+    if (shift && d_out_vector_grad) {
+        take_rows(rq, p->dtype, 0, p->nq, plan, ws + plan.off_clean, &pre.m[2], &q_rows, &q_ld);
+        pre.m[2].clean = 1;
+    } else if (!rq.ready && (!f32 || rq.raw)) {
         q_rows = w.mm.a, q_ld = w.mm.lda;
     } else if (d_out_vector_grad && plan.path_b == JV_SX_PLANES) {
         rb = rows_of(p->queries, p->query_stride, p, plan, JV_SX_RAW, false);
@@ -377,10 +390,12 @@ int jv_softmax_grad_device(const jv_softmax_params* p, const float* d_lse, const
         if (d_out_query_grad) {   // G times the piece's vectors: k = its rows
             o.mm.M = p->nq, o.mm.k = w.kv, o.mm.kph = w.kv / 32;
             o.mm.b = w.mm.b, o.mm.ldb = w.mm.ldb, o.mm.kb = rows, o.mm.cb = rv.cols(p->d);
+            o.mm.tail_b = shift && at + rows == p->n ? ws + plan.off_tail : nullptr;
             o.mul = 1.0f, o.out = ws + plan.off_slab, o.ldo = plan.dp, o.add = at > 0;
             o.splits = std::min(plan.splits_q, splits_of(plan, rows));   // (only the last piece can be that short: it adds to the first ranges)
             if (direct) o.mul = p->scale, o.out = d_out_query_grad, o.ldo = query_grad_stride;
             q = o;
+            o.mm.tail_b = nullptr;
         }
         if (d_out_vector_grad) {   // G across times the queries: k = the queries
             o.mm.M = rows, o.mm.k = (int)up(p->nq, 32), o.mm.kph = plan.kq / 32, o.mm.ka = p->nq % (f32 ? 32 : 64) ? p->nq + 1 : p->nq, o.mm.ca = w.kv;

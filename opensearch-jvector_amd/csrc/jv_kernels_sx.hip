@@ -78,7 +78,10 @@ __device__ __forceinline__ void pack(const JvSxPrepare& a, const JvSxPrepare::Ma
             __builtin_memcpy(x, row + at, sizeof(x));   // (no alignment is asked for)
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = at + e < d ? row[at + e] : (T)0.0f;
+            for (int e = 0; e < 8; e++) {
+                const int c = m.shift && at < d ? d - 8 + e : at + e;
+                x[e] = c >= at && c < d ? row[c] : (T)0.0f;
+            }
         }
         uint16_t p[3][8];
 #pragma unroll
@@ -130,6 +133,7 @@ __device__ __forceinline__ void queries(const JvSxPrepare& a, int part) {
     const float unit = a.w && top > 0.0f && top < __builtin_inff() ? top : 1.0f;
     const int i = part * 256 + threadIdx.x;
     if (i == 0) *a.norm = unit;
+    if (a.last && i < 8) ((__bf16*)a.tail)[i] = a.d / 8 * 8 + i < a.d ? ((const __bf16*)a.last)[a.d / 8 * 8 + i] : (__bf16)0.0f;
     if (i >= a.nq) return;
     JvSxQuery q = query_of(a.lse, a.w, a.targets, a.n, i);
     q.w /= unit;
@@ -635,7 +639,7 @@ extern "C" hipError_t jvk_sx_grads(const JvMmOut* q, const JvMmOut* v, int path,
     path = grads_path(path, q ? q->mm.N : v->mm.N);
     hipError_t e = hipSuccess;
     if (path == JV_SX_LARGE) {
-        if (q) e = mm_out_pipe<BF16, false, true>(*q, s);
+        if (q) e = q->mm.tail_b ? mm_out_pipe<BF16, false, true, true>(*q, s) : mm_out_pipe<BF16, false, true>(*q, s);
         if (v && e == hipSuccess) e = aligned_rows(*v) ? mm_out_pipe<BF16, true, true>(*v, s) : mm_out_tile<Tile<BF16, 2, 2, 2, 2, 2, true, true>>(*v, s);
         return e;
     }

@@ -101,6 +101,7 @@ struct Tile {
         const int lr = lane >> 3, lp = (lane & 7) ^ lr;
         const char* src[PER];   // k along rows: the row's piece; k across: the column's piece of row 0
         int krow[PER];          // k across: the row inside a step
+        bool ends[CB];          // k across: this piece is the last of B's row
 #pragma unroll
         for (int i = 0; i < CA; i++) {
             krow[i] = (i * WAVES + w) * (64 / GA) + lane / GA;   // (a row of TM columns is GA pieces)
@@ -111,7 +112,10 @@ struct Tile {
         for (int i = 0; i < CB; i++) {
             krow[CA + i] = (i * WAVES + w) * (64 / GB) + lane / GB;
             if constexpr (!TB) src[CA + i] = a.b + (int64_t)min(n0 + 8 * (i * WAVES + w) + lr, a.N - 1) * a.ldb + lp * 16;
-            else src[CA + i] = a.b + (int64_t)min(n0 + 8 * ((lane % GB) ^ (swirl<GB>(krow[CA + i]) << 2)), a.cb - 8) * 2;
+            else {
+                const int col = min(n0 + 8 * ((lane % GB) ^ (swirl<GB>(krow[CA + i]) << 2)), a.cb - 8);
+                src[CA + i] = a.b + (int64_t)col * 2, ends[i] = a.tail_b && col == a.cb - 8;
+            }
         }
         const int wm = w % WM, wn = w / WM, h = lane >> 5, r31 = lane & 31;
         int aoff[MT], boff[NT], ax, bx;
@@ -148,8 +152,12 @@ struct Tile {
             for (int i = 0; i < CA; i++)
                 glds16(src[i] + (TA ? (int64_t)min(kin * 64 + krow[i], a.ka - 1) * a.lda : off), dst + (i * WAVES + w) * (TA ? 1024 : GROUP));
 #pragma unroll
-            for (int i = 0; i < CB; i++)
-                glds16(src[CA + i] + (TB ? (int64_t)min(kin * 64 + krow[CA + i], a.kb - 1) * a.ldb : min(off, (int64_t)(a.end_b - 16 - lp * 16))), dst + GA * GROUP + (i * WAVES + w) * (TB ? 1024 : GROUP));
+            for (int i = 0; i < CB; i++) {
+                const int k = kin * 64 + krow[CA + i];
+                const char* p = src[CA + i] + (TB ? (int64_t)min(k, a.kb - 1) * a.ldb : min(off, (int64_t)(a.end_b - 16 - lp * 16)));
+                if (TB && ends[i] && k >= a.kb - 1) p = a.tail_b;
+                glds16(p, dst + GA * GROUP + (i * WAVES + w) * (TB ? 1024 : GROUP));
+            }
             kin++;
         };
 #pragma unroll

@@ -34,9 +34,9 @@ static hipError_t lds_of(int bytes) {
     return e;
 }
 
-template <int TY, bool TA, bool TB>
+template <int TY, bool TA, bool TB, bool ENDS>
 __global__ __launch_bounds__(512) void jvm_out_pipe_kernel(const JvMmOut a) {
-    using P = Pipe<TY, TA, TB>;
+    using P = Pipe<TY, TA, TB, ENDS>;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int tm = (a.mm.M + P::TM - 1) / P::TM, tn = (a.mm.N + P::TN - 1) / P::TN, tiles = tm * tn;
     const Share share(tiles * a.splits);
@@ -61,15 +61,15 @@ __global__ __launch_bounds__(512) void jvm_out_pipe_kernel(const JvMmOut a) {
     });
 }
 
-template <int TY, bool TA = false, bool TB = false>
+template <int TY, bool TA = false, bool TB = false, bool ENDS = false>
 static hipError_t mm_out_pipe(const JvMmOut& a, hipStream_t s) {
-    using P = Pipe<TY, TA, TB>;
+    using P = Pipe<TY, TA, TB, ENDS>;
     if (a.mm.M <= 0 || a.mm.N <= 0) return hipSuccess;
     const int64_t all = (int64_t)((a.mm.M + P::TM - 1) / P::TM) * ((a.mm.N + P::TN - 1) / P::TN) * a.splits;
     if (all > 0x7fffffffll || a.splits < 1 || a.splits > a.mm.kph || !aligned_rows(a)) return hipErrorInvalidValue;
-    hipError_t e = lds_of<jvm_out_pipe_kernel<TY, TA, TB>>(P::LDS);
+    hipError_t e = lds_of<jvm_out_pipe_kernel<TY, TA, TB, ENDS>>(P::LDS);
     if (e != hipSuccess) return e;
-    jvm_out_pipe_kernel<TY, TA, TB><<<(unsigned)(all < 256 ? (all + 7) / 8 * 8 : 256), P::THREADS, P::LDS, s>>>(a);
+    jvm_out_pipe_kernel<TY, TA, TB, ENDS><<<(unsigned)(all < 256 ? (all + 7) / 8 * 8 : 256), P::THREADS, P::LDS, s>>>(a);
     return hipGetLastError();
 }
 

@@ -15,7 +15,9 @@ struct JvMm {
     int32_t kph;             // phases (bf16, e4m3)
     int64_t plane_a;         // float32 as bf16 planes: bytes from plane to plane
     int32_t ka, kb, ca, cb;  // operands with k across their rows
-    int32_t end_b;           // bytes of k that a row of B has, a multiple of 16 (bf16, k along its rows): what lies behind reads as the last 16, A holds zeros there
+    int32_t end_b;           // bytes of k that a row of B has, 16 at least (bf16, k along its rows): the 16 B that would pass its end, and those behind,
+                             // are read from 16 B before it instead, and A holds the 16 B that pass its end in that order, zeros for what was there already
+    const char* tail_b;      // bf16, k across B's rows: 16 B that stand for the last 16 B of columns of B's last row, which may pass the matrix's end
     const uint8_t *sa, *sb;  // e4m3: scale bytes [M][kph / 2] / [N][kph / 2]
 };
 
@@ -87,6 +89,7 @@ struct JvSxPrepare {
         int32_t kp;
         int32_t raw;            // float32 rows [rows][kp] as they are
         int32_t clean;          // rows without a target become zeros
+        int32_t shift;          // bf16: the last components as JvMm.end_b wants them of A
     } m[3];
     int32_t dtype, d;
     const int32_t* targets;     // of the queries, for n rows
@@ -96,6 +99,8 @@ struct JvSxPrepare {
     int32_t nq;
     JvSxQuery* query;
     float *norm, *rest;
+    const void* last;       // bf16: the last row, whose last components (a multiple of 8 of them in front) become `tail`; nullptr = none
+    void* tail;
 };
 
 // sets jv_last_error() and returns `code` (jv_abi.cpp)

@@ -26,7 +26,8 @@ struct Work {
     int part;        // which k range
 };
 
-template <int TY, bool TA = false, bool TB = false>
+// ENDS: JvMm.tail_b is there (looking for it costs 1 % otherwise).
+template <int TY, bool TA = false, bool TB = false, bool ENDS = false>
 struct Pipe {
     using acc_t = f32x16;
     static constexpr bool RAW = false;
@@ -35,6 +36,7 @@ struct Pipe {
     static constexpr int REGION = 32768, SCALES = 4 * REGION, SCRATCH = SCALES + (TY == BF16 ? 0 : 2 * 8192);
     static constexpr int LDS = SCRATCH + 4 * 4096;   // 4 KB for waves w and w + 4: they are never in their epilogue at the same time
     static_assert(TY == BF16 || (!TA && !TB), "8-bit operands have k along their rows");
+    static_assert(TB || !ENDS);
 
     template <int N>
     static __device__ __forceinline__ void wait_copies() {
@@ -70,6 +72,7 @@ struct Pipe {
         work(0, sw);
         int si = 0, sk = sw.k0, sreg = 0;
         const char *pa[2], *pb[2];   // k along rows: the row's piece; k across: the column's piece of row 0
+        bool ends = false;           // k across: this piece is the last of B's row
         auto rows = [&]() {
 #pragma unroll
             for (int i = 0; i < 2; i++) {
@@ -77,7 +80,10 @@ struct Pipe {
                 if constexpr (!TA) pa[i] = a.a + (int64_t)min(sw.m0 + 16 * (i * 8 + w) + (lane >> 2), a.M - 1) * a.lda + ((lane & 3) ^ ((lane >> 4) & 3)) * 16;
                 else pa[i] = a.a + (int64_t)min(sw.m0 + 8 * ((lane & 31) ^ (((2 * w + (lane >> 5)) & 3) << 2)), a.ca - 8) * 2;
                 if constexpr (!TB) pb[i] = a.b + (int64_t)min(sw.n0 + 16 * (i * 8 + w) + (lane >> 2), a.N - 1) * a.ldb + ((lane & 3) ^ ((lane >> 4) & 3)) * 16;
-                else pb[i] = a.b + (int64_t)min(sw.n0 + 8 * ((lane & 31) ^ (((2 * w + (lane >> 5)) & 3) << 2)), a.cb - 8) * 2;
+                else {
+                    const int col = min(sw.n0 + 8 * ((lane & 31) ^ (((2 * w + (lane >> 5)) & 3) << 2)), a.cb - 8);
+                    pb[i] = a.b + (int64_t)col * 2, ends = ENDS && col == a.cb - 8;
+                }
             }
         };
         rows();
@@ -89,7 +95,9 @@ struct Pipe {
             for (int i = 0; i < 2; i++) {
                 const int k = sk * 32 + 16 * i + 2 * w + (lane >> 5);
                 glds16(pa[i] + (TA ? (int64_t)min(k, a.ka - 1) * a.lda : off), dst + i * 8192);
-                glds16(pb[i] + (TB ? (int64_t)min(k, a.kb - 1) * a.ldb : min(off, end_b)), dst + 16384 + i * 8192);
+                const char* p = pb[i] + (TB ? (int64_t)min(k, a.kb - 1) * a.ldb : min(off, end_b));
+                if (ENDS && ends && k >= a.kb - 1) p = a.tail_b;
+                glds16(p, dst + 16384 + i * 8192);
             }
             sreg = (sreg + 1) & 3;
             if (++sk == sw.k1) {   // on to the next tile (behind the last: the same one again, never read)
