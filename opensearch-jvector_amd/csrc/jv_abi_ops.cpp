@@ -300,7 +300,7 @@ int jv_softmax_loss_device(const jv_softmax_params* p, float* d_out_loss, float*
             pre.m[0].rows = 0;
             CHK(jvk_sx_loss(&a, s));
         }
-        CHK(jvk_sx_join(a.part, a.splits, p->nq, a.hit, p->targets, p->n, d_out_loss, d_out_lse, s));
+        CHK(jvk_sx_join(a.part, a.splits, p->nq, a.c, a.hit, p->targets, p->n, d_out_loss, d_out_lse, s));
     }
     return done(hip_stream);
 }

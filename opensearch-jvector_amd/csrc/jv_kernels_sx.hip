@@ -107,8 +107,11 @@ __device__ __forceinline__ void pack(const JvSxPrepare& a, const JvSxPrepare::Ma
 
 __device__ __forceinline__ JvSxQuery query_of(const float* lse, const float* w, const int32_t* targets, int64_t n, int i) {
     const int t = targets[i];
-    const bool has = known(t, n);
-    return {has ? lse[i] * 1.44269504088896341f : __builtin_inff(), has ? (w ? w[i] : 1.0f) : 0.0f, has ? t : -1, 0};
+    if (!known(t, n)) return {__builtin_inff(), 0.0f, -1, 0.0f};
+    const float w0 = w ? w[i] : 1.0f, lse2 = lse[i] * 1.44269504088896341f;
+    // lse log2(e) - lse2: what both roundings left out, up to 2^-19 for a logarithm of 40 and as much of p
+    const float lacks = fabsf(lse2) < __builtin_inff() ? fmaf(lse[i], 1.44269504088896341f, -lse2) + lse[i] * 1.92596299112661747e-8f : 0.0f;
+    return {lse2, w0 * exp2_(-lacks), t, w0};
 }
 
 // The weights are divided by the largest of them (`norm`, multiplied back in float32 at the end): an entry of g at a target is then just
@@ -136,7 +139,7 @@ __device__ __forceinline__ void queries(const JvSxPrepare& a, int part) {
     if (a.last && i < 8) ((__bf16*)a.tail)[i] = a.d / 8 * 8 + i < a.d ? ((const __bf16*)a.last)[a.d / 8 * 8 + i] : (__bf16)0.0f;
     if (i >= a.nq) return;
     JvSxQuery q = query_of(a.lse, a.w, a.targets, a.n, i);
-    q.w /= unit;
+    q.w /= unit, q.whole /= unit;
     a.query[i] = q;
     a.rest[i] = 0.0f;
 }
@@ -174,7 +177,7 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
 
 // A lane's part of a tile: MT queries, NT * 16 rows each.  `rows`: how many rows the tile has in all.  Four instructions a logit: the maximum, the
 // scaled difference (c <= 0: the smallest product is the largest logit), the exponential, the sum.
-// `m0`, `n0`: where the tile lies; the target's own logit is taken from the same product, so that a loss near 0 keeps its digits.
+// `m0`, `n0`: where the tile lies; the target's own product is the same one, so that a loss near 0 keeps its digits.
 template <class Core, int MT, int NT>
 __device__ __forceinline__ void add_tile(const JvSxLoss& a, typename Core::acc_t (&acc)[MT][NT], int m0, int n0, const int (&want)[MT], float (&top)[MT], float (&sum)[MT]) {
     const float c = a.c;
@@ -188,7 +191,7 @@ __device__ __forceinline__ void add_tile(const JvSxLoss& a, typename Core::acc_t
             for (int n = 0; n < NT; n++)
 #pragma unroll
                 for (int e = 0; e < Core::E; e++)
-                    if (Core::col(n, e) == at) a.hit[m0 + Core::row(m)] = acc[m][n][e] * c;
+                    if (Core::col(n, e) == at) a.hit[m0 + Core::row(m)] = acc[m][n][e];
         }
     }
     const float none = c < 0.0f ? __builtin_inff() : -__builtin_inff();   // (what is behind the last row: its logit is -inf)
@@ -408,8 +411,9 @@ extern "C" hipError_t jvk_sx_loss(const JvSxLoss* a, hipStream_t s) {
     return hipGetLastError();
 }
 
-// one wave a query: join the partials
-__global__ __launch_bounds__(256) void jvs_join_kernel(const float2* __restrict__ part, int splits, int nq, const float* __restrict__ hit,
+// One wave a query: join the partials.  The few operations behind the sums are in 64 bits: a logarithm of 40 has a float32 step of 4e-6, and a loss
+// near 0 is the difference of two such.
+__global__ __launch_bounds__(256) void jvs_join_kernel(const float2* __restrict__ part, int splits, int nq, float c, const float* __restrict__ hit,
                                                        const int32_t* __restrict__ targets, int64_t n, float* __restrict__ loss, float* __restrict__ lse) {
     const int i = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
     if (i >= nq) return;
@@ -421,14 +425,16 @@ __global__ __launch_bounds__(256) void jvs_join_kernel(const float2* __restrict_
     }
     for (int off = 32; off >= 1; off >>= 1) join(m, s, __shfl_xor(m, off, 64), __shfl_xor(s, off, 64));
     if (lane != 0) return;
-    const int t = targets ? targets[i] : -1;
-    lse[i] = (m + log2_(s)) * 0.69314718055994531f;
-    loss[i] = t >= 0 && t < n ? ((m - hit[i]) + log2_(s)) * 0.69314718055994531f : 0.0f;
+    constexpr double ln2 = 0.69314718055994530942;
+    const double all = (double)m * ln2 + log((double)s);
+    lse[i] = (float)all;
+    loss[i] = targets && known(targets[i], n) ? (float)(all - (c == 0.0f ? 0.0 : (double)hit[i] * c * ln2)) : 0.0f;
 }
 
-extern "C" hipError_t jvk_sx_join(const float2* part, int splits, int nq, const float* hit, const int32_t* targets, int64_t n, float* loss, float* lse, hipStream_t s) {
+extern "C" hipError_t jvk_sx_join(const float2* part, int splits, int nq, float c, const float* hit, const int32_t* targets, int64_t n, float* loss, float* lse,
+                                  hipStream_t s) {
     if (nq <= 0) return hipSuccess;
-    jvs_join_kernel<<<(nq + 3) / 4, 256, 0, s>>>(part, splits, nq, hit, targets, n, loss, lse);
+    jvs_join_kernel<<<(nq + 3) / 4, 256, 0, s>>>(part, splits, nq, c, hit, targets, n, loss, lse);
     return hipGetLastError();
 }
 
@@ -450,7 +456,7 @@ __device__ __forceinline__ void weigh(typename Core::acc_t (&acc)[NT], const JvS
 #pragma unroll
             for (int e = 0; e < Core::E; e++)
                 if (Core::col(n, e) == hit) {
-                    acc[n][e] -= q.w;
+                    acc[n][e] -= q.whole;
                     if (lossy) *rest = acc[n][e] - (float)(__bf16)acc[n][e];   // (one lane holds it; three planes lack nothing)
                 }
     }
@@ -478,7 +484,7 @@ __global__ __launch_bounds__(512) void jvs_weights_kernel(const JvSxWeights a, i
 #pragma unroll
     for (int m = 0; m < 4; m++) {
         const int r = m0 + P::row(m);
-        q[m] = {__builtin_inff(), 0.0f, -1, 0};
+        q[m] = {__builtin_inff(), 0.0f, -1, 0.0f};
         if (r < a.mm.M) q[m] = a.query[r];
         const int64_t t = q[m].target - a.row0;
         at[m] = q[m].target >= 0 && t >= 0 && t < a.mm.N ? (int)t : -1;
@@ -534,7 +540,7 @@ __global__ __launch_bounds__(T::THREADS, T::RESIDENT) void jvs_weights_tile_kern
 #pragma unroll
     for (int m = 0; m < MT; m++) {
         const int r = m0 + T::row(m);
-        JvSxQuery q = {__builtin_inff(), 0.0f, -1, 0};
+        JvSxQuery q = {__builtin_inff(), 0.0f, -1, 0.0f};
         if (r < a.mm.M) q = a.query ? a.query[r] : query_of(a.lse, a.w, a.targets, a.n, r);
         weigh<T>(acc[m], q, a.c, a.mm.N - n0, q.target >= 0 ? (int)(q.target - a.row0) - n0 : -1, a.path == JV_SX_TILES, a.rest + r);
         // (kv is a multiple of 64: four columns are in or out together)

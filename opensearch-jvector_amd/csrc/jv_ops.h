@@ -42,14 +42,14 @@ struct JvSxLoss {
     int32_t first;         // 0: partials of an earlier piece of the rows are in `part` already, join them
     const int32_t* targets;  // nullptr = none
     int64_t row0;          // first row of this piece
-    float* hit;            // [M] the target's logit (log2 domain), written by the piece that has it
+    float* hit;            // [M] the target's product, written by the piece that has it
 };
 // what the gradient needs of a query
 struct JvSxQuery {
     float lse2;            // base-2 logarithm
-    float w;               // weight / norm; 0 = the query takes no part
+    float w;               // weight / norm, times 2^-(what lse2 lacks of its value); 0 = the query takes no part
     int32_t target;        // row, -1 = none
-    int32_t pad;
+    float whole;           // weight / norm
 };
 // partial sums of a gradient, [splits][rows][lds], to be joined
 struct JvSxFinish {
@@ -122,7 +122,7 @@ enum JvSxPath {
 int jvk_sx_path(int nq, int64_t rows, int f32);
 int jvk_sx_loss_splits(int path, int nq, int64_t rows, int d);   // workgroups that share a panel of queries
 hipError_t jvk_sx_loss(const JvSxLoss* a, hipStream_t s);
-hipError_t jvk_sx_join(const float2* part, int splits, int nq, const float* hit, const int32_t* targets, int64_t n, float* loss, float* lse, hipStream_t s);
+hipError_t jvk_sx_join(const float2* part, int splits, int nq, float c, const float* hit, const int32_t* targets, int64_t n, float* loss, float* lse, hipStream_t s);
 hipError_t jvk_sx_weights(const JvSxWeights* a, hipStream_t s);
 // dq = G V and dv = G^T Q (nullptr: not asked for)
 int jvk_sx_grad_splits(int path, int64_t rows, int d, int64_t k, int across);
