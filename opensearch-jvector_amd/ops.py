@@ -32,39 +32,41 @@ def _workspace_bytes(dtype: int, nq: int, n: int, d: int, flags: int) -> int:
     return binding.softmax_workspace(binding.softmax_params(0, dtype, nq, n, d, 1.0), flags)   # (the shape alone decides)
 
 
-def _matrix(x: torch.Tensor, what: str):
+def _matrix(x: torch.Tensor, what: str, name: str):
     """(dtype, rows, components, row stride) of a matrix of vectors."""
     if x.dim() != 2 or not x.is_cuda:
-        raise ValueError(f"{what}: a 2-D tensor on a GPU is wanted, got shape {tuple(x.shape)} on {x.device}")
-    if x.dtype not in _DTYPES:
-        raise ValueError(f"{what}: float32 or bfloat16 is wanted, got {x.dtype}")
+        raise ValueError(f"{what}: {name}: a 2-D tensor on a GPU is wanted, got shape {tuple(x.shape)} on {x.device}")
+    dtype = _DTYPES.get(x.dtype)
+    if dtype is None:
+        raise ValueError(f"{what}: {name}: float32 or bfloat16 is wanted, got {x.dtype}")
     n, d = x.shape
-    if d > 1 and n > 0 and x.stride(1) != 1:
-        raise ValueError(f"{what}: the components of a row have to be contiguous, got strides {x.stride()}")
-    return _DTYPES[x.dtype], n, d, x.stride(0) if n > 1 else d
+    apart, step = x.stride()
+    if step != 1 and d > 1 and n > 0:
+        raise ValueError(f"{what}: {name}: the components of a row have to be contiguous, got strides {x.stride()}")
+    return dtype, n, d, apart if n > 1 else d
 
 
-def _like(x: torch.Tensor, to: torch.Tensor, shape, dtype, what: str) -> torch.Tensor:
-    if x.device != to.device or tuple(x.shape) != tuple(shape) or x.dtype != dtype or not x.is_contiguous():
-        raise ValueError(f"{what}: a contiguous {dtype} tensor of shape {tuple(shape)} on {to.device} is wanted, got {x.dtype} {tuple(x.shape)} on {x.device}")
-    return x
+def _like(x: torch.Tensor, device, shape, dtype, what: str, name: str):
+    if x.dtype is not dtype or x.shape != shape or x.device != device or not x.is_contiguous():
+        raise ValueError(f"{what}: {name}: a contiguous {dtype} tensor of shape {tuple(shape)} on {device} is wanted, got {x.dtype} {tuple(x.shape)} on {x.device}")
 
 
 def _codes(codes: torch.Tensor, scales: torch.Tensor, d: int, what: str) -> int:
     blocks = -(-d // BLOCK)
     if codes.dim() != 2 or not codes.is_cuda:
         raise ValueError(f"{what}: 2-D codes on a GPU are wanted")
-    _like(codes, codes, (codes.shape[0], blocks * BLOCK), torch.uint8, f"{what}: codes")
-    _like(scales, codes, (codes.shape[0], blocks), torch.uint8, f"{what}: scales")
-    return codes.shape[0]
+    n, device = codes.shape[0], codes.device
+    _like(codes, device, (n, blocks * BLOCK), torch.uint8, what, "codes")
+    _like(scales, device, (n, blocks), torch.uint8, what, "scales")
+    return n
 
 
 def encode_blocks(vectors: torch.Tensor):
     """(codes [n][blocks * 128] uint8, scales [n][blocks] uint8) of [n][d] vectors; see jv_encode_blocks_device."""
-    dtype, n, d, stride = _matrix(vectors, "encode_blocks")
+    dtype, n, d, stride = _matrix(vectors, "encode_blocks", "vectors")
     dev, blocks = vectors.device, -(-d // BLOCK)
-    codes = torch.empty((n, blocks * BLOCK), dtype=torch.uint8, device=dev)
-    scales = torch.empty((n, blocks), dtype=torch.uint8, device=dev)
+    codes = vectors.new_empty((n, blocks * BLOCK), dtype=torch.uint8)
+    scales = vectors.new_empty((n, blocks), dtype=torch.uint8)
     binding.encode_blocks_device(dev.index, vectors.data_ptr(), dtype, stride, n, d, codes.data_ptr(), scales.data_ptr(), _stream(dev))
     return codes, scales
 
@@ -74,7 +76,7 @@ def decode_blocks(codes: torch.Tensor, scales: torch.Tensor, d: int, dtype: torc
     n = _codes(codes, scales, d, "decode_blocks")
     if dtype not in _DTYPES:
         raise ValueError(f"decode_blocks: float32 or bfloat16 is wanted, got {dtype}")
-    out = torch.empty((n, d), dtype=dtype, device=codes.device)
+    out = codes.new_empty((n, d), dtype=dtype)
     binding.decode_blocks_device(codes.device.index, codes.data_ptr(), scales.data_ptr(), n, d, _DTYPES[dtype], out.data_ptr(), d, _stream(codes.device))
     return out
 
@@ -85,36 +87,38 @@ def score_blocks(query_codes: torch.Tensor, query_scales: torch.Tensor, codes: t
     nq, n = _codes(query_codes, query_scales, d, "score_blocks: queries"), _codes(codes, scales, d, "score_blocks: rows")
     if query_codes.device != codes.device or dtype not in _DTYPES:
         raise ValueError("score_blocks: queries and rows on one device and float32 or bfloat16 scores are wanted")
-    out = torch.empty((nq, n), dtype=dtype, device=codes.device)
+    out = codes.new_empty((nq, n), dtype=dtype)
     binding.score_blocks_device(codes.device.index, query_codes.data_ptr(), query_scales.data_ptr(), nq, codes.data_ptr(), scales.data_ptr(), n, d,
                                 _DTYPES[dtype], out.data_ptr(), n, _stream(codes.device))
     return out
 
 
 def _softmax(queries, vectors, targets, scale, what, flags):
-    """(params with a workspace, the workspace) of a softmax call."""
-    dtype, nq, d, q_stride = _matrix(queries, f"{what}: queries")
-    v_dtype, n, v_d, v_stride = _matrix(vectors, f"{what}: vectors")
-    if v_dtype != dtype or v_d != d or vectors.device != queries.device:
+    """(params with a workspace, the workspace, the device) of a softmax call."""
+    dtype, nq, d, q_stride = _matrix(queries, what, "queries")
+    v_dtype, n, v_d, v_stride = _matrix(vectors, what, "vectors")
+    device = queries.device
+    if v_dtype != dtype or v_d != d or vectors.device != device:
         raise ValueError(f"{what}: queries {queries.dtype} {tuple(queries.shape)} on {queries.device} and vectors {vectors.dtype} "
                          f"{tuple(vectors.shape)} on {vectors.device} do not match")
     if targets is not None:
-        _like(targets, queries, (nq,), torch.int32, f"{what}: targets")
-    params = binding.softmax_params(queries.device.index, dtype, nq, n, d, scale, queries.data_ptr(), q_stride, vectors.data_ptr(), v_stride,
+        _like(targets, device, (nq,), torch.int32, what, "targets")
+    params = binding.softmax_params(device.index, dtype, nq, n, d, scale, queries.data_ptr(), q_stride, vectors.data_ptr(), v_stride,
                                     0 if targets is None else targets.data_ptr())
-    params.workspace_bytes = _workspace_bytes(dtype, nq, n, d, flags)
-    workspace = torch.empty(params.workspace_bytes, dtype=torch.uint8, device=queries.device)
-    params.workspace = workspace.data_ptr()
-    return params, workspace
+    need = _workspace_bytes(dtype, nq, n, d, flags)
+    workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    params.workspace_bytes, params.workspace = need, workspace.data_ptr()
+    return params, workspace, device
 
 
 def softmax_loss(queries: torch.Tensor, vectors: torch.Tensor, targets, scale: float):
     """(loss [nq], lse [nq]), float32: loss_i = lse_i - scale q_i . v_targets[i], lse_i = log sum_j exp(scale q_i . v_j).  ``targets``: int32, a value
     outside [0, n) (or None in place of the tensor) = no target, loss 0; see jv_softmax_loss_device."""
-    params, workspace = _softmax(queries, vectors, targets, scale, "softmax_loss", binding.SOFTMAX_LOSS)
-    loss = torch.empty(params.nq, dtype=torch.float32, device=queries.device)
-    lse = torch.empty(params.nq, dtype=torch.float32, device=queries.device)
-    binding.softmax_loss_device(params, loss.data_ptr(), lse.data_ptr(), _stream(queries.device))
+    params, workspace, device = _softmax(queries, vectors, targets, scale, "softmax_loss", binding.SOFTMAX_LOSS)
+    nq = queries.shape[0]
+    loss = torch.empty(nq, dtype=torch.float32, device=device)
+    lse = torch.empty(nq, dtype=torch.float32, device=device)
+    binding.softmax_loss_device(params, loss.data_ptr(), lse.data_ptr(), _stream(device))
     return loss, lse
 
 
@@ -125,15 +129,16 @@ def softmax_loss_grad(queries: torch.Tensor, vectors: torch.Tensor, targets, sca
     if not queries_grad and not vectors_grad:
         return None, None
     flags = (binding.SOFTMAX_QUERY_GRAD if queries_grad else 0) | (binding.SOFTMAX_VECTOR_GRAD if vectors_grad else 0)
-    params, workspace = _softmax(queries, vectors, targets, scale, "softmax_loss_grad", flags)
-    _like(lse, queries, (params.nq,), torch.float32, "softmax_loss_grad: lse")
+    params, workspace, device = _softmax(queries, vectors, targets, scale, "softmax_loss_grad", flags)
+    nq, d = queries.shape
+    _like(lse, device, (nq,), torch.float32, "softmax_loss_grad", "lse")
     if loss_grad is not None:
-        _like(loss_grad, queries, (params.nq,), torch.float32, "softmax_loss_grad: loss_grad")
-    dq = torch.empty(queries.shape, dtype=queries.dtype, device=queries.device) if queries_grad else None
-    dv = torch.empty(vectors.shape, dtype=vectors.dtype, device=vectors.device) if vectors_grad else None
+        _like(loss_grad, device, (nq,), torch.float32, "softmax_loss_grad", "loss_grad")
+    dq = queries.new_empty((nq, d)) if queries_grad else None
+    dv = vectors.new_empty(vectors.shape) if vectors_grad else None
     # (an empty tensor has no address: its gradient has nothing to write either)
     if (dq is None or dq.numel() == 0) and (dv is None or dv.numel() == 0):
         return dq, dv
     binding.softmax_grad_device(params, lse.data_ptr(), 0 if loss_grad is None else loss_grad.data_ptr(), 0 if dq is None else dq.data_ptr(),
-                                params.d, 0 if dv is None else dv.data_ptr(), params.d, _stream(queries.device))
+                                d, 0 if dv is None else dv.data_ptr(), d, _stream(device))
     return dq, dv
