@@ -86,6 +86,8 @@ struct Plan {
 // MB of one piece's weights g: few large pieces, for every piece writes and reads dq's partial sums again and starts its tiles anew (step
 // 4096 x 131072 x 1024: 4.67 ms with 128, 4.54 with 384, 4.32 with 1024, all of it in one piece)
 constexpr int64_t kWeights = 1024;
+// MB of one piece's rows, where a gradient needs them laid out
+constexpr int64_t kLaid = 2048;
 
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
@@ -96,7 +98,15 @@ int64_t piece(int64_t n, int64_t most) {
     return std::max<int64_t>(up((n + pieces - 1) / pieces, 256), 256);
 }
 
-Plan make_plan(int dtype, int nq, int64_t n, int d, uint32_t what) {
+// The products take the vectors as they lie (take_rows): float32 with at least four components; bf16, 4-B aligned, with an even number of them,
+// eight at least.
+bool can_lie(int dtype, int d) { return dtype == JV_DTYPE_F32 ? d >= 4 : d >= 8 && d % 2 == 0; }
+bool lies(const jv_softmax_params* p) {
+    return can_lie(p->dtype, p->d) && (p->dtype == JV_DTYPE_F32 || ((uintptr_t)p->vectors % 4 == 0 && p->vector_stride % 2 == 0));
+}
+
+// `as_is`: the vectors are taken as they lie
+Plan make_plan(int dtype, int nq, int64_t n, int d, uint32_t what, bool as_is) {
     Plan p{};
     p.P = dtype == JV_DTYPE_F32 ? 3 : 1;
     p.dp = (int)up(d, 64);
@@ -105,7 +115,8 @@ Plan make_plan(int dtype, int nq, int64_t n, int d, uint32_t what) {
     const int64_t panels = std::max((nq + 255) / 256, 1), row = (int64_t)p.P * p.dp * 2;
     const int64_t fill = 256 * ((1024 + panels - 1) / panels);   // rows whose tiles fill the chip four times
     p.rows_f = piece(n, std::max<int64_t>((128ll << 20) / row, fill));
-    p.rows_b = piece(n, std::max<int64_t>((kWeights << 20) / ((int64_t)p.P * 2 * p.gq), fill));
+    const int64_t most = (kWeights << 20) / ((int64_t)p.P * 2 * p.gq);
+    p.rows_b = piece(n, std::max<int64_t>(as_is ? most : std::min(most, (kLaid << 20) / row), fill));
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
         const int64_t o = at;
@@ -118,11 +129,11 @@ Plan make_plan(int dtype, int nq, int64_t n, int d, uint32_t what) {
         p.splits_f = jvk_sx_loss_splits(p.path_f, nq, n, d);
         p.off_part = take((int64_t)p.splits_f * nq * 8);
         p.off_hit = take((int64_t)nq * 4);
-        p.off_v = take(std::min<int64_t>(p.rows_f, n) * row);
+        p.off_v = take(as_is ? 0 : std::min<int64_t>(p.rows_f, n) * row);
     }
     if (what & (JV_SOFTMAX_QUERY_GRAD | JV_SOFTMAX_VECTOR_GRAD)) {
         p.path_b = jvk_sx_path(nq, std::min<int64_t>(p.rows_b, n), dtype == JV_DTYPE_F32);
-        p.off_v = take(std::min<int64_t>(p.rows_b, n) * row);
+        p.off_v = take(as_is ? 0 : std::min<int64_t>(p.rows_b, n) * row);
         p.off_query = take((int64_t)nq * sizeof(JvSxQuery));
         p.off_norm = take(4);
         p.off_tail = take(16);
@@ -143,10 +154,8 @@ Plan make_plan(int dtype, int nq, int64_t n, int d, uint32_t what) {
     return p;
 }
 
-// Rows as a product takes them: the caller's own where they are
-//   bf16, 4-B aligned, with an even number of components, eight at least (the queries, whose padding stands for zeros behind the vectors', with
-//   whole steps of 64), or
-//   float32 with at least four components, and the path takes them as they lie (JV_SX_RAW all of them, JV_SX_PLANES the vectors).
+// Rows as a product takes them: the caller's own (the vectors where lies(); queries in bf16 where they are 4-B aligned and whole steps of 64, for
+// their padding stands for zeros behind the vectors', and in float32 where the path takes them as they lie), or laid out.
 struct Rows {
     const char* p;
     int64_t stride;   // bytes
@@ -157,8 +166,8 @@ struct Rows {
 };
 Rows rows_of(const void* p, int64_t stride, const jv_softmax_params* q, const Plan& plan, int path, bool vectors) {
     Rows r{(const char*)p, stride * size_of(q->dtype), false, plan.dp, false};
-    if (q->dtype == JV_DTYPE_BF16) r.ready = (uintptr_t)p % 4 == 0 && stride % 2 == 0 && (vectors ? q->d % 2 == 0 && q->d >= 8 : q->d % 64 == 0);
-    else if (path == JV_SX_RAW || (path == JV_SX_PLANES && vectors)) r.ready = q->d >= 4, r.kp = 4, r.raw = true;
+    if (q->dtype == JV_DTYPE_BF16) r.ready = vectors ? lies(q) : (uintptr_t)p % 4 == 0 && stride % 2 == 0 && q->d % 64 == 0;
+    else if (path == JV_SX_RAW || vectors) r.ready = q->d >= 4, r.kp = 4, r.raw = true;
     return r;
 }
 
@@ -264,14 +273,16 @@ int jv_softmax_workspace(const jv_softmax_params* params, uint32_t what, int64_t
     if (!out_bytes || !what || (what & ~7u)) return jvi_fail(JV_EINVAL, "softmax: out_bytes is NULL or unknown flags %#x", what);
     int64_t need = 256;   // (the loss and its gradient are separate calls: the larger of the two)
     for (uint32_t part : {what & JV_SOFTMAX_LOSS, what & (JV_SOFTMAX_QUERY_GRAD | JV_SOFTMAX_VECTOR_GRAD)})
-        if (part) need = std::max(need, make_plan(params->dtype, params->nq, params->n, params->d, part).bytes);
+        for (bool as_is : {false, true})   // (bf16: where the vectors lie decides, which is not known here)
+            if (part && (as_is ? can_lie(params->dtype, params->d) : params->dtype == JV_DTYPE_BF16 || !can_lie(params->dtype, params->d)))
+                need = std::max(need, make_plan(params->dtype, params->nq, params->n, params->d, part, as_is).bytes);
     *out_bytes = need;
     return JV_OK;
 }
 
 int jv_softmax_loss_device(const jv_softmax_params* p, float* d_out_loss, float* d_out_lse, void* hip_stream) {
     TRY(check_softmax(p));
-    const Plan plan = make_plan(p->dtype, p->nq, p->n, p->d, JV_SOFTMAX_LOSS);
+    const Plan plan = make_plan(p->dtype, p->nq, p->n, p->d, JV_SOFTMAX_LOSS, lies(p));
     TRY(check_softmax_call(p, plan));
     if (p->nq > 0 && (!d_out_loss || !d_out_lse)) return jvi_fail(JV_EINVAL, "softmax: output pointer is NULL");
     OnDevice on(p->device);
@@ -310,7 +321,7 @@ int jv_softmax_grad_device(const jv_softmax_params* p, const float* d_lse, const
     TRY(check_softmax(p));
     const uint32_t what = (d_out_query_grad ? JV_SOFTMAX_QUERY_GRAD : 0) | (d_out_vector_grad ? JV_SOFTMAX_VECTOR_GRAD : 0);
     if (!what) return jvi_fail(JV_EINVAL, "softmax: no gradient asked for");
-    const Plan plan = make_plan(p->dtype, p->nq, p->n, p->d, what);
+    const Plan plan = make_plan(p->dtype, p->nq, p->n, p->d, what, lies(p));
     TRY(check_softmax_call(p, plan));
     if (p->nq > 0 && !d_lse) return jvi_fail(JV_EINVAL, "softmax: lse is NULL");
     if (d_out_query_grad) TRY(check_rows(d_out_query_grad, p->nq, query_grad_stride, p->d, p->dtype, "softmax: query gradient"));

@@ -115,8 +115,9 @@ __device__ __forceinline__ JvSxQuery query_of(const float* lse, const float* w, 
 }
 
 // The weights are divided by the largest of them (`norm`, multiplied back in float32 at the end): an entry of g at a target is then just
-// below 1 for the largest weight, where bf16's step is finest in relation.  Every workgroup finds the largest anew and sees to 256 queries.
-__device__ __forceinline__ void queries(const JvSxPrepare& a, int part) {
+// below 1 for the largest weight, where bf16's step is finest in relation.  Every workgroup finds the largest anew: no
+// more than 64 of them.
+__device__ __forceinline__ void queries(const JvSxPrepare& a, int part, int parts) {
     __shared__ float tops[4];
     float top = 0.0f;
     if (a.w) {
@@ -134,14 +135,15 @@ __device__ __forceinline__ void queries(const JvSxPrepare& a, int part) {
     top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
     // (no weights, none but zeros, or one that is not finite: 1, so that what is not finite shows in the gradient)
     const float unit = a.w && top > 0.0f && top < __builtin_inff() ? top : 1.0f;
-    const int i = part * 256 + threadIdx.x;
+    int i = part * 256 + threadIdx.x;
     if (i == 0) *a.norm = unit;
     if (a.last && i < 8) ((__bf16*)a.tail)[i] = a.d / 8 * 8 + i < a.d ? ((const __bf16*)a.last)[a.d / 8 * 8 + i] : (__bf16)0.0f;
-    if (i >= a.nq) return;
-    JvSxQuery q = query_of(a.lse, a.w, a.targets, a.n, i);
-    q.w /= unit, q.whole /= unit;
-    a.query[i] = q;
-    a.rest[i] = 0.0f;
+    for (; i < a.nq; i += parts * 256) {
+        JvSxQuery q = query_of(a.lse, a.w, a.targets, a.n, i);
+        q.w /= unit, q.whole /= unit;
+        a.query[i] = q;
+        a.rest[i] = 0.0f;
+    }
 }
 
 template <typename T>
@@ -152,12 +154,12 @@ __global__ __launch_bounds__(256) void jvs_prepare_kernel(const JvSxPrepare a, i
     if (i < g1) return pack<T>(a, a.m[1], (int64_t)i * 256 + threadIdx.x, (int64_t)g1 * 256);
     i -= g1;
     if (i < g2) return pack<T>(a, a.m[2], (int64_t)i * 256 + threadIdx.x, (int64_t)g2 * 256);
-    queries(a, i - g2);
+    queries(a, i - g2, gridDim.x - g0 - g1 - g2);
 }
 extern "C" hipError_t jvk_sx_prepare(const JvSxPrepare* a, hipStream_t s) {
     int g[3];
     for (int k = 0; k < 3; k++) g[k] = (int)std::min<int64_t>((a->m[k].rows * std::max(a->m[k].kp / 8, 1) + 255) / 256, 32768);
-    const unsigned grid = (unsigned)(g[0] + g[1] + g[2] + (a->query ? (a->nq + 255) / 256 : 0));
+    const unsigned grid = (unsigned)(g[0] + g[1] + g[2] + (a->query ? std::min((a->nq + 255) / 256, 64) : 0));
     if (grid == 0) return hipSuccess;
     if (a->dtype == 0) jvs_prepare_kernel<float><<<grid, 256, 0, s>>>(*a, g[0], g[1], g[2]);
     else jvs_prepare_kernel<__bf16><<<grid, 256, 0, s>>>(*a, g[0], g[1], g[2]);
