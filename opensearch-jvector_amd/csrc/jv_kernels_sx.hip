@@ -638,7 +638,8 @@ static int grads_path(int path, int d) { return path == JV_SX_LARGE && d <= 128 
 extern "C" int jvk_sx_grad_splits(int path, int64_t rows, int d, int64_t k, int across) {
     path = grads_path(path, d);
     const bool large = path == JV_SX_LARGE;
-    const int tm = large ? 256 : path == JV_SX_PLANES && !across ? shape_of(path, (int)rows, k, 0).m : 128, tn = large ? 256 : 128;
+    const bool few = path == JV_SX_RAW && !across && rows <= 64;
+    const int tm = large ? 256 : few ? 64 : path == JV_SX_PLANES && !across ? shape_of(path, (int)rows, k, 0).m : 128, tn = large ? 256 : few ? 64 : 128;
     const int64_t tiles = std::max<int64_t>((rows + tm - 1) / tm, 1) * ((d + tn - 1) / tn);
     const int64_t steps = path == JV_SX_RAW || path == JV_SX_PLANES ? (k + 31) / 32 : (k + 63) / 64;
     return (int)std::max<int64_t>(std::min<int64_t>((large ? 256 : 512) / tiles, steps / ((large ? 4 : 8) * (across ? 2 : 1))), 1);
@@ -659,13 +660,16 @@ extern "C" hipError_t jvk_sx_grads(const JvMmOut* q, const JvMmOut* v, int path,
         if (v && e == hipSuccess) e = mm_out_tile<Tile3<4, true, true>>(*v, s);
         return e;
     }
-    // 64 x 64 where 128 x 128 would be no more than one tile a CU
+    // 64 x 64 where 128 x 128 would be no more than one tile a CU; in float32, whose operands are split for every tile, for dq of up to 64 queries too
+    // (adapter 43 x 13 015 x 1296: 131 -> 122 us; bf16: 2 % either way)
     int64_t tiles = 0;
     for (const JvMmOut* o : {q, v})
         if (o) tiles += (int64_t)((o->mm.M + 127) / 128) * ((o->mm.N + 127) / 128) * o->splits;
     if (path == JV_SX_RAW) {
-        if (tiles <= 256) return grads_tile<Tile32<1, 1, 2, 2, 4, false, true>, Tile32<1, 1, 2, 2, 4, true, true>>(q, v, s);
-        return grads_tile<Tile32<2, 2, 2, 2, 2, false, true>, Tile32<2, 2, 2, 2, 2, true, true>>(q, v, s);
+        using Q64 = Tile32<1, 1, 2, 2, 4, false, true>;
+        using V128 = Tile32<2, 2, 2, 2, 2, true, true>;
+        if (tiles <= 256) return grads_tile<Q64, Tile32<1, 1, 2, 2, 4, true, true>>(q, v, s);
+        return q && q->mm.M <= 64 ? grads_tile<Q64, V128>(q, v, s) : grads_tile<Tile32<2, 2, 2, 2, 2, false, true>, V128>(q, v, s);
     }
     if (tiles <= 256) return grads_tile<Tile<BF16, 1, 1, 2, 2, 4, false, true>, Tile<BF16, 1, 1, 2, 2, 4, true, true>>(q, v, s);
     return grads_tile<Tile<BF16, 2, 2, 2, 2, 2, false, true>, Tile<BF16, 2, 2, 2, 2, 2, true, true>>(q, v, s);
