@@ -633,8 +633,7 @@ static hipError_t grads_tile(const JvMmOut* q, const JvMmOut* v, hipStream_t s) 
 static int grads_path(int path, int d) { return path == JV_SX_LARGE && d <= 128 ? JV_SX_TILES : path; }
 
 // k ranges of a gradient of `rows` rows: once around the CUs with the large tiles, twice with the small ones; at least four and eight steps in
-// each.  dv (`across`) is written as it is if it has one range, joining more costs a launch: twice as many steps (step 4096 x 4096 x 768, bf16:
-// dv 104 us of one range, 40 of five).
+// each.  (dv, `across`, step 4096 x 4096 x 768, bf16: 104 us of one range, 40 of five.)
 extern "C" int jvk_sx_grad_splits(int path, int64_t rows, int d, int64_t k, int across) {
     path = grads_path(path, d);
     const bool large = path == JV_SX_LARGE;
@@ -642,7 +641,7 @@ extern "C" int jvk_sx_grad_splits(int path, int64_t rows, int d, int64_t k, int 
     const int tm = large ? 256 : few ? 64 : path == JV_SX_PLANES && !across ? shape_of(path, (int)rows, k, 0).m : 128, tn = large ? 256 : few ? 64 : 128;
     const int64_t tiles = std::max<int64_t>((rows + tm - 1) / tm, 1) * ((d + tn - 1) / tn);
     const int64_t steps = path == JV_SX_RAW || path == JV_SX_PLANES ? (k + 31) / 32 : (k + 63) / 64;
-    return (int)std::max<int64_t>(std::min<int64_t>((large ? 256 : 512) / tiles, steps / ((large ? 4 : 8) * (across ? 2 : 1))), 1);
+    return (int)std::max<int64_t>(std::min<int64_t>((large ? 256 : 512) / tiles, steps / (large ? 4 : 8)), 1);
 }
 extern "C" hipError_t jvk_sx_grads(const JvMmOut* q, const JvMmOut* v, int path, hipStream_t s) {
     path = grads_path(path, q ? q->mm.N : v->mm.N);

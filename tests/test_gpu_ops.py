@@ -181,7 +181,7 @@ def test_softmax_loss_and_gradients(torch, ops, dtype, nq, n, d, pad, shift, sca
 
 
 @pytest.mark.parametrize("dtype,nq,n,d", [("bf16", 4096, 20011, 64), ("f32", 2500, 20011, 130), ("bf16", 1500, 70001, 64), ("f32", 64, 140001, 200),
-                                          ("bf16", 4096, 140003, 64), ("f32", 4100, 45001, 20), ("f32", 3, 400001, 3), ("bf16", 5, 70001, 1001), ("bf16", 4096, 140003, 50), ("bf16", 4096, 140003, 51)])
+                                          ("bf16", 4096, 140003, 64), ("f32", 4100, 45001, 20), ("f32", 3, 400001, 3), ("bf16", 5, 70001, 1001), ("bf16", 4096, 140003, 50), ("bf16", 4096, 140003, 51), ("bf16", 4096, 140003, 134)])
 def test_softmax_over_several_pieces_of_the_rows(torch, ops, dtype, nq, n, d):
     """Sizes whose rows take several pieces: against a float64 computation on the GPU, with the bound's largest terms alone."""
     q, v, t, w, _, _, t64, _ = loss_case(torch, nq, n, d, dtype)
