@@ -579,7 +579,7 @@ template <class T>
 static hipError_t weights_tile(const JvSxWeights& a, hipStream_t s) {
     const int64_t all = (int64_t)((padded_queries(a) + T::TM - 1) / T::TM) * ((a.kv + T::TN - 1) / T::TN);
     const int64_t extra = a.clean ? ((int64_t)a.mm.M * a.mm.k + CLEANED - 1) / CLEANED : 0;
-    if (all + extra > 0x7fffffffll || extra * CLEANED > 0x7fffffffll) return hipErrorInvalidValue;
+    if (all + extra > 0x7fffffffll || extra * CLEANED > 0xffffffffll) return hipErrorInvalidValue;   // (256 tiles of 128 x 128 have 2^15 queries at most)
     hipError_t e = lds_of<jvs_weights_tile_kernel<T>>(T::LDS);
     if (e != hipSuccess) return e;
     jvs_weights_tile_kernel<T><<<(unsigned)(all + extra), T::THREADS, T::LDS, s>>>(a);

@@ -490,6 +490,35 @@ def test_a_gradient_of_more_than_4_gib(torch, ops):
         assert ((dv[rows].double() - want).abs() <= off + 1e-30).all()
 
 
+def test_as_many_and_as_long_queries_as_few_tiles_take(torch, ops):
+    """2^15 queries of 2^16 components against 16 rows: 8 GiB of queries, of their gradient and of their copy."""
+    nq, n, d = 1 << 15, 16, 1 << 16
+    g = torch.Generator(device="cuda").manual_seed(8)
+    v = torch.randn((n, d), generator=g, device="cuda") / 256
+    q = torch.empty((nq, d), device="cuda")
+    for at in range(0, nq, 4096):
+        q[at:at + 4096] = torch.randn((4096, d), generator=g, device="cuda") / 256
+    t = (torch.arange(nq, device="cuda") % 17).int()   # (every 17th has none)
+    loss, lse = ops.softmax_loss(q, v, t, 2.0)
+    dq, dv = ops.softmax_loss_grad(q, v, t, 2.0, lse)
+    want, reach = torch.zeros((n, d), dtype=torch.float64, device="cuda"), torch.zeros((n, d), dtype=torch.float64, device="cuda")
+    # a dot product is 6 d / 16 additions of partial sums below 2^-5 (256 terms' root of 2^-16 each is 2^-8), half a step each, times the scale;
+    # the exponentials and the logarithm of 16 of them: a few steps of 4
+    de = 2 * 6 * d / 16 * 2.0 ** -24 * 2.0 ** -5 + 2.0 ** -20
+    for at in range(0, nq, 2048):
+        x = q[at:at + 2048].double()
+        z = 2.0 * x @ v.double().t()
+        assert (lse[at:at + 2048] - torch.logsumexp(z, 1)).abs().max().item() <= de
+        p = torch.softmax(z, 1)
+        p[torch.arange(2048, device="cuda"), t[at:at + 2048].long().clamp(max=15)] -= 1
+        p *= 2.0 * (t[at:at + 2048] < 16).double()[:, None]
+        want += p.t() @ x
+        reach += p.abs().t() @ x.abs()
+        if at % 8192 == 0:
+            assert ((dq[at:at + 2048].double() - p @ v.double()).abs() <= 8 * de * (p.abs() @ v.double().abs())).all()
+    assert ((dv.double() - want).abs() <= (8 * de + 6 * nq / 16 * 2.0 ** -24) * reach).all()
+
+
 def test_codes_and_scores_of_more_than_4_gib(torch, ops):
     n, d = 4500001, 1000
     g = torch.Generator(device="cuda").manual_seed(6)
