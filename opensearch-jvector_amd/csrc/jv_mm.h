@@ -10,6 +10,8 @@
 // Both operands are staged with 16-B copies straight into LDS; a copy's 64 lanes fill an 8-row group of 1 024 B in
 // order, so the swizzle (16-B piece p of row r at p ^ (r & 7)) is on the source address.  Groups are 1 152 B apart: a 16-B fragment
 // read serves 16 consecutive rows at a time, the pad puts the two groups of such a pair on opposite halves of the 256-B bank row.
+// Bound by the rows' bytes with few queries (loss 8 x 87 332 x 384, bf16: 14 us, 4.8 TB/s), by the way through a tile's steps where there are few
+// tiles (loss 2048 x 2048 x 768: 18 us, 360 TFLOP/s).
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -47,7 +49,8 @@ __device__ __forceinline__ s16x4 read_across(const unsigned char* p) {   // 16 l
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
 }
 
-// This wave's copies of a step have landed and everybody's have (SOLO: a wave with LDS of its own), `left` steps (PER copies each, NS - 1 at most) being under way behind it.
+// This wave's copies of a step have landed and everybody's have (SOLO: a wave with LDS of its own), `left` steps (PER copies each, NS - 1 at most)
+// being under way behind it.
 template <int NS, int PER, bool SOLO = false>
 __device__ __forceinline__ void wait_step(int left) {
     static_assert(NS >= 2 && NS <= 4);

@@ -15,6 +15,8 @@
 // are k, as a gradient's operands lie).  k along rows: a row's 64 bytes are four 16-B pieces, piece p at p ^ ((row >> 2) & 3), so a
 // fragment read's 16 consecutive rows cover the 64 banks once.  k across rows: 32 rows of 256 columns, read through the transposing
 // LDS read (16 lanes give four rows of 16 and take 16 columns of four); piece p of row k at p ^ ((k & 3) << 2), so four rows cover the banks.
+// Bound by the matrix unit: 8192^3 in bf16 1277 TFLOP/s (a library's product: 1423), at the 1.6 - 1.8 GHz that power leaves; tiles of 1024 components
+// with an epilogue each 1000 - 1075.  Four waves of 128 x 128 each, which read a third less from LDS, were slower.
 #pragma once
 #include "jv_mm.h"
 
@@ -272,7 +274,8 @@ struct Pipe {
 
     // Writes a tile whose elements are value(m, n, e) as rows of float32 or bf16, `ldo` elements apart, rows < M and columns < N; the rows
     // are 16-B aligned.  They go through LDS, so that a store writes whole 128-B lines: 32 rows of 128 B at a time, piece p of row r at
-    // p ^ ((r >> 1) & 7).  (Other rows go to the small tiles: element by element from here, scores of 256 x 500 001 x 768 took 496 us, there 343.)  Returns the stores that every wave has issued.
+    // p ^ ((r >> 1) & 7).  (Other rows go to the small tiles: element by element from here, scores of 256 x 500 001 x 768 took 496 us, there 343.)
+    // Returns the stores that every wave has issued.
     template <class V>
     static __device__ __forceinline__ int write_bf16(unsigned char* smem, uint16_t* out, int64_t ldo, const Work& at, int M, int N, V&& value) {
         const int tid = own_thread(), lane = tid & 63, w = tid >> 6, h = lane >> 5, r31 = lane & 31;
