@@ -179,12 +179,14 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
 
 // A lane's part of a tile: MT queries, NT * 16 rows each.  `rows`: how many rows the tile has in all.  Four instructions a logit: the maximum, the
 // scaled difference (c <= 0: the smallest product is the largest logit), the exponential, the sum.
-// `m0`, `n0`: where the tile lies; the target's own product is the same one, so that a loss near 0 keeps its digits.
+// `m0`, `n0`: where the tile lies.  The target's own product is kept apart (`hit`) and left out of the maximum and the sum: where a pair is learnt its
+// term would be the 1 that all other terms together, which are the loss, are rounded against.
 template <class Core, int MT, int NT>
 __device__ __forceinline__ void add_tile(const JvSxLoss& a, typename Core::acc_t (&acc)[MT][NT], int m0, int n0, const int (&want)[MT], float (&top)[MT], float (&sum)[MT]) {
     const float c = a.c;
     const int rows = a.mm.N - n0;
     const int first = Core::col(0, 0) & ~(Core::WIDE < 32 ? 7 : 31);   // this wave's columns
+    const float none = c < 0.0f ? __builtin_inff() : -__builtin_inff();   // (the target and what is behind the last row: the logit is -inf)
 #pragma unroll
     for (int m = 0; m < MT; m++) {
         const int at = want[m] - n0;
@@ -193,10 +195,9 @@ __device__ __forceinline__ void add_tile(const JvSxLoss& a, typename Core::acc_t
             for (int n = 0; n < NT; n++)
 #pragma unroll
                 for (int e = 0; e < Core::E; e++)
-                    if (Core::col(n, e) == at) a.hit[m0 + Core::row(m)] = acc[m][n][e];
+                    if (Core::col(n, e) == at) a.hit[m0 + Core::row(m)] = acc[m][n][e], acc[m][n][e] = none;
         }
     }
-    const float none = c < 0.0f ? __builtin_inff() : -__builtin_inff();   // (what is behind the last row: its logit is -inf)
     if (rows < Core::TN) {
 #pragma unroll
         for (int m = 0; m < MT; m++)
@@ -227,7 +228,7 @@ __device__ __forceinline__ void add_tile(const JvSxLoss& a, typename Core::acc_t
     }
 #pragma unroll
     for (int m = 0; m < MT; m++) {
-        // (c = 0: every logit is 0, also that of an infinite product, but those behind the last row are left out)
+        // (c = 0: every logit is 0, also that of an infinite product, but the target's and those behind the last row are left out)
         const float now = fmaxf(top[m], best[m] == none ? -__builtin_inff() : best[m] * c), ref = now == -__builtin_inff() ? 0.0f : now;
         float s = sum[m] * exp2_(top[m] - ref);
         if (c == 0.0f) {
@@ -413,8 +414,10 @@ extern "C" hipError_t jvk_sx_loss(const JvSxLoss* a, hipStream_t s) {
     return hipGetLastError();
 }
 
-// One wave a query: join the partials.  The few operations behind the sums are in 64 bits: a logarithm of 40 has a float32 step of 4e-6, and a loss
-// near 0 is the difference of two such.
+// One wave a query: join the partials, which are o = log sum_(j not the target) exp z_j; with the target's logit z
+//   loss = log(1 + exp(o - z)),   lse = z + loss,
+// each as the larger of the two and log1p of what is behind it.  The few operations behind the sums are in 64 bits: as float32 o and z would be rounded
+// by 2e-6 near 40, and a loss near 0, exp(o - z), by that share of itself.
 __global__ __launch_bounds__(256) void jvs_join_kernel(const float2* __restrict__ part, int splits, int nq, float c, const float* __restrict__ hit,
                                                        const int32_t* __restrict__ targets, int64_t n, float* __restrict__ loss, float* __restrict__ lse) {
     const int i = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -427,10 +430,21 @@ __global__ __launch_bounds__(256) void jvs_join_kernel(const float2* __restrict_
     }
     for (int off = 32; off >= 1; off >>= 1) join(m, s, __shfl_xor(m, off, 64), __shfl_xor(s, off, 64));
     if (lane != 0) return;
-    constexpr double ln2 = 0.69314718055994530942;
-    const double all = (double)m * ln2 + log((double)s);
+    constexpr double ln2 = 0.69314718055994530942, inf = __builtin_inf();
+    const double rest = (double)m * ln2 + log((double)s);
+    double all = rest, own = 0.0;
+    if (targets && known(targets[i], n)) {
+        const double z = (double)hit[i] * c * ln2;
+        if (z == -inf) {   // probability 0
+            own = rest - z;
+        } else {           // (an infinite logit leaves no probabilities)
+            const double behind = log1p(exp(-fabs(rest - z))), none = z == inf ? z - z : 0.0;
+            all = (rest > z ? rest : z) + behind + none;
+            own = (rest > z ? rest - z : 0.0) + behind + none;
+        }
+    }
     lse[i] = (float)all;
-    loss[i] = targets && known(targets[i], n) ? (float)(all - (c == 0.0f ? 0.0 : (double)hit[i] * c * ln2)) : 0.0f;
+    loss[i] = (float)own;
 }
 
 extern "C" hipError_t jvk_sx_join(const float2* part, int splits, int nq, float c, const float* hit, const int32_t* targets, int64_t n, float* loss, float* lse,

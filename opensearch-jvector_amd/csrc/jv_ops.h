@@ -38,7 +38,7 @@ struct JvSxLoss {
     float c;               // scale * log2(e)
     int32_t path;          // JvSxPath
     int32_t splits;        // jvk_sx_loss_splits
-    float2* part;          // [M][splits]: maximum and sum (log2 domain)
+    float2* part;          // [M][splits]: maximum and sum (log2 domain) over the rows but for the target
     int32_t first;         // 0: partials of an earlier piece of the rows are in `part` already, join them
     const int32_t* targets;  // nullptr = none
     int64_t row0;          // first row of this piece
