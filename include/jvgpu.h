@@ -336,9 +336,14 @@ int jv_softmax_workspace(const jv_softmax_params* params, uint32_t what, int64_t
 /* out_loss [nq], out_lse [nq] (natural logarithm; -inf if n == 0). */
 int jv_softmax_loss_device(const jv_softmax_params* params, float* d_out_loss, float* d_out_lse, void* hip_stream);
 /* Gradients of sum_i loss_grad_i loss_i (loss_grad NULL = 1 each) for the lse that jv_softmax_loss_device returned, each row rounded once
- * to `dtype` and overwritten; a gradient whose pointer is NULL is not computed.  Sums are taken in a fixed order: two calls agree bit for bit. */
+ * to `dtype` and overwritten; a gradient whose pointer is NULL is not computed.  Sums are taken in a fixed order: two calls agree bit for bit.
+ * The lse alone, as a float32, says what a target's probability lacks to 1 to about 1e-6 only: the gradient of a pair with a loss of 1e-4 has two
+ * right digits.  With the losses beside it (jv_softmax_grad_device_ex) it has them all. */
 int jv_softmax_grad_device(const jv_softmax_params* params, const float* d_lse, const float* d_loss_grad, void* d_out_query_grad,
                            int64_t query_grad_stride, void* d_out_vector_grad, int64_t vector_grad_stride, void* hip_stream);
+/* The same with the losses that jv_softmax_loss_device returned beside d_lse (NULL: jv_softmax_grad_device). */
+int jv_softmax_grad_device_ex(const jv_softmax_params* params, const float* d_lse, const float* d_loss, const float* d_loss_grad, void* d_out_query_grad,
+                              int64_t query_grad_stride, void* d_out_vector_grad, int64_t vector_grad_stride, void* hip_stream);
 
 /* Introspection used by the benchmark's roofline accounting. */
 typedef struct jv_index_info {

@@ -28,7 +28,7 @@ ABI_SYMBOLS = [
     "jv_shard_group_destroy", "jv_search_sharded_batch", "jv_search_sharded_batch_ex", "jv_shard_group_set_option",
     "jv_score_ordinals_batch", "jv_score_ordinals_batch_device", "jv_exact_search",
     "jv_encode_blocks_device", "jv_decode_blocks_device", "jv_score_blocks_device", "jv_softmax_workspace", "jv_softmax_loss_device",
-    "jv_softmax_grad_device",
+    "jv_softmax_grad_device", "jv_softmax_grad_device_ex",
 ]
 DTYPE_F32, DTYPE_BF16 = 0, 1
 OPS_MAX_D, SOFTMAX_MAX_QUERIES = 65536, 1 << 22
@@ -273,6 +273,8 @@ def load_library(path: str = LIB_PATH) -> C.CDLL:
     lib.jv_softmax_loss_device.restype = C.c_int
     lib.jv_softmax_grad_device.argtypes = [C.POINTER(JvSoftmaxParams), vp, vp, vp, i64, vp, i64, vp]
     lib.jv_softmax_grad_device.restype = C.c_int
+    lib.jv_softmax_grad_device_ex.argtypes = [C.POINTER(JvSoftmaxParams), vp, vp, vp, vp, i64, vp, i64, vp]
+    lib.jv_softmax_grad_device_ex.restype = C.c_int
     lib.jv_index_get_info.argtypes = [vp, C.POINTER(JvIndexInfo)]
     lib.jv_index_get_info.restype = C.c_int
     lib.jv_set_option.argtypes = [C.c_char_p, i64]
@@ -636,7 +638,7 @@ def softmax_loss_device(params: JvSoftmaxParams, d_out_loss: int, d_out_lse: int
 
 
 def softmax_grad_device(params: JvSoftmaxParams, d_lse: int, d_loss_grad: int, d_out_query_grad: int, query_grad_stride: int, d_out_vector_grad: int,
-                        vector_grad_stride: int, stream: int = 0):
+                        vector_grad_stride: int, stream: int = 0, d_loss: int = 0):
     lib = load_library()
-    _check(lib, lib.jv_softmax_grad_device(C.byref(params), d_lse, d_loss_grad or None, d_out_query_grad or None, query_grad_stride,
-                                           d_out_vector_grad or None, vector_grad_stride, stream or None))
+    _check(lib, lib.jv_softmax_grad_device_ex(C.byref(params), d_lse, d_loss or None, d_loss_grad or None, d_out_query_grad or None, query_grad_stride,
+                                              d_out_vector_grad or None, vector_grad_stride, stream or None))

@@ -318,6 +318,11 @@ int jv_softmax_loss_device(const jv_softmax_params* p, float* d_out_loss, float*
 
 int jv_softmax_grad_device(const jv_softmax_params* p, const float* d_lse, const float* d_loss_grad, void* d_out_query_grad, int64_t query_grad_stride,
                            void* d_out_vector_grad, int64_t vector_grad_stride, void* hip_stream) {
+    return jv_softmax_grad_device_ex(p, d_lse, nullptr, d_loss_grad, d_out_query_grad, query_grad_stride, d_out_vector_grad, vector_grad_stride, hip_stream);
+}
+
+int jv_softmax_grad_device_ex(const jv_softmax_params* p, const float* d_lse, const float* d_loss, const float* d_loss_grad, void* d_out_query_grad,
+                              int64_t query_grad_stride, void* d_out_vector_grad, int64_t vector_grad_stride, void* hip_stream) {
     TRY(check_softmax(p));
     const uint32_t what = (d_out_query_grad ? JV_SOFTMAX_QUERY_GRAD : 0) | (d_out_vector_grad ? JV_SOFTMAX_VECTOR_GRAD : 0);
     if (!what) return jvi_fail(JV_EINVAL, "softmax: no gradient asked for");
@@ -342,7 +347,7 @@ int jv_softmax_grad_device(const jv_softmax_params* p, const float* d_lse, const
     w.mm = logits(plan, p->nq, p->d);
     w.c = p->scale * 1.44269504088896341f;
     if (rv.ready && !f32) w.mm.end_b = p->d * 2;
-    w.path = plan.path_b, w.g = ws + plan.off_g;
+    w.path = plan.path_b, w.g = ws + plan.off_g, w.loss = d_loss;
     // float32 g needs no common unit and lacks nothing at a target
     JvSxPrepare pre{};
     pre.dtype = p->dtype, pre.d = p->d;
@@ -352,7 +357,7 @@ int jv_softmax_grad_device(const jv_softmax_params* p, const float* d_lse, const
         w.lse = d_lse, w.w = d_loss_grad, w.targets = p->targets, w.n = p->n;
     } else {
         w.query = query = (JvSxQuery*)(ws + plan.off_query), w.rest = (float*)(ws + plan.off_rest), norm = (float*)(ws + plan.off_norm);
-        pre.lse = d_lse, pre.w = d_loss_grad, pre.nq = p->nq, pre.query = query, pre.norm = norm, pre.rest = w.rest;
+        pre.lse = d_lse, pre.loss = d_loss, pre.w = d_loss_grad, pre.nq = p->nq, pre.query = query, pre.norm = norm, pre.rest = w.rest;
     }
     const bool direct = raw && plan.splits_q == 1 && plan.rows_b >= p->n;   // dq is complete at once
     // Queries without a target are laid out as zeros.  dv's product reads them so: bf16 as they are laid out (again if the end is shifted),

@@ -105,13 +105,15 @@ __device__ __forceinline__ void pack(const JvSxPrepare& a, const JvSxPrepare::Ma
     }
 }
 
-__device__ __forceinline__ JvSxQuery query_of(const float* lse, const float* w, const int32_t* targets, int64_t n, int i) {
+// `unit`: what the weights are divided by.  `loss` (nullptr: not known): g at the target is w (exp(-loss) - 1), with all the digits that the loss has; from lse,
+// p - 1 is left with what a float32 lse leaves of it (half a step of 20 is 1e-6).
+__device__ __forceinline__ JvSxQuery query_of(const float* lse, const float* loss, const float* w, const int32_t* targets, int64_t n, int i, float unit) {
     const int t = targets[i];
     if (!known(t, n)) return {__builtin_inff(), 0.0f, -1, 0.0f};
     const float w0 = w ? w[i] : 1.0f, lse2 = lse[i] * 1.44269504088896341f;
     // lse log2(e) - lse2: what both roundings left out, up to 2^-19 for a logarithm of 40 and as much of p
     const float lacks = fabsf(lse2) < __builtin_inff() ? fmaf(lse[i], 1.44269504088896341f, -lse2) + lse[i] * 1.92596299112661747e-8f : 0.0f;
-    return {lse2, w0 * exp2_(-lacks), t, w0};
+    return {lse2, w0 * exp2_(-lacks) / unit, t, loss ? w0 / unit * expm1f(-loss[i]) : w0 / unit};
 }
 
 // The weights are divided by the largest of them (`norm`, multiplied back in float32 at the end): an entry of g at a target is then just
@@ -139,9 +141,7 @@ __device__ __forceinline__ void queries(const JvSxPrepare& a, int part, int part
     if (i == 0) *a.norm = unit;
     if (a.last && i < 8) ((__bf16*)a.tail)[i] = a.d / 8 * 8 + i < a.d ? ((const __bf16*)a.last)[a.d / 8 * 8 + i] : (__bf16)0.0f;
     for (; i < a.nq; i += parts * 256) {
-        JvSxQuery q = query_of(a.lse, a.w, a.targets, a.n, i);
-        q.w /= unit, q.whole /= unit;
-        a.query[i] = q;
+        a.query[i] = query_of(a.lse, a.loss, a.w, a.targets, a.n, i, unit);
         a.rest[i] = 0.0f;
     }
 }
@@ -458,9 +458,9 @@ extern "C" hipError_t jvk_sx_join(const float2* part, int splits, int nq, float 
 // backward: the logits again, as weights g
 // ---------------------------------------------------------------------------------------------
 // g of a lane's columns of one query, in place of the logits; `cols`: how many of the tile's columns are rows of the piece; `hit`: the target's
-// column.  Three instructions a value; the target, which few tiles hold, and the last tile's end are seen to apart.
+// column; `told`: the losses are known.  Three instructions a value; the target, which few tiles hold, and the last tile's end are seen to apart.
 template <class Core, int NT>
-__device__ __forceinline__ void weigh(typename Core::acc_t (&acc)[NT], const JvSxQuery& q, float c, int cols, int hit, bool lossy, float* rest) {
+__device__ __forceinline__ void weigh(typename Core::acc_t (&acc)[NT], const JvSxQuery& q, float c, int cols, int hit, bool told, bool lossy, float* rest) {
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -472,7 +472,7 @@ __device__ __forceinline__ void weigh(typename Core::acc_t (&acc)[NT], const JvS
 #pragma unroll
             for (int e = 0; e < Core::E; e++)
                 if (Core::col(n, e) == hit) {
-                    acc[n][e] -= q.whole;
+                    acc[n][e] = told ? q.own : acc[n][e] - q.own;
                     if (lossy) *rest = acc[n][e] - (float)(__bf16)acc[n][e];   // (one lane holds it; three planes lack nothing)
                 }
     }
@@ -516,7 +516,7 @@ __global__ __launch_bounds__(512) void jvs_weights_kernel(const JvSxWeights a, i
         },
         [&](const Work& w, f32x16 (&acc)[4][2]) -> int {
 #pragma unroll
-            for (int m = 0; m < 4; m++) weigh<P>(acc[m], q[m], a.c, a.mm.N - w.n0, at[m] - w.n0, true, a.rest + w.m0 + P::row(m));
+            for (int m = 0; m < 4; m++) weigh<P>(acc[m], q[m], a.c, a.mm.N - w.n0, at[m] - w.n0, a.loss, true, a.rest + w.m0 + P::row(m));
             return P::write_bf16(smem, (uint16_t*)a.g, a.kv, w, padded, a.kv, [&](int m, int n, int e) { return acc[m][n][e]; });
         });
 }
@@ -557,8 +557,8 @@ __global__ __launch_bounds__(T::THREADS, T::RESIDENT) void jvs_weights_tile_kern
     for (int m = 0; m < MT; m++) {
         const int r = m0 + T::row(m);
         JvSxQuery q = {__builtin_inff(), 0.0f, -1, 0.0f};
-        if (r < a.mm.M) q = a.query ? a.query[r] : query_of(a.lse, a.w, a.targets, a.n, r);
-        weigh<T>(acc[m], q, a.c, a.mm.N - n0, q.target >= 0 ? (int)(q.target - a.row0) - n0 : -1, a.path == JV_SX_TILES, a.rest + r);
+        if (r < a.mm.M) q = a.query ? a.query[r] : query_of(a.lse, a.loss, a.w, a.targets, a.n, r, 1.0f);
+        weigh<T>(acc[m], q, a.c, a.mm.N - n0, q.target >= 0 ? (int)(q.target - a.row0) - n0 : -1, a.loss, a.path == JV_SX_TILES, a.rest + r);
         // (kv is a multiple of 64: four columns are in or out together)
         auto put = [&](int r, int c, f32x4 v) {
             if (r >= padded || c >= a.kv) return;

@@ -49,7 +49,7 @@ struct JvSxQuery {
     float lse2;            // base-2 logarithm
     float w;               // weight / norm, times 2^-(what lse2 lacks of its value); 0 = the query takes no part
     int32_t target;        // row, -1 = none
-    float whole;           // weight / norm
+    float own;             // weight / norm, to be taken off p at the target; where the losses are known, g there: weight / norm * (exp(-loss) - 1)
 };
 // partial sums of a gradient, [splits][rows][lds], to be joined
 struct JvSxFinish {
@@ -69,8 +69,8 @@ struct JvSxWeights {
     JvMm mm;               // A = queries, B = vectors of this piece
     float c;
     int64_t row0;          // first row of this piece
-    const JvSxQuery* query;   // nullptr: from lse, w (nullptr = 1) and targets as they are
-    const float *lse, *w;
+    const JvSxQuery* query;   // nullptr: from lse, loss, w (nullptr = 1) and targets as they are
+    const float *lse, *loss, *w;   // loss: nullptr = not known
     const int32_t* targets;
     int64_t n;             // rows in all
     int32_t path;          // JvSxPath
@@ -95,7 +95,7 @@ struct JvSxPrepare {
     const int32_t* targets;     // of the queries, for n rows
     int64_t n;
     // the gradient's queries (query == nullptr: none)
-    const float *lse, *w;
+    const float *lse, *loss, *w;
     int32_t nq;
     JvSxQuery* query;
     float *norm, *rest;

@@ -123,15 +123,18 @@ def softmax_loss(queries: torch.Tensor, vectors: torch.Tensor, targets, scale: f
 
 
 def softmax_loss_grad(queries: torch.Tensor, vectors: torch.Tensor, targets, scale: float, lse: torch.Tensor, loss_grad=None, queries_grad: bool = True,
-                      vectors_grad: bool = True):
+                      vectors_grad: bool = True, loss=None):
     """Gradients of sum_i loss_grad[i] * loss[i] (``loss_grad`` None = 1 each) by the queries and by the vectors, in their dtype; None in the place
-    of one that is not asked for.  ``lse`` as ``softmax_loss`` returned it; see jv_softmax_grad_device."""
+    of one that is not asked for.  ``lse`` and ``loss`` as ``softmax_loss`` returned them; without ``loss`` the gradient of a pair that is nearly
+    learnt keeps only the digits that a float32 lse leaves (two at a loss of 1e-4); see jv_softmax_grad_device."""
     if not queries_grad and not vectors_grad:
         return None, None
     flags = (binding.SOFTMAX_QUERY_GRAD if queries_grad else 0) | (binding.SOFTMAX_VECTOR_GRAD if vectors_grad else 0)
     params, workspace, device = _softmax(queries, vectors, targets, scale, "softmax_loss_grad", flags)
     nq, d = queries.shape
     _like(lse, device, (nq,), torch.float32, "softmax_loss_grad", "lse")
+    if loss is not None:
+        _like(loss, device, (nq,), torch.float32, "softmax_loss_grad", "loss")
     if loss_grad is not None:
         _like(loss_grad, device, (nq,), torch.float32, "softmax_loss_grad", "loss_grad")
     dq = queries.new_empty((nq, d)) if queries_grad else None
@@ -140,5 +143,5 @@ def softmax_loss_grad(queries: torch.Tensor, vectors: torch.Tensor, targets, sca
     if (dq is None or dq.numel() == 0) and (dv is None or dv.numel() == 0):
         return dq, dv
     binding.softmax_grad_device(params, lse.data_ptr(), 0 if loss_grad is None else loss_grad.data_ptr(), 0 if dq is None else dq.data_ptr(),
-                                d, 0 if dv is None else dv.data_ptr(), d, _stream(device))
+                                d, 0 if dv is None else dv.data_ptr(), d, _stream(device), 0 if loss is None else loss.data_ptr())
     return dq, dv

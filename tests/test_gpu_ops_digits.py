@@ -107,3 +107,74 @@ def test_a_target_of_minus_infinity(torch, ops):
     q, t = torch.ones((2, 64), device="cuda", dtype=torch.bfloat16), torch.tensor([5, 6], dtype=torch.int32, device="cuda")
     loss, lse = ops.softmax_loss(q, v, t, 0.125)
     assert loss[0] == float("inf") and abs(loss[1].item() - np.log(39)) <= 2.0 ** -20 and ((lse - (8 + np.log(39))).abs() <= 2.0 ** -20).all()
+
+
+# ------------------------------------------------------------------------------------------------ gradients of learnt pairs
+def gradients(torch, q, v, t, scale, w):
+    """(dq, dv, reach of dq, reach of dv) in float64: g at the target from what its probability lacks to 1."""
+    z, apart, hit = others(torch, q, v, t, scale)
+    loss = torch.log1p(torch.exp(apart))
+    g = torch.exp(z - (hit + loss)[:, None]).scatter(1, t.long()[:, None], torch.expm1(-loss)[:, None]) * (scale * w.double())[:, None]
+    a, b = q.double(), v.double()
+    return g @ b, g.t() @ a, g.abs() @ b.abs(), g.abs().t() @ a.abs()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("nq,n,d", PAIRS)
+def test_a_learnt_pairs_gradient_keeps_its_digits(torch, ops, dtype, nq, n, d):
+    """Row by row: an entry of g is off by SLIP (the target's), or by the lse's half step and the exponential's argument (the others': 2^-24 * 32 + SLIP); float32 g
+    is held in three parts (2^-24), bf16 g in one (2^-8; the target's whole in dq); a sum of k terms in chains of k / 16 products of parts, six for
+    float32, and so many half steps; the result is rounded once."""
+    q, v, t, scale = learnt(torch, nq, n, d, dtype)
+    w = torch.linspace(0.25, 1.0, nq, device="cuda")
+    loss, lse = ops.softmax_loss(q, v, t, scale)
+    dq, dv = ops.softmax_loss_grad(q, v, t, scale, lse, w, loss=loss)
+    want_q, want_v, reach_q, reach_v = gradients(torch, q, v, t, scale, w)
+    entry, last, parts = 2.0 ** -19 + SLIP + (2.0 ** -24 if dtype == "f32" else 2.0 ** -8), (2.0 ** -24 if dtype == "f32" else 2.0 ** -8), (6 if dtype == "f32" else 1)
+    for got, want, reach, k in ((dq, want_q, reach_q, n), (dv, want_v, reach_v, nq)):
+        off = (entry + (parts * k / 16 + 8) * 2.0 ** -24) * reach
+        assert ((got.double() - want).abs() <= off + last * (want.abs() + off)).all(), ((got.double() - want).abs() / (off + last * want.abs())).max()
+    # a row that is one query's target alone: its gradient is that query's, times the entry
+    loss64 = torch.log1p(torch.exp(others(torch, q, v, t, scale)[1]))
+    if nq == 1:
+        own = (scale * w.double() * torch.expm1(-loss64))[:, None] * q.double()
+        assert ((dv[t.long()].double() - own).abs() <= (2 * SLIP + 2 * last + (2.0 ** -8 if dtype == "bf16" else 0)) * own.abs()).all()
+    one, none = ops.softmax_loss_grad(q, v, t, scale, lse, w, vectors_grad=False, loss=loss)
+    assert none is None and torch.equal(one, dq)
+    none, one = ops.softmax_loss_grad(q, v, t, scale, lse, w, queries_grad=False, loss=loss)
+    assert none is None and torch.equal(one, dv)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_losses_of_queries_that_take_no_part_are_not_read(torch, ops, dtype):
+    q, v, t, scale = learnt(torch, 9, 500, 96, dtype)
+    t[[2, 5]] = torch.tensor([-1, 500], dtype=torch.int32, device="cuda")
+    loss, lse = ops.softmax_loss(q, v, t, scale)
+    want = ops.softmax_loss_grad(q, v, t, scale, lse, loss=loss)
+    loss[[2, 5]] = torch.tensor([float("nan"), float("inf")], device="cuda")
+    got = ops.softmax_loss_grad(q, v, t, scale, lse, loss=loss)
+    assert all(torch.equal(a, b) for a, b in zip(want, got)) and (got[0][[2, 5]] == 0).all()
+    with pytest.raises(ValueError):
+        ops.softmax_loss_grad(q, v, t, scale, lse, loss=loss[:8])
+    with pytest.raises(ValueError):
+        ops.softmax_loss_grad(q, v, t, scale, lse, loss=loss.double())
+
+
+def test_the_gradient_of_a_learnt_pair_is_the_losss_slope(torch, ops):
+    """Against differences, at a loss of 1e-6, along the target's row and along another: components move by 2^-9, so that products stay exact.  A logit moves
+    by r = SCALE 2^-9 at most; near 0 the loss is an exponential of the logits, so a central difference is off by (r^2 / 6) e^r of its reach, SCALE
+    loss a unit, and the losses' own digits add SLIP e^r / r, the gradient's SLIP."""
+    q, v, t, scale = learnt(torch, 1, 3770, 1000, "f32")
+    loss, lse = ops.softmax_loss(q, v, t, scale)
+    dq, dv = ops.softmax_loss_grad(q, v, t, scale, lse, loss=loss)
+    h, r = 2.0 ** -9, SCALE * 2.0 ** -9
+    off = SCALE * loss.item() * (r * r / 6 * np.exp(r) + SLIP * np.exp(r) / r + 2 * SLIP)
+    assert loss.item() < 1e-5
+    for step in (v[t.long()], v[:1]):
+        up, down = (ops.softmax_loss(q + sign * h * step, v, t, scale)[0].item() for sign in (1, -1))
+        assert abs((up - down) / (2 * h) - (dq.double() * step.double()).sum().item()) <= off
+    moved = [v.clone(), v.clone()]
+    for x, sign in zip(moved, (1, -1)):
+        x[t.long()] += sign * h * q
+    up, down = (ops.softmax_loss(q, x, t, scale)[0].item() for x in moved)
+    assert abs((up - down) / (2 * h) - (dv[t.long()].double() * q.double()).sum().item()) <= off
