@@ -205,7 +205,7 @@ def _framework(state):
     loss, lse = ops.softmax_loss(q, v, t, case["scale"])
     out = {"loss": loss, "lse": lse}
     if case["kind"] != "loss":
-        grads = ops.softmax_loss_grad(q, v, t, case["scale"], lse, state["weights"], queries_grad=True, vectors_grad=case["kind"] == "step")
+        grads = ops.softmax_loss_grad(q, v, t, case["scale"], lse, state["weights"], queries_grad=True, vectors_grad=case["kind"] == "step", loss=loss)
         out["grad_queries"] = grads[0]
         if case["kind"] == "step":
             out["grad_vectors"] = grads[1]
