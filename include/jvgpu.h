@@ -309,8 +309,10 @@ int jv_score_blocks_device(int32_t device, const uint8_t* d_query_codes, const u
 /* Softmax cross entropy of queries over ALL rows of a matrix, as an embedding model or a query adapter is trained against a corpus:
  *   lse_i = log sum_j exp(scale q_i . v_j),   loss_i = lse_i - scale q_i . v_t(i)
  * in pieces of the rows: the nq x n logits are never held.  A target outside [0, n) is none: its loss is 0, its gradient 0, and it adds to no
- * row's gradient, whatever the query holds (a batch's padding may be NaN).  What is not finite in a row reaches every query's loss, in a
- * query with a target every row's gradient.  Components of float32 beyond 3.38e38 (bf16's largest) count as infinite.
+ * row's gradient, whatever the query (a batch's padding may be NaN) or a row holds.  A logit of NaN or +infinity makes its query's lse NaN and, where the
+ * query has a target, its loss, its gradient and every row's gradient; so does NaN for its lse or weight.  A bf16 logit of -infinity has probability 0, or is
+ * NaN (zeros that a product adds behind a row's end meet the infinity).  Infinite components of float32 make NaN; beyond 3.38e38 (bf16's largest) they
+ * count as infinite.
  * Logits are float32 sums of exact products; the gradient of bf16 rounds each probability to bf16 once (relative to the largest loss_grad). */
 #define JV_SOFTMAX_MAX_QUERIES (1 << 22)
 typedef struct jv_softmax_params {

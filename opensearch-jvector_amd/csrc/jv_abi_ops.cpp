@@ -392,6 +392,7 @@ int jv_softmax_grad_device_ex(const jv_softmax_params* p, const float* d_lse, co
         fq.slab = (const float*)(ws + plan.off_slab), fq.splits = std::min(plan.splits_q, splits_of(plan, std::min<int64_t>(plan.rows_b, p->n)));
         fq.rows = p->nq, fq.out = d_out_query_grad, fq.ldo = query_grad_stride;
         fq.rest = w.rest, fq.query = query, fq.vectors = p->vectors, fq.v_stride = p->vector_stride;
+        fq.targets = p->targets, fq.n = p->n;
     }
     for (int64_t at = 0; at < p->n; at += plan.rows_b) {
         const int rows = (int)std::min<int64_t>(plan.rows_b, p->n - at);
@@ -411,6 +412,7 @@ int jv_softmax_grad_device_ex(const jv_softmax_params* p, const float* d_lse, co
             o.splits = std::min(plan.splits_q, splits_of(plan, rows));   // (only the last piece can be that short: it adds to the first ranges)
             if (direct) o.mul = p->scale, o.out = d_out_query_grad, o.ldo = query_grad_stride;
             q = o;
+            if (direct) q.targets = p->targets, q.n = p->n;
             o.mm.tail_b = nullptr;
         }
         if (d_out_vector_grad) {   // G across times the queries: k = the queries

@@ -31,6 +31,8 @@ using namespace jvmm;
 
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float log2_(float x) { return __builtin_amdgcn_logf(x); }
+// v_mul_legacy_f32: 0 where one of them is, also beside NaN and infinity (the compiler has it as an intrinsic without a builtin)
+__device__ float times_or_0(float x, float w) __asm("llvm.amdgcn.fmul.legacy");
 
 __device__ __forceinline__ uint16_t bf16_bits(float x) {
     const __bf16 b = (__bf16)x;
@@ -49,10 +51,8 @@ __device__ __forceinline__ void planes3(float x, uint16_t (&p)[3]) {
 // ---------------------------------------------------------------------------------------------
 // what has to be laid out: rows as padded bf16 planes [rows][planes][kp], and what the gradient needs of each query
 // ---------------------------------------------------------------------------------------------
-// A query without a target takes no part in the gradients, whatever it holds (a batch's padding may be NaN): its row of g is zeros, and so is
-// its row among dv's operands.
-__device__ __forceinline__ bool known(int target, int64_t n) { return target >= 0 && target < n; }
-
+// A query without a target (jvmm::known) takes no part in the gradients, whatever it (a batch's padding may be NaN) or a row holds: its row of g is zeros, and so
+// are its row among dv's operands and its own gradient.
 template <typename T>
 __device__ __forceinline__ void pack(const JvSxPrepare& a, const JvSxPrepare::Matrix& m, int64_t first, int64_t step) {   // eight components a thread
     constexpr int P = sizeof(T) == 4 ? 3 : 1;
@@ -111,6 +111,8 @@ __device__ __forceinline__ JvSxQuery query_of(const float* lse, const float* los
     const int t = targets[i];
     if (!known(t, n)) return {__builtin_inff(), 0.0f, -1, 0.0f};
     const float w0 = w ? w[i] : 1.0f, lse2 = lse[i] * 1.44269504088896341f;
+    // no probabilities (a logit was NaN or +inf, or all of them -inf): NaN shows, also beside a weight of 0 (times_or_0)
+    if (!(lse[i] > -__builtin_inff()) || w0 != w0) return {__builtin_nanf(""), __builtin_nanf(""), t, __builtin_nanf("")};
     // lse log2(e) - lse2: what both roundings left out, up to 2^-19 for a logarithm of 40 and as much of p
     const float lacks = fabsf(lse2) < __builtin_inff() ? fmaf(lse[i], 1.44269504088896341f, -lse2) + lse[i] * 1.92596299112661747e-8f : 0.0f;
     return {lse2, w0 * exp2_(-lacks) / unit, t, loss ? w0 / unit * expm1f(-loss[i]) : w0 / unit};
@@ -464,7 +466,7 @@ __device__ __forceinline__ void weigh(typename Core::acc_t (&acc)[NT], const JvS
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
-        for (int e = 0; e < Core::E; e++) acc[n][e] = exp2_(fmaf(acc[n][e], c, -q.lse2)) * q.w;
+        for (int e = 0; e < Core::E; e++) acc[n][e] = times_or_0(exp2_(fmaf(acc[n][e], c, -q.lse2)), q.w);   // (no target: 0)
     const int first = Core::col(0, 0) & ~(Core::WIDE < 32 ? 7 : 31);   // this wave's columns
     if (__any(hit >= first && hit < first + Core::WIDE)) {
 #pragma unroll
@@ -476,11 +478,11 @@ __device__ __forceinline__ void weigh(typename Core::acc_t (&acc)[NT], const JvS
                     if (lossy) *rest = acc[n][e] - (float)(__bf16)acc[n][e];   // (one lane holds it; three planes lack nothing)
                 }
     }
-    if (cols < Core::TN || (Core::RAW && __any(q.target < 0))) {   // (laid out, a query without a target is zeros)
+    if (cols < Core::TN) {
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int e = 0; e < Core::E; e++) acc[n][e] = (!Core::RAW || q.target >= 0) && Core::col(n, e) < cols ? acc[n][e] : 0.0f;
+            for (int e = 0; e < Core::E; e++) acc[n][e] = Core::col(n, e) < cols ? acc[n][e] : 0.0f;
     }
 }
 
@@ -630,7 +632,7 @@ extern "C" hipError_t jvk_sx_weights(const JvSxWeights* a, hipStream_t s) {
 template <class TQ, class TV>
 __global__ __launch_bounds__(256) void jvs_grads_tile_kernel(const JvMmOut q, const JvMmOut v, int first) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    if ((int)blockIdx.x < first) out_tile<TQ>(q, blockIdx.x, smem);
+    if ((int)blockIdx.x < first) out_tile<TQ, true>(q, blockIdx.x, smem);
     else out_tile<TV>(v, blockIdx.x - first, smem);
 }
 template <class TQ, class TV>
@@ -717,9 +719,10 @@ __global__ __launch_bounds__(256) void jvs_finish_kernel(const JvSxFinish q, con
     const float by = norm ? mul * *norm : mul, lack = a.rest ? a.rest[r] : 0.0f;
     const T* target = lack != 0.0f ? (const T*)a.vectors + a.query[r].target * a.v_stride : nullptr;
     T* out = (T*)a.out + r * a.ldo;
+    const bool dead = a.targets && !known(a.targets[r], a.n);   // (0 times a row that is not finite)
 #pragma unroll
     for (int e = 0; e < 4; e++)
-        if (c + e < d) out[c + e] = (T)((lack != 0.0f ? fmaf(lack, (float)target[c + e], x[e]) : x[e]) * by);
+        if (c + e < d) out[c + e] = (T)(dead ? 0.0f : (lack != 0.0f ? fmaf(lack, (float)target[c + e], x[e]) : x[e]) * by);
 }
 template <typename T>
 __global__ __launch_bounds__(256) void jvs_fill_kernel(T* __restrict__ out, int64_t stride, int64_t rows, int d, float value) {

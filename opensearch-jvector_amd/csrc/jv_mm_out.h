@@ -11,6 +11,9 @@ typedef __attribute__((ext_vector_type(2))) float f32x2;
 typedef __attribute__((ext_vector_type(1))) float f32x1;
 typedef __attribute__((ext_vector_type(1))) __bf16 bf16x1;
 
+// a query's target is one of n rows
+__device__ __forceinline__ bool known(int target, int64_t n) { return target >= 0 && target < n; }
+
 // the output's rows are 16-B aligned
 __host__ __device__ __forceinline__ bool aligned_rows(const JvMmOut& a) { return (uintptr_t)a.out % 16 == 0 && a.ldo % (a.dtype == 0 ? 4 : 8) == 0; }
 
@@ -112,8 +115,8 @@ struct Turn {
     }
 };
 
-// workgroup `i` of tiles * splits: one tile over one k range
-template <class T>
+// workgroup `i` of tiles * splits: one tile over one k range.  TARGETS: JvMmOut.targets is looked at.
+template <class T, bool TARGETS = false>
 __device__ __forceinline__ void out_tile(const JvMmOut& a, int i, unsigned char* smem) {
     constexpr int MT = T::MT, NT = T::NT;
     const int tm = (a.mm.M + T::TM - 1) / T::TM, tn = (a.mm.N + T::TN - 1) / T::TN, tiles = tm * tn;
@@ -141,6 +144,7 @@ __device__ __forceinline__ void out_tile(const JvMmOut& a, int i, unsigned char*
             V v = turn.template get<V>(i, r, c) * mul;
             r += m0, c += n0;
             if (r >= a.mm.M || c >= a.mm.N) continue;
+            if (TARGETS && a.targets && !known(a.targets[r], a.n)) v = V{};
             const int64_t at = (int64_t)r * a.ldo + c;
             if (a.dtype == 0) {
                 float* p = (float*)a.out + slab + at;

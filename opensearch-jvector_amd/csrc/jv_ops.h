@@ -31,6 +31,8 @@ struct JvMmOut {
     int64_t ldo;           // elements
     int32_t splits;        // partial sums over `splits` k ranges, float32 [splits][M][ldo] at `out`
     int32_t add;           // to what is there (float32)
+    const int32_t* targets;   // rows of C are queries, those without a target among `n` rows become zeros (jvs_grads_tile_kernel's first product); nullptr = all have one
+    int64_t n;
 };
 // the logits' forward pass: A = queries, B = vectors
 struct JvSxLoss {
@@ -62,6 +64,8 @@ struct JvSxFinish {
     const JvSxQuery* query;
     const void* vectors;
     int64_t v_stride;
+    const int32_t* targets;   // rows without a target among `n` become zeros; nullptr = all have one
+    int64_t n;
 };
 // One piece of the gradient's weights G = w (p - [j = target]), zeros where a query has no target: bf16 [M][kv]; float32 as three
 // planes [M][3][kv] (JV_SX_PLANES) or as it is [M][kv] (JV_SX_RAW).  Behind the last query: zeros, one row of them or up to a multiple of 64.
