@@ -320,7 +320,7 @@ typedef struct jv_softmax_params {
     int32_t device;
     int32_t dtype;          /* jv_dtype of the queries, the vectors and their gradients */
     int32_t nq, n, d;       /* queries, rows, components */
-    float scale;            /* 1 / temperature; finite */
+    float scale;            /* 1 / temperature; finite, as is its product with log2(e): below 2.35e38 */
     int32_t reserved;
     const void* queries;    /* [nq] rows, query_stride components apart */
     int64_t query_stride;

@@ -20,6 +20,7 @@ namespace {
 
 constexpr int64_t kMaxRows = 0x7fffffffll - 65536;   // a tile behind the last row still has an int32 number
 constexpr int64_t kMaxStride = 1ll << 31;
+constexpr float kLog2E = 1.44269504088896341f;
 constexpr int32_t kNoEnd = 0x7fffff00;          // JvMm.end_b of rows that have all of k
 
 // the caller's current device comes back on every way out
@@ -179,7 +180,7 @@ int check_softmax(const jv_softmax_params* p) {
     TRY(check_shape(p->n, p->d, "softmax: vectors"));
     TRY(check_shape(p->nq, p->d, "softmax: queries"));
     if (p->nq > JV_SOFTMAX_MAX_QUERIES) return jvi_fail(JV_EUNSUPPORTED, "softmax: %d queries (> %d)", p->nq, JV_SOFTMAX_MAX_QUERIES);
-    if (!std::isfinite(p->scale)) return jvi_fail(JV_EINVAL, "softmax: scale is not finite");
+    if (!std::isfinite(p->scale * kLog2E)) return jvi_fail(JV_EINVAL, "softmax: scale or its product with log2(e) is not finite");
     return JV_OK;
 }
 int check_softmax_call(const jv_softmax_params* p, const Plan& plan) {
@@ -294,7 +295,7 @@ int jv_softmax_loss_device(const jv_softmax_params* p, float* d_out_loss, float*
         const int64_t step = rv.ready ? std::max<int64_t>(p->n, 1) : plan.rows_f;
         JvSxLoss a{};
         a.mm = logits(plan, p->nq, p->d);
-        a.c = p->scale * 1.44269504088896341f;
+        a.c = p->scale * kLog2E;
         a.targets = p->targets, a.hit = (float*)(ws + plan.off_hit);
         const bool shift = rv.ready && p->dtype == JV_DTYPE_BF16 && p->d % 8;   // (JvMm.end_b)
         if (rv.ready && p->dtype == JV_DTYPE_BF16) a.mm.end_b = p->d * 2;
@@ -345,7 +346,7 @@ int jv_softmax_grad_device_ex(const jv_softmax_params* p, const float* d_lse, co
     const bool f32 = p->dtype == JV_DTYPE_F32, raw = plan.path_b == JV_SX_RAW;
     JvSxWeights w{};
     w.mm = logits(plan, p->nq, p->d);
-    w.c = p->scale * 1.44269504088896341f;
+    w.c = p->scale * kLog2E;
     if (rv.ready && !f32) w.mm.end_b = p->d * 2;
     w.path = plan.path_b, w.g = ws + plan.off_g, w.loss = d_loss;
     // float32 g needs no common unit and lacks nothing at a target
