@@ -230,14 +230,17 @@ __device__ __forceinline__ void add_tile(const JvSxLoss& a, typename Core::acc_t
     }
 #pragma unroll
     for (int m = 0; m < MT; m++) {
-        // (c = 0: every logit is 0, also that of an infinite product, but the target's and those behind the last row are left out)
+        // (c = 0: a lane that has rows has 0 for its maximum)
         const float now = fmaxf(top[m], best[m] == none ? -__builtin_inff() : best[m] * c), ref = now == -__builtin_inff() ? 0.0f : now;
         float s = sum[m] * exp2_(top[m] - ref);
         if (c == 0.0f) {
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
-                for (int e = 0; e < Core::E; e++) s += acc[m][n][e] == none ? 0.0f : exp2_(acc[m][n][e] * 0.0f);
+                for (int e = 0; e < Core::E; e++) {   // (by their places: -inf may be a product, and 0 times that is NaN)
+                    const int col = Core::col(n, e);
+                    s += col < rows && col != want[m] - n0 ? exp2_(acc[m][n][e] * 0.0f) : 0.0f;
+                }
         } else {
 #pragma unroll
             for (int n = 0; n < NT; n++)

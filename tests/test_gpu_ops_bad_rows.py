@@ -104,3 +104,15 @@ def test_a_row_of_minus_infinite_logits_is_left_out(torch, ops):
     # (one rounding of g and one of the result may fall the other way: half a step each, twice)
     assert (dv[299] == 0).all() and ((dv[:299].double() - want.double()).abs() <= 4 * half_step("bf16") * np.abs(want.abs().double().max().item())).all()
     assert (dq[3] == 0).all()
+
+
+@pytest.mark.parametrize("dtype,nq,n,d", SHAPES)
+def test_a_scale_of_zero_beside_an_infinite_product(torch, ops, dtype, nq, n, d):
+    """0 times infinity is NaN, whatever its sign; no row is left out of the others' sum."""
+    q, v, t, w = inputs(torch, dtype, nq, n, d)
+    loss, lse = ops.softmax_loss(q, v, t, 0.0)
+    assert ((lse - np.log(n)).abs() <= 2.0 ** -19).all() and ((loss - np.log(n)).abs() <= 2.0 ** -19).all()
+    for bad in (float("inf"), -float("inf")):
+        v[n // 2, 0] = bad
+        loss, lse = ops.softmax_loss(q.abs() + 1, v, t, 0.0)
+        assert torch.isnan(loss).all() and torch.isnan(lse).all()
