@@ -333,7 +333,10 @@ typedef struct jv_softmax_params {
 #define JV_SOFTMAX_LOSS 0x1u
 #define JV_SOFTMAX_QUERY_GRAD 0x2u
 #define JV_SOFTMAX_VECTOR_GRAD 0x4u
-/* Bytes of workspace that the calls named by `what` (JV_SOFTMAX_*) need for this dtype, nq, n and d. */
+#define JV_SOFTMAX_AS_THEY_LIE 0x8u /* with the others, in jv_softmax_workspace: for vectors of this alignment and stride only */
+/* Bytes of workspace that the calls named by `what` (JV_SOFTMAX_*) need for this dtype, nq, n and d: wherever the vectors lie, or, with
+ * JV_SOFTMAX_AS_THEY_LIE, for `vectors` (its alignment counts, nothing is read) and `vector_stride` as they are.  bf16 rows that are 4-byte aligned, of an even number
+ * of components, need no room to be laid out in, which may be 2 GiB. */
 int jv_softmax_workspace(const jv_softmax_params* params, uint32_t what, int64_t* out_bytes);
 /* out_loss [nq], out_lse [nq] (natural logarithm; -inf if n == 0). */
 int jv_softmax_loss_device(const jv_softmax_params* params, float* d_out_loss, float* d_out_lse, void* hip_stream);

@@ -32,7 +32,7 @@ ABI_SYMBOLS = [
 ]
 DTYPE_F32, DTYPE_BF16 = 0, 1
 OPS_MAX_D, SOFTMAX_MAX_QUERIES = 65536, 1 << 22
-SOFTMAX_LOSS, SOFTMAX_QUERY_GRAD, SOFTMAX_VECTOR_GRAD = 0x1, 0x2, 0x4
+SOFTMAX_LOSS, SOFTMAX_QUERY_GRAD, SOFTMAX_VECTOR_GRAD, SOFTMAX_AS_THEY_LIE = 0x1, 0x2, 0x4, 0x8
 XB_NO_PREFILTER, XB_FORCE_PREFILTER, XB_TOPK_MAX, XB_INFO_WORDS = 0x1, 0x2, 1024, 4
 QFLAG_RETRIED_BIG, QFLAG_EARLY_TERMINATED = 0x1, 0x2
 

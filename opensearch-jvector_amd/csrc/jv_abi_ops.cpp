@@ -271,11 +271,12 @@ int jv_score_blocks_device(int32_t device, const uint8_t* d_query_codes, const u
 
 int jv_softmax_workspace(const jv_softmax_params* params, uint32_t what, int64_t* out_bytes) {
     TRY(check_softmax(params));
-    if (!out_bytes || !what || (what & ~7u)) return jvi_fail(JV_EINVAL, "softmax: out_bytes is NULL or unknown flags %#x", what);
+    if (!out_bytes || !(what & 7u) || (what & ~15u)) return jvi_fail(JV_EINVAL, "softmax: out_bytes is NULL, no call is named or unknown flags %#x", what);
+    const bool here = what & JV_SOFTMAX_AS_THEY_LIE;
     int64_t need = 256;   // (the loss and its gradient are separate calls: the larger of the two)
     for (uint32_t part : {what & JV_SOFTMAX_LOSS, what & (JV_SOFTMAX_QUERY_GRAD | JV_SOFTMAX_VECTOR_GRAD)})
-        for (bool as_is : {false, true})   // (bf16: where the vectors lie decides, which is not known here)
-            if (part && (as_is ? can_lie(params->dtype, params->d) : params->dtype == JV_DTYPE_BF16 || !can_lie(params->dtype, params->d)))
+        for (bool as_is : {false, true})   // (bf16: where the vectors lie decides)
+            if (part && (here ? as_is == lies(params) : as_is ? can_lie(params->dtype, params->d) : params->dtype == JV_DTYPE_BF16 || !can_lie(params->dtype, params->d)))
                 need = std::max(need, make_plan(params->dtype, params->nq, params->n, params->d, part, as_is).bytes);
     *out_bytes = need;
     return JV_OK;

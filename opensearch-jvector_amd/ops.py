@@ -28,8 +28,10 @@ def _stream(device) -> int:
 
 
 @functools.lru_cache(maxsize=1024)
-def _workspace_bytes(dtype: int, nq: int, n: int, d: int, flags: int) -> int:
-    return binding.softmax_workspace(binding.softmax_params(0, dtype, nq, n, d, 1.0), flags)   # (the shape alone decides)
+def _workspace_bytes(dtype: int, nq: int, n: int, d: int, flags: int, offset: int, odd: bool) -> int:
+    # the shape decides, and whether the vectors can be taken as they lie: `offset`: their address to 4 bytes, `odd`: their stride
+    params = binding.softmax_params(0, dtype, nq, n, d, 1.0, d_vectors=4 + offset, vector_stride=int(odd))
+    return binding.softmax_workspace(params, flags | binding.SOFTMAX_AS_THEY_LIE)
 
 
 def _matrix(x: torch.Tensor, what: str, name: str):
@@ -105,7 +107,7 @@ def _softmax(queries, vectors, targets, scale, what, flags):
         _like(targets, device, (nq,), torch.int32, what, "targets")
     params = binding.softmax_params(device.index, dtype, nq, n, d, scale, queries.data_ptr(), q_stride, vectors.data_ptr(), v_stride,
                                     0 if targets is None else targets.data_ptr())
-    need = _workspace_bytes(dtype, nq, n, d, flags)
+    need = _workspace_bytes(dtype, nq, n, d, flags, vectors.data_ptr() % 4, v_stride % 2 == 1)
     workspace = torch.empty(need, dtype=torch.uint8, device=device)
     params.workspace_bytes, params.workspace = need, workspace.data_ptr()
     return params, workspace, device
