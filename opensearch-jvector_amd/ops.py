@@ -8,7 +8,8 @@
 Plumbing only: argument checks, output tensors and workspaces from torch's allocator, the calls of the C ABI on torch's current
 stream of the tensors' device (which need not be the current device).  Nothing here waits for the GPU or keeps anything between calls, so
 every function can be captured into a graph; there is no CPU fallback.  Vectors are float32 or bfloat16 matrices whose rows are
-contiguous; the rows may lie any distance apart.  Not differentiable by autograd: the gradient is a call of its own.
+contiguous; the rows may lie any distance apart.  Not differentiable by autograd: the gradient is a call of its own, and a loss of tensors that
+autograd records is refused (detach them, or call under ``torch.no_grad()``).
 """
 from __future__ import annotations
 
@@ -116,6 +117,9 @@ def _softmax(queries, vectors, targets, scale, what, flags):
 def softmax_loss(queries: torch.Tensor, vectors: torch.Tensor, targets, scale: float):
     """(loss [nq], lse [nq]), float32: loss_i = lse_i - scale q_i . v_targets[i], lse_i = log sum_j exp(scale q_i . v_j).  ``targets``: int32, a value
     outside [0, n) (or None in place of the tensor) = no target, loss 0; see jv_softmax_loss_device."""
+    if torch.is_grad_enabled() and (queries.requires_grad or vectors.requires_grad):
+        raise ValueError("softmax_loss: autograd does not see this loss: detach the queries and vectors, or call it under torch.no_grad(), and take the gradient "
+                         "from softmax_loss_grad")
     params, workspace, device = _softmax(queries, vectors, targets, scale, "softmax_loss", binding.SOFTMAX_LOSS)
     nq = queries.shape[0]
     loss = torch.empty(nq, dtype=torch.float32, device=device)
