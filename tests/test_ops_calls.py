@@ -39,3 +39,27 @@ def test_a_workspace_for_vectors_as_they_lie(pkg):
         with pytest.raises(b.JvError) as e:
             need(1, 10, 8, what)
         assert e.value.code == b.JV_EINVAL
+
+
+def test_the_gradient_without_losses_refuses_what_the_one_with_them_refuses(pkg):
+    """jv_softmax_grad_device itself (the binding calls jv_softmax_grad_device_ex)."""
+    import ctypes
+    b = pkg.binding
+    lib, A = b.load_library(), 1 << 20
+
+    def call(name, params, lse=A, dq=A, dq_stride=64, dv=A, dv_stride=64):
+        between = (None,) if name.endswith("_ex") else ()
+        return getattr(lib, name)(ctypes.byref(params), lse, *between, None, dq, dq_stride, dv, dv_stride, None)
+
+    def params(**kw):
+        p = b.softmax_params(0, kw.pop("dtype", 1), 5, 100, 64, kw.pop("scale", 1.0), A, 64, A, 64, A)
+        p.workspace, p.workspace_bytes = A, 1 << 40
+        for k, x in kw.items():
+            setattr(p, k, x)
+        return p
+    for name in ("jv_softmax_grad_device", "jv_softmax_grad_device_ex"):
+        for kw in (dict(struct_size=80), dict(dtype=3), dict(scale=float("inf")), dict(queries=A + 1), dict(vector_stride=0), dict(workspace=None), dict(workspace_bytes=255)):
+            assert call(name, params(**kw)) == b.JV_EINVAL, (name, kw)
+        assert call(name, params(), lse=None) == b.JV_EINVAL and call(name, params(), dq=None, dv=None) == b.JV_EINVAL
+        assert call(name, params(), dq_stride=63) == b.JV_EINVAL and call(name, params(), dv=A + 1) == b.JV_EINVAL
+        assert call(name, params(d=b.OPS_MAX_D + 1)) == b.JV_EUNSUPPORTED
