@@ -308,11 +308,13 @@ int jv_score_blocks_device(int32_t device, const uint8_t* d_query_codes, const u
 
 /* Softmax cross entropy of queries over ALL rows of a matrix, as an embedding model or a query adapter is trained against a corpus:
  *   lse_i = log sum_j exp(scale q_i . v_j),   loss_i = lse_i - scale q_i . v_t(i)
- * in pieces of the rows: the nq x n logits are never held.  A target outside [0, n) is none: its loss is 0, its gradient 0, and it adds to no
- * row's gradient, whatever the query (a batch's padding may be NaN) or a row holds.  A logit of NaN or +infinity makes its query's lse NaN and, where the
- * query has a target, its loss, its gradient and every row's gradient; so does NaN for its lse or weight.  A bf16 logit of -infinity has probability 0, or is
- * NaN (zeros that a product adds behind a row's end meet the infinity).  Infinite components of float32 make NaN; beyond 3.38e38 (bf16's largest) they
- * count as infinite.
+ * in pieces of the rows.  The loss holds none of the nq x n logits; the gradient holds a weight in the place of each, in the workspace, for one
+ * piece of the rows: up to about 1 GiB (or 256 rows', where that is more).  A loss near 0 has all the digits of its float32 logits.
+ * A target outside [0, n) is none: its loss is 0, its gradient 0, and it adds to no row's gradient, whatever the query (a batch's padding may
+ * be NaN) or a row holds.  A logit of NaN or +infinity makes its query's lse NaN and, where the query has a target, its loss, its gradient and
+ * every row's gradient; so does NaN for its lse or weight.  A bf16 logit of -infinity has probability 0 (its query's gradient is 0 times infinity, NaN),
+ * or is NaN itself (zeros that a product adds behind a row's end meet the infinity).  Infinite components of float32 make NaN; beyond 3.38e38
+ * (bf16's largest) they count as infinite.
  * Logits are float32 sums of exact products; the gradient of bf16 rounds each probability to bf16 once (relative to the largest loss_grad). */
 #define JV_SOFTMAX_MAX_QUERIES (1 << 22)
 typedef struct jv_softmax_params {
@@ -335,8 +337,8 @@ typedef struct jv_softmax_params {
 #define JV_SOFTMAX_VECTOR_GRAD 0x4u
 #define JV_SOFTMAX_AS_THEY_LIE 0x8u /* with the others, in jv_softmax_workspace: for vectors of this alignment and stride only */
 /* Bytes of workspace that the calls named by `what` (JV_SOFTMAX_*) need for this dtype, nq, n and d: wherever the vectors lie, or, with
- * JV_SOFTMAX_AS_THEY_LIE, for `vectors` (its alignment counts, nothing is read) and `vector_stride` as they are.  bf16 rows that are 4-byte aligned, of an even number
- * of components, need no room to be laid out in, which may be 2 GiB. */
+ * JV_SOFTMAX_AS_THEY_LIE, for `vectors` (its alignment counts, nothing is read) and `vector_stride` as they are.  bf16 rows of an even number of components (eight
+ * at least) and an even stride, 4-byte aligned, need no room to be laid out in, which may be 2 GiB. */
 int jv_softmax_workspace(const jv_softmax_params* params, uint32_t what, int64_t* out_bytes);
 /* out_loss [nq], out_lse [nq] (natural logarithm; -inf if n == 0). */
 int jv_softmax_loss_device(const jv_softmax_params* params, float* d_out_loss, float* d_out_lse, void* hip_stream);

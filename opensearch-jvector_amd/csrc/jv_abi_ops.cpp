@@ -85,7 +85,8 @@ struct Plan {
 };
 
 // MB of one piece's weights g: few large pieces, for every piece writes and reads dq's partial sums again and starts its tiles anew (step
-// 4096 x 131072 x 1024: 4.67 ms with 128, 4.54 with 384, 4.32 with 1024, all of it in one piece)
+// 4096 x 131072 x 1024: 4.67 ms with 128, 4.54 with 384, 4.32 with 1024, all of it in one piece).  A piece has whole tiles of 256 rows and at least one: 6 GiB
+// of g with 2^22 float32 queries.
 constexpr int64_t kWeights = 1024;
 // MB of one piece's rows, where a gradient needs them laid out
 constexpr int64_t kLaid = 2048;

@@ -145,8 +145,9 @@ extern "C" hipError_t jvk_f8_decode(const uint8_t* codes, const uint8_t* scales,
 //   1 x 100 000 x 768: 22 us, the launches of the two calls (the query's encoding and this) and 77 MB of codes.
 //   256 x 500 000 x 768, float32: 265 us, 3.4 TB/s, more than half of it the scores; the stores of one tile and the products of the next
 //     share a wave's order of memory operations, so they overlap by two phases only.  d = 128: 133 us, 4.3 TB/s (large copy: 4.7).
-//   4096 x 65 536 x 1536, bf16: 465 us, 1770 TFLOP/s (a large library product of 8-bit floats: 2785); 8-bit products draw the most power and the
-//     clock gives way.  256 x 256 against 128 x 128 tiles: 1024 x 100 000 x 768, bf16: 128 and 178 us.
+//   4096 x 65 536 x 1536, bf16: 470 us, 1750 TFLOP/s (a large library product of 8-bit floats: 2785).  The matrix unit has work in 42 % of the cycles; 15 %
+//     of the LDS cycles are bank conflicts (float32 scores: 25 %), which bf16 products on these tiles do not have: the scales' reads or the
+//     epilogue's writes, not found out which.  256 x 256 against 128 x 128 tiles: 1024 x 100 000 x 768, bf16: 128 and 178 us.
 template <int TY>
 static hipError_t score(const JvMmOut& a, hipStream_t s) {
     const int64_t M = a.mm.M, N = a.mm.N, tiles = (M + 127) / 128 * ((N + 127) / 128);

@@ -1,7 +1,10 @@
-// jv_kernels_sx.hip — softmax cross entropy of queries over all rows of an index, and its gradient, without keeping the logits (gfx950).
+// jv_kernels_sx.hip — softmax cross entropy of queries over all rows of an index without keeping the logits, and its gradient, which keeps a weight in the place
+// of each, a piece of the rows at a time (gfx950).
 //
-//   z_ij = scale q_i . v_j     lse_i = log sum_j exp z_ij     loss_i = lse_i - z_i,t(i)
+//   z_ij = scale q_i . v_j     lse_i = log sum_j exp z_ij     loss_i = lse_i - z_i,t(i) = log(1 + sum_(j != t(i)) exp(z_ij - z_i,t(i)))
 //   g_ij = w_i scale (exp(z_ij - lse_i) - [j = t(i)])         dq_i = sum_j g_ij v_j         dv_j = sum_i g_ij q_i
+// The sums leave the target out, and g at the target is w_i scale (exp(-loss_i) - 1) where the losses are given: a learnt pair's loss and gradient have all the
+// digits of float32 products, not those that are left behind a 1.
 //
 // Forward: a workgroup walks tiles of rows for one panel of queries, and every lane keeps the running maximum and sum of ITS rows (one column of
 // the accumulators is one query: no exchange until the end); the workgroups' partials are joined by a second kernel.  Backward: the logits
@@ -14,11 +17,11 @@
 // pairs of them that reach 2^-24: float32's accuracy at 1.5 times the rate of its own matrix instruction (1423 / 6 against 154 TFLOP/s).
 //
 // What bounds it (MI355X; a large copy moves 4.7 TB/s, a large bf16 product runs at 1423 TFLOP/s):
-//   few queries (bf16 300, float32 100: as many operations as a byte of rows pays for): the rows' bytes.  Loss 256 x 1 000 000 x 768 bf16: 445 us,
-//     3.5 TB/s and 880 TFLOP/s, near both; loss 11 x 257 776 x 1272 float32: 268 us, 4.9 TB/s.
+//   few queries (bf16 300, float32 100: as many operations as a byte of rows pays for): the rows' bytes.  Loss 256 x 1 000 000 x 768 bf16: 450 us,
+//     3.4 TB/s and 870 TFLOP/s, near both; loss 11 x 257 776 x 1272 float32: 268 us, 4.9 TB/s.
 //   many queries: the matrix unit, and behind each tile the exponentials (a quarter of the rate of other instructions), which no product runs
-//     beside.  Step 4096 x 131 072 x 1024 bf16: 4.15 ms, 1060 TFLOP/s over its four products; float32 777 x 30 011 x 381: 550 us, 775 TFLOP/s.
-//   little of everything: the launches.  Step 32 x 1000 x 64 float32: 42 us for four.
+//     beside.  Step 4096 x 131 072 x 1024 bf16: 4.17 ms, 1055 TFLOP/s over its four products; float32 777 x 30 011 x 381: 550 us, 775 TFLOP/s.
+//   little of everything: the launches.  Step 32 x 1000 x 64 float32: 37 us for five.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
