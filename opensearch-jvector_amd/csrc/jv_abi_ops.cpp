@@ -125,17 +125,22 @@ Plan make_plan(int dtype, int nq, int64_t n, int d, uint32_t what, bool as_is) {
         at += up(bytes, 256);
         return o;
     };
-    p.off_q = take((int64_t)nq * row);
+    // bytes of a query or row that is laid out: float32 of fewer than four components as four of them (rows_of), queries of JV_SX_RAW not at all otherwise
+    const bool f32 = dtype == JV_DTYPE_F32;
+    auto query = [&](int path) { return f32 && path == JV_SX_RAW ? d < 4 ? 16 : 0 : row; };
+    const int64_t laid = f32 ? 16 : row;
     if (what & JV_SOFTMAX_LOSS) {
-        p.path_f = jvk_sx_path(nq, n, dtype == JV_DTYPE_F32);
+        p.path_f = jvk_sx_path(nq, n, f32);
+        p.off_q = take(nq * query(p.path_f));
         p.splits_f = jvk_sx_loss_splits(p.path_f, nq, n, d);
         p.off_part = take((int64_t)p.splits_f * nq * 8);
         p.off_hit = take((int64_t)nq * 4);
-        p.off_v = take(as_is ? 0 : std::min<int64_t>(p.rows_f, n) * row);
+        p.off_v = take(as_is ? 0 : std::min<int64_t>(p.rows_f, n) * laid);
     }
     if (what & (JV_SOFTMAX_QUERY_GRAD | JV_SOFTMAX_VECTOR_GRAD)) {
-        p.path_b = jvk_sx_path(nq, std::min<int64_t>(p.rows_b, n), dtype == JV_DTYPE_F32);
-        p.off_v = take(as_is ? 0 : std::min<int64_t>(p.rows_b, n) * row);
+        p.path_b = jvk_sx_path(nq, std::min<int64_t>(p.rows_b, n), f32);
+        p.off_q = take(nq * query(p.path_b));
+        p.off_v = take(as_is ? 0 : std::min<int64_t>(p.rows_b, n) * laid);
         p.off_query = take((int64_t)nq * sizeof(JvSxQuery));
         p.off_norm = take(4);
         p.off_tail = take(16);
@@ -148,7 +153,7 @@ Plan make_plan(int dtype, int nq, int64_t n, int d, uint32_t what, bool as_is) {
         if (what & JV_SOFTMAX_VECTOR_GRAD) {
             const int64_t rows = std::min<int64_t>(p.rows_b, n);
             p.splits_v = jvk_sx_grad_splits(p.path_b, rows, d, nq, 1);
-            p.off_clean = take(dtype == JV_DTYPE_F32 ? (int64_t)nq * std::max(d, 4) * 4 : d % 8 ? (int64_t)nq * p.dp * 2 : 0);
+            p.off_clean = take(f32 ? (int64_t)nq * std::max(d, 4) * 4 : d % 8 ? (int64_t)nq * p.dp * 2 : 0);
             p.off_slab_v = take(p.splits_v > 1 ? p.splits_v * rows * p.dp * 4 : 0);
         }
     }

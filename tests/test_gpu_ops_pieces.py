@@ -57,7 +57,7 @@ def test_every_row_counts(torch, ops, pkg, dtype, nq, n, d, forward, backward):
     kind = b.DTYPE_F32 if dtype == "f32" else b.DTYPE_BF16
     v, q, a, t, block = counted(torch, dtype, nq, n, d)
     planes = 3 if dtype == "f32" else 1
-    laid = planes * -(-d // 64) * 64 * 2 if (d % 2 if dtype == "bf16" else d < 4) else 0   # bytes of a row that is laid out
+    laid = (-(-d // 64) * 128 if d % 2 else 0) if dtype == "bf16" else (16 if d < 4 else 0)   # bytes of a row that is laid out
     if forward > 1:
         assert pieces(b, kind, nq, n, d, b.SOFTMAX_LOSS, v, laid) >= forward
     if backward > 1:

@@ -63,3 +63,19 @@ def test_the_gradient_without_losses_refuses_what_the_one_with_them_refuses(pkg)
         assert call(name, params(), lse=None) == b.JV_EINVAL and call(name, params(), dq=None, dv=None) == b.JV_EINVAL
         assert call(name, params(), dq_stride=63) == b.JV_EINVAL and call(name, params(), dv=A + 1) == b.JV_EINVAL
         assert call(name, params(d=b.OPS_MAX_D + 1)) == b.JV_EUNSUPPORTED
+
+
+def test_a_float32_workspace_has_room_for_what_is_laid_out_alone(pkg):
+    """Rows and queries of fewer than four components are laid out with four (16 bytes), others of few tiles not at all."""
+    b = pkg.binding
+
+    def need(nq, n, d, what):
+        return b.softmax_workspace(b.softmax_params(0, b.DTYPE_F32, nq, n, d, 1.0), what)
+    # 2^15 queries of 2^16 components against 16 rows: taken as they lie; dv's copy of those without a target as zeros is 8 GiB
+    nq, d = 1 << 15, 1 << 16
+    assert need(nq, 16, d, b.SOFTMAX_LOSS) < 1 << 20
+    assert need(nq, 16, d, b.SOFTMAX_QUERY_GRAD) < (nq * d * 4) + (64 << 20)          # one range of dq's partial sums
+    assert need(nq, 16, d, b.SOFTMAX_VECTOR_GRAD) < (nq * d * 4) + (64 << 20)
+    # rows of three components: no more than 16 bytes each of one piece, and the partial sums
+    assert need(64, 6000001, 3, b.SOFTMAX_LOSS) < 6000001 * 16
+    assert need(1, 1000, 3, b.SOFTMAX_LOSS) < 1000 * 16 + 8192
